@@ -307,6 +307,31 @@ NB200_API int nb200_blob_mean_pooling(void* stream, int batch, int h, int w, int
 NB200_API int nb200_blob_resize_image(void* stream, int batch, int h, int w, int c, int delta_left, int delta_right,
 	int delta_top, int delta_bottom, int padding, float default_value, const float* x, float* y);
 
+/* ---- language-model operators -------------------------------------------------------------------------------- */
+/* The operators below take their data in one of three types; what they sum, normalise or carry along is fp32 in all.
+ * Data pointers are aligned to their element's size or better, row sizes count elements, int arrays are 32-bit. */
+enum {
+	NB200_TYPE_FP32 = 0,
+	NB200_TYPE_FP16 = 1,
+	NB200_TYPE_BF16 = 2
+};
+/* CObjectNormalizationLayer's arithmetic (SumMatrixColumns, NME.h:439-440; AddVectorToMatrixColumns, NME.h:423-424;
+ * MultiplyDiagMatrixByMatrix, NME.h:570-572; MultiplyMatrixByDiagMatrix, NME.h:588-596) as one pass over the rows:
+ * y[h][w] = (x[h][w] - mean[h]) * inverse_deviation[h] * scale[w] + free_term[w], inverse_deviation = 1 / sqrt(variance +
+ * epsilon), the variance being that of the width elements (not width - 1).  scale and free_term are of parameter_type, which is `type`
+ * or NB200_TYPE_FP32; NULL: ones, zeros.  mean and inverse_deviation (NULL: not wanted) get a float per row.  y may be x. */
+NB200_API int nb200_layer_normalization(void* stream, int type, int parameter_type, const void* x, int height, int width,
+	long long x_row_size, const void* scale, const void* free_term, float epsilon, void* y, long long y_row_size, float* mean,
+	float* inverse_deviation);
+/* Its gradients (the training half of the same layer; NME.h:433-436 sums the parameters' over the rows): dx from dy, x and
+ * the two vectors of the forward pass; scale_diff and free_term_diff, of parameter_type, each NULL where not wanted.  The
+ * sums over the rows are made in a fixed order: the same bits from run to run.  dx may be dy or x.  `scratch` holds
+ * nb200_layer_normalization_backward_scratch_floats(type, height, width) floats; NULL when both are NULL. */
+NB200_API size_t nb200_layer_normalization_backward_scratch_floats(int type, int height, int width);
+NB200_API int nb200_layer_normalization_backward(void* stream, int type, int parameter_type, const void* dy,
+	long long dy_row_size, const void* x, int height, int width, long long x_row_size, const void* scale, const float* mean,
+	const float* inverse_deviation, void* dx, long long dx_row_size, void* scale_diff, void* free_term_diff, float* scratch);
+
 #ifdef __cplusplus
 }
 #endif

@@ -22,6 +22,7 @@ def native_path() -> Path:
 OK, EINVAL, ENODEVICE, ELAUNCH, EDEVICE, ETOOBIG = 0, -1, -2, -3, -4, -5
 PREC_3XTF32, PREC_TF32, PREC_FP32_SIMT = 0, 1, 2
 ACT_NONE, ACT_RELU, ACT_HSWISH = 0, 1, 2
+TYPE_FP32, TYPE_FP16, TYPE_BF16 = 0, 1, 2
 
 VEC_OPS = ["COPY", "FILL", "FILL_HANDLE", "ADD", "SUB", "ELTWISE_MUL", "MULTIPLY", "NEG_MULTIPLY", "ADD_VALUE",
            "RELU", "SIGMOID", "SQRT", "INV", "TANH", "EXP", "HSWISH", "ELTWISE_MAX", "ELTWISE_DIV", "MUL_ADD"]
@@ -50,7 +51,7 @@ class Mbv2Desc(C.Structure):
                                                                 ("act_dw_param", C.c_float)]
 
 
-_vp, _i, _f = C.c_void_p, C.c_int, C.c_float
+_vp, _i, _f, _ll = C.c_void_p, C.c_int, C.c_float, C.c_longlong
 _EP = C.POINTER(Epilogue)
 
 # name -> (restype, argtypes); the single source of truth for tests that check exported symbols
@@ -102,6 +103,10 @@ SIGNATURES = {
     "nb200_blob_max_pooling_padded": (_i, [_vp, _i, _i, _i, _i, _i, _i, _i, _i, _f, _i, _i, _i, _i, _vp, _vp]),
     "nb200_blob_mean_pooling": (_i, [_vp, _i, _i, _i, _i, _i, _i, _i, _i, _vp, _vp]),
     "nb200_blob_resize_image": (_i, [_vp, _i, _i, _i, _i, _i, _i, _i, _i, _i, _f, _vp, _vp]),
+    "nb200_layer_normalization": (_i, [_vp, _i, _i, _vp, _i, _i, _ll, _vp, _vp, _f, _vp, _ll, _vp, _vp]),
+    "nb200_layer_normalization_backward_scratch_floats": (C.c_size_t, [_i, _i, _i]),
+    "nb200_layer_normalization_backward": (_i, [_vp, _i, _i, _vp, _ll, _vp, _i, _i, _ll, _vp, _vp, _vp, _vp, _ll, _vp, _vp,
+                                                _vp]),
 }
 
 # Diagnostic entry points (neoml_b200/csrc/diagnostics.h): exported for the benchmark and the tests, not part of the

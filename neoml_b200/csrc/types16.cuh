@@ -1,0 +1,92 @@
+// Element types of the row, sequence and loss kernels: fp32, fp16 and bf16 data in global memory, fp32 in registers.
+// Conversions to 16 bits happen once, at the final store, to nearest even.
+#pragma once
+#include "common.cuh"
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+namespace nb200 {
+
+inline int type_size(int type) { return type == NB200_TYPE_FP32 ? 4 : 2; }
+inline bool type_valid(int type) { return type == NB200_TYPE_FP32 || type == NB200_TYPE_FP16 || type == NB200_TYPE_BF16; }
+// every address of a row-addressed operand is a multiple of its element's size
+inline bool type_aligned(const void* p, int type) { return (reinterpret_cast<uintptr_t>(p) & (type_size(type) - 1)) == 0; }
+
+#ifdef __CUDACC__
+
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+template<typename T> __device__ __forceinline__ T from_float(float v);
+template<> __device__ __forceinline__ float from_float<float>(float v) { return v; }
+template<> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
+template<> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// Two 16-bit values in one register, and back.
+template<typename T> __device__ __forceinline__ float2 unpack2(uint32_t v);
+template<> __device__ __forceinline__ float2 unpack2<__half>(uint32_t v)
+{
+	return __half22float2(*reinterpret_cast<const __half2*>(&v));
+}
+template<> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t v)
+{
+	return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u)); // a bf16 is the upper half of a float
+}
+template<typename T> __device__ __forceinline__ uint32_t pack2(float a, float b);
+template<> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b)
+{
+	const __half2 h = __floats2half2_rn(a, b);
+	return *reinterpret_cast<const uint32_t*>(&h);
+}
+template<> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b)
+{
+	const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+	return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// 16 bytes as they lie in memory <-> the floats they hold (four or eight).
+template<typename T> struct Unit16 {
+	static constexpr int N = 16 / static_cast<int>(sizeof(T));
+	static __device__ __forceinline__ void unpack(const uint4& r, float* v)
+	{
+		const uint32_t w[4] = { r.x, r.y, r.z, r.w };
+#pragma unroll
+		for(int i = 0; i < 4; ++i) {
+			const float2 f = unpack2<T>(w[i]);
+			v[2 * i] = f.x;
+			v[2 * i + 1] = f.y;
+		}
+	}
+	static __device__ __forceinline__ uint4 pack(const float* v)
+	{
+		return make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
+	}
+};
+template<> struct Unit16<float> {
+	static constexpr int N = 4;
+	static __device__ __forceinline__ void unpack(const uint4& r, float* v)
+	{
+		v[0] = __uint_as_float(r.x); v[1] = __uint_as_float(r.y); v[2] = __uint_as_float(r.z); v[3] = __uint_as_float(r.w);
+	}
+	static __device__ __forceinline__ uint4 pack(const float* v)
+	{
+		return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+	}
+};
+
+__device__ __forceinline__ float warp_sum_all(float v)
+{
+#pragma unroll
+	for(int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+	return v;
+}
+__device__ __forceinline__ float warp_max_all(float v)
+{
+#pragma unroll
+	for(int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+	return v;
+}
+
+#endif // __CUDACC__
+
+} // namespace nb200

@@ -4,6 +4,10 @@ torch is used for device memory and streams only; every computation is a call in
 (include/neoml_b200.h) on the tensors' device pointers, enqueued on torch's current stream.
 Method names and argument meaning follow NeoMathEngine/include/NeoMathEngine/NeoMathEngine.h; blobs are
 channels-last ``[batch, height, width, channels]`` fp32 tensors, filters ``[count, height, width, channels]``.
+
+The operators of language models at the end of the file (normalisation, recurrence, losses) take fp32, fp16 or bf16 data
+and run on the device that their tensors are on, on torch's current stream of that device.  What they record nowhere is a
+gradient: the backward pass of each is a call of its own, as in NeoML's engine.
 """
 from __future__ import annotations
 
@@ -414,3 +418,95 @@ def BlobResizeImage(source, delta_left, delta_right, delta_top, delta_bottom, pa
         _stream(), n, h, w, c, delta_left, delta_right, delta_top, delta_bottom, padding, float(default_value),
         _ptr(source), _ptr(result)))
     return result
+
+
+# ---- operators of language models: fp32, fp16 and bf16 data, fp32 sums -----------------------------------------------
+
+_TYPES = {torch.float32: capi.TYPE_FP32, torch.float16: capi.TYPE_FP16, torch.bfloat16: capi.TYPE_BF16}
+
+
+def _typed(t: torch.Tensor) -> int:
+    assert t.dtype in _TYPES, f"fp32, fp16 or bf16 tensors only, not {t.dtype}"
+    return _TYPES[t.dtype]
+
+
+def _device_of(*tensors) -> torch.device:
+    """The one device that all of them (None left out) are on."""
+    devices = {t.device for t in tensors if t is not None}
+    assert len(devices) == 1 and next(iter(devices)).type == "cuda", "tensors on one CUDA device only"
+    return next(iter(devices))
+
+
+def _current(device) -> int:
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _matrix(t: torch.Tensor) -> tuple[int, int, int]:
+    """Rows, width and row size of a tensor seen as a matrix of its last dimension; a 2-D one may be a view of some
+    columns or of every n-th row."""
+    assert t.dim() >= 1 and t.shape[-1] >= 1, "rows of at least one element"
+    width = t.shape[-1]
+    if t.dim() == 2 and t.shape[0] > 1:
+        assert (width == 1 or t.stride(1) == 1) and t.stride(0) >= width, "rows of adjacent elements that do not overlap"
+        return t.shape[0], width, t.stride(0)
+    assert t.is_contiguous(), "contiguous tensors, or matrices of contiguous rows"
+    return t.numel() // width, width, width
+
+
+def _vector(t: torch.Tensor | None, count: int, *types) -> int | None:
+    """Pointer of an optional contiguous vector with `count` elements of one of the types."""
+    if t is None:
+        return None
+    assert t.numel() == count and t.is_contiguous() and t.dtype in types, f"{count} contiguous elements of {types}"
+    return t.data_ptr()
+
+
+def LayerNormalization(source, scale=None, free_term=None, *, epsilon=1e-5, result=None):
+    """The rows of `source` [..., width], each less its mean and over its deviation, times `scale` plus `free_term`.  Returns
+    (result, mean, inverse_deviation); the last two are what the backward pass takes, fp32, one per row.  scale and
+    free_term have `width` elements, both of the source's type or both fp32; None stands for ones and zeros.  `result` may
+    be `source`."""
+    height, width, row = _matrix(source)
+    code, parameter = _typed(source), next((p.dtype for p in (scale, free_term) if p is not None), source.dtype)
+    assert parameter in (source.dtype, torch.float32), "parameters of the rows' type or fp32"
+    if result is None:
+        result = torch.empty(source.shape, dtype=source.dtype, device=source.device)
+    assert result.shape == source.shape and result.dtype == source.dtype, "a result like the source"
+    device = _device_of(source, scale, free_term, result)
+    scale_at, free_at = _vector(scale, width, parameter), _vector(free_term, width, parameter)
+    mean, inverse = torch.empty((2, *source.shape[:-1]), dtype=torch.float32, device=device).unbind()
+    with torch.cuda.device(device):
+        capi.check("LayerNormalization", capi.load().nb200_layer_normalization(
+            _current(device), code, _TYPES[parameter], source.data_ptr(), height, width, row, scale_at, free_at, float(epsilon),
+            result.data_ptr(), _matrix(result)[2], mean.data_ptr(), inverse.data_ptr()))
+    return result, mean, inverse
+
+
+def LayerNormalizationBackward(result_diff, source, mean, inverse_deviation, scale=None, *, source_diff=None,
+                               parameters=True, parameter_type=None):
+    """The gradients of LayerNormalization: (source_diff, scale_diff, free_term_diff) from the result's, what went in and
+    the two vectors that the forward pass returned.  The parameters' gradients are of the scale's type (without a scale
+    `parameter_type`, or the source's); None with parameters=False.  `source_diff` may be `result_diff`."""
+    height, width, row = _matrix(source)
+    code = _typed(source)
+    parameter = scale.dtype if scale is not None else parameter_type or source.dtype
+    assert parameter in (source.dtype, torch.float32), "parameters of the rows' type or fp32"
+    if source_diff is None:
+        source_diff = torch.empty(source.shape, dtype=source.dtype, device=source.device)
+    for t in (result_diff, source_diff):
+        assert t.shape == source.shape and t.dtype == source.dtype, "gradients like the source"
+    device = _device_of(result_diff, source, mean, inverse_deviation, scale, source_diff)
+    mean_at, inverse_at = _vector(mean, height, torch.float32), _vector(inverse_deviation, height, torch.float32)
+    scale_at = _vector(scale, width, parameter)
+    lib = capi.load()
+    scale_diff = free_diff = scratch = None
+    with torch.cuda.device(device):
+        if parameters:
+            scale_diff, free_diff = (torch.empty(width, dtype=parameter, device=device) for _ in range(2))
+            need = lib.nb200_layer_normalization_backward_scratch_floats(code, height, width)
+            scratch = torch.empty(need, dtype=torch.float32, device=device)
+        capi.check("LayerNormalizationBackward", lib.nb200_layer_normalization_backward(
+            _current(device), code, _TYPES[parameter], result_diff.data_ptr(), _matrix(result_diff)[2], source.data_ptr(), height,
+            width, row, scale_at, mean_at, inverse_at, source_diff.data_ptr(), _matrix(source_diff)[2], _ptr(scale_diff),
+            _ptr(free_diff), _ptr(scratch)))
+    return source_diff, scale_diff, free_diff
