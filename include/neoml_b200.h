@@ -332,6 +332,28 @@ NB200_API int nb200_layer_normalization_backward(void* stream, int type, int par
 	long long dy_row_size, const void* x, int height, int width, long long x_row_size, const void* scale, const float* mean,
 	const float* inverse_deviation, void* dx, long long dx_row_size, void* scale_diff, void* free_term_diff, float* scratch);
 
+/* A gated linear recurrence, the pooling step of NeoML's quasi-recurrent layers (IDnnEngine::QrnnFPooling, QrnnIfPooling) with
+ * the gates' VectorSigmoid (NME.h:311) inside: over [batch][length][channels],
+ *   h[t] = sigmoid(forget[t]) * h[t-1] + u[t] * update[t],   u = sigmoid(input), or 1 - sigmoid(forget) where input is NULL.
+ * The gates come as they are before the sigmoid: 0.999 rounded to 16 bits would be one.  `result` is dense and gets every
+ * h[t]; initial_state (NULL: zeros) and final_state (NULL: not wanted) are fp32 [batch][channels], and may be the same
+ * memory.  lengths (NULL: all of `length`) ends sequences early: behind a sequence's end nothing is read, the result is
+ * zero and the state stays (values outside 0..length count as the nearer of the two).  Strides of the three inputs are in elements, channels are adjacent; a stride of
+ * zero repeats a sequence or a step. */
+typedef struct nb200_recurrence_desc {
+	int batch, length, channels;
+	long long update_batch, update_row, forget_batch, forget_row, input_batch, input_row; /* from sequence to sequence, step to step */
+} nb200_recurrence_desc;
+NB200_API int nb200_gated_recurrence(void* stream, int type, const nb200_recurrence_desc* desc, const void* update,
+	const void* forget, const void* input, const float* initial_state, const int* lengths, void* result, float* final_state);
+/* Its gradients (QrnnFPoolingBackward, QrnnIfPoolingBackward; the slope of VectorSigmoid, NME.h:311, inside): of update,
+ * forget and input (dense, zero behind a sequence's end; input_diff is NULL exactly where input is) and of the initial
+ * state, from those of the result and of the final state (NULL: zeros).  `result` is what the forward pass wrote. */
+NB200_API int nb200_gated_recurrence_backward(void* stream, int type, const nb200_recurrence_desc* desc,
+	const void* result_diff, long long result_diff_batch, long long result_diff_row, const void* result, const void* update,
+	const void* forget, const void* input, const float* initial_state, const float* final_state_diff, const int* lengths,
+	void* update_diff, void* forget_diff, void* input_diff, float* initial_state_diff);
+
 #ifdef __cplusplus
 }
 #endif

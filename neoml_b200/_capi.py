@@ -51,8 +51,14 @@ class Mbv2Desc(C.Structure):
                                                                 ("act_dw_param", C.c_float)]
 
 
+class RecurrenceDesc(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("batch", "length", "channels")] + [
+        (n, C.c_longlong) for n in ("update_batch", "update_row", "forget_batch", "forget_row", "input_batch", "input_row")]
+
+
 _vp, _i, _f, _ll = C.c_void_p, C.c_int, C.c_float, C.c_longlong
 _EP = C.POINTER(Epilogue)
+_RD = C.POINTER(RecurrenceDesc)
 
 # name -> (restype, argtypes); the single source of truth for tests that check exported symbols
 SIGNATURES = {
@@ -107,6 +113,9 @@ SIGNATURES = {
     "nb200_layer_normalization_backward_scratch_floats": (C.c_size_t, [_i, _i, _i]),
     "nb200_layer_normalization_backward": (_i, [_vp, _i, _i, _vp, _ll, _vp, _i, _i, _ll, _vp, _vp, _vp, _vp, _ll, _vp, _vp,
                                                 _vp]),
+    "nb200_gated_recurrence": (_i, [_vp, _i, _RD, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "nb200_gated_recurrence_backward": (_i, [_vp, _i, _RD, _vp, _ll, _ll, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+                                             _vp]),
 }
 
 # Diagnostic entry points (neoml_b200/csrc/diagnostics.h): exported for the benchmark and the tests, not part of the

@@ -1,0 +1,475 @@
+// A gated linear recurrence over [batch][length][channels], forward and backward.
+//
+//   a = sigmoid(forget), u = sigmoid(input), or 1 - a without input gates;   h_t = a_t h_{t-1} + u_t z_t
+//   backward:  S_t = dh_t + a_{t+1} S_{t+1};  dz = S u,  d(forget) = S h_{t-1} a (1 - a)  [coupled: S (h_{t-1} - z) a (1 - a)],
+//   d(input) = S z u (1 - u),  dh_0 = a_1 S_1
+//
+// Both are first-order linear recurrences, s' = A s + H, whose steps compose: (A2, H2) after (A1, H1) is (A2 A1, A2 H1 + H2).
+// The work is bound by memory as long as every element is read once and both gates are formed once, so a chunk of the time
+// axis is read into registers, folded there, joined with the chunks around it, and its states are written out of the
+// same registers:
+//   thread   one channel (two 16-bit channels where rows are aligned for it) times STEPS steps: loads them all at once,
+//            folds them to one (A, H)
+//   block    its warps hold consecutive stretches of time for the same 32 or 64 channels; the folds meet in shared memory
+//   cluster  up to 8 blocks hold consecutive stretches again and tell each other their folds through distributed shared
+//            memory; a cluster walks its channels' whole time axis, carrying the state in a register
+// The gates' pre-activations are the inputs: a gate of 0.999 rounded to bf16 is 1 and would never forget.
+#include "types16.cuh"
+#include <cooperative_groups.h>
+
+namespace nb200 {
+
+namespace {
+
+namespace cg = cooperative_groups;
+
+constexpr int STEPS = 8;       // of a thread
+constexpr int MAX_WARPS = 16;  // of a block
+constexpr int MAX_CLUSTER = 8;
+
+struct RecurrenceParams {
+	const void *z, *f, *i;          // update, forget, input (null: coupled)
+	const void *dh, *h;             // backward: gradient of the result, the result
+	void *out, *df, *di;            // out: result, or gradient of the update
+	const float* first;             // initial state [batch][channels], null: zeros; backward too
+	const float* lastDiff;          // backward: gradient of the final state, null: zeros
+	float* last;                    // final state, or gradient of the initial one; null: not wanted
+	const int* lengths;             // null: all `length`
+	long long zBatch, zRow, fBatch, fRow, iBatch, iRow, dhBatch, dhRow; // elements between sequences and steps
+	int length, channels;
+};
+
+struct Gate {
+	float keep, take; // sigmoid(x), 1 - sigmoid(x)
+};
+
+// Both without cancellation; exp never overflows.
+__device__ __forceinline__ Gate gate(float x)
+{
+	const float e = __expf(-fabsf(x));
+	const float large = __fdividef(1.f, 1.f + e), small = e * large;
+	return x >= 0.f ? Gate{ large, small } : Gate{ small, large };
+}
+
+// W channels of one step as they lie in memory: one register
+template<typename T, int W>
+__device__ __forceinline__ uint32_t load_raw(const T* p)
+{
+	if constexpr(sizeof(T) * W == 4) return *reinterpret_cast<const uint32_t*>(p);
+	else return *reinterpret_cast<const unsigned short*>(p);
+}
+template<typename T, int W>
+__device__ __forceinline__ float2 floats(uint32_t raw)
+{
+	if constexpr(sizeof(T) == 4) return make_float2(__uint_as_float(raw), 0.f);
+	else return unpack2<T>(raw);
+}
+template<typename T, int W>
+__device__ __forceinline__ void store_raw(T* p, float a, float b)
+{
+	if constexpr(sizeof(T) == 4) *p = a;
+	else if constexpr(W == 2) *reinterpret_cast<uint32_t*>(p) = pack2<T>(a, b);
+	else *p = from_float<T>(a);
+}
+
+template<int W>
+struct Fold {
+	float a[W], h[W];
+};
+
+// What a block's threads share: their folds, and those of the cluster's blocks (two sets, for alternating rounds).
+template<int W>
+struct Shared {
+	Fold<W> warps[MAX_WARPS][32];
+	Fold<W> blocks[2][MAX_CLUSTER][32];
+};
+
+// Joins the folds of a round: `mine` is this thread's stretch; the state before it is returned in `state`, and `carry` moves on by
+// the whole round.  Stretches follow one another warp by warp, block by block.
+template<int W>
+__device__ __forceinline__ void join(Shared<W>& s, const Fold<W>& mine, int round, int rank, int blocks, int warps, float* carry,
+	float* state)
+{
+	const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+	Fold<W> before, all;
+#pragma unroll
+	for(int w = 0; w < W; ++w) {
+		before.a[w] = 1.f;
+		before.h[w] = 0.f;
+	}
+	all = mine;
+	if(warps > 1) {
+		s.warps[warp][lane] = mine;
+		__syncthreads();
+		Fold<W> run = before;
+		for(int k = 0; k < warps; ++k) {
+			if(k == warp) before = run;
+			const Fold<W> next = s.warps[k][lane];
+#pragma unroll
+			for(int w = 0; w < W; ++w) {
+				run.h[w] = fmaf(next.a[w], run.h[w], next.h[w]);
+				run.a[w] *= next.a[w];
+			}
+		}
+		all = run;
+	}
+	float start[W];
+	if(blocks > 1) {
+		cg::cluster_group cluster = cg::this_cluster();
+		for(int k = warp; k < blocks; k += warps) cluster.map_shared_rank(&s, k)->blocks[round & 1][rank][lane] = all;
+		cluster.sync(); // the other set of the next round is free again: everybody has read it before this barrier
+#pragma unroll
+		for(int w = 0; w < W; ++w) start[w] = carry[w];
+		for(int k = 0; k < blocks; ++k) {
+			if(k == rank) {
+#pragma unroll
+				for(int w = 0; w < W; ++w) start[w] = carry[w];
+			}
+			const Fold<W> next = s.blocks[round & 1][k][lane];
+#pragma unroll
+			for(int w = 0; w < W; ++w) carry[w] = fmaf(next.a[w], carry[w], next.h[w]);
+		}
+	} else {
+#pragma unroll
+		for(int w = 0; w < W; ++w) {
+			start[w] = carry[w];
+			carry[w] = fmaf(all.a[w], carry[w], all.h[w]);
+		}
+		if(warps > 1) __syncthreads(); // the folds have been read
+	}
+#pragma unroll
+	for(int w = 0; w < W; ++w) state[w] = fmaf(before.a[w], start[w], before.h[w]);
+}
+
+__device__ __forceinline__ int sequence_length(const RecurrenceParams& p, int b)
+{
+	if(p.lengths == nullptr) return p.length;
+	const int n = __ldg(p.lengths + b);
+	return n < 0 ? 0 : n > p.length ? p.length : n;
+}
+
+template<typename T, int W, bool INPUT>
+__global__ void __launch_bounds__(MAX_WARPS * 32) recurrence_forward_kernel(const RecurrenceParams p)
+{
+	__shared__ Shared<W> s;
+	const int blocks = gridDim.y, rank = blockIdx.y; // the blocks of a cluster
+	const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5;
+	if(blocks > 1) cg::this_cluster().sync(); // the others' shared memory exists from here on
+	const int b = blockIdx.z;
+	const int c = (blockIdx.x * 32 + (threadIdx.x & 31)) * W;
+	const bool on = c < p.channels;
+	const int n = sequence_length(p, b);
+	const T* const z = static_cast<const T*>(p.z) + b * p.zBatch + c;
+	const T* const f = static_cast<const T*>(p.f) + b * p.fBatch + c;
+	const T* const i = INPUT ? static_cast<const T*>(p.i) + b * p.iBatch + c : nullptr;
+	T* const out = static_cast<T*>(p.out) + static_cast<long long>(b) * p.length * p.channels + c;
+	const long long state0 = static_cast<long long>(b) * p.channels + c;
+	float carry[W];
+#pragma unroll
+	for(int w = 0; w < W; ++w) carry[w] = on && p.first != nullptr ? p.first[state0 + w] : 0.f;
+	const int span = warps * STEPS, stride = span * blocks;
+	int round = 0;
+	for(int t0 = 0; t0 < p.length; t0 += stride, ++round) {
+		const int t = t0 + rank * span + warp * STEPS;
+		if(t0 >= n) { // behind the sequence (the whole cluster agrees): its results are zeros
+#pragma unroll
+			for(int k = 0; k < STEPS; ++k) {
+				if(on && t + k < p.length) store_raw<T, W>(out + static_cast<long long>(t + k) * p.channels, 0.f, 0.f);
+			}
+			continue;
+		}
+		uint32_t rz[STEPS], rf[STEPS], ri[STEPS];
+#pragma unroll
+		for(int k = 0; k < STEPS; ++k) {
+			const bool in = on && t + k < n;
+			rz[k] = in ? load_raw<T, W>(z + (t + k) * p.zRow) : 0u;
+			rf[k] = in ? load_raw<T, W>(f + (t + k) * p.fRow) : 0u;
+			if constexpr(INPUT) ri[k] = in ? load_raw<T, W>(i + (t + k) * p.iRow) : 0u;
+		}
+		float a[STEPS][W], h[STEPS][W];
+		Fold<W> mine;
+#pragma unroll
+		for(int w = 0; w < W; ++w) {
+			mine.a[w] = 1.f;
+			mine.h[w] = 0.f;
+		}
+#pragma unroll
+		for(int k = 0; k < STEPS; ++k) {
+			const float2 vz = floats<T, W>(rz[k]), vf = floats<T, W>(rf[k]);
+			float2 vi = make_float2(0.f, 0.f);
+			if constexpr(INPUT) vi = floats<T, W>(ri[k]);
+			const bool in = t + k < n;
+#pragma unroll
+			for(int w = 0; w < W; ++w) {
+				const Gate forget = gate(w == 0 ? vf.x : vf.y);
+				const float take = INPUT ? gate(w == 0 ? vi.x : vi.y).keep : forget.take;
+				a[k][w] = in ? forget.keep : 1.f;
+				h[k][w] = in ? take * (w == 0 ? vz.x : vz.y) : 0.f;
+				mine.h[w] = fmaf(a[k][w], mine.h[w], h[k][w]);
+				mine.a[w] *= a[k][w];
+			}
+		}
+		float state[W];
+		join<W>(s, mine, round, rank, blocks, warps, carry, state);
+#pragma unroll
+		for(int k = 0; k < STEPS; ++k) {
+#pragma unroll
+			for(int w = 0; w < W; ++w) state[w] = fmaf(a[k][w], state[w], h[k][w]);
+			if(on && t + k < p.length) {
+				const bool in = t + k < n;
+				store_raw<T, W>(out + static_cast<long long>(t + k) * p.channels, in ? state[0] : 0.f, in ? state[W - 1] : 0.f);
+			}
+		}
+	}
+	if(on && p.last != nullptr && rank == 0 && warp == 0) {
+#pragma unroll
+		for(int w = 0; w < W; ++w) p.last[state0 + w] = carry[w];
+	}
+	if(blocks > 1) cg::this_cluster().sync(); // nobody leaves while its shared memory may be written
+}
+
+// Time runs backwards: step k of a stretch is t - k.
+template<typename T, int W, bool INPUT>
+__global__ void __launch_bounds__(MAX_WARPS * 32) recurrence_backward_kernel(const RecurrenceParams p)
+{
+	__shared__ Shared<W> s;
+	const int blocks = gridDim.y, rank = blockIdx.y;
+	const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5;
+	if(blocks > 1) cg::this_cluster().sync(); // the others' shared memory exists from here on
+	const int b = blockIdx.z;
+	const int c = (blockIdx.x * 32 + (threadIdx.x & 31)) * W;
+	const bool on = c < p.channels;
+	const int n = sequence_length(p, b);
+	const long long own = static_cast<long long>(b) * p.length * p.channels + c;
+	const T* const z = static_cast<const T*>(p.z) + b * p.zBatch + c;
+	const T* const f = static_cast<const T*>(p.f) + b * p.fBatch + c;
+	const T* const i = INPUT ? static_cast<const T*>(p.i) + b * p.iBatch + c : nullptr;
+	const T* const dh = static_cast<const T*>(p.dh) + b * p.dhBatch + c;
+	const T* const h = static_cast<const T*>(p.h) + own;
+	T* const dz = static_cast<T*>(p.out) + own;
+	T* const df = static_cast<T*>(p.df) + own;
+	T* const di = INPUT ? static_cast<T*>(p.di) + own : nullptr;
+	const long long state0 = static_cast<long long>(b) * p.channels + c;
+	float carry[W], first[W]; // carry: what step t + 1 hands back, a_{t+1} S_{t+1}
+#pragma unroll
+	for(int w = 0; w < W; ++w) {
+		carry[w] = on && p.lastDiff != nullptr ? p.lastDiff[state0 + w] : 0.f;
+		first[w] = on && p.first != nullptr ? p.first[state0 + w] : 0.f;
+	}
+	// behind the sequence the gradients are zeros
+	for(int t = n + rank * warps + warp; t < p.length; t += blocks * warps) {
+		if(!on) break;
+		const long long at = static_cast<long long>(t) * p.channels;
+		store_raw<T, W>(dz + at, 0.f, 0.f);
+		store_raw<T, W>(df + at, 0.f, 0.f);
+		if constexpr(INPUT) store_raw<T, W>(di + at, 0.f, 0.f);
+	}
+	const int span = warps * STEPS, stride = span * blocks;
+	int round = 0;
+	for(int done = 0; done < n; done += stride, ++round) {
+		const int t = n - 1 - done - rank * span - warp * STEPS;
+		uint32_t rz[STEPS], rf[STEPS], ri[STEPS], rd[STEPS], rh[STEPS];
+#pragma unroll
+		for(int k = 0; k < STEPS; ++k) {
+			const bool in = on && t - k >= 0;
+			rf[k] = in ? load_raw<T, W>(f + (t - k) * p.fRow) : 0u;
+			rd[k] = in ? load_raw<T, W>(dh + (t - k) * p.dhRow) : 0u;
+			rz[k] = in ? load_raw<T, W>(z + (t - k) * p.zRow) : 0u;
+			rh[k] = in && t - k > 0 ? load_raw<T, W>(h + static_cast<long long>(t - k - 1) * p.channels) : 0u;
+			if constexpr(INPUT) ri[k] = in ? load_raw<T, W>(i + (t - k) * p.iRow) : 0u;
+		}
+		float a[STEPS][W], u[STEPS][W];
+		Fold<W> mine;
+#pragma unroll
+		for(int w = 0; w < W; ++w) {
+			mine.a[w] = 1.f;
+			mine.h[w] = 0.f;
+		}
+#pragma unroll
+		for(int k = 0; k < STEPS; ++k) {
+			const float2 vf = floats<T, W>(rf[k]), vd = floats<T, W>(rd[k]);
+			const bool in = t - k >= 0;
+#pragma unroll
+			for(int w = 0; w < W; ++w) {
+				const Gate forget = gate(w == 0 ? vf.x : vf.y);
+				a[k][w] = in ? forget.keep : 1.f;
+				u[k][w] = forget.take;
+				const float d = w == 0 ? vd.x : vd.y;
+				// a (dh + s): this step's own part is a dh
+				mine.h[w] = a[k][w] * (mine.h[w] + d);
+				mine.a[w] *= a[k][w];
+			}
+		}
+		float state[W];
+		join<W>(s, mine, round, rank, blocks, warps, carry, state);
+#pragma unroll
+		for(int k = 0; k < STEPS; ++k) {
+			const float2 vd = floats<T, W>(rd[k]), vz = floats<T, W>(rz[k]);
+			float2 vh = floats<T, W>(rh[k]), vi = make_float2(0.f, 0.f);
+			if(t - k == 0) vh = make_float2(first[0], first[W - 1]);
+			if constexpr(INPUT) vi = floats<T, W>(ri[k]);
+			float oz[W], of[W], oi[W];
+#pragma unroll
+			for(int w = 0; w < W; ++w) {
+				const float S = state[w] + (w == 0 ? vd.x : vd.y), zz = w == 0 ? vz.x : vz.y, before = w == 0 ? vh.x : vh.y;
+				const float slope = a[k][w] * u[k][w];
+				if constexpr(INPUT) {
+					const Gate take = gate(w == 0 ? vi.x : vi.y);
+					oz[w] = S * take.keep;
+					of[w] = S * before * slope;
+					oi[w] = S * zz * (take.keep * take.take);
+				} else {
+					oz[w] = S * u[k][w];
+					of[w] = S * (before - zz) * slope;
+				}
+				state[w] = a[k][w] * S;
+			}
+			if(on && t - k >= 0) {
+				const long long at = static_cast<long long>(t - k) * p.channels;
+				store_raw<T, W>(dz + at, oz[0], oz[W - 1]);
+				store_raw<T, W>(df + at, of[0], of[W - 1]);
+				if constexpr(INPUT) store_raw<T, W>(di + at, oi[0], oi[W - 1]);
+			}
+		}
+	}
+	if(on && p.last != nullptr && rank == 0 && warp == 0) {
+#pragma unroll
+		for(int w = 0; w < W; ++w) p.last[state0 + w] = carry[w];
+	}
+	if(blocks > 1) cg::this_cluster().sync();
+}
+
+using Kernel = void (*)(const RecurrenceParams);
+
+template<typename T, bool BACKWARD>
+Kernel kernel_of(int pair, bool input)
+{
+	if constexpr(sizeof(T) == 2) {
+		if(pair) {
+			if(BACKWARD) return input ? recurrence_backward_kernel<T, 2, true> : recurrence_backward_kernel<T, 2, false>;
+			return input ? recurrence_forward_kernel<T, 2, true> : recurrence_forward_kernel<T, 2, false>;
+		}
+	}
+	if(BACKWARD) return input ? recurrence_backward_kernel<T, 1, true> : recurrence_backward_kernel<T, 1, false>;
+	return input ? recurrence_forward_kernel<T, 1, true> : recurrence_forward_kernel<T, 1, false>;
+}
+
+// Warps for the time axis first, then blocks of a cluster, until the device has about two thousand threads on every SM.
+int launch(int type, bool pair, bool backward, const RecurrenceParams& p, int batch, cudaStream_t stream)
+{
+	const bool input = p.i != nullptr;
+	const Kernel kernel = type == NB200_TYPE_FP32 ? (backward ? kernel_of<float, true>(pair, input) : kernel_of<float, false>(pair, input))
+		: type == NB200_TYPE_FP16 ? (backward ? kernel_of<__half, true>(pair, input) : kernel_of<__half, false>(pair, input))
+		: (backward ? kernel_of<__nv_bfloat16, true>(pair, input) : kernel_of<__nv_bfloat16, false>(pair, input));
+	const int perWarp = pair ? 64 : 32;
+	const int tiles = (p.channels + perWarp - 1) / perWarp;
+	const int stretches = (p.length + STEPS - 1) / STEPS;
+	const long long groups = static_cast<long long>(tiles) * batch;
+	int warps = 1;
+	while(warps < MAX_WARPS && warps < stretches) warps *= 2;
+	int blocks = 1;
+	while(blocks < MAX_CLUSTER && blocks * warps < stretches && groups * blocks < sm_count() * 2) blocks *= 2;
+	cudaLaunchConfig_t config = {};
+	config.blockDim = dim3(warps * 32);
+	config.gridDim = dim3(tiles, blocks, batch);
+	config.stream = stream;
+	cudaLaunchAttribute attribute[1];
+	attribute[0].id = cudaLaunchAttributeClusterDimension;
+	attribute[0].val.clusterDim.x = 1;
+	attribute[0].val.clusterDim.y = blocks;
+	attribute[0].val.clusterDim.z = 1;
+	config.attrs = attribute;
+	config.numAttrs = blocks > 1 ? 1 : 0;
+	cudaLaunchKernelEx(&config, kernel, p);
+	count_launch();
+	return check_launch();
+}
+
+// 16-bit channels go in pairs where every pair lies in one aligned word
+struct Strided {
+	const void* p;
+	long long batch, row;
+};
+bool pairs_aligned(int type, int batch, int length, int channels, const Strided* s, int n)
+{
+	if(type == NB200_TYPE_FP32 || channels % 2 != 0) return false;
+	for(int k = 0; k < n; ++k) {
+		if(s[k].p == nullptr) continue;
+		if((reinterpret_cast<uintptr_t>(s[k].p) & 3u) != 0) return false;
+		if((batch > 1 && s[k].batch % 2 != 0) || (length > 1 && s[k].row % 2 != 0)) return false;
+	}
+	return true;
+}
+
+bool desc_valid(int type, const nb200_recurrence_desc* d)
+{
+	if(d == nullptr || !type_valid(type) || d->batch < 0 || d->length < 0 || d->channels < 0) return false;
+	const long long rows[] = { d->update_row, d->forget_row, d->input_row };
+	const long long batches[] = { d->update_batch, d->forget_batch, d->input_batch };
+	for(int k = 0; k < 3; ++k) {
+		if(rows[k] < 0 || batches[k] < 0) return false;
+	}
+	return true;
+}
+
+bool floats_aligned(const float* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
+
+} // namespace
+
+} // namespace nb200
+
+using namespace nb200;
+
+extern "C" {
+
+int nb200_gated_recurrence(void* stream, int type, const nb200_recurrence_desc* d, const void* update, const void* forget,
+	const void* input, const float* initial_state, const int* lengths, void* result, float* final_state)
+{
+	if(!desc_valid(type, d)) return NB200_EINVAL;
+	if(d->batch == 0 || d->channels == 0) return NB200_OK;
+	if(d->length > 0 && (update == nullptr || forget == nullptr || result == nullptr)) return NB200_EINVAL;
+	if(!type_aligned(update, type) || !type_aligned(forget, type) || !type_aligned(input, type) || !type_aligned(result, type)
+		|| !floats_aligned(initial_state) || !floats_aligned(final_state)) return NB200_EINVAL;
+	if(d->batch > 65535 || d->length > (1 << 30)) return NB200_ETOOBIG;
+	if(device_status_word() == nullptr) return NB200_ENODEVICE;
+	RecurrenceParams p = {};
+	p.z = update; p.f = forget; p.i = input; p.out = result; p.first = initial_state; p.last = final_state; p.lengths = lengths;
+	p.zBatch = d->update_batch; p.zRow = d->update_row; p.fBatch = d->forget_batch; p.fRow = d->forget_row;
+	p.iBatch = d->input_batch; p.iRow = d->input_row;
+	p.length = d->length; p.channels = d->channels;
+	const Strided all[] = { { update, d->update_batch, d->update_row }, { forget, d->forget_batch, d->forget_row },
+		{ input, d->input_batch, d->input_row }, { result, 0, 0 } };
+	return launch(type, pairs_aligned(type, d->batch, d->length, d->channels, all, 4), false, p, d->batch, as_stream(stream));
+}
+
+int nb200_gated_recurrence_backward(void* stream, int type, const nb200_recurrence_desc* d, const void* result_diff,
+	long long result_diff_batch, long long result_diff_row, const void* result, const void* update, const void* forget,
+	const void* input, const float* initial_state, const float* final_state_diff, const int* lengths, void* update_diff,
+	void* forget_diff, void* input_diff, float* initial_state_diff)
+{
+	if(!desc_valid(type, d) || result_diff_batch < 0 || result_diff_row < 0) return NB200_EINVAL;
+	if(d->batch == 0 || d->channels == 0) return NB200_OK;
+	if(d->length > 0 && (result_diff == nullptr || result == nullptr || update == nullptr || forget == nullptr
+		|| update_diff == nullptr || forget_diff == nullptr)) return NB200_EINVAL;
+	if(d->length > 0 && (input == nullptr) != (input_diff == nullptr)) return NB200_EINVAL;
+	const void* const typed[] = { result_diff, result, update, forget, input, update_diff, forget_diff, input_diff };
+	for(const void* t : typed) {
+		if(!type_aligned(t, type)) return NB200_EINVAL;
+	}
+	if(!floats_aligned(initial_state) || !floats_aligned(final_state_diff) || !floats_aligned(initial_state_diff)) return NB200_EINVAL;
+	if(d->batch > 65535 || d->length > (1 << 30)) return NB200_ETOOBIG;
+	if(device_status_word() == nullptr) return NB200_ENODEVICE;
+	RecurrenceParams p = {};
+	p.z = update; p.f = forget; p.i = input; p.dh = result_diff; p.h = result;
+	p.out = update_diff; p.df = forget_diff; p.di = input_diff;
+	p.first = initial_state; p.lastDiff = final_state_diff; p.last = initial_state_diff; p.lengths = lengths;
+	p.zBatch = d->update_batch; p.zRow = d->update_row; p.fBatch = d->forget_batch; p.fRow = d->forget_row;
+	p.iBatch = d->input_batch; p.iRow = d->input_row; p.dhBatch = result_diff_batch; p.dhRow = result_diff_row;
+	p.length = d->length; p.channels = d->channels;
+	const Strided all[] = { { update, d->update_batch, d->update_row }, { forget, d->forget_batch, d->forget_row },
+		{ input, d->input_batch, d->input_row }, { result_diff, result_diff_batch, result_diff_row }, { result, 0, 0 },
+		{ update_diff, 0, 0 }, { forget_diff, 0, 0 }, { input_diff, 0, 0 } };
+	return launch(type, pairs_aligned(type, d->batch, d->length, d->channels, all, 8), true, p, d->batch, as_stream(stream));
+}
+
+} // extern "C"

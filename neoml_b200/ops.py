@@ -510,3 +510,65 @@ def LayerNormalizationBackward(result_diff, source, mean, inverse_deviation, sca
             width, row, scale_at, mean_at, inverse_at, source_diff.data_ptr(), _matrix(source_diff)[2], _ptr(scale_diff),
             _ptr(free_diff), _ptr(scratch)))
     return source_diff, scale_diff, free_diff
+
+
+def _steps(t: torch.Tensor, shape, dtype) -> tuple[int, int]:
+    """Strides of a [batch, length, channels] operand with adjacent channels; expanded ones repeat."""
+    assert t.shape == shape and t.dtype == dtype, f"{list(shape)} of {dtype}"
+    assert shape[2] <= 1 or t.stride(2) == 1, "adjacent channels"
+    return (t.stride(0) if shape[0] > 1 else 0), (t.stride(1) if shape[1] > 1 else 0)
+
+
+def _recurrence_desc(update, forget, input):
+    assert update.dim() == 3, "[batch, length, channels]"
+    shape, dtype = update.shape, update.dtype
+    return capi.RecurrenceDesc(*shape, *_steps(update, shape, dtype), *_steps(forget, shape, dtype),
+                               *(_steps(input, shape, dtype) if input is not None else (0, 0)))
+
+
+def GatedRecurrence(update, forget, input=None, *, initial_state=None, lengths=None, result=None, final_state=None):
+    """h[t] = sigmoid(forget[t]) h[t-1] + u[t] update[t] over [batch, length, channels], u = sigmoid(input) or, without
+    input gates, 1 - sigmoid(forget): QrnnIfPooling and QrnnFPooling with the gates' sigmoid inside.  Returns (result,
+    final_state): every h[t] in the update's type, and the last state, fp32 [batch, channels].  initial_state is fp32 too
+    (None: zeros); `final_state` may be the same tensor, as when tokens are served one at a time.  lengths (int32 [batch])
+    ends sequences early: behind their end the result is zero and the state stays.  The three inputs may be strided views or
+    expanded; channels are adjacent."""
+    desc, code = _recurrence_desc(update, forget, input), _typed(update)
+    batch, length, channels = update.shape
+    if result is None:
+        result = torch.empty(update.shape, dtype=update.dtype, device=update.device)
+    if final_state is None:
+        final_state = torch.empty((batch, channels), dtype=torch.float32, device=update.device)
+    assert result.shape == update.shape and result.dtype == update.dtype and result.is_contiguous(), "a dense result like the update"
+    device = _device_of(update, forget, input, initial_state, lengths, result, final_state)
+    states = _vector(initial_state, batch * channels, torch.float32), _vector(final_state, batch * channels, torch.float32)
+    lengths_at = _vector(lengths, batch, torch.int32)
+    with torch.cuda.device(device):
+        capi.check("GatedRecurrence", capi.load().nb200_gated_recurrence(
+            _current(device), code, C.byref(desc), update.data_ptr(), forget.data_ptr(),
+            None if input is None else input.data_ptr(), states[0], lengths_at, result.data_ptr(), states[1]))
+    return result, final_state
+
+
+def GatedRecurrenceBackward(result_diff, result, update, forget, input=None, *, initial_state=None, final_state_diff=None,
+                            lengths=None):
+    """The gradients of GatedRecurrence: (update_diff, forget_diff, input_diff, initial_state_diff); input_diff is None
+    without input gates.  `result` is what the forward pass returned; final_state_diff (fp32, None: zeros) is the gradient
+    of the last state.  Gradients are dense, one for every element that an expanded input stands for, and zero behind a
+    sequence's end."""
+    desc, code = _recurrence_desc(update, forget, input), _typed(update)
+    batch, length, channels = update.shape
+    diff_strides = _steps(result_diff, update.shape, update.dtype)
+    assert result.shape == update.shape and result.dtype == update.dtype and result.is_contiguous(), "the forward pass's result"
+    device = _device_of(result_diff, result, update, forget, input, initial_state, final_state_diff, lengths)
+    states = _vector(initial_state, batch * channels, torch.float32), _vector(final_state_diff, batch * channels, torch.float32)
+    lengths_at = _vector(lengths, batch, torch.int32)
+    update_diff, forget_diff = torch.empty_like(result), torch.empty_like(result)
+    input_diff = None if input is None else torch.empty_like(result)
+    initial_diff = torch.empty((batch, channels), dtype=torch.float32, device=device)
+    with torch.cuda.device(device):
+        capi.check("GatedRecurrenceBackward", capi.load().nb200_gated_recurrence_backward(
+            _current(device), code, C.byref(desc), result_diff.data_ptr(), *diff_strides, result.data_ptr(), update.data_ptr(),
+            forget.data_ptr(), None if input is None else input.data_ptr(), states[0], states[1], lengths_at,
+            update_diff.data_ptr(), forget_diff.data_ptr(), _ptr(input_diff), initial_diff.data_ptr()))
+    return update_diff, forget_diff, input_diff, initial_diff
