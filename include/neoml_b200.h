@@ -354,6 +354,22 @@ NB200_API int nb200_gated_recurrence_backward(void* stream, int type, const nb20
 	const void* forget, const void* input, const float* initial_state, const float* final_state_diff, const int* lengths,
 	void* update_diff, void* forget_diff, void* input_diff, float* initial_state_diff);
 
+/* Distillation from a teacher's top logits, beside MatrixSoftmaxByRows (NME.h:450): per row, with p the softmax of the `kept`
+ * teacher logits over temperature and q that of all the row's logits over temperature,
+ *   loss = temperature^2 * sum_k p[k] * (log p[k] - log q[index[k]]),   log_sum = log sum_j exp(logits[j] / temperature).
+ * teacher_logits (of teacher_type: `type` or NB200_TYPE_FP32) and teacher_indices are [rows][kept].  An index outside
+ * 0..vocabulary-1 marks an entry that is not used; a row without one has loss zero and no gradient.  An index that is
+ * kept twice counts twice.  kept <= NB200_DISTILLATION_KEPT_MAX (NB200_ETOOBIG otherwise). */
+#define NB200_DISTILLATION_KEPT_MAX 1024
+NB200_API int nb200_distillation_loss(void* stream, int type, int teacher_type, const void* logits, int rows, int vocabulary,
+	long long row_size, const void* teacher_logits, const int* teacher_indices, int kept, float temperature, float* loss,
+	float* log_sum);
+/* Its gradient by the logits (the softmax of NME.h:450 less the teacher's probabilities, times temperature * loss_diff[row]);
+ * log_sum is the forward pass's.  logits_diff may be logits. */
+NB200_API int nb200_distillation_loss_backward(void* stream, int type, int teacher_type, const float* loss_diff,
+	const void* logits, int rows, int vocabulary, long long row_size, const void* teacher_logits, const int* teacher_indices,
+	int kept, float temperature, const float* log_sum, void* logits_diff, long long logits_diff_row_size);
+
 #ifdef __cplusplus
 }
 #endif

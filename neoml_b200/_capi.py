@@ -116,6 +116,8 @@ SIGNATURES = {
     "nb200_gated_recurrence": (_i, [_vp, _i, _RD, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "nb200_gated_recurrence_backward": (_i, [_vp, _i, _RD, _vp, _ll, _ll, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
                                              _vp]),
+    "nb200_distillation_loss": (_i, [_vp, _i, _i, _vp, _i, _i, _ll, _vp, _vp, _i, _f, _vp, _vp]),
+    "nb200_distillation_loss_backward": (_i, [_vp, _i, _i, _vp, _vp, _i, _i, _ll, _vp, _vp, _i, _f, _vp, _vp, _ll]),
 }
 
 # Diagnostic entry points (neoml_b200/csrc/diagnostics.h): exported for the benchmark and the tests, not part of the

@@ -74,6 +74,83 @@ template<> struct Unit16<float> {
 	}
 };
 
+// ---- rows in 16-byte units of memory -----------------------------------------------------------------------------------
+// A row is cut into the aligned 16-byte units that it touches, so that rows of any width and first address move at full
+// rate: the units at its two ends hold elements of the neighbouring rows too, which the caller leaves out of what it
+// computes.  V: elements of a unit, or 1 for units of single elements (operands that are aligned differently).
+// A row and the matrix that it lies in.  A unit is addressed by the column of its element 0, negative at a row's head.
+template<typename T, int V>
+struct Row {
+	const T* p;      // element 0 of the row
+	const T* begin;  // of the matrix
+	const T* end;
+};
+
+template<typename T, int V>
+__device__ __forceinline__ void load_unit(const Row<T, V>& row, int first, int width, uint4& raw)
+{
+	if constexpr(V == 1) {
+		raw.x = 0u;
+		if(first < width) {
+			if constexpr(sizeof(T) == 4) raw.x = __float_as_uint(reinterpret_cast<const float*>(row.p)[first]);
+			else raw.x = reinterpret_cast<const unsigned short*>(row.p)[first];
+		}
+	} else {
+		const T* at = row.p + first;
+		raw = make_uint4(0u, 0u, 0u, 0u);
+		if(first >= width) return;
+		if(at >= row.begin && at + V <= row.end) {
+			raw = *reinterpret_cast<const uint4*>(at);
+		} else { // the first unit of the first row, the last one of the last
+			float v[V];
+#pragma unroll
+			for(int j = 0; j < V; ++j) v[j] = first + j >= 0 && first + j < width ? to_float(at[j]) : 0.f;
+			raw = Unit16<T>::pack(v);
+		}
+	}
+}
+
+template<typename T, int V>
+__device__ __forceinline__ void unit_floats(const uint4& raw, float* v)
+{
+	if constexpr(V == 1) {
+		if constexpr(sizeof(T) == 4) v[0] = __uint_as_float(raw.x);
+		else v[0] = unpack2<T>(raw.x).x;
+	} else {
+		Unit16<T>::unpack(raw, v);
+	}
+}
+
+template<typename T, int V>
+__device__ __forceinline__ void store_unit(T* row, int first, int width, const float* v)
+{
+	if constexpr(V == 1) {
+		if(first < width) row[first] = from_float<T>(v[0]);
+	} else {
+		if(first >= 0 && first + V <= width) {
+			*reinterpret_cast<uint4*>(row + first) = Unit16<T>::pack(v);
+		} else {
+#pragma unroll
+			for(int j = 0; j < V; ++j) {
+				if(first + j >= 0 && first + j < width) row[first + j] = from_float<T>(v[j]);
+			}
+		}
+	}
+}
+
+template<int V>
+__device__ __forceinline__ bool inside(int first, int j, int width)
+{
+	return V == 1 ? first < width : first + j >= 0 && first + j < width;
+}
+
+// elements by which a row's first address lies behind a 16-byte boundary
+template<typename T, int V>
+__device__ __forceinline__ int row_offset(const T* row)
+{
+	return V == 1 ? 0 : static_cast<int>((reinterpret_cast<uintptr_t>(row) & 15u) / sizeof(T));
+}
+
 __device__ __forceinline__ float warp_sum_all(float v)
 {
 #pragma unroll

@@ -572,3 +572,47 @@ def GatedRecurrenceBackward(result_diff, result, update, forget, input=None, *, 
             forget.data_ptr(), None if input is None else input.data_ptr(), states[0], states[1], lengths_at,
             update_diff.data_ptr(), forget_diff.data_ptr(), _ptr(input_diff), initial_diff.data_ptr()))
     return update_diff, forget_diff, input_diff, initial_diff
+
+
+def _teacher(logits, teacher_logits, teacher_indices, rows, temperature):
+    assert teacher_logits.shape == teacher_indices.shape and teacher_logits.shape[:-1] == logits.shape[:-1], \
+        "the kept logits and their columns, for every row"
+    assert teacher_logits.dtype in (logits.dtype, torch.float32), "a teacher of the logits' type or fp32"
+    assert 0.0 < temperature < float("inf"), "a positive temperature"
+    kept = teacher_logits.shape[-1]
+    return kept, _vector(teacher_logits, rows * kept, teacher_logits.dtype), _vector(teacher_indices, rows * kept, torch.int32)
+
+
+def DistillationLoss(logits, teacher_logits, teacher_indices, *, temperature=1.0):
+    """temperature^2 times the divergence of a student's rows of `logits` [..., vocabulary] from a teacher of which each row
+    kept some top logits: teacher_logits and teacher_indices (int32) [..., kept], at most 1024 of them, renormalised among
+    themselves.  An index outside the vocabulary marks an entry that is not used; rows without one have loss zero.
+    Returns (loss, log_sum), fp32, one per row; log_sum, of logits / temperature, is what the backward pass takes."""
+    rows, vocabulary, row = _matrix(logits)
+    code = _typed(logits)
+    kept, teacher_at, indices_at = _teacher(logits, teacher_logits, teacher_indices, rows, temperature)
+    device = _device_of(logits, teacher_logits, teacher_indices)
+    loss, log_sum = torch.empty((2, *logits.shape[:-1]), dtype=torch.float32, device=device).unbind()
+    with torch.cuda.device(device):
+        capi.check("DistillationLoss", capi.load().nb200_distillation_loss(
+            _current(device), code, _TYPES[teacher_logits.dtype], logits.data_ptr(), rows, vocabulary, row, teacher_at, indices_at,
+            kept, float(temperature), loss.data_ptr(), log_sum.data_ptr()))
+    return loss, log_sum
+
+
+def DistillationLossBackward(loss_diff, logits, teacher_logits, teacher_indices, log_sum, *, temperature=1.0, result=None):
+    """The gradient of DistillationLoss by the logits, from that of each row's loss (fp32) and the log_sum of the forward
+    pass.  `result` may be `logits`, which the gradient then replaces."""
+    rows, vocabulary, row = _matrix(logits)
+    code = _typed(logits)
+    kept, teacher_at, indices_at = _teacher(logits, teacher_logits, teacher_indices, rows, temperature)
+    if result is None:
+        result = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    assert result.shape == logits.shape and result.dtype == logits.dtype, "a gradient like the logits"
+    device = _device_of(loss_diff, logits, teacher_logits, teacher_indices, log_sum, result)
+    diff_at, sum_at = _vector(loss_diff, rows, torch.float32), _vector(log_sum, rows, torch.float32)
+    with torch.cuda.device(device):
+        capi.check("DistillationLossBackward", capi.load().nb200_distillation_loss_backward(
+            _current(device), code, _TYPES[teacher_logits.dtype], diff_at, logits.data_ptr(), rows, vocabulary, row, teacher_at,
+            indices_at, kept, float(temperature), sum_at, result.data_ptr(), _matrix(result)[2]))
+    return result
