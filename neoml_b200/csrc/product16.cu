@@ -1,0 +1,417 @@
+// The 16-bit products behind the cross entropy over a vocabulary (product16.cuh): a persistent tcgen05 kernel.
+//
+//   warp 0      loads: tiles of A (128 x 64) and B (256 x 64) by TMA into a ring of four stages
+//   warp 1      issues the MMAs (128 x 256 x 16) into one of two accumulators of 256 tensor-memory columns
+//   warps 4-11  epilogue: two warps per lane quarter, 128 columns each, while the next tile is multiplied
+//
+// Operands whose m or n is adjacent in memory need no transposition: the tensor core reads them MN-major.  A box of 64 adjacent
+// indices x 64 k lands as 64 rows of 128 bytes; eight rows are a swizzle atom of 1024 bytes (stride byte offset), the next 64
+// indices lie 8192 bytes further (leading byte offset).  Every wait is bounded (common.cuh).
+#include "product16.cuh"
+
+#include <cuda.h>
+#include <mutex>
+
+namespace nb200 {
+
+namespace {
+
+constexpr int BM = PRODUCT16_M, BN = PRODUCT16_N, BK = PRODUCT16_K;
+constexpr int STAGES = 4;
+constexpr int A_BYTES = BM * BK * 2, B_BYTES = BN * BK * 2, STAGE_BYTES = A_BYTES + B_BYTES;
+constexpr int EPILOGUE_WARPS = 8;
+constexpr int THREADS = (4 + EPILOGUE_WARPS) * 32;
+constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 + 256;
+constexpr int KERNEL_ID = 0x70;       // in the status word: (KERNEL_ID << 8) | site
+constexpr float LOG2E = 1.4426950408889634f;
+enum { SITE_LOAD = 1, SITE_MMA = 2, SITE_MMA_ACC = 3, SITE_EPILOGUE = 4 };
+enum { B_FULL = 0, B_EMPTY = STAGES, B_ACCFULL = 2 * STAGES, B_ACCEMPTY = 2 * STAGES + 2, B_DONE = 2 * STAGES + 4, BARS };
+
+__device__ __forceinline__ float exp2_fast(float x)
+{
+	float y;
+	asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+	return y;
+}
+
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const void* map, uint64_t* bar, int x, int y)
+{
+	asm volatile(
+		"cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+		::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y) : "memory");
+}
+
+// MN-major operand of 16-bit elements: see the head of this file.
+__device__ __forceinline__ uint64_t desc_across(uint32_t smemAddr)
+{
+	uint64_t d = 0;
+	d |= static_cast<uint64_t>((smemAddr >> 4) & 0x3FFFu);
+	d |= static_cast<uint64_t>(8192 >> 4) << 16;
+	d |= static_cast<uint64_t>(1024 >> 4) << 32;
+	d |= static_cast<uint64_t>(1) << 46;
+	d |= static_cast<uint64_t>(2) << 61;
+	return d;
+}
+
+__device__ __forceinline__ void umma_f16_ss(uint32_t tmemD, uint64_t descA, uint64_t descB, uint32_t idesc, uint32_t accumulate)
+{
+	asm volatile(
+		"{\n\t.reg .pred p;\n\t"
+		"setp.ne.b32 p, %4, 0;\n\t"
+		"tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+		::"r"(tmemD), "l"(descA), "l"(descB), "r"(idesc), "r"(accumulate) : "memory");
+}
+
+__device__ __forceinline__ void store32(void* p, const uint32_t* v) // 32 bytes, aligned
+{
+	asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+		::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
+}
+__device__ __forceinline__ void load32(const void* p, uint32_t* v)
+{
+	asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+		: "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]) : "l"(p) : "memory");
+}
+
+struct Tile {
+	int m0, n0, mTile, nTile, split, kBegin, kEnd;
+};
+
+__device__ __forceinline__ Tile tile_of(const Product16Params& p, int tile)
+{
+	Tile t;
+	const int perSplit = p.mTiles * p.nTiles;
+	t.split = tile / perSplit;
+	const int r = tile - t.split * perSplit;
+	if(p.mFast) {
+		t.nTile = r / p.mTiles;
+		t.mTile = r - t.nTile * p.mTiles;
+	} else {
+		t.mTile = r / p.nTiles;
+		t.nTile = r - t.mTile * p.nTiles;
+	}
+	t.m0 = t.mTile * BM;
+	t.n0 = t.nTile * BN;
+	t.kBegin = t.split * p.kBlocksPerSplit;
+	t.kEnd = min(p.kBlocks, t.kBegin + p.kBlocksPerSplit);
+	return t;
+}
+
+__device__ __forceinline__ uint32_t pack16(float a, float b, int bf16)
+{
+	return bf16 ? pack2<__nv_bfloat16>(a, b) : pack2<__half>(a, b);
+}
+
+template<int EPILOGUE, bool A_ACROSS, bool B_ACROSS>
+__global__ void __launch_bounds__(THREADS, 1) product16_kernel(const Product16Params p, const __grid_constant__ CUtensorMap mapA,
+	const __grid_constant__ CUtensorMap mapB)
+{
+	extern __shared__ uint8_t smemRaw[];
+	uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smemRaw) + 1023) & ~static_cast<uintptr_t>(1023));
+	uint64_t* const bars = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE_BYTES);
+	uint32_t* const tmemSlot = reinterpret_cast<uint32_t*>(bars + BARS);
+	volatile int* const abortFlag = reinterpret_cast<volatile int*>(tmemSlot + 1);
+	const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+	const uint32_t smemBase = smem_u32(smem);
+	if(threadIdx.x == 0) {
+		for(int i = 0; i < STAGES; ++i) {
+			mbar_init(bars + B_FULL + i, 1);
+			mbar_init(bars + B_EMPTY + i, 1);
+		}
+		for(int i = 0; i < 2; ++i) {
+			mbar_init(bars + B_ACCFULL + i, 1);
+			mbar_init(bars + B_ACCEMPTY + i, EPILOGUE_WARPS);
+		}
+		mbar_init(bars + B_DONE, 1);
+		mbar_init_fence();
+		*abortFlag = 0;
+		tma_prefetch_descriptor(&mapA);
+		tma_prefetch_descriptor(&mapB);
+	}
+	if(warp == 2) {
+		tmem_alloc(tmemSlot, 512);
+		tmem_relinquish();
+	}
+	tc_fence_before_sync();
+	__syncthreads();
+	tc_fence_after_sync();
+	const uint32_t tmemBase = *tmemSlot;
+	const int tiles = p.mTiles * p.nTiles * p.splits;
+	dependent_wait();
+
+	if(warp == 0) {
+		if(elect_one()) {
+			int it = 0;
+			bool ok = true;
+			for(int tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x) {
+				const Tile t = tile_of(p, tile);
+				for(int kb = t.kBegin; kb < t.kEnd; ++kb, ++it) {
+					const int s = it % STAGES;
+					if(it >= STAGES && !mbar_wait_bounded(bars + B_EMPTY + s, (it / STAGES - 1) & 1, abortFlag, p.status, (KERNEL_ID << 8) | SITE_LOAD)) {
+						ok = false;
+						break;
+					}
+					uint64_t* const full = bars + B_FULL + s;
+					const uint32_t a = smemBase + s * STAGE_BYTES, b = a + A_BYTES;
+					mbar_arrive_expect_tx(full, STAGE_BYTES);
+					const int ka = p.akOffset + kb * BK, kbB = p.bkOffset + kb * BK;
+					if constexpr(A_ACROSS) {
+#pragma unroll
+						for(int i = 0; i < BM / 64; ++i) tma_load_2d(a + i * 8192, &mapA, full, p.aOffset + t.m0 + i * 64, ka);
+					} else {
+						tma_load_2d(a, &mapA, full, ka, p.aOffset + t.m0);
+					}
+					if constexpr(B_ACROSS) {
+#pragma unroll
+						for(int i = 0; i < BN / 64; ++i) tma_load_2d(b + i * 8192, &mapB, full, p.bOffset + t.n0 + i * 64, kbB);
+					} else {
+						tma_load_2d(b, &mapB, full, kbB, p.bOffset + t.n0);
+					}
+				}
+			}
+			if(!ok) { // let what is in flight land before the shared memory goes
+				int ignored = 0;
+				for(int i = it > STAGES ? it - STAGES : 0; i < it; ++i) {
+					mbar_wait_bounded(bars + B_FULL + i % STAGES, (i / STAGES) & 1, &ignored, nullptr, 0);
+				}
+			}
+		}
+		__syncwarp();
+	} else if(warp == 1) {
+		if(elect_one()) {
+			const uint32_t format = p.bf16 ? (1u << 7) | (1u << 10) : 0u;
+			const uint32_t idesc = umma_idesc_f16(BM, BN) | format | (A_ACROSS ? 1u << 15 : 0u) | (B_ACROSS ? 1u << 16 : 0u);
+			int it = 0, n = 0;
+			bool ok = true;
+			for(int tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x, ++n) {
+				const Tile t = tile_of(p, tile);
+				const int acc = n & 1;
+				if(n >= 2 && !mbar_wait_bounded(bars + B_ACCEMPTY + acc, (n / 2 - 1) & 1, abortFlag, p.status, (KERNEL_ID << 8) | SITE_MMA_ACC)) break;
+				tc_fence_after_sync();
+				const uint32_t d = tmemBase + acc * BN;
+				for(int kb = t.kBegin; kb < t.kEnd; ++kb, ++it) {
+					const int s = it % STAGES;
+					if(!mbar_wait_bounded(bars + B_FULL + s, (it / STAGES) & 1, abortFlag, p.status, (KERNEL_ID << 8) | SITE_MMA)) {
+						ok = false;
+						break;
+					}
+					tc_fence_after_sync();
+					const uint32_t a = smemBase + s * STAGE_BYTES, b = a + A_BYTES;
+#pragma unroll
+					for(int k = 0; k < BK / 16; ++k) {
+						const uint64_t da = A_ACROSS ? desc_across(a + k * 2048) : umma_desc_k128(a + k * 32);
+						const uint64_t db = B_ACROSS ? desc_across(b + k * 2048) : umma_desc_k128(b + k * 32);
+						umma_f16_ss(d, da, db, idesc, kb > t.kBegin || k > 0 ? 1u : 0u);
+					}
+					umma_commit(bars + B_EMPTY + s);
+				}
+				if(ok) umma_commit(bars + B_ACCFULL + acc);
+			}
+			if(*abortFlag != 0) { // nothing may still write tensor memory when it is freed
+				int ignored = 0;
+				umma_commit(bars + B_DONE);
+				mbar_wait_bounded(bars + B_DONE, 0, &ignored, nullptr, 0);
+			}
+		}
+		__syncwarp();
+	} else if(warp >= 4) {
+		const int quarter = warp & 3, half = (warp - 4) >> 2;
+		int n = 0;
+		for(int tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++n) {
+			const Tile t = tile_of(p, tile);
+			const int acc = n & 1;
+			const int row = t.m0 + quarter * 32 + lane;
+			const bool on = row < p.m;
+			const int col0 = t.n0 + half * 128;
+			const uint32_t at = tmemBase + (static_cast<uint32_t>(quarter * 32) << 16) + acc * BN + half * 128;
+			int label = -1;
+			float logSum2 = 0.f, by = 0.f;
+			if(on && (EPILOGUE == PRODUCT16_STATS || EPILOGUE == PRODUCT16_DIFF)) {
+				label = __ldg(p.labels + row);
+				if(label < 0 || label >= p.columns) label = -1;
+			}
+			if(on && EPILOGUE == PRODUCT16_DIFF) {
+				logSum2 = __ldg(p.logSum + row) * LOG2E;
+				by = __ldg(p.rowScale + row) * __ldg(p.scale);
+				if(label < 0) by = 0.f;
+			}
+			if(EPILOGUE == PRODUCT16_STORE) by = __ldg(p.resultScale);
+			const int own = label - p.firstColumn - col0; // the label's place in this thread's columns, if it is there
+			if(!mbar_wait_bounded_warp(bars + B_ACCFULL + acc, (n >> 1) & 1, abortFlag, p.status, (KERNEL_ID << 8) | SITE_EPILOGUE)) break;
+			tc_fence_after_sync();
+			float top = -INFINITY, sum = 0.f;
+#pragma unroll 1
+			for(int c = 0; c < 128; c += 32) {
+				uint32_t r[32];
+				tmem_ld32_issue(at + c, r);
+				tmem_ld_wait();
+				if(EPILOGUE == PRODUCT16_SUM && t.kBegin >= t.kEnd) { // a part of K without steps: nothing was multiplied
+#pragma unroll
+					for(int i = 0; i < 32; ++i) r[i] = 0u;
+				}
+				if(c == 96) { // the accumulator is free
+					tc_fence_before_sync();
+					if(lane == 0) mbar_arrive(bars + B_ACCEMPTY + acc);
+				}
+				if constexpr(EPILOGUE == PRODUCT16_STATS) {
+					const int left = p.columns - p.firstColumn - col0 - c; // valid ones of these 32
+					if(left < 32) {
+#pragma unroll
+						for(int i = 0; i < 32; ++i) {
+							if(i >= left) r[i] = 0xff800000u;
+						}
+					}
+					const bool here = own >= c && own < c + 32;
+					if(__any_sync(0xffffffffu, here)) {
+						float value = 0.f;
+#pragma unroll
+						for(int i = 0; i < 32; ++i) {
+							if(own - c == i) value = __uint_as_float(r[i]);
+						}
+						if(here && left > own - c) p.labelled[row] = value;
+					}
+					float newTop = top;
+#pragma unroll
+					for(int i = 0; i < 32; ++i) newTop = fmaxf(newTop, __uint_as_float(r[i]) * LOG2E);
+					const float reference = newTop == -INFINITY ? 0.f : newTop;
+					float part[4] = { 0.f, 0.f, 0.f, 0.f };
+#pragma unroll
+					for(int i = 0; i < 32; ++i) part[i & 3] += exp2_fast(fmaf(__uint_as_float(r[i]), LOG2E, -reference));
+					sum = sum * exp2_fast(top - reference) + ((part[0] + part[1]) + (part[2] + part[3]));
+					top = newTop;
+				} else if constexpr(EPILOGUE == PRODUCT16_DIFF) {
+					const int left = p.columns - p.firstColumn - col0 - c;
+					float v[32];
+#pragma unroll
+					for(int i = 0; i < 32; ++i) v[i] = by * exp2_fast(fmaf(__uint_as_float(r[i]), LOG2E, -logSum2));
+					if(__any_sync(0xffffffffu, own >= c && own < c + 32)) {
+#pragma unroll
+						for(int i = 0; i < 32; ++i) {
+							if(own - c == i) v[i] -= by;
+						}
+					}
+					// a row without a target has no gradient, whatever its logits; columns behind the vocabulary are zeros,
+					// which the products that read them count on
+					if(by == 0.f || left < 32) {
+#pragma unroll
+						for(int i = 0; i < 32; ++i) {
+							if(by == 0.f || i >= left) v[i] = 0.f;
+						}
+					}
+					if(on) {
+						uint16_t* const out = static_cast<uint16_t*>(p.out16) + row * p.ldOut + col0 + c;
+#pragma unroll
+						for(int j = 0; j < 2; ++j) {
+							uint32_t w[8];
+#pragma unroll
+							for(int i = 0; i < 8; ++i) w[i] = pack16(v[j * 16 + 2 * i], v[j * 16 + 2 * i + 1], p.bf16);
+							store32(out + j * 16, w);
+						}
+					}
+				} else if constexpr(EPILOGUE == PRODUCT16_SUM) {
+					if(on) {
+						float* const out = p.plane + (static_cast<long long>(t.split) * p.m + row) * p.ldPlane + col0 + c;
+#pragma unroll
+						for(int j = 0; j < 4; ++j) {
+							if(col0 + c + j * 8 < p.n) { // ldPlane is a multiple of 8
+								if(p.accumulate) {
+									uint32_t before[8];
+									load32(out + j * 8, before);
+#pragma unroll
+									for(int i = 0; i < 8; ++i) r[j * 8 + i] = __float_as_uint(__uint_as_float(r[j * 8 + i]) + __uint_as_float(before[i]));
+								}
+								store32(out + j * 8, r + j * 8);
+							}
+						}
+					}
+				} else {
+					if(on) {
+						uint16_t* const out = static_cast<uint16_t*>(p.out16) + row * p.ldOut + col0 + c;
+						const bool aligned = (p.ldOut & 7) == 0 && (reinterpret_cast<uintptr_t>(p.out16) & 15u) == 0;
+#pragma unroll
+						for(int j = 0; j < 4; ++j) {
+							uint32_t w[4];
+#pragma unroll
+							for(int i = 0; i < 4; ++i) {
+								w[i] = pack16(__uint_as_float(r[j * 8 + 2 * i]) * by, __uint_as_float(r[j * 8 + 2 * i + 1]) * by, p.bf16);
+							}
+							const int left = p.n - (col0 + c + j * 8);
+							if(aligned && left >= 8) {
+								*reinterpret_cast<uint4*>(out + j * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+							} else {
+#pragma unroll
+								for(int i = 0; i < 8; ++i) {
+									if(i < left) out[j * 8 + i] = static_cast<uint16_t>(i & 1 ? w[i >> 1] >> 16 : w[i >> 1] & 0xffffu);
+								}
+							}
+						}
+					}
+				}
+			}
+			if(EPILOGUE == PRODUCT16_STATS && on) {
+				p.partial[static_cast<long long>(t.nTile * 2 + half) * p.m + row] = make_float2(top, sum);
+			}
+		}
+	}
+	tc_fence_before_sync();
+	__syncthreads();
+	if(warp == 2) tmem_dealloc(tmemBase, 512);
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+	const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encoder()
+{
+	static EncodeTiledFn found = nullptr;
+	static std::once_flag once;
+	std::call_once(once, [] {
+		void* fn = nullptr;
+		cudaDriverEntryPointQueryResult q;
+		if(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess) {
+			found = reinterpret_cast<EncodeTiledFn>(fn);
+		}
+		cudaGetLastError();
+	});
+	return found;
+}
+
+using Kernel = void (*)(const Product16Params, const CUtensorMap, const CUtensorMap);
+
+} // namespace
+
+bool product16_map(void* map, const void* base, bool bf16, long long inner, long long rows, long long rowSize, int boxRows)
+{
+	const EncodeTiledFn encode = encoder();
+	if(encode == nullptr || !aligned16(base) || rowSize % 8 != 0 || rowSize * 2 >= (1ll << 40)) return false;
+	const cuuint64_t dims[2] = { static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(rows) };
+	const cuuint64_t strides[1] = { static_cast<cuuint64_t>(rowSize) * 2 };
+	const cuuint32_t box[2] = { 64, static_cast<cuuint32_t>(boxRows) };
+	const cuuint32_t steps[2] = { 1, 1 };
+	return encode(static_cast<CUtensorMap*>(map), bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
+		const_cast<void*>(base), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+		CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+int product16(Product16Epilogue epilogue, bool aAcross, bool bAcross, const Product16Params& p, const void* mapA, const void* mapB,
+	cudaStream_t stream)
+{
+	Kernel kernel = nullptr;
+	if(epilogue == PRODUCT16_STATS && !aAcross && !bAcross) kernel = product16_kernel<PRODUCT16_STATS, false, false>;
+	else if(epilogue == PRODUCT16_DIFF && !aAcross && !bAcross) kernel = product16_kernel<PRODUCT16_DIFF, false, false>;
+	else if(epilogue == PRODUCT16_SUM && !aAcross && bAcross) kernel = product16_kernel<PRODUCT16_SUM, false, true>;
+	else if(epilogue == PRODUCT16_SUM && aAcross && bAcross) kernel = product16_kernel<PRODUCT16_SUM, true, true>;
+	else if(epilogue == PRODUCT16_STORE && aAcross && bAcross) kernel = product16_kernel<PRODUCT16_STORE, true, true>;
+	else return NB200_EINVAL;
+	const long long tiles = static_cast<long long>(p.mTiles) * p.nTiles * p.splits;
+	if(tiles > 0x7fffffffLL - 1024) return NB200_ETOOBIG;
+	if(tiles == 0) return NB200_OK;
+	if(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES) != cudaSuccess) return check_launch();
+	const int grid = tiles < sm_count() ? static_cast<int>(tiles) : sm_count();
+	launch_dependent(false, kernel, dim3(grid), dim3(THREADS), SMEM_BYTES, stream, p, *static_cast<const CUtensorMap*>(mapA),
+		*static_cast<const CUtensorMap*>(mapB));
+	count_launch();
+	return check_launch();
+}
+
+} // namespace nb200

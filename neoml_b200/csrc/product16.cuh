@@ -1,0 +1,57 @@
+// Products of 16-bit matrices on the tensor core (fp16 or bf16 in, fp32 accumulators), with the epilogues of the cross entropy over a
+// vocabulary (vocabulary_loss.cu).  D[m][n] = sum_k A[m][k] B[n][k]; either operand may lie with its k adjacent (rows of k) or with
+// its m or n adjacent (rows per k, as a gradient's product meets what the forward pass stored).
+#pragma once
+#include "types16.cuh"
+
+namespace nb200 {
+
+enum Product16Epilogue {
+	PRODUCT16_STATS, // per row and 128 columns: maximum and sum of exponentials, and the labelled column's value
+	PRODUCT16_DIFF,  // 16-bit gradient by the logits: coefficient[row] * (softmax - [column is the label])
+	PRODUCT16_SUM,   // fp32 planes, one per part of K; added to what is there where `accumulate` is set
+	PRODUCT16_STORE  // 16-bit result times *resultScale
+};
+
+struct Product16Params {
+	int m, n;            // rows and columns of the result
+	int mTiles, nTiles, splits;
+	int kBlocks, kBlocksPerSplit;
+	int mFast;           // consecutive tiles go down the rows (A stays near) rather than along the columns
+	int aOffset, bOffset;   // added to the m and n coordinates of the loads
+	int akOffset, bkOffset; // and to their k coordinates
+	int bf16;            // operands are bf16 rather than fp16
+	int* status;
+	// STATS
+	float2* partial;     // [2 * nTiles][m]: maximum in units of log 2, sum of 2^(x - maximum)
+	float* labelled;     // [m]
+	// STATS, DIFF
+	const int* labels;   // [m]
+	int firstColumn;     // the column that column 0 of this result stands for
+	int columns;         // of all: columns behind are left out
+	// DIFF
+	const float* logSum; // [m]
+	const float* rowScale; // [m], times *scale
+	const float* scale;
+	// DIFF, STORE
+	void* out16;
+	long long ldOut;
+	// STORE
+	const float* resultScale;
+	// SUM
+	float* plane;        // [splits][m][ldPlane]
+	long long ldPlane;   // a multiple of 8
+	int accumulate;
+};
+
+// Enqueues the product.  mapA and mapB are the operands' tensor maps (product16_map).
+int product16(Product16Epilogue epilogue, bool aAcross, bool bAcross, const Product16Params& p, const void* mapA, const void* mapB,
+	cudaStream_t stream);
+// Map of a matrix of 16-bit elements, `inner` adjacent ones in each of `rows` rows; boxes of 64 x boxRows land as 128-byte rows
+// with the 128-byte swizzle.  False where TMA cannot describe it (base or rows off a 16-byte boundary).
+bool product16_map(void* map, const void* base, bool bf16, long long inner, long long rows, long long rowSize, int boxRows);
+
+constexpr int PRODUCT16_M = 128, PRODUCT16_N = 256, PRODUCT16_K = 64; // of a tile
+constexpr int PRODUCT16_BOX_A = 128, PRODUCT16_BOX_B = 256, PRODUCT16_BOX_ACROSS = 64; // boxRows of the operands' maps
+
+} // namespace nb200

@@ -616,3 +616,59 @@ def DistillationLossBackward(loss_diff, logits, teacher_logits, teacher_indices,
             _current(device), code, _TYPES[teacher_logits.dtype], diff_at, logits.data_ptr(), rows, vocabulary, row, teacher_at,
             indices_at, kept, float(temperature), sum_at, result.data_ptr(), _matrix(result)[2]))
     return result
+
+
+def _head(hidden, weights, labels):
+    rows, width, row = _matrix(hidden)
+    assert weights.dim() == 2 and weights.shape[1] == width and weights.dtype == hidden.dtype, \
+        f"weights [vocabulary, {width}] of the hidden rows' type"
+    vocabulary, _, weights_row = _matrix(weights)
+    assert vocabulary >= 1, "a vocabulary"
+    assert labels.shape == hidden.shape[:-1], "a label for every row"
+    return _typed(hidden), rows, width, row, vocabulary, weights_row
+
+
+def _head_scratch(code, hidden, rows, width, row, weights, vocabulary, weights_row, backward):
+    need = capi.load().nb200_vocabulary_cross_entropy_scratch_bytes(code, hidden.data_ptr(), rows, width, row, weights.data_ptr(),
+                                                                    vocabulary, weights_row, int(backward))
+    return torch.empty(need, dtype=torch.uint8, device=hidden.device)
+
+
+def VocabularyCrossEntropy(hidden, weights, labels, *, precision=PREC_3XTF32):
+    """Softmax cross entropy of the logits hidden @ weights^T against labels (int32), without keeping the logits: hidden
+    [..., width], weights [vocabulary, width], labels [...].  Returns (loss, log_sum), fp32, one per row; log_sum is what the
+    backward pass takes.  A label outside the vocabulary marks a row without a target (padding, a prompt): loss zero.
+    `precision` is that of the products of fp32 matrices."""
+    code, rows, width, row, vocabulary, weights_row = _head(hidden, weights, labels)
+    device = _device_of(hidden, weights, labels)
+    labels_at = _vector(labels, rows, torch.int32)
+    loss, log_sum = torch.empty((2, *labels.shape), dtype=torch.float32, device=device).unbind()
+    with torch.cuda.device(device):
+        scratch = _head_scratch(code, hidden, rows, width, row, weights, vocabulary, weights_row, False)
+        capi.check("VocabularyCrossEntropy", capi.load().nb200_vocabulary_cross_entropy(
+            _current(device), code, hidden.data_ptr(), rows, width, row, weights.data_ptr(), vocabulary, weights_row, labels_at,
+            loss.data_ptr(), log_sum.data_ptr(), scratch.data_ptr(), precision))
+    return loss, log_sum
+
+
+def VocabularyCrossEntropyBackward(loss_diff, hidden, weights, labels, log_sum, *, hidden_diff=True, weights_diff=True,
+                                   precision=PREC_3XTF32):
+    """The gradients of VocabularyCrossEntropy by hidden and weights, from that of each row's loss (fp32) and the forward
+    pass's log_sum.  hidden_diff and weights_diff: True for a new tensor, False where that gradient is not wanted (None comes
+    back), or the tensor to write.  Rows without a target have no gradient."""
+    code, rows, width, row, vocabulary, weights_row = _head(hidden, weights, labels)
+    device = _device_of(loss_diff, hidden, weights, labels, log_sum)
+    pointers = (_vector(loss_diff, rows, torch.float32), _vector(labels, rows, torch.int32), _vector(log_sum, rows, torch.float32))
+    diffs, places = [], []
+    for wanted, like in ((hidden_diff, hidden), (weights_diff, weights)):
+        diff = torch.empty(like.shape, dtype=like.dtype, device=device) if wanted is True else None if wanted is False else wanted
+        diffs.append(diff)
+        if diff is not None:
+            assert diff.shape == like.shape and diff.dtype == like.dtype and diff.device == device, "gradients like their operands"
+        places += (None, 0) if diff is None else (diff.data_ptr(), _matrix(diff)[2])
+    with torch.cuda.device(device):
+        scratch = _head_scratch(code, hidden, rows, width, row, weights, vocabulary, weights_row, True)
+        capi.check("VocabularyCrossEntropyBackward", capi.load().nb200_vocabulary_cross_entropy_backward(
+            _current(device), code, pointers[0], hidden.data_ptr(), rows, width, row, weights.data_ptr(), vocabulary, weights_row,
+            pointers[1], pointers[2], *places, scratch.data_ptr(), precision))
+    return tuple(diffs)
