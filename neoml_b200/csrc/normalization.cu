@@ -19,8 +19,9 @@ namespace nb200 {
 namespace {
 
 constexpr int MAX_WARPS = 32;     // of the kernels that loop over a row
-constexpr int MAX_ROW_WARPS = 16; // of those that hold it: 128 registers a thread
-constexpr int ROWS_PER_WARP_BLOCK = 4; // rows at a time of a block whose warps have a row each
+constexpr int MAX_ROW_WARPS = 16; // of those that hold it
+constexpr int SMALL_BLOCK = 128;  // threads of a block whose rows are a warp's or less: several rows at a time
+constexpr int SMALL_WIDTH = 1024; // and what such a row holds at most
 
 struct NormParams {
 	const void* x;
@@ -32,91 +33,114 @@ struct NormParams {
 	float* inv;
 	float* partial;        // backward: [blocks][2][width]
 	long long xRow, dyRow, outRow; // elements between rows
-	int height, width, warpsPerRow;
-	int rowStep;           // rows between two that a warp (or a block) takes
+	int height, width;
+	int lanes;             // threads that share a row: 4 to 32, or whole warps
+	int rowStep;           // rows between two that a thread takes
 	float epsilon;
 };
 
 // Sum over the threads that share a row; every one of them gets it.  `slots` holds a float per warp; the two calls of a
 // row use different ones, so that one barrier each is enough.
-__device__ __forceinline__ float row_sum(float v, int warps, float* slots)
+__device__ __forceinline__ float row_sum(float v, int lanes, float* slots)
 {
+	if(lanes <= 32) {
+		for(int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+		return v;
+	}
 	v = warp_sum_all(v);
-	if(warps == 1) return v;
 	if((threadIdx.x & 31) == 0) slots[threadIdx.x >> 5] = v;
 	__syncthreads();
-	float s = (threadIdx.x & 31) < warps ? slots[threadIdx.x & 31] : 0.f;
-	return warp_sum_all(s);
+	return warp_sum_all((threadIdx.x & 31) < (lanes >> 5) ? slots[threadIdx.x & 31] : 0.f);
 }
 
-// C units per thread.  A row per block of warpsPerRow warps, or (warpsPerRow == 1) a row per warp.
-template<typename T, typename P, int V, int C>
-__global__ void __launch_bounds__(MAX_ROW_WARPS * 32) norm_forward_kernel(const NormParams p)
+// The parameters of a thread's columns.
+template<typename P, int V, int C, bool EDGES>
+__device__ __forceinline__ void load_parameters(const void* from, float missing, int t, int lanes, int offset, int width, float (&v)[C][V])
 {
-	__shared__ float slots[2][MAX_WARPS];
-	const int warps = p.warpsPerRow;
-	const int lanes = warps * 32;
-	const int t = warps == 1 ? threadIdx.x & 31 : threadIdx.x;
-	int r = warps == 1 ? blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
-	if(r >= p.height) return; // a whole warp, or a whole block
-	const T* const x = static_cast<const T*>(p.x);
-	Row<T, V> row;
-	row.begin = x;
-	row.end = x + (p.height - 1) * p.xRow + p.width;
-	const int offset = row_offset<T, V>(x + r * p.xRow);
-	float scale[C][V], free[C][V];
 #pragma unroll
 	for(int c = 0; c < C; ++c) {
 		const int first = (c * lanes + t) * V - offset;
 #pragma unroll
 		for(int j = 0; j < V; ++j) {
-			const bool in = inside<V>(first, j, p.width);
-			scale[c][j] = in && p.scale != nullptr ? to_float(static_cast<const P*>(p.scale)[first + j]) : 1.f;
-			free[c][j] = in && p.free_term != nullptr ? to_float(static_cast<const P*>(p.free_term)[first + j]) : 0.f;
+			v[c][j] = from != nullptr && inside<V, EDGES>(first, j, width) ? to_float(static_cast<const P*>(from)[first + j]) : missing;
 		}
 	}
+}
+
+// C units per thread; the next row is under way while a row is worked on.
+template<typename T, typename P, int V, int C, bool EDGES>
+__global__ void __launch_bounds__(MAX_ROW_WARPS * 32, V * C <= 8 ? 2 : 1) norm_forward_kernel(const NormParams p)
+{
+	__shared__ float slots[2][MAX_WARPS];
+	const int lanes = p.lanes;
+	const int t = threadIdx.x & (lanes <= 32 ? lanes - 1 : 1023);
+	const int rowsAtOnce = lanes <= 32 ? blockDim.x / lanes : 1;
+	int r = blockIdx.x * rowsAtOnce + (lanes <= 32 ? threadIdx.x / lanes : 0);
+	const T* const x = static_cast<const T*>(p.x);
+	Row<T, V> row;
+	row.begin = x;
+	row.end = x + (p.height - 1) * p.xRow + p.width;
+	const int offset = EDGES ? row_offset<T, V>(x + r * p.xRow) : 0;
+	float scale[C][V], free[C][V];
+	load_parameters<P, V, C, EDGES>(p.scale, 1.f, t, lanes, offset, p.width, scale);
+	load_parameters<P, V, C, EDGES>(p.free_term, 0.f, t, lanes, offset, p.width, free);
 	const float overWidth = 1.f / static_cast<float>(p.width);
-	for(; r < p.height; r += p.rowStep) {
-		row.p = x + r * p.xRow;
+	uint4 next[C];
+	auto load = [&](int at) {
+		row.p = x + at * p.xRow;
+#pragma unroll
+		for(int c = 0; c < C; ++c) {
+			next[c] = make_uint4(0u, 0u, 0u, 0u);
+			if(at < p.height) load_unit<T, V, EDGES>(row, (c * lanes + t) * V - offset, p.width, next[c]);
+		}
+	};
+	load(r);
+	// all threads of a warp stay to the end of its last row
+	for(int left = r - (lanes <= 32 ? (threadIdx.x & 31) / lanes : 0); left < p.height; left += p.rowStep, r += p.rowStep) {
 		uint4 raw[C];
 #pragma unroll
-		for(int c = 0; c < C; ++c) load_unit<T, V>(row, (c * lanes + t) * V - offset, p.width, raw[c]);
+		for(int c = 0; c < C; ++c) raw[c] = next[c];
+		load(r + p.rowStep);
 		float sum = 0.f;
 #pragma unroll
 		for(int c = 0; c < C; ++c) {
-			const int first = (c * lanes + t) * V - offset;
 			float v[V];
-			unit_floats<T, V>(raw[c], v);
+			whole_floats<T, V, EDGES>(raw[c], (c * lanes + t) * V - offset, p.width, v);
 #pragma unroll
-			for(int j = 0; j < V; ++j) sum += inside<V>(first, j, p.width) ? v[j] : 0.f;
+			for(int j = 0; j < V; ++j) sum += v[j];
 		}
-		const float mean = row_sum(sum, warps, slots[0]) * overWidth;
+		const float mean = row_sum(sum, lanes, slots[0]) * overWidth;
 		float square = 0.f;
 #pragma unroll
 		for(int c = 0; c < C; ++c) {
 			const int first = (c * lanes + t) * V - offset;
 			float v[V];
 			unit_floats<T, V>(raw[c], v);
+			if(whole<V, EDGES>(first, p.width)) {
 #pragma unroll
-			for(int j = 0; j < V; ++j) {
-				const float d = inside<V>(first, j, p.width) ? v[j] - mean : 0.f;
-				square = fmaf(d, d, square);
+				for(int j = 0; j < V; ++j) square = fmaf(v[j] - mean, v[j] - mean, square);
+			} else {
+#pragma unroll
+				for(int j = 0; j < V; ++j) {
+					if(inside<V, EDGES>(first, j, p.width)) square = fmaf(v[j] - mean, v[j] - mean, square);
+				}
 			}
 		}
-		const float inv = rsqrtf(row_sum(square, warps, slots[1]) * overWidth + p.epsilon);
-		T* const out = static_cast<T*>(p.out) + r * p.outRow;
+		const float inv = rsqrtf(row_sum(square, lanes, slots[1]) * overWidth + p.epsilon);
+		if(r < p.height) {
+			T* const out = static_cast<T*>(p.out) + r * p.outRow;
 #pragma unroll
-		for(int c = 0; c < C; ++c) {
-			const int first = (c * lanes + t) * V - offset;
-			float v[V];
-			unit_floats<T, V>(raw[c], v);
+			for(int c = 0; c < C; ++c) {
+				float v[V];
+				unit_floats<T, V>(raw[c], v);
 #pragma unroll
-			for(int j = 0; j < V; ++j) v[j] = fmaf((v[j] - mean) * inv, scale[c][j], free[c][j]);
-			store_unit<T, V>(out, first, p.width, v);
-		}
-		if(t == 0) {
-			if(p.mean != nullptr) p.mean[r] = mean;
-			if(p.inv != nullptr) p.inv[r] = inv;
+				for(int j = 0; j < V; ++j) v[j] = fmaf((v[j] - mean) * inv, scale[c][j], free[c][j]);
+				store_unit<T, V, EDGES>(out, (c * lanes + t) * V - offset, p.width, v);
+			}
+			if(t == 0) {
+				if(p.mean != nullptr) p.mean[r] = mean;
+				if(p.inv != nullptr) p.inv[r] = inv;
+			}
 		}
 	}
 }
@@ -132,13 +156,13 @@ __global__ void __launch_bounds__(1024) norm_forward_wide_kernel(const NormParam
 		T* const out = static_cast<T*>(p.out) + r * p.outRow;
 		float sum = 0.f;
 		for(int i = threadIdx.x; i < p.width; i += blockDim.x) sum += to_float(x[i]);
-		const float mean = row_sum(sum, MAX_WARPS, slots[0]) * overWidth;
+		const float mean = row_sum(sum, MAX_WARPS * 32, slots[0]) * overWidth;
 		float square = 0.f;
 		for(int i = threadIdx.x; i < p.width; i += blockDim.x) {
 			const float d = to_float(x[i]) - mean;
 			square = fmaf(d, d, square);
 		}
-		const float inv = rsqrtf(row_sum(square, MAX_WARPS, slots[1]) * overWidth + p.epsilon);
+		const float inv = rsqrtf(row_sum(square, MAX_WARPS * 32, slots[1]) * overWidth + p.epsilon);
 		for(int i = threadIdx.x; i < p.width; i += blockDim.x) {
 			const float s = p.scale != nullptr ? to_float(static_cast<const P*>(p.scale)[i]) : 1.f;
 			const float b = p.free_term != nullptr ? to_float(static_cast<const P*>(p.free_term)[i]) : 0.f;
@@ -152,15 +176,16 @@ __global__ void __launch_bounds__(1024) norm_forward_wide_kernel(const NormParam
 	}
 }
 
-// Backward.  A block's sums of dy u and dy stay in registers over all its rows and go to `partial` once.
-template<typename T, typename P, int V, int C>
+// Backward.  A thread's sums of dy u and dy stay in registers over all its rows; a block's go to `partial` once.
+template<typename T, typename P, int V, int C, bool EDGES>
 __global__ void __launch_bounds__(MAX_ROW_WARPS * 32) norm_backward_kernel(const NormParams p)
 {
 	__shared__ float slots[2][2][MAX_WARPS];
-	const int warps = p.warpsPerRow;
-	const int lanes = warps * 32;
-	const int t = warps == 1 ? threadIdx.x & 31 : threadIdx.x;
-	int r = warps == 1 ? blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
+	__shared__ float sums[2][SMALL_WIDTH];
+	const int lanes = p.lanes;
+	const int t = threadIdx.x & (lanes <= 32 ? lanes - 1 : 1023);
+	const int rowsAtOnce = lanes <= 32 ? blockDim.x / lanes : 1;
+	int r = blockIdx.x * rowsAtOnce + (lanes <= 32 ? threadIdx.x / lanes : 0);
 	const T* const x = static_cast<const T*>(p.x);
 	const T* const dy = static_cast<const T*>(p.dy);
 	Row<T, V> xr, dr;
@@ -168,88 +193,121 @@ __global__ void __launch_bounds__(MAX_ROW_WARPS * 32) norm_backward_kernel(const
 	xr.end = x + (p.height - 1) * p.xRow + p.width;
 	dr.begin = dy;
 	dr.end = dy + (p.height - 1) * p.dyRow + p.width;
-	const int offset = row_offset<T, V>(x + (r < p.height ? r : 0) * p.xRow);
+	const int offset = EDGES ? row_offset<T, V>(x + r * p.xRow) : 0;
 	float scale[C][V], ds[C][V], db[C][V];
+	load_parameters<P, V, C, EDGES>(p.scale, 1.f, t, lanes, offset, p.width, scale);
 #pragma unroll
 	for(int c = 0; c < C; ++c) {
-		const int first = (c * lanes + t) * V - offset;
 #pragma unroll
-		for(int j = 0; j < V; ++j) {
-			scale[c][j] = inside<V>(first, j, p.width) && p.scale != nullptr ? to_float(static_cast<const P*>(p.scale)[first + j]) : 1.f;
-			ds[c][j] = db[c][j] = 0.f;
-		}
+		for(int j = 0; j < V; ++j) ds[c][j] = db[c][j] = 0.f;
 	}
 	const float overWidth = 1.f / static_cast<float>(p.width);
 	int phase = 0;
-	for(; r < p.height; r += p.rowStep, phase ^= 1) {
-		xr.p = x + r * p.xRow;
-		dr.p = dy + r * p.dyRow;
+	uint4 nextX[C], nextD[C];
+	float nextMean = 0.f, nextInv = 0.f;
+	auto load = [&](int at) {
+		xr.p = x + at * p.xRow;
+		dr.p = dy + at * p.dyRow;
+#pragma unroll
+		for(int c = 0; c < C; ++c) {
+			nextX[c] = nextD[c] = make_uint4(0u, 0u, 0u, 0u);
+			if(at < p.height) {
+				load_unit<T, V, EDGES>(xr, (c * lanes + t) * V - offset, p.width, nextX[c]);
+				load_unit<T, V, EDGES>(dr, (c * lanes + t) * V - offset, p.width, nextD[c]);
+			}
+		}
+		if(at < p.height) {
+			nextMean = __ldg(p.mean + at);
+			nextInv = __ldg(p.inv + at);
+		}
+	};
+	load(r);
+	for(int left = r - (lanes <= 32 ? (threadIdx.x & 31) / lanes : 0); left < p.height; left += p.rowStep, r += p.rowStep, phase ^= 1) {
 		uint4 rx[C], rd[C];
 #pragma unroll
 		for(int c = 0; c < C; ++c) {
-			load_unit<T, V>(xr, (c * lanes + t) * V - offset, p.width, rx[c]);
-			load_unit<T, V>(dr, (c * lanes + t) * V - offset, p.width, rd[c]);
+			rx[c] = nextX[c];
+			rd[c] = nextD[c];
 		}
-		const float mean = __ldg(p.mean + r), inv = __ldg(p.inv + r);
+		const float mean = nextMean, inv = nextInv;
+		load(r + p.rowStep);
 		float sumG = 0.f, sumGu = 0.f;
 #pragma unroll
 		for(int c = 0; c < C; ++c) {
 			const int first = (c * lanes + t) * V - offset;
 			float u[V], g[V];
-			unit_floats<T, V>(rx[c], u);
-			unit_floats<T, V>(rd[c], g);
+			whole_floats<T, V, EDGES>(rx[c], first, p.width, u); // the neighbours' may be infinite
+			whole_floats<T, V, EDGES>(rd[c], first, p.width, g); // zeros outside, and so is what they are multiplied by
 #pragma unroll
 			for(int j = 0; j < V; ++j) {
-				const bool in = inside<V>(first, j, p.width);
-				const float d = in ? g[j] : 0.f, unit = in ? (u[j] - mean) * inv : 0.f;
-				ds[c][j] = fmaf(d, unit, ds[c][j]);
-				db[c][j] += d;
-				const float by = d * scale[c][j];
+				const float unit = (u[j] - mean) * inv;
+				ds[c][j] = fmaf(g[j], unit, ds[c][j]);
+				db[c][j] += g[j];
+				const float by = g[j] * scale[c][j];
 				sumG += by;
 				sumGu = fmaf(by, unit, sumGu);
 			}
 		}
-		sumG = warp_sum_all(sumG);
-		sumGu = warp_sum_all(sumGu);
-		if(warps > 1) {
+		if(lanes <= 32) {
+			for(int o = lanes >> 1; o > 0; o >>= 1) {
+				sumG += __shfl_xor_sync(0xffffffffu, sumG, o);
+				sumGu += __shfl_xor_sync(0xffffffffu, sumGu, o);
+			}
+		} else {
+			sumG = warp_sum_all(sumG);
+			sumGu = warp_sum_all(sumGu);
 			if((threadIdx.x & 31) == 0) {
 				slots[phase][0][threadIdx.x >> 5] = sumG;
 				slots[phase][1][threadIdx.x >> 5] = sumGu;
 			}
 			__syncthreads(); // one a row: the slots alternate
 			const int w = threadIdx.x & 31;
-			sumG = warp_sum_all(w < warps ? slots[phase][0][w] : 0.f);
-			sumGu = warp_sum_all(w < warps ? slots[phase][1][w] : 0.f);
+			sumG = warp_sum_all(w < (lanes >> 5) ? slots[phase][0][w] : 0.f);
+			sumGu = warp_sum_all(w < (lanes >> 5) ? slots[phase][1][w] : 0.f);
 		}
-		const float meanG = sumG * overWidth, meanGu = sumGu * overWidth;
-		T* const out = static_cast<T*>(p.out) + r * p.outRow;
+		if(r < p.height) {
+			const float meanG = sumG * overWidth, meanGu = sumGu * overWidth;
+			T* const out = static_cast<T*>(p.out) + r * p.outRow;
 #pragma unroll
-		for(int c = 0; c < C; ++c) {
-			const int first = (c * lanes + t) * V - offset;
-			float u[V], g[V];
-			unit_floats<T, V>(rx[c], u);
-			unit_floats<T, V>(rd[c], g);
+			for(int c = 0; c < C; ++c) {
+				float u[V], g[V];
+				unit_floats<T, V>(rx[c], u);
+				unit_floats<T, V>(rd[c], g);
 #pragma unroll
-			for(int j = 0; j < V; ++j) {
-				const float unit = (u[j] - mean) * inv;
-				g[j] = (fmaf(g[j], scale[c][j], -meanG) - unit * meanGu) * inv;
+				for(int j = 0; j < V; ++j) {
+					const float unit = (u[j] - mean) * inv;
+					g[j] = (fmaf(g[j], scale[c][j], -meanG) - unit * meanGu) * inv;
+				}
+				store_unit<T, V, EDGES>(out, (c * lanes + t) * V - offset, p.width, g);
 			}
-			store_unit<T, V>(out, first, p.width, g);
 		}
 	}
 	if(p.partial == nullptr) return;
-	// one row of partial sums per block; the warps that had rows of their own write one each
-	float* const mine = p.partial + static_cast<long long>(warps == 1 ? blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x) * 2 * p.width;
+	float* const mine = p.partial + static_cast<long long>(blockIdx.x) * 2 * p.width;
+	// rows that are worked on at the same time add up in turn
+	for(int g = 0; g < rowsAtOnce; ++g) {
+		if(rowsAtOnce == 1 || threadIdx.x / lanes == g) {
 #pragma unroll
-	for(int c = 0; c < C; ++c) {
-		const int first = (c * lanes + t) * V - offset;
+			for(int c = 0; c < C; ++c) {
+				const int first = (c * lanes + t) * V - offset;
 #pragma unroll
-		for(int j = 0; j < V; ++j) {
-			if(inside<V>(first, j, p.width)) {
-				mine[first + j] = ds[c][j];
-				mine[p.width + first + j] = db[c][j];
+				for(int j = 0; j < V; ++j) {
+					if(!inside<V, EDGES>(first, j, p.width)) continue;
+					const int column = first + j;
+					if(rowsAtOnce == 1) {
+						mine[column] = ds[c][j];
+						mine[p.width + column] = db[c][j];
+					} else {
+						sums[0][column] = (g > 0 ? sums[0][column] : 0.f) + ds[c][j];
+						sums[1][column] = (g > 0 ? sums[1][column] : 0.f) + db[c][j];
+					}
+				}
 			}
 		}
+		if(rowsAtOnce > 1) __syncthreads();
+	}
+	if(rowsAtOnce > 1) {
+		for(int i = threadIdx.x; i < 2 * p.width; i += blockDim.x) mine[i] = i < p.width ? sums[0][i] : sums[1][i - p.width];
 	}
 }
 
@@ -279,8 +337,8 @@ __global__ void __launch_bounds__(1024) norm_backward_wide_kernel(const NormPara
 			}
 		}
 		started = true;
-		const float meanG = row_sum(sumG, MAX_WARPS, slots[phase][0]) * overWidth;
-		const float meanGu = row_sum(sumGu, MAX_WARPS, slots[phase][1]) * overWidth;
+		const float meanG = row_sum(sumG, MAX_WARPS * 32, slots[phase][0]) * overWidth;
+		const float meanGu = row_sum(sumGu, MAX_WARPS * 32, slots[phase][1]) * overWidth;
 		for(int i = threadIdx.x; i < p.width; i += blockDim.x) {
 			const float unit = (to_float(x[i]) - mean) * inv;
 			const float s = p.scale != nullptr ? to_float(static_cast<const P*>(p.scale)[i]) : 1.f;
@@ -329,45 +387,59 @@ __global__ void __launch_bounds__(256) zero_parameters_kernel(P* a, P* b, int wi
 struct Shape {
 	bool wide;      // rows longer than registers hold
 	int unit;       // elements of a unit
-	int units;      // per thread: 1, 2, 4 (or 16 units of one element)
-	int warps;      // per row
+	bool edges;     // rows may begin or end inside a unit
+	int units;      // per thread: 1 to 4, 6 or 8, or 16 units of one element
+	int lanes;      // threads of a row
 	int threads;    // per block
 	int rowsAtOnce; // of a block
 	int blocks;
-	int parts() const { return wide || warps > 1 ? blocks : blocks * rowsAtOnce; }
 };
 
-// `most`: elements a thread may hold.  Few enough warps that a block's barriers cost little, enough threads that the
-// device is filled: the fewest warps per row whose threads hold the row.
-Shape shape_of(int type, int height, int width, bool alike, int most)
+// A thread holds 16 elements (forward: 24 of 16 bits in a row that is one warp's, 32 in rows that are too long for MAX_ROW_WARPS
+// warps otherwise): more of them, with the parameters or sums beside them, would not stay in registers.
+// Rows of at most 32 lanes need no barrier.  Longer ones take the fewest threads, then the fewest warps, that hold them.
+Shape shape_of(int type, int height, int width, bool alike, bool aligned, bool forward)
 {
 	Shape s = {};
-	const int whole = alike ? 16 / type_size(type) : 1;
-	s.unit = whole;
-	const int units = (width + whole - 1) / whole + (whole > 1 ? 1 : 0); // the row may begin inside a unit
-	const int unitsPerThread = alike ? most / whole : 16;
-	s.warps = 1;
-	while(s.warps < MAX_ROW_WARPS && static_cast<long long>(s.warps) * 32 * unitsPerThread < units) s.warps *= 2;
-	const int perThread = (units + s.warps * 32 - 1) / (s.warps * 32);
-	s.wide = perThread > unitsPerThread;
-	if(s.wide) {
-		s.warps = MAX_WARPS;
-		s.threads = 1024;
+	const int size = type_size(type);
+	s.unit = alike ? 16 / size : 1;
+	s.edges = !aligned || width % s.unit != 0;
+	// a row that begins inside a unit touches one more
+	const int units = alike && !aligned ? (width + 2 * (s.unit - 1)) / s.unit : (width + s.unit - 1) / s.unit;
+	const int most = alike ? 16 / s.unit : 16;
+	if(units <= 32 * (forward && alike && size == 2 ? 3 : most) && width <= SMALL_WIDTH) {
+		s.lanes = 32;
+		while(s.lanes > 4 && units <= s.lanes / 2) s.lanes /= 2;
+		s.threads = SMALL_BLOCK;
+		s.rowsAtOnce = SMALL_BLOCK / s.lanes;
+		s.units = alike ? (units + s.lanes - 1) / s.lanes : 16;
+	} else {
+		int hold = units > MAX_ROW_WARPS * 32 * most && forward && alike ? 2 * most : most;
+		auto warps_for = [&](int h) { return (units + 32 * h - 1) / (32 * h); };
+		s.wide = warps_for(hold) > MAX_ROW_WARPS;
+		if(alike && !s.wide) {
+			for(int h = hold - 1; h >= 1 && warps_for(h) <= MAX_ROW_WARPS; --h) {
+				if(warps_for(h) * h < warps_for(hold) * hold) hold = h;
+			}
+		}
+		s.threads = s.lanes = (s.wide ? MAX_WARPS : warps_for(hold)) * 32;
 		s.rowsAtOnce = 1;
+		s.units = alike ? (units + s.lanes - 1) / s.lanes : 16;
+	}
+	// by the kernels' registers
+	const int residentThreads = s.units * s.unit <= 8 ? (forward ? 1024 : 768) : forward && s.units * s.unit <= 16 ? 640 : 512;
+	if(s.wide) {
 		s.blocks = height < sm_count() * 2 ? height : sm_count() * 2;
 		return s;
 	}
-	s.units = alike ? (perThread <= 1 ? 1 : perThread <= 2 ? 2 : perThread <= 4 ? 4 : 8) : 16;
-	s.rowsAtOnce = s.warps == 1 ? ROWS_PER_WARP_BLOCK : 1;
-	s.threads = s.warps * 32 * s.rowsAtOnce;
-	// a block's rows are a multiple of a unit's elements apart
-	const long long wanted = (static_cast<long long>(height) + s.rowsAtOnce - 1) / s.rowsAtOnce;
-	long long resident = static_cast<long long>(sm_count()) * (1024 / s.threads > 0 ? 1024 / s.threads : 1);
+	// a block's rows are a multiple of a unit's elements apart: all of them begin at the same offset in a unit
+	const int wanted = (height + s.rowsAtOnce - 1) / s.rowsAtOnce;
+	int resident = sm_count() * (residentThreads / s.threads > 1 ? residentThreads / s.threads : 1);
 	if(wanted > resident) {
-		while(resident * s.rowsAtOnce % whole != 0) ++resident;
-		s.blocks = static_cast<int>(resident);
+		while(resident * s.rowsAtOnce % s.unit != 0) ++resident;
+		s.blocks = resident;
 	} else {
-		s.blocks = static_cast<int>(wanted);
+		s.blocks = wanted;
 	}
 	return s;
 }
@@ -388,32 +460,62 @@ bool aligned_alike(int type, int height, const Operand* o, int n)
 	return true;
 }
 
+// Every operand's rows all begin on a 16-byte boundary.
+bool all_aligned(int type, int height, const Operand* o, int n)
+{
+	for(int i = 0; i < n; ++i) {
+		if(!aligned16(o[i].p) || (height > 1 && (o[i].row * type_size(type) & 15) != 0)) return false;
+	}
+	return true;
+}
+
+template<typename T, typename P, bool EDGES>
+void launch_forward_units(const NormParams& p, const Shape& s, cudaStream_t stream)
+{
+	constexpr int V = Unit16<T>::N;
+	if(s.units <= 1) norm_forward_kernel<T, P, V, 1, EDGES><<<s.blocks, s.threads, 0, stream>>>(p);
+	else if(s.units == 2) norm_forward_kernel<T, P, V, 2, EDGES><<<s.blocks, s.threads, 0, stream>>>(p);
+	else if(s.units == 3) norm_forward_kernel<T, P, V, 3, EDGES><<<s.blocks, s.threads, 0, stream>>>(p);
+	else if(s.units == 4) norm_forward_kernel<T, P, V, 4, EDGES><<<s.blocks, s.threads, 0, stream>>>(p);
+	else if constexpr(V == 4) {
+		if(s.units <= 6) norm_forward_kernel<T, P, V, 6, EDGES><<<s.blocks, s.threads, 0, stream>>>(p);
+		else norm_forward_kernel<T, P, V, 8, EDGES><<<s.blocks, s.threads, 0, stream>>>(p);
+	}
+}
+
 template<typename T, typename P>
 void launch_forward(const NormParams& p, const Shape& s, cudaStream_t stream)
 {
-	constexpr int V = Unit16<T>::N;
 	if(s.wide) norm_forward_wide_kernel<T, P><<<s.blocks, s.threads, 0, stream>>>(p);
-	else if(s.unit == 1) norm_forward_kernel<T, P, 1, 16><<<s.blocks, s.threads, 0, stream>>>(p);
-	else if(s.units == 1) norm_forward_kernel<T, P, V, 1><<<s.blocks, s.threads, 0, stream>>>(p);
-	else if(s.units == 2) norm_forward_kernel<T, P, V, 2><<<s.blocks, s.threads, 0, stream>>>(p);
-	else if(s.units == 4) norm_forward_kernel<T, P, V, 4><<<s.blocks, s.threads, 0, stream>>>(p);
-	else if constexpr(V == 4) norm_forward_kernel<T, P, V, 8><<<s.blocks, s.threads, 0, stream>>>(p);
+	else if(s.unit == 1) norm_forward_kernel<T, P, 1, 16, true><<<s.blocks, s.threads, 0, stream>>>(p);
+	else if(s.edges) launch_forward_units<T, P, true>(p, s, stream);
+	else launch_forward_units<T, P, false>(p, s, stream);
+}
+
+template<typename T, typename P, bool EDGES>
+void launch_backward_units(const NormParams& p, const Shape& s, cudaStream_t stream)
+{
+	constexpr int V = Unit16<T>::N;
+	if(s.units <= 1) norm_backward_kernel<T, P, V, 1, EDGES><<<s.blocks, s.threads, 0, stream>>>(p);
+	else if(s.units == 2) norm_backward_kernel<T, P, V, 2, EDGES><<<s.blocks, s.threads, 0, stream>>>(p);
+	else if constexpr(V == 4) {
+		if(s.units == 3) norm_backward_kernel<T, P, V, 3, EDGES><<<s.blocks, s.threads, 0, stream>>>(p);
+		else norm_backward_kernel<T, P, V, 4, EDGES><<<s.blocks, s.threads, 0, stream>>>(p);
+	}
 }
 
 template<typename T, typename P>
 void launch_backward(const NormParams& p, const Shape& s, void* scaleDiff, void* freeDiff, cudaStream_t stream)
 {
-	constexpr int V = Unit16<T>::N;
 	if(s.wide) norm_backward_wide_kernel<T, P><<<s.blocks, s.threads, 0, stream>>>(p);
-	else if(s.unit == 1) norm_backward_kernel<T, P, 1, 16><<<s.blocks, s.threads, 0, stream>>>(p);
-	else if(s.units == 1) norm_backward_kernel<T, P, V, 1><<<s.blocks, s.threads, 0, stream>>>(p);
-	else if(s.units == 2) norm_backward_kernel<T, P, V, 2><<<s.blocks, s.threads, 0, stream>>>(p);
-	else if constexpr(V == 4) norm_backward_kernel<T, P, V, 4><<<s.blocks, s.threads, 0, stream>>>(p);
+	else if(s.unit == 1) norm_backward_kernel<T, P, 1, 16, true><<<s.blocks, s.threads, 0, stream>>>(p);
+	else if(s.edges) launch_backward_units<T, P, true>(p, s, stream);
+	else launch_backward_units<T, P, false>(p, s, stream);
 	count_launch();
 	if(p.partial != nullptr) {
 		const dim3 grid((p.width + 31) / 32, 2);
 		launch_dependent(true, norm_parameters_kernel<P>, grid, dim3(512), 0, stream, static_cast<const float*>(p.partial),
-			s.parts(), p.width, static_cast<P*>(scaleDiff), static_cast<P*>(freeDiff));
+			s.blocks, p.width, static_cast<P*>(scaleDiff), static_cast<P*>(freeDiff));
 		count_launch();
 	}
 }
@@ -431,8 +533,6 @@ bool sizes_valid(int type, int parameterType, int height, int width)
 {
 	return type_valid(type) && (parameterType == type || parameterType == NB200_TYPE_FP32) && height >= 0 && width >= 1;
 }
-
-constexpr int FORWARD_ELEMENTS = 32, BACKWARD_ELEMENTS = 16; // registers: three floats an element there, one more sum here
 
 } // namespace
 
@@ -452,11 +552,11 @@ int nb200_layer_normalization(void* stream, int type, int parameter_type, const 
 		|| !type_aligned(scale, parameter_type) || !type_aligned(free_term, parameter_type)) return NB200_EINVAL;
 	if(device_status_word() == nullptr) return NB200_ENODEVICE;
 	const Operand operands[] = { { x, x_row_size }, { y, y_row_size } };
-	const Shape s = shape_of(type, height, width, aligned_alike(type, height, operands, 2), FORWARD_ELEMENTS);
+	const Shape s = shape_of(type, height, width, aligned_alike(type, height, operands, 2), all_aligned(type, height, operands, 2), true);
 	NormParams p = {};
 	p.x = x; p.scale = scale; p.free_term = free_term; p.out = y; p.mean = mean; p.inv = inverse_deviation;
 	p.xRow = x_row_size; p.outRow = y_row_size;
-	p.height = height; p.width = width; p.warpsPerRow = s.warps; p.rowStep = s.blocks * s.rowsAtOnce; p.epsilon = epsilon;
+	p.height = height; p.width = width; p.lanes = s.lanes; p.rowStep = s.blocks * s.rowsAtOnce; p.epsilon = epsilon;
 	with_types(type, parameter_type, [&](auto t, auto q) { launch_forward<decltype(t), decltype(q)>(p, s, as_stream(stream)); });
 	count_launch();
 	return check_launch();
@@ -466,9 +566,12 @@ size_t nb200_layer_normalization_backward_scratch_floats(int type, int height, i
 {
 	if(!type_valid(type) || height <= 0 || width <= 0) return 0;
 	// whichever form the operands' alignment selects
-	const int a = shape_of(type, height, width, true, BACKWARD_ELEMENTS).parts();
-	const int b = shape_of(type, height, width, false, BACKWARD_ELEMENTS).parts();
-	return static_cast<size_t>(a > b ? a : b) * 2 * width;
+	int blocks = 0;
+	for(int form = 0; form < 3; ++form) {
+		const int n = shape_of(type, height, width, form > 0, form > 1, false).blocks;
+		if(n > blocks) blocks = n;
+	}
+	return static_cast<size_t>(blocks) * 2 * width;
 }
 
 int nb200_layer_normalization_backward(void* stream, int type, int parameter_type, const void* dy, long long dy_row_size,
@@ -496,13 +599,13 @@ int nb200_layer_normalization_backward(void* stream, int type, int parameter_typ
 		return check_launch();
 	}
 	const Operand operands[] = { { x, x_row_size }, { dy, dy_row_size }, { dx, dx_row_size } };
-	const Shape s = shape_of(type, height, width, aligned_alike(type, height, operands, 3), BACKWARD_ELEMENTS);
+	const Shape s = shape_of(type, height, width, aligned_alike(type, height, operands, 3), all_aligned(type, height, operands, 3), false);
 	NormParams p = {};
 	p.x = x; p.dy = dy; p.scale = scale; p.out = dx;
 	p.mean = const_cast<float*>(mean); p.inv = const_cast<float*>(inverse_deviation);
 	p.partial = parameters ? scratch : nullptr;
 	p.xRow = x_row_size; p.dyRow = dy_row_size; p.outRow = dx_row_size;
-	p.height = height; p.width = width; p.warpsPerRow = s.warps; p.rowStep = s.blocks * s.rowsAtOnce;
+	p.height = height; p.width = width; p.lanes = s.lanes; p.rowStep = s.blocks * s.rowsAtOnce;
 	with_types(type, parameter_type, [&](auto t, auto q) {
 		launch_backward<decltype(t), decltype(q)>(p, s, scale_diff, free_term_diff, as_stream(stream));
 	});

@@ -86,7 +86,9 @@ struct Row {
 	const T* end;
 };
 
-template<typename T, int V>
+// A unit as it lies in memory, neighbouring rows' elements included (whole_floats leaves them out): what has just been asked
+// for is not looked at here, so that loads stay under way.  EDGES false: rows that begin and end with whole units.
+template<typename T, int V, bool EDGES = true>
 __device__ __forceinline__ void load_unit(const Row<T, V>& row, int first, int width, uint4& raw)
 {
 	if constexpr(V == 1) {
@@ -96,10 +98,10 @@ __device__ __forceinline__ void load_unit(const Row<T, V>& row, int first, int w
 			else raw.x = reinterpret_cast<const unsigned short*>(row.p)[first];
 		}
 	} else {
-		const T* at = row.p + first;
+		const T* const at = row.p + first;
 		raw = make_uint4(0u, 0u, 0u, 0u);
 		if(first >= width) return;
-		if(at >= row.begin && at + V <= row.end) {
+		if(!EDGES || (at >= row.begin && at + V <= row.end)) {
 			raw = *reinterpret_cast<const uint4*>(at);
 		} else { // the first unit of the first row, the last one of the last
 			float v[V];
@@ -121,11 +123,13 @@ __device__ __forceinline__ void unit_floats(const uint4& raw, float* v)
 	}
 }
 
-template<typename T, int V>
+template<typename T, int V, bool EDGES = true>
 __device__ __forceinline__ void store_unit(T* row, int first, int width, const float* v)
 {
 	if constexpr(V == 1) {
 		if(first < width) row[first] = from_float<T>(v[0]);
+	} else if constexpr(!EDGES) {
+		if(first < width) *reinterpret_cast<uint4*>(row + first) = Unit16<T>::pack(v);
 	} else {
 		if(first >= 0 && first + V <= width) {
 			*reinterpret_cast<uint4*>(row + first) = Unit16<T>::pack(v);
@@ -138,10 +142,28 @@ __device__ __forceinline__ void store_unit(T* row, int first, int width, const f
 	}
 }
 
-template<int V>
+template<int V, bool EDGES = true>
 __device__ __forceinline__ bool inside(int first, int j, int width)
 {
-	return V == 1 ? first < width : first + j >= 0 && first + j < width;
+	return V == 1 || !EDGES ? first < width : first + j >= 0 && first + j < width;
+}
+
+// the whole unit belongs to the row
+template<int V, bool EDGES = true>
+__device__ __forceinline__ bool whole(int first, int width)
+{
+	return V == 1 || !EDGES ? first < width : first >= 0 && first + V <= width;
+}
+
+// a unit's floats, with zeros for what is not the row's
+template<typename T, int V, bool EDGES>
+__device__ __forceinline__ void whole_floats(const uint4& raw, int first, int width, float* v)
+{
+	unit_floats<T, V>(raw, v);
+	if(V > 1 && EDGES && !whole<V>(first, width)) {
+#pragma unroll
+		for(int j = 0; j < V; ++j) v[j] = inside<V>(first, j, width) ? v[j] : 0.f;
+	}
 }
 
 // elements by which a row's first address lies behind a 16-byte boundary
