@@ -11,8 +11,10 @@
 //   thread   one channel (two 16-bit channels where rows are aligned for it) times STEPS steps: loads them all at once,
 //            folds them to one (A, H)
 //   block    its warps hold consecutive stretches of time for the same 32 or 64 channels; the folds meet in shared memory
-//   cluster  up to 8 blocks hold consecutive stretches again and tell each other their folds through distributed shared
-//            memory; a cluster walks its channels' whole time axis, carrying the state in a register
+//   cluster  up to 8 blocks hold consecutive stretches again; a cluster walks its channels' whole time axis, carrying the state
+//            in a register.  Blocks send each other their folds by asynchronous stores that count on the receiver's
+//            mbarrier: a cluster-wide barrier would wait for the results' stores to global memory too, every round
+// The next round's loads are issued before this one is folded.
 // The gates' pre-activations are the inputs: a gate of 0.999 rounded to bf16 is 1 and would never forget.
 #include "types16.cuh"
 #include <cooperative_groups.h>
@@ -24,8 +26,9 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int STEPS = 8;       // of a thread
-constexpr int MAX_WARPS = 16;  // of a block
+constexpr int MAX_WARPS = 8;   // of a block
 constexpr int MAX_CLUSTER = 8;
+constexpr int KERNEL_ID = 0x71; // in the status word: (KERNEL_ID << 8) | site
 
 struct RecurrenceParams {
 	const void *z, *f, *i;          // update, forget, input (null: coupled)
@@ -37,6 +40,7 @@ struct RecurrenceParams {
 	const int* lengths;             // null: all `length`
 	long long zBatch, zRow, fBatch, fRow, iBatch, iRow, dhBatch, dhRow; // elements between sequences and steps
 	int length, channels;
+	int* status;
 };
 
 struct Gate {
@@ -80,17 +84,54 @@ struct Fold {
 // What a block's threads share: their folds, and those of the cluster's blocks (two sets, for alternating rounds).
 template<int W>
 struct Shared {
-	Fold<W> warps[MAX_WARPS][32];
+	Fold<W> warps[2][MAX_WARPS][32];
 	Fold<W> blocks[2][MAX_CLUSTER][32];
+	uint64_t arrived[2];
+	int abortFlag;
 };
+
+// Stores a fold in the shared memory of block `rank` of the cluster and counts its bytes on that block's barrier.
+__device__ __forceinline__ void send(const Fold<1>& f, Fold<1>* at, uint64_t* bar, int rank)
+{
+	asm volatile("{\n\t.reg .b32 a, m;\n\t"
+		"mapa.shared::cluster.u32 a, %0, %2;\n\t"
+		"mapa.shared::cluster.u32 m, %1, %2;\n\t"
+		"st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.b32 [a], {%3, %4}, [m];\n\t}"
+		::"r"(smem_u32(at)), "r"(smem_u32(bar)), "r"(rank), "r"(__float_as_uint(f.a[0])), "r"(__float_as_uint(f.h[0])) : "memory");
+}
+__device__ __forceinline__ void send(const Fold<2>& f, Fold<2>* at, uint64_t* bar, int rank)
+{
+	asm volatile("{\n\t.reg .b32 a, m;\n\t"
+		"mapa.shared::cluster.u32 a, %0, %2;\n\t"
+		"mapa.shared::cluster.u32 m, %1, %2;\n\t"
+		"st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [a], {%3, %4, %5, %6}, [m];\n\t}"
+		::"r"(smem_u32(at)), "r"(smem_u32(bar)), "r"(rank), "r"(__float_as_uint(f.a[0])), "r"(__float_as_uint(f.a[1])),
+		  "r"(__float_as_uint(f.h[0])), "r"(__float_as_uint(f.h[1])) : "memory");
+}
+
+template<int W>
+__device__ __forceinline__ void begin_sharing(Shared<W>& s, int blocks)
+{
+	if(blocks == 1) return;
+	if(threadIdx.x == 0) {
+		mbar_init(s.arrived, 1);
+		mbar_init(s.arrived + 1, 1);
+		mbar_init_fence();
+		s.abortFlag = 0;
+	}
+	cg::this_cluster().sync(); // the others' shared memory and barriers exist from here on
+}
 
 // Joins the folds of a round: `mine` is this thread's stretch; the state before it is returned in `state`, and `carry` moves on by
 // the whole round.  Stretches follow one another warp by warp, block by block.
+//   A set of folds is written again two rounds later.  Within the block, the barrier of the round between keeps the writers
+// behind the readers.  Between blocks: a block sends its folds of a round after its own barrier, when all its warps have read
+// the set of the round before, and nobody sends the round after next without having received those.
 template<int W>
-__device__ __forceinline__ void join(Shared<W>& s, const Fold<W>& mine, int round, int rank, int blocks, int warps, float* carry,
-	float* state)
+__device__ __forceinline__ void join(Shared<W>& s, const Fold<W>& mine, int round, int rank, int blocks, int warps, int* status,
+	float* carry, float* state)
 {
-	const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+	const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, set = round & 1;
 	Fold<W> before, all;
 #pragma unroll
 	for(int w = 0; w < W; ++w) {
@@ -99,12 +140,14 @@ __device__ __forceinline__ void join(Shared<W>& s, const Fold<W>& mine, int roun
 	}
 	all = mine;
 	if(warps > 1) {
-		s.warps[warp][lane] = mine;
+		s.warps[set][warp][lane] = mine;
 		__syncthreads();
 		Fold<W> run = before;
-		for(int k = 0; k < warps; ++k) {
+#pragma unroll
+		for(int k = 0; k < MAX_WARPS; ++k) {
+			if(k >= warps) break;
 			if(k == warp) before = run;
-			const Fold<W> next = s.warps[k][lane];
+			const Fold<W> next = s.warps[set][k][lane];
 #pragma unroll
 			for(int w = 0; w < W; ++w) {
 				run.h[w] = fmaf(next.a[w], run.h[w], next.h[w]);
@@ -114,28 +157,25 @@ __device__ __forceinline__ void join(Shared<W>& s, const Fold<W>& mine, int roun
 		all = run;
 	}
 	float start[W];
-	if(blocks > 1) {
-		cg::cluster_group cluster = cg::this_cluster();
-		for(int k = warp; k < blocks; k += warps) cluster.map_shared_rank(&s, k)->blocks[round & 1][rank][lane] = all;
-		cluster.sync(); // the other set of the next round is free again: everybody has read it before this barrier
 #pragma unroll
-		for(int w = 0; w < W; ++w) start[w] = carry[w];
+	for(int w = 0; w < W; ++w) start[w] = carry[w];
+	if(blocks > 1) {
+		if(threadIdx.x == 0) mbar_arrive_expect_tx(s.arrived + set, static_cast<uint32_t>(blocks * 32 * sizeof(Fold<W>)));
+		for(int k = warp; k < blocks; k += warps) send(all, &s.blocks[set][rank][lane], s.arrived + set, k);
+		// should the wait give up, the rounds go on with what is there: every block has to reach the end
+		mbar_wait_bounded_warp(s.arrived + set, (round >> 1) & 1, &s.abortFlag, status, (KERNEL_ID << 8) | 1);
 		for(int k = 0; k < blocks; ++k) {
 			if(k == rank) {
 #pragma unroll
 				for(int w = 0; w < W; ++w) start[w] = carry[w];
 			}
-			const Fold<W> next = s.blocks[round & 1][k][lane];
+			const Fold<W> next = s.blocks[set][k][lane];
 #pragma unroll
 			for(int w = 0; w < W; ++w) carry[w] = fmaf(next.a[w], carry[w], next.h[w]);
 		}
 	} else {
 #pragma unroll
-		for(int w = 0; w < W; ++w) {
-			start[w] = carry[w];
-			carry[w] = fmaf(all.a[w], carry[w], all.h[w]);
-		}
-		if(warps > 1) __syncthreads(); // the folds have been read
+		for(int w = 0; w < W; ++w) carry[w] = fmaf(all.a[w], carry[w], all.h[w]);
 	}
 #pragma unroll
 	for(int w = 0; w < W; ++w) state[w] = fmaf(before.a[w], start[w], before.h[w]);
@@ -149,12 +189,12 @@ __device__ __forceinline__ int sequence_length(const RecurrenceParams& p, int b)
 }
 
 template<typename T, int W, bool INPUT>
-__global__ void __launch_bounds__(MAX_WARPS * 32) recurrence_forward_kernel(const RecurrenceParams p)
+__global__ void __launch_bounds__(MAX_WARPS * 32, 3) recurrence_forward_kernel(const RecurrenceParams p)
 {
 	__shared__ Shared<W> s;
 	const int blocks = gridDim.y, rank = blockIdx.y; // the blocks of a cluster
 	const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5;
-	if(blocks > 1) cg::this_cluster().sync(); // the others' shared memory exists from here on
+	begin_sharing<W>(s, blocks);
 	const int b = blockIdx.z;
 	const int c = (blockIdx.x * 32 + (threadIdx.x & 31)) * W;
 	const bool on = c < p.channels;
@@ -168,24 +208,34 @@ __global__ void __launch_bounds__(MAX_WARPS * 32) recurrence_forward_kernel(cons
 #pragma unroll
 	for(int w = 0; w < W; ++w) carry[w] = on && p.first != nullptr ? p.first[state0 + w] : 0.f;
 	const int span = warps * STEPS, stride = span * blocks;
-	int round = 0;
-	for(int t0 = 0; t0 < p.length; t0 += stride, ++round) {
-		const int t = t0 + rank * span + warp * STEPS;
-		if(t0 >= n) { // behind the sequence (the whole cluster agrees): its results are zeros
-#pragma unroll
-			for(int k = 0; k < STEPS; ++k) {
-				if(on && t + k < p.length) store_raw<T, W>(out + static_cast<long long>(t + k) * p.channels, 0.f, 0.f);
-			}
-			continue;
-		}
-		uint32_t rz[STEPS], rf[STEPS], ri[STEPS];
+	uint32_t nz[STEPS], nf[STEPS], ni[STEPS];
+	auto load = [&](int t) {
+		const T *az = z + t * p.zRow, *af = f + t * p.fRow, *ai = INPUT ? i + t * p.iRow : nullptr;
 #pragma unroll
 		for(int k = 0; k < STEPS; ++k) {
 			const bool in = on && t + k < n;
-			rz[k] = in ? load_raw<T, W>(z + (t + k) * p.zRow) : 0u;
-			rf[k] = in ? load_raw<T, W>(f + (t + k) * p.fRow) : 0u;
-			if constexpr(INPUT) ri[k] = in ? load_raw<T, W>(i + (t + k) * p.iRow) : 0u;
+			nz[k] = in ? load_raw<T, W>(az) : 0u;
+			nf[k] = in ? load_raw<T, W>(af) : 0u;
+			az += p.zRow;
+			af += p.fRow;
+			if constexpr(INPUT) {
+				ni[k] = in ? load_raw<T, W>(ai) : 0u;
+				ai += p.iRow;
+			}
 		}
+	};
+	int round = 0, t = rank * span + warp * STEPS;
+	load(t);
+	// the whole cluster agrees on n, and on the number of rounds
+	for(; round * stride < n; ++round, t += stride) {
+		uint32_t rz[STEPS], rf[STEPS], ri[STEPS];
+#pragma unroll
+		for(int k = 0; k < STEPS; ++k) {
+			rz[k] = nz[k];
+			rf[k] = nf[k];
+			if constexpr(INPUT) ri[k] = ni[k];
+		}
+		load(t + stride);
 		float a[STEPS][W], h[STEPS][W];
 		Fold<W> mine;
 #pragma unroll
@@ -210,16 +260,19 @@ __global__ void __launch_bounds__(MAX_WARPS * 32) recurrence_forward_kernel(cons
 			}
 		}
 		float state[W];
-		join<W>(s, mine, round, rank, blocks, warps, carry, state);
+		join<W>(s, mine, round, rank, blocks, warps, p.status, carry, state);
+		T* to = out + static_cast<long long>(t) * p.channels;
 #pragma unroll
 		for(int k = 0; k < STEPS; ++k) {
 #pragma unroll
 			for(int w = 0; w < W; ++w) state[w] = fmaf(a[k][w], state[w], h[k][w]);
-			if(on && t + k < p.length) {
-				const bool in = t + k < n;
-				store_raw<T, W>(out + static_cast<long long>(t + k) * p.channels, in ? state[0] : 0.f, in ? state[W - 1] : 0.f);
-			}
+			if(on && t + k < n) store_raw<T, W>(to, state[0], state[W - 1]);
+			to += p.channels;
 		}
+	}
+	// behind the sequence the results are zeros
+	for(int k = n + rank * warps + warp; k < p.length; k += blocks * warps) {
+		if(on) store_raw<T, W>(out + static_cast<long long>(k) * p.channels, 0.f, 0.f);
 	}
 	if(on && p.last != nullptr && rank == 0 && warp == 0) {
 #pragma unroll
@@ -230,12 +283,12 @@ __global__ void __launch_bounds__(MAX_WARPS * 32) recurrence_forward_kernel(cons
 
 // Time runs backwards: step k of a stretch is t - k.
 template<typename T, int W, bool INPUT>
-__global__ void __launch_bounds__(MAX_WARPS * 32) recurrence_backward_kernel(const RecurrenceParams p)
+__global__ void __launch_bounds__(MAX_WARPS * 32, 2) recurrence_backward_kernel(const RecurrenceParams p)
 {
 	__shared__ Shared<W> s;
 	const int blocks = gridDim.y, rank = blockIdx.y;
 	const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5;
-	if(blocks > 1) cg::this_cluster().sync(); // the others' shared memory exists from here on
+	begin_sharing<W>(s, blocks);
 	const int b = blockIdx.z;
 	const int c = (blockIdx.x * 32 + (threadIdx.x & 31)) * W;
 	const bool on = c < p.channels;
@@ -265,19 +318,40 @@ __global__ void __launch_bounds__(MAX_WARPS * 32) recurrence_backward_kernel(con
 		if constexpr(INPUT) store_raw<T, W>(di + at, 0.f, 0.f);
 	}
 	const int span = warps * STEPS, stride = span * blocks;
-	int round = 0;
-	for(int done = 0; done < n; done += stride, ++round) {
-		const int t = n - 1 - done - rank * span - warp * STEPS;
-		uint32_t rz[STEPS], rf[STEPS], ri[STEPS], rd[STEPS], rh[STEPS];
+	uint32_t nz[STEPS], nf[STEPS], ni[STEPS], nd[STEPS], nh[STEPS];
+	auto load = [&](int t) {
+		const T *az = z + t * p.zRow, *af = f + t * p.fRow, *ai = INPUT ? i + t * p.iRow : nullptr, *ad = dh + t * p.dhRow;
+		const T* ah = h + static_cast<long long>(t - 1) * p.channels;
 #pragma unroll
 		for(int k = 0; k < STEPS; ++k) {
 			const bool in = on && t - k >= 0;
-			rf[k] = in ? load_raw<T, W>(f + (t - k) * p.fRow) : 0u;
-			rd[k] = in ? load_raw<T, W>(dh + (t - k) * p.dhRow) : 0u;
-			rz[k] = in ? load_raw<T, W>(z + (t - k) * p.zRow) : 0u;
-			rh[k] = in && t - k > 0 ? load_raw<T, W>(h + static_cast<long long>(t - k - 1) * p.channels) : 0u;
-			if constexpr(INPUT) ri[k] = in ? load_raw<T, W>(i + (t - k) * p.iRow) : 0u;
+			nf[k] = in ? load_raw<T, W>(af) : 0u;
+			nd[k] = in ? load_raw<T, W>(ad) : 0u;
+			nz[k] = in ? load_raw<T, W>(az) : 0u;
+			nh[k] = in && t - k > 0 ? load_raw<T, W>(ah) : 0u;
+			af -= p.fRow;
+			ad -= p.dhRow;
+			az -= p.zRow;
+			ah -= p.channels;
+			if constexpr(INPUT) {
+				ni[k] = in ? load_raw<T, W>(ai) : 0u;
+				ai -= p.iRow;
+			}
 		}
+	};
+	int round = 0, t = n - 1 - rank * span - warp * STEPS;
+	load(t);
+	for(; round * stride < n; ++round, t -= stride) {
+		uint32_t rz[STEPS], rf[STEPS], ri[STEPS], rd[STEPS], rh[STEPS];
+#pragma unroll
+		for(int k = 0; k < STEPS; ++k) {
+			rz[k] = nz[k];
+			rf[k] = nf[k];
+			rd[k] = nd[k];
+			rh[k] = nh[k];
+			if constexpr(INPUT) ri[k] = ni[k];
+		}
+		load(t - stride);
 		float a[STEPS][W], u[STEPS][W];
 		Fold<W> mine;
 #pragma unroll
@@ -301,7 +375,8 @@ __global__ void __launch_bounds__(MAX_WARPS * 32) recurrence_backward_kernel(con
 			}
 		}
 		float state[W];
-		join<W>(s, mine, round, rank, blocks, warps, carry, state);
+		join<W>(s, mine, round, rank, blocks, warps, p.status, carry, state);
+		long long to = static_cast<long long>(t) * p.channels;
 #pragma unroll
 		for(int k = 0; k < STEPS; ++k) {
 			const float2 vd = floats<T, W>(rd[k]), vz = floats<T, W>(rz[k]);
@@ -324,8 +399,9 @@ __global__ void __launch_bounds__(MAX_WARPS * 32) recurrence_backward_kernel(con
 				}
 				state[w] = a[k][w] * S;
 			}
+			const long long at = to;
+			to -= p.channels;
 			if(on && t - k >= 0) {
-				const long long at = static_cast<long long>(t - k) * p.channels;
 				store_raw<T, W>(dz + at, oz[0], oz[W - 1]);
 				store_raw<T, W>(df + at, of[0], of[W - 1]);
 				if constexpr(INPUT) store_raw<T, W>(di + at, oi[0], oi[W - 1]);
@@ -354,21 +430,31 @@ Kernel kernel_of(int pair, bool input)
 	return input ? recurrence_forward_kernel<T, 1, true> : recurrence_forward_kernel<T, 1, false>;
 }
 
-// Warps for the time axis first, then blocks of a cluster, until the device has about two thousand threads on every SM.
-int launch(int type, bool pair, bool backward, const RecurrenceParams& p, int batch, cudaStream_t stream)
+// Warps for the time axis first, then blocks of a cluster: as many as give the fewest rounds, one after another, of the blocks
+// that the device holds at a time (by the kernels' registers).
+int launch(int type, bool pair, bool backward, RecurrenceParams p, int batch, cudaStream_t stream)
 {
 	const bool input = p.i != nullptr;
 	const Kernel kernel = type == NB200_TYPE_FP32 ? (backward ? kernel_of<float, true>(pair, input) : kernel_of<float, false>(pair, input))
 		: type == NB200_TYPE_FP16 ? (backward ? kernel_of<__half, true>(pair, input) : kernel_of<__half, false>(pair, input))
 		: (backward ? kernel_of<__nv_bfloat16, true>(pair, input) : kernel_of<__nv_bfloat16, false>(pair, input));
+	p.status = device_status_word();
 	const int perWarp = pair ? 64 : 32;
 	const int tiles = (p.channels + perWarp - 1) / perWarp;
 	const int stretches = (p.length + STEPS - 1) / STEPS;
 	const long long groups = static_cast<long long>(tiles) * batch;
 	int warps = 1;
 	while(warps < MAX_WARPS && warps < stretches) warps *= 2;
+	const long long held = static_cast<long long>(sm_count()) * (backward ? 2 : 3) * (MAX_WARPS / warps);
 	int blocks = 1;
-	while(blocks < MAX_CLUSTER && blocks * warps < stretches && groups * blocks < sm_count() * 2) blocks *= 2;
+	long long least = 0;
+	for(int n = 1; n <= MAX_CLUSTER && (n == 1 || n / 2 * warps < stretches); n *= 2) {
+		const long long rounds = (groups * n + held - 1) / held * ((stretches + n * warps - 1) / (n * warps));
+		if(n == 1 || rounds < least) {
+			least = rounds;
+			blocks = n;
+		}
+	}
 	cudaLaunchConfig_t config = {};
 	config.blockDim = dim3(warps * 32);
 	config.gridDim = dim3(tiles, blocks, batch);
