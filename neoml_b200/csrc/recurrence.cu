@@ -47,12 +47,28 @@ struct Gate {
 	float keep, take; // sigmoid(x), 1 - sigmoid(x)
 };
 
-// Both without cancellation; exp never overflows.
+__device__ __forceinline__ float exp2_fast(float x)
+{
+	float y;
+	asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+	return y;
+}
+__device__ __forceinline__ float inverse_fast(float x)
+{
+	float y;
+	asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+	return y;
+}
+// Both without cancellation; the exponential never overflows.
 __device__ __forceinline__ Gate gate(float x)
 {
-	const float e = __expf(-fabsf(x));
-	const float large = __fdividef(1.f, 1.f + e), small = e * large;
+	const float e = exp2_fast(fabsf(x) * -1.4426950408889634f);
+	const float large = inverse_fast(1.f + e), small = e * large;
 	return x >= 0.f ? Gate{ large, small } : Gate{ small, large };
+}
+__device__ __forceinline__ float sigmoid(float x)
+{
+	return inverse_fast(1.f + exp2_fast(x * -1.4426950408889634f)); // of infinity: zero
 }
 
 // W channels of one step as they lie in memory: one register
@@ -112,70 +128,67 @@ __device__ __forceinline__ void send(const Fold<2>& f, Fold<2>* at, uint64_t* ba
 template<int W>
 __device__ __forceinline__ void begin_sharing(Shared<W>& s, int blocks)
 {
-	if(blocks == 1) return;
 	if(threadIdx.x == 0) {
 		mbar_init(s.arrived, 1);
 		mbar_init(s.arrived + 1, 1);
 		mbar_init_fence();
 		s.abortFlag = 0;
 	}
-	cg::this_cluster().sync(); // the others' shared memory and barriers exist from here on
+	if(blocks > 1) cg::this_cluster().sync(); // the others' shared memory and barriers exist from here on
+	else __syncthreads();
 }
 
 // Joins the folds of a round: `mine` is this thread's stretch; the state before it is returned in `state`, and `carry` moves on by
 // the whole round.  Stretches follow one another warp by warp, block by block.
 //   A set of folds is written again two rounds later.  Within the block, the barrier of the round between keeps the writers
-// behind the readers.  Between blocks: a block sends its folds of a round after its own barrier, when all its warps have read
-// the set of the round before, and nobody sends the round after next without having received those.
+// behind the readers.  Between blocks: a block sends its fold of a round after its own barrier, when all its warps have read
+// the set of the round before, and nobody sends the round after next without having received that fold.
 template<int W>
 __device__ __forceinline__ void join(Shared<W>& s, const Fold<W>& mine, int round, int rank, int blocks, int warps, int* status,
 	float* carry, float* state)
 {
 	const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, set = round & 1;
-	Fold<W> before, all;
+	Fold<W> before;
 #pragma unroll
 	for(int w = 0; w < W; ++w) {
 		before.a[w] = 1.f;
 		before.h[w] = 0.f;
 	}
-	all = mine;
+	auto after = [](Fold<W>& f, const Fold<W>& next) {
+#pragma unroll
+		for(int w = 0; w < W; ++w) {
+			f.h[w] = fmaf(next.a[w], f.h[w], next.h[w]);
+			f.a[w] *= next.a[w];
+		}
+	};
 	if(warps > 1) {
-		s.warps[set][warp][lane] = mine;
+		if(warp < warps - 1) s.warps[set][warp][lane] = mine;
 		__syncthreads();
-		Fold<W> run = before;
-#pragma unroll
-		for(int k = 0; k < MAX_WARPS; ++k) {
-			if(k >= warps) break;
-			if(k == warp) before = run;
-			const Fold<W> next = s.warps[set][k][lane];
-#pragma unroll
-			for(int w = 0; w < W; ++w) {
-				run.h[w] = fmaf(next.a[w], run.h[w], next.h[w]);
-				run.a[w] *= next.a[w];
-			}
-		}
-		all = run;
+		for(int k = 0; k < warp; ++k) after(before, s.warps[set][k][lane]);
 	}
-	float start[W];
-#pragma unroll
-	for(int w = 0; w < W; ++w) start[w] = carry[w];
-	if(blocks > 1) {
-		if(threadIdx.x == 0) mbar_arrive_expect_tx(s.arrived + set, static_cast<uint32_t>(blocks * 32 * sizeof(Fold<W>)));
-		for(int k = warp; k < blocks; k += warps) send(all, &s.blocks[set][rank][lane], s.arrived + set, k);
-		// should the wait give up, the rounds go on with what is there: every block has to reach the end
-		mbar_wait_bounded_warp(s.arrived + set, (round >> 1) & 1, &s.abortFlag, status, (KERNEL_ID << 8) | 1);
-		for(int k = 0; k < blocks; ++k) {
-			if(k == rank) {
-#pragma unroll
-				for(int w = 0; w < W; ++w) start[w] = carry[w];
-			}
-			const Fold<W> next = s.blocks[set][k][lane];
-#pragma unroll
-			for(int w = 0; w < W; ++w) carry[w] = fmaf(next.a[w], carry[w], next.h[w]);
+	if(warp == warps - 1) { // the block's fold, to every block of the cluster, this one too
+		Fold<W> all = before;
+		after(all, mine);
+		if(blocks == 1) { // launched without a cluster: st.async is not an instruction of such a kernel
+			s.blocks[set][0][lane] = all;
+			__syncwarp();
+			if(lane == 0) mbar_arrive(s.arrived + set);
+		} else {
+			if(lane == 0) mbar_arrive_expect_tx(s.arrived + set, static_cast<uint32_t>(blocks * 32 * sizeof(Fold<W>)));
+			for(int k = 0; k < blocks; ++k) send(all, &s.blocks[set][rank][lane], s.arrived + set, k);
 		}
-	} else {
+	}
+	// should the wait give up, the rounds go on with what is there: every block has to reach the end
+	mbar_wait_bounded_warp(s.arrived + set, (round >> 1) & 1, &s.abortFlag, status, (KERNEL_ID << 8) | 1);
+	float start[W];
+	for(int k = 0; k < blocks; ++k) {
+		if(k == rank) {
 #pragma unroll
-		for(int w = 0; w < W; ++w) carry[w] = fmaf(all.a[w], carry[w], all.h[w]);
+			for(int w = 0; w < W; ++w) start[w] = carry[w];
+		}
+		const Fold<W> next = s.blocks[set][k][lane];
+#pragma unroll
+		for(int w = 0; w < W; ++w) carry[w] = fmaf(next.a[w], carry[w], next.h[w]);
 	}
 #pragma unroll
 	for(int w = 0; w < W; ++w) state[w] = fmaf(before.a[w], start[w], before.h[w]);
@@ -188,54 +201,65 @@ __device__ __forceinline__ int sequence_length(const RecurrenceParams& p, int b)
 	return n < 0 ? 0 : n > p.length ? p.length : n;
 }
 
-template<typename T, int W, bool INPUT>
-__global__ void __launch_bounds__(MAX_WARPS * 32, 3) recurrence_forward_kernel(const RecurrenceParams p)
+// Where a block's part of a round lies in an operand.  DENSE operands (channels adjacent, steps `channels` apart) share one 32-bit
+// offset per step, the same in every round, on a base that is uniform in the block: no address arithmetic per load.
+template<typename T, bool DENSE>
+struct Operand {
+	const uint8_t* base; // step 0 of this block's sequence; DENSE: of the round
+	long long row;       // bytes between steps
+	__device__ __forceinline__ const T* at(uint32_t offset, int t, int c) const
+	{
+		return DENSE ? reinterpret_cast<const T*>(base + offset) : reinterpret_cast<const T*>(base + t * row) + c;
+	}
+};
+
+// Runs f(integral constant) as true where every step of the thread's stretch exists, without a test per step.
+struct Yes { static constexpr bool value = true; };
+struct No { static constexpr bool value = false; };
+
+template<typename T, int W, bool INPUT, bool DENSE>
+__global__ void __launch_bounds__(MAX_WARPS * 32, W == 1 ? 3 : 2) recurrence_forward_kernel(const RecurrenceParams p)
 {
 	__shared__ Shared<W> s;
 	const int blocks = gridDim.y, rank = blockIdx.y; // the blocks of a cluster
 	const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5;
 	begin_sharing<W>(s, blocks);
 	const int b = blockIdx.z;
-	const int c = (blockIdx.x * 32 + (threadIdx.x & 31)) * W;
-	const bool on = c < p.channels;
+	const int own = (blockIdx.x * 32 + (threadIdx.x & 31)) * W;
+	const bool on = own < p.channels;
+	const int c = on ? own : p.channels - W; // lanes behind the last channel read what others read, and write nothing
 	const int n = sequence_length(p, b);
-	const T* const z = static_cast<const T*>(p.z) + b * p.zBatch + c;
-	const T* const f = static_cast<const T*>(p.f) + b * p.fBatch + c;
-	const T* const i = INPUT ? static_cast<const T*>(p.i) + b * p.iBatch + c : nullptr;
-	T* const out = static_cast<T*>(p.out) + static_cast<long long>(b) * p.length * p.channels + c;
+	const int span = warps * STEPS, stride = span * blocks;
+	const int first = rank * span + warp * STEPS;
+	Operand<T, DENSE> z = { static_cast<const uint8_t*>(p.z) + b * p.zBatch * sizeof(T), p.zRow * static_cast<long long>(sizeof(T)) };
+	Operand<T, DENSE> f = { static_cast<const uint8_t*>(p.f) + b * p.fBatch * sizeof(T), p.fRow * static_cast<long long>(sizeof(T)) };
+	Operand<T, DENSE> i = { static_cast<const uint8_t*>(p.i) + b * p.iBatch * sizeof(T), p.iRow * static_cast<long long>(sizeof(T)) };
+	T* const out = static_cast<T*>(p.out) + static_cast<long long>(b) * p.length * p.channels;
+	uint8_t* outRound = reinterpret_cast<uint8_t*>(out);
+	const long long roundBytes = static_cast<long long>(stride) * p.channels * sizeof(T);
+	uint32_t offset[STEPS];
+#pragma unroll
+	for(int k = 0; k < STEPS; ++k) offset[k] = (static_cast<uint32_t>(first + k) * p.channels + c) * static_cast<uint32_t>(sizeof(T));
 	const long long state0 = static_cast<long long>(b) * p.channels + c;
 	float carry[W];
 #pragma unroll
-	for(int w = 0; w < W; ++w) carry[w] = on && p.first != nullptr ? p.first[state0 + w] : 0.f;
-	const int span = warps * STEPS, stride = span * blocks;
-	uint32_t nz[STEPS], nf[STEPS], ni[STEPS];
-	auto load = [&](int t) {
-		const T *az = z + t * p.zRow, *af = f + t * p.fRow, *ai = INPUT ? i + t * p.iRow : nullptr;
+	for(int w = 0; w < W; ++w) carry[w] = p.first != nullptr ? p.first[state0 + w] : 0.f;
+
+	uint32_t rz[STEPS], rf[STEPS], ri[STEPS];
+	auto load = [&](int t, auto full) {
 #pragma unroll
 		for(int k = 0; k < STEPS; ++k) {
-			const bool in = on && t + k < n;
-			nz[k] = in ? load_raw<T, W>(az) : 0u;
-			nf[k] = in ? load_raw<T, W>(af) : 0u;
-			az += p.zRow;
-			af += p.fRow;
-			if constexpr(INPUT) {
-				ni[k] = in ? load_raw<T, W>(ai) : 0u;
-				ai += p.iRow;
-			}
+			const bool in = decltype(full)::value || t + k < n;
+			rz[k] = in ? load_raw<T, W>(z.at(offset[k], t + k, c)) : 0u;
+			rf[k] = in ? load_raw<T, W>(f.at(offset[k], t + k, c)) : 0u;
+			if constexpr(INPUT) ri[k] = in ? load_raw<T, W>(i.at(offset[k], t + k, c)) : 0u;
 		}
 	};
-	int round = 0, t = rank * span + warp * STEPS;
-	load(t);
+	int round = 0, t = first;
+	if(t + STEPS <= n) load(t, Yes());
+	else load(t, No());
 	// the whole cluster agrees on n, and on the number of rounds
-	for(; round * stride < n; ++round, t += stride) {
-		uint32_t rz[STEPS], rf[STEPS], ri[STEPS];
-#pragma unroll
-		for(int k = 0; k < STEPS; ++k) {
-			rz[k] = nz[k];
-			rf[k] = nf[k];
-			if constexpr(INPUT) ri[k] = ni[k];
-		}
-		load(t + stride);
+	for(; round * stride < n; ++round) {
 		float a[STEPS][W], h[STEPS][W];
 		Fold<W> mine;
 #pragma unroll
@@ -243,36 +267,53 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 3) recurrence_forward_kernel(c
 			mine.a[w] = 1.f;
 			mine.h[w] = 0.f;
 		}
+		auto fold = [&](auto full) {
 #pragma unroll
-		for(int k = 0; k < STEPS; ++k) {
-			const float2 vz = floats<T, W>(rz[k]), vf = floats<T, W>(rf[k]);
-			float2 vi = make_float2(0.f, 0.f);
-			if constexpr(INPUT) vi = floats<T, W>(ri[k]);
-			const bool in = t + k < n;
+			for(int k = 0; k < STEPS; ++k) {
+				const float2 vz = floats<T, W>(rz[k]), vf = floats<T, W>(rf[k]);
+				float2 vi = make_float2(0.f, 0.f);
+				if constexpr(INPUT) vi = floats<T, W>(ri[k]);
+				const bool in = decltype(full)::value || t + k < n;
 #pragma unroll
-			for(int w = 0; w < W; ++w) {
-				const Gate forget = gate(w == 0 ? vf.x : vf.y);
-				const float take = INPUT ? gate(w == 0 ? vi.x : vi.y).keep : forget.take;
-				a[k][w] = in ? forget.keep : 1.f;
-				h[k][w] = in ? take * (w == 0 ? vz.x : vz.y) : 0.f;
-				mine.h[w] = fmaf(a[k][w], mine.h[w], h[k][w]);
-				mine.a[w] *= a[k][w];
+				for(int w = 0; w < W; ++w) {
+					const Gate forget = gate(w == 0 ? vf.x : vf.y);
+					const float take = INPUT ? sigmoid(w == 0 ? vi.x : vi.y) : forget.take;
+					a[k][w] = in ? forget.keep : 1.f;
+					h[k][w] = in ? take * (w == 0 ? vz.x : vz.y) : 0.f;
+					mine.h[w] = fmaf(a[k][w], mine.h[w], h[k][w]);
+					mine.a[w] *= a[k][w];
+				}
 			}
+		};
+		const bool whole = t + STEPS <= n;
+		if(whole) fold(Yes());
+		else fold(No());
+		if constexpr(DENSE) {
+			z.base += roundBytes;
+			f.base += roundBytes;
+			if constexpr(INPUT) i.base += roundBytes;
 		}
+		if(t + stride + STEPS <= n) load(t + stride, Yes());
+		else load(t + stride, No());
 		float state[W];
 		join<W>(s, mine, round, rank, blocks, warps, p.status, carry, state);
-		T* to = out + static_cast<long long>(t) * p.channels;
+		auto apply = [&](auto full) {
 #pragma unroll
-		for(int k = 0; k < STEPS; ++k) {
+			for(int k = 0; k < STEPS; ++k) {
 #pragma unroll
-			for(int w = 0; w < W; ++w) state[w] = fmaf(a[k][w], state[w], h[k][w]);
-			if(on && t + k < n) store_raw<T, W>(to, state[0], state[W - 1]);
-			to += p.channels;
-		}
+				for(int w = 0; w < W; ++w) state[w] = fmaf(a[k][w], state[w], h[k][w]);
+				T* const to = DENSE ? reinterpret_cast<T*>(outRound + offset[k]) : out + static_cast<long long>(t + k) * p.channels + c;
+				if(on && (decltype(full)::value || t + k < n)) store_raw<T, W>(to, state[0], state[W - 1]);
+			}
+		};
+		if(whole) apply(Yes());
+		else apply(No());
+		outRound += roundBytes;
+		t += stride;
 	}
 	// behind the sequence the results are zeros
 	for(int k = n + rank * warps + warp; k < p.length; k += blocks * warps) {
-		if(on) store_raw<T, W>(out + static_cast<long long>(k) * p.channels, 0.f, 0.f);
+		if(on) store_raw<T, W>(out + static_cast<long long>(k) * p.channels + c, 0.f, 0.f);
 	}
 	if(on && p.last != nullptr && rank == 0 && warp == 0) {
 #pragma unroll
@@ -282,7 +323,7 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 3) recurrence_forward_kernel(c
 }
 
 // Time runs backwards: step k of a stretch is t - k.
-template<typename T, int W, bool INPUT>
+template<typename T, int W, bool INPUT, bool DENSE>
 __global__ void __launch_bounds__(MAX_WARPS * 32, 2) recurrence_backward_kernel(const RecurrenceParams p)
 {
 	__shared__ Shared<W> s;
@@ -290,68 +331,73 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 2) recurrence_backward_kernel(
 	const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5;
 	begin_sharing<W>(s, blocks);
 	const int b = blockIdx.z;
-	const int c = (blockIdx.x * 32 + (threadIdx.x & 31)) * W;
-	const bool on = c < p.channels;
+	const int own = (blockIdx.x * 32 + (threadIdx.x & 31)) * W;
+	const bool on = own < p.channels;
+	const int c = on ? own : p.channels - W;
 	const int n = sequence_length(p, b);
-	const long long own = static_cast<long long>(b) * p.length * p.channels + c;
-	const T* const z = static_cast<const T*>(p.z) + b * p.zBatch + c;
-	const T* const f = static_cast<const T*>(p.f) + b * p.fBatch + c;
-	const T* const i = INPUT ? static_cast<const T*>(p.i) + b * p.iBatch + c : nullptr;
-	const T* const dh = static_cast<const T*>(p.dh) + b * p.dhBatch + c;
-	const T* const h = static_cast<const T*>(p.h) + own;
-	T* const dz = static_cast<T*>(p.out) + own;
-	T* const df = static_cast<T*>(p.df) + own;
-	T* const di = INPUT ? static_cast<T*>(p.di) + own : nullptr;
+	const int span = warps * STEPS, stride = span * blocks;
+	const int back = rank * span + warp * STEPS; // steps between the round's last one and this thread's first
+	const long long roundBytes = static_cast<long long>(stride) * p.channels * sizeof(T);
+	const long long sequence = static_cast<long long>(b) * p.length * p.channels;
+	// DENSE: bases of the round, which ends behind step n - 1; nothing in front of step 0 is read
+	const long long begin = DENSE ? static_cast<long long>(n - stride) * p.channels * static_cast<long long>(sizeof(T)) : 0;
+	Operand<T, DENSE> z = { static_cast<const uint8_t*>(p.z) + b * p.zBatch * sizeof(T) + begin, p.zRow * static_cast<long long>(sizeof(T)) };
+	Operand<T, DENSE> f = { static_cast<const uint8_t*>(p.f) + b * p.fBatch * sizeof(T) + begin, p.fRow * static_cast<long long>(sizeof(T)) };
+	Operand<T, DENSE> i = { static_cast<const uint8_t*>(p.i) + b * p.iBatch * sizeof(T) + begin, p.iRow * static_cast<long long>(sizeof(T)) };
+	Operand<T, DENSE> dh = { static_cast<const uint8_t*>(p.dh) + b * p.dhBatch * sizeof(T) + begin, p.dhRow * static_cast<long long>(sizeof(T)) };
+	const long long denseRow = static_cast<long long>(p.channels) * sizeof(T);
+	Operand<T, DENSE> h = { static_cast<const uint8_t*>(p.h) + sequence * sizeof(T) + begin - denseRow, denseRow }; // the step before
+	T* const dz = static_cast<T*>(p.out) + sequence;
+	T* const df = static_cast<T*>(p.df) + sequence;
+	T* const di = INPUT ? static_cast<T*>(p.di) + sequence : nullptr;
+	long long outRound = begin;
+	uint32_t offset[STEPS];
+#pragma unroll
+	for(int k = 0; k < STEPS; ++k) offset[k] = (static_cast<uint32_t>(stride - 1 - back - k) * p.channels + c) * static_cast<uint32_t>(sizeof(T));
 	const long long state0 = static_cast<long long>(b) * p.channels + c;
 	float carry[W], first[W]; // carry: what step t + 1 hands back, a_{t+1} S_{t+1}
 #pragma unroll
 	for(int w = 0; w < W; ++w) {
-		carry[w] = on && p.lastDiff != nullptr ? p.lastDiff[state0 + w] : 0.f;
-		first[w] = on && p.first != nullptr ? p.first[state0 + w] : 0.f;
+		carry[w] = p.lastDiff != nullptr ? p.lastDiff[state0 + w] : 0.f;
+		first[w] = p.first != nullptr ? p.first[state0 + w] : 0.f;
 	}
 	// behind the sequence the gradients are zeros
-	for(int t = n + rank * warps + warp; t < p.length; t += blocks * warps) {
+	for(int k = n + rank * warps + warp; k < p.length; k += blocks * warps) {
+		const long long at = static_cast<long long>(k) * p.channels + c;
 		if(!on) break;
-		const long long at = static_cast<long long>(t) * p.channels;
 		store_raw<T, W>(dz + at, 0.f, 0.f);
 		store_raw<T, W>(df + at, 0.f, 0.f);
 		if constexpr(INPUT) store_raw<T, W>(di + at, 0.f, 0.f);
 	}
-	const int span = warps * STEPS, stride = span * blocks;
-	uint32_t nz[STEPS], nf[STEPS], ni[STEPS], nd[STEPS], nh[STEPS];
-	auto load = [&](int t) {
-		const T *az = z + t * p.zRow, *af = f + t * p.fRow, *ai = INPUT ? i + t * p.iRow : nullptr, *ad = dh + t * p.dhRow;
-		const T* ah = h + static_cast<long long>(t - 1) * p.channels;
+	// The gates and the gradients are wanted when a round begins, the rest only when its state has arrived: the former are
+	// loaded a whole round ahead, the latter while the round before them ends.
+	uint32_t rz[STEPS], rf[STEPS], ri[STEPS], rd[STEPS], nd[STEPS], rh[STEPS];
+	auto load_gates = [&](int t, auto full) {
 #pragma unroll
 		for(int k = 0; k < STEPS; ++k) {
-			const bool in = on && t - k >= 0;
-			nf[k] = in ? load_raw<T, W>(af) : 0u;
-			nd[k] = in ? load_raw<T, W>(ad) : 0u;
-			nz[k] = in ? load_raw<T, W>(az) : 0u;
-			nh[k] = in && t - k > 0 ? load_raw<T, W>(ah) : 0u;
-			af -= p.fRow;
-			ad -= p.dhRow;
-			az -= p.zRow;
-			ah -= p.channels;
-			if constexpr(INPUT) {
-				ni[k] = in ? load_raw<T, W>(ai) : 0u;
-				ai -= p.iRow;
-			}
+			const bool in = decltype(full)::value || t - k >= 0;
+			rf[k] = in ? load_raw<T, W>(f.at(offset[k], t - k, c)) : 0u;
+			nd[k] = in ? load_raw<T, W>(dh.at(offset[k], t - k, c)) : 0u;
 		}
 	};
-	int round = 0, t = n - 1 - rank * span - warp * STEPS;
-	load(t);
-	for(; round * stride < n; ++round, t -= stride) {
-		uint32_t rz[STEPS], rf[STEPS], ri[STEPS], rd[STEPS], rh[STEPS];
+	auto load_rest = [&](int t, auto full) {
 #pragma unroll
 		for(int k = 0; k < STEPS; ++k) {
-			rz[k] = nz[k];
-			rf[k] = nf[k];
-			rd[k] = nd[k];
-			rh[k] = nh[k];
-			if constexpr(INPUT) ri[k] = ni[k];
+			const bool in = decltype(full)::value || t - k >= 0;
+			rz[k] = in ? load_raw<T, W>(z.at(offset[k], t - k, c)) : 0u;
+			rh[k] = decltype(full)::value || t - k > 0 ? load_raw<T, W>(h.at(offset[k], t - k, c)) : 0u;
+			if constexpr(INPUT) ri[k] = in ? load_raw<T, W>(i.at(offset[k], t - k, c)) : 0u;
 		}
-		load(t - stride);
+	};
+	int round = 0, t = n - 1 - back;
+	if(t - STEPS >= 0) {
+		load_gates(t, Yes());
+		load_rest(t, Yes());
+	} else {
+		load_gates(t, No());
+		load_rest(t, No());
+	}
+	for(; round * stride < n; ++round) {
 		float a[STEPS][W], u[STEPS][W];
 		Fold<W> mine;
 #pragma unroll
@@ -359,54 +405,78 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 2) recurrence_backward_kernel(
 			mine.a[w] = 1.f;
 			mine.h[w] = 0.f;
 		}
+		auto fold = [&](auto full) {
 #pragma unroll
-		for(int k = 0; k < STEPS; ++k) {
-			const float2 vf = floats<T, W>(rf[k]), vd = floats<T, W>(rd[k]);
-			const bool in = t - k >= 0;
+			for(int k = 0; k < STEPS; ++k) {
+				rd[k] = nd[k];
+				const float2 vf = floats<T, W>(rf[k]), vd = floats<T, W>(rd[k]);
+				const bool in = decltype(full)::value || t - k >= 0;
 #pragma unroll
-			for(int w = 0; w < W; ++w) {
-				const Gate forget = gate(w == 0 ? vf.x : vf.y);
-				a[k][w] = in ? forget.keep : 1.f;
-				u[k][w] = forget.take;
-				const float d = w == 0 ? vd.x : vd.y;
-				// a (dh + s): this step's own part is a dh
-				mine.h[w] = a[k][w] * (mine.h[w] + d);
-				mine.a[w] *= a[k][w];
+				for(int w = 0; w < W; ++w) {
+					const Gate forget = gate(w == 0 ? vf.x : vf.y);
+					a[k][w] = in ? forget.keep : 1.f;
+					u[k][w] = forget.take;
+					// a (dh + s): this step's own part is a dh
+					mine.h[w] = a[k][w] * (mine.h[w] + (w == 0 ? vd.x : vd.y));
+					mine.a[w] *= a[k][w];
+				}
 			}
+		};
+		const bool whole = t - STEPS >= 0, nextWhole = t - stride - STEPS >= 0;
+		if(whole) fold(Yes());
+		else fold(No());
+		if constexpr(DENSE) {
+			f.base -= roundBytes;
+			dh.base -= roundBytes;
 		}
+		if(nextWhole) load_gates(t - stride, Yes());
+		else load_gates(t - stride, No());
 		float state[W];
 		join<W>(s, mine, round, rank, blocks, warps, p.status, carry, state);
-		long long to = static_cast<long long>(t) * p.channels;
+		auto apply = [&](auto full) {
 #pragma unroll
-		for(int k = 0; k < STEPS; ++k) {
-			const float2 vd = floats<T, W>(rd[k]), vz = floats<T, W>(rz[k]);
-			float2 vh = floats<T, W>(rh[k]), vi = make_float2(0.f, 0.f);
-			if(t - k == 0) vh = make_float2(first[0], first[W - 1]);
-			if constexpr(INPUT) vi = floats<T, W>(ri[k]);
-			float oz[W], of[W], oi[W];
+			for(int k = 0; k < STEPS; ++k) {
+				const float2 vd = floats<T, W>(rd[k]), vz = floats<T, W>(rz[k]);
+				float2 vh = floats<T, W>(rh[k]), vi = make_float2(0.f, 0.f);
+				if(!decltype(full)::value && t - k == 0) vh = make_float2(first[0], first[W - 1]);
+				if constexpr(INPUT) vi = floats<T, W>(ri[k]);
+				float oz[W], of[W], oi[W];
 #pragma unroll
-			for(int w = 0; w < W; ++w) {
-				const float S = state[w] + (w == 0 ? vd.x : vd.y), zz = w == 0 ? vz.x : vz.y, before = w == 0 ? vh.x : vh.y;
-				const float slope = a[k][w] * u[k][w];
-				if constexpr(INPUT) {
-					const Gate take = gate(w == 0 ? vi.x : vi.y);
-					oz[w] = S * take.keep;
-					of[w] = S * before * slope;
-					oi[w] = S * zz * (take.keep * take.take);
-				} else {
-					oz[w] = S * u[k][w];
-					of[w] = S * (before - zz) * slope;
+				for(int w = 0; w < W; ++w) {
+					const float S = state[w] + (w == 0 ? vd.x : vd.y), zz = w == 0 ? vz.x : vz.y, before = w == 0 ? vh.x : vh.y;
+					const float slope = a[k][w] * u[k][w];
+					if constexpr(INPUT) {
+						const Gate take = gate(w == 0 ? vi.x : vi.y);
+						oz[w] = S * take.keep;
+						of[w] = S * before * slope;
+						oi[w] = oz[w] * zz * take.take;
+					} else {
+						oz[w] = S * u[k][w];
+						of[w] = S * (before - zz) * slope;
+					}
+					state[w] = a[k][w] * S;
 				}
-				state[w] = a[k][w] * S;
+				if(on && (decltype(full)::value || t - k >= 0)) {
+					const long long step = DENSE ? 0 : static_cast<long long>(t - k) * p.channels + c;
+					store_raw<T, W>(DENSE ? reinterpret_cast<T*>(reinterpret_cast<uint8_t*>(dz) + outRound + offset[k]) : dz + step, oz[0], oz[W - 1]);
+					store_raw<T, W>(DENSE ? reinterpret_cast<T*>(reinterpret_cast<uint8_t*>(df) + outRound + offset[k]) : df + step, of[0], of[W - 1]);
+					if constexpr(INPUT) {
+						store_raw<T, W>(DENSE ? reinterpret_cast<T*>(reinterpret_cast<uint8_t*>(di) + outRound + offset[k]) : di + step, oi[0], oi[W - 1]);
+					}
+				}
 			}
-			const long long at = to;
-			to -= p.channels;
-			if(on && t - k >= 0) {
-				store_raw<T, W>(dz + at, oz[0], oz[W - 1]);
-				store_raw<T, W>(df + at, of[0], of[W - 1]);
-				if constexpr(INPUT) store_raw<T, W>(di + at, oi[0], oi[W - 1]);
-			}
+		};
+		if(whole) apply(Yes());
+		else apply(No());
+		if constexpr(DENSE) {
+			z.base -= roundBytes;
+			h.base -= roundBytes;
+			if constexpr(INPUT) i.base -= roundBytes;
 		}
+		if(nextWhole) load_rest(t - stride, Yes());
+		else load_rest(t - stride, No());
+		outRound -= roundBytes;
+		t -= stride;
 	}
 	if(on && p.last != nullptr && rank == 0 && warp == 0) {
 #pragma unroll
@@ -417,17 +487,23 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 2) recurrence_backward_kernel(
 
 using Kernel = void (*)(const RecurrenceParams);
 
-template<typename T, bool BACKWARD>
-Kernel kernel_of(int pair, bool input)
+template<typename T, int W, bool BACKWARD>
+Kernel kernel_of(bool input, bool dense)
 {
-	if constexpr(sizeof(T) == 2) {
-		if(pair) {
-			if(BACKWARD) return input ? recurrence_backward_kernel<T, 2, true> : recurrence_backward_kernel<T, 2, false>;
-			return input ? recurrence_forward_kernel<T, 2, true> : recurrence_forward_kernel<T, 2, false>;
-		}
+	if(BACKWARD) {
+		if(dense) return input ? recurrence_backward_kernel<T, W, true, true> : recurrence_backward_kernel<T, W, false, true>;
+		return input ? recurrence_backward_kernel<T, W, true, false> : recurrence_backward_kernel<T, W, false, false>;
 	}
-	if(BACKWARD) return input ? recurrence_backward_kernel<T, 1, true> : recurrence_backward_kernel<T, 1, false>;
-	return input ? recurrence_forward_kernel<T, 1, true> : recurrence_forward_kernel<T, 1, false>;
+	if(dense) return input ? recurrence_forward_kernel<T, W, true, true> : recurrence_forward_kernel<T, W, false, true>;
+	return input ? recurrence_forward_kernel<T, W, true, false> : recurrence_forward_kernel<T, W, false, false>;
+}
+
+template<bool BACKWARD>
+Kernel kernel_for(int type, bool pair, bool input, bool dense)
+{
+	if(type == NB200_TYPE_FP32) return kernel_of<float, 1, BACKWARD>(input, dense);
+	if(type == NB200_TYPE_FP16) return pair ? kernel_of<__half, 2, BACKWARD>(input, dense) : kernel_of<__half, 1, BACKWARD>(input, dense);
+	return pair ? kernel_of<__nv_bfloat16, 2, BACKWARD>(input, dense) : kernel_of<__nv_bfloat16, 1, BACKWARD>(input, dense);
 }
 
 // Warps for the time axis first, then blocks of a cluster: as many as give the fewest rounds, one after another, of the blocks
@@ -435,9 +511,10 @@ Kernel kernel_of(int pair, bool input)
 int launch(int type, bool pair, bool backward, RecurrenceParams p, int batch, cudaStream_t stream)
 {
 	const bool input = p.i != nullptr;
-	const Kernel kernel = type == NB200_TYPE_FP32 ? (backward ? kernel_of<float, true>(pair, input) : kernel_of<float, false>(pair, input))
-		: type == NB200_TYPE_FP16 ? (backward ? kernel_of<__half, true>(pair, input) : kernel_of<__half, false>(pair, input))
-		: (backward ? kernel_of<__nv_bfloat16, true>(pair, input) : kernel_of<__nv_bfloat16, false>(pair, input));
+	const long long row = p.channels;
+	const bool dense = row * type_size(type) * (MAX_CLUSTER + 1) * MAX_WARPS * STEPS < (1ll << 32)
+		&& (p.length <= 1 || (p.zRow == row && p.fRow == row && (!input || p.iRow == row) && (!backward || p.dhRow == row)));
+	const Kernel kernel = backward ? kernel_for<true>(type, pair, input, dense) : kernel_for<false>(type, pair, input, dense);
 	p.status = device_status_word();
 	const int perWarp = pair ? 64 : 32;
 	const int tiles = (p.channels + perWarp - 1) / perWarp;
@@ -445,10 +522,10 @@ int launch(int type, bool pair, bool backward, RecurrenceParams p, int batch, cu
 	const long long groups = static_cast<long long>(tiles) * batch;
 	int warps = 1;
 	while(warps < MAX_WARPS && warps < stretches) warps *= 2;
-	const long long held = static_cast<long long>(sm_count()) * (backward ? 2 : 3) * (MAX_WARPS / warps);
+	const long long held = static_cast<long long>(sm_count()) * (backward || pair ? 2 : 3) * (MAX_WARPS / warps);
 	int blocks = 1;
 	long long least = 0;
-	for(int n = 1; n <= MAX_CLUSTER && (n == 1 || n / 2 * warps < stretches); n *= 2) {
+	for(int n = 1; n <= MAX_CLUSTER && (n - 1) * warps < stretches; ++n) {
 		const long long rounds = (groups * n + held - 1) / held * ((stretches + n * warps - 1) / (n * warps));
 		if(n == 1 || rounds < least) {
 			least = rounds;
