@@ -506,8 +506,11 @@ Kernel kernel_for(int type, bool pair, bool input, bool dense)
 	return pair ? kernel_of<__nv_bfloat16, 2, BACKWARD>(input, dense) : kernel_of<__nv_bfloat16, 1, BACKWARD>(input, dense);
 }
 
-// Warps for the time axis first, then blocks of a cluster: as many as give the fewest rounds, one after another, of the blocks
-// that the device holds at a time (by the kernels' registers).
+// How many warps and blocks share a sequence's time axis: the fewest that fill three quarters of the warps that the SMs hold
+// (16, or 24 in the kernels of fewer registers).  Blocks of four warps: 16 x 2048 x 2048 bf16 took 98 us in blocks of four, 102
+// in blocks of eight and 146 of two, in clusters of two (of four, eight) of the first 102 (109, 125); 64 x 100 x 4096 fp16, where a
+// warp per sequence is enough, 47 us in blocks of two and 63 of eight.  Where there are few channels (2 x 16384 x 2048) clusters
+// of eight blocks of four are fastest: 113 us, 159 in clusters of four, 477 without.
 int launch(int type, bool pair, bool backward, RecurrenceParams p, int batch, cudaStream_t stream)
 {
 	const bool input = p.i != nullptr;
@@ -520,18 +523,12 @@ int launch(int type, bool pair, bool backward, RecurrenceParams p, int batch, cu
 	const int tiles = (p.channels + perWarp - 1) / perWarp;
 	const int stretches = (p.length + STEPS - 1) / STEPS;
 	const long long groups = static_cast<long long>(tiles) * batch;
-	int warps = 1;
-	while(warps < MAX_WARPS && warps < stretches) warps *= 2;
-	const long long held = static_cast<long long>(sm_count()) * (backward || pair ? 2 : 3) * (MAX_WARPS / warps);
-	int blocks = 1;
-	long long least = 0;
-	for(int n = 1; n <= MAX_CLUSTER && (n - 1) * warps < stretches; ++n) {
-		const long long rounds = (groups * n + held - 1) / held * ((stretches + n * warps - 1) / (n * warps));
-		if(n == 1 || rounds < least) {
-			least = rounds;
-			blocks = n;
-		}
-	}
+	const long long wanted = static_cast<long long>(sm_count()) * (backward || pair ? 12 : 18);
+	int warps = stretches < 2 ? 1 : 2, blocks = 1;
+	auto more = [&](int w, int n) { return groups * w * n < wanted && w * n < stretches; };
+	while(warps < 4 && more(warps, blocks)) warps *= 2;
+	while(blocks < MAX_CLUSTER && more(warps, blocks)) blocks *= 2;
+	while(warps < MAX_WARPS && more(warps, blocks)) warps *= 2;
 	cudaLaunchConfig_t config = {};
 	config.blockDim = dim3(warps * 32);
 	config.gridDim = dim3(tiles, blocks, batch);
