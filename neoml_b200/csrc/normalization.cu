@@ -13,6 +13,7 @@
 // alignment and a thread's columns never change.  This is why rows of odd width run at the same rate as even ones.
 // Operands whose rows are aligned differently from one another (a view of some columns) take the form with units of one element.
 #include "types16.cuh"
+#include <atomic>
 
 namespace nb200 {
 
@@ -43,27 +44,63 @@ struct NormParams {
 // row use different ones, so that one barrier each is enough.
 __device__ __forceinline__ float row_sum(float v, int lanes, float* slots)
 {
-	if(lanes <= 32) {
-		for(int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-		return v;
-	}
 	v = warp_sum_all(v);
 	if((threadIdx.x & 31) == 0) slots[threadIdx.x >> 5] = v;
 	__syncthreads();
 	return warp_sum_all((threadIdx.x & 31) < (lanes >> 5) ? slots[threadIdx.x & 31] : 0.f);
 }
 
+// Sum over groups of `lanes` threads of a warp.
+__device__ __forceinline__ float lane_sum(float v, int lanes)
+{
+#pragma unroll
+	for(int o = 16; o > 0; o >>= 1) {
+		if(o < lanes) v += __shfl_xor_sync(0xffffffffu, v, o);
+	}
+	return v;
+}
+
+// A unit's floats in pairs; the second of a unit of one element stays zero.
+template<int V>
+struct Pairs {
+	static constexpr int N = V > 1 ? V / 2 : 1;
+	float2 v[N];
+};
+
+template<typename T, int V, bool EDGES>
+__device__ __forceinline__ void unit_pairs(const uint4& raw, int first, int width, Pairs<V>& out)
+{
+	float v[V > 1 ? V : 2];
+	v[1] = 0.f;
+	whole_floats<T, V, EDGES>(raw, first, width, v);
+#pragma unroll
+	for(int j = 0; j < Pairs<V>::N; ++j) out.v[j] = make_float2(v[2 * j], v[2 * j + 1]);
+}
+
+// Zeros where the unit is not the row's (units of one element: where the row has ended, and beside the element).
+template<int V, bool EDGES>
+__device__ __forceinline__ void clear_outside(int first, int width, Pairs<V>& p)
+{
+	if(V > 1 && whole<V, EDGES>(first, width)) return;
+#pragma unroll
+	for(int j = 0; j < Pairs<V>::N; ++j) {
+		if(!inside<V, EDGES>(first, 2 * j, width)) p.v[j].x = 0.f;
+		if(V == 1 || !inside<V, EDGES>(first, 2 * j + 1, width)) p.v[j].y = 0.f;
+	}
+}
+
 // The parameters of a thread's columns.
 template<typename P, int V, int C, bool EDGES>
-__device__ __forceinline__ void load_parameters(const void* from, float missing, int t, int lanes, int offset, int width, float (&v)[C][V])
+__device__ __forceinline__ void load_parameters(const void* from, float missing, int t, int lanes, int offset, int width, Pairs<V> (&v)[C])
 {
 #pragma unroll
 	for(int c = 0; c < C; ++c) {
 		const int first = (c * lanes + t) * V - offset;
+		auto one = [&](int j) {
+			return from != nullptr && j < V && inside<V, EDGES>(first, j, width) ? to_float(static_cast<const P*>(from)[first + j]) : missing;
+		};
 #pragma unroll
-		for(int j = 0; j < V; ++j) {
-			v[c][j] = from != nullptr && inside<V, EDGES>(first, j, width) ? to_float(static_cast<const P*>(from)[first + j]) : missing;
-		}
+		for(int j = 0; j < Pairs<V>::N; ++j) v[c].v[j] = make_float2(one(2 * j), one(2 * j + 1));
 	}
 }
 
@@ -71,7 +108,7 @@ __device__ __forceinline__ void load_parameters(const void* from, float missing,
 template<typename T, typename P, int V, int C, bool EDGES>
 __global__ void __launch_bounds__(MAX_ROW_WARPS * 32, V * C <= 8 ? 2 : 1) norm_forward_kernel(const NormParams p)
 {
-	__shared__ float slots[2][MAX_WARPS];
+	__shared__ float4 joined[2][MAX_ROW_WARPS];
 	const int lanes = p.lanes;
 	const int t = threadIdx.x & (lanes <= 32 ? lanes - 1 : 1023);
 	const int rowsAtOnce = lanes <= 32 ? blockDim.x / lanes : 1;
@@ -81,10 +118,21 @@ __global__ void __launch_bounds__(MAX_ROW_WARPS * 32, V * C <= 8 ? 2 : 1) norm_f
 	row.begin = x;
 	row.end = x + (p.height - 1) * p.xRow + p.width;
 	const int offset = EDGES ? row_offset<T, V>(x + r * p.xRow) : 0;
-	float scale[C][V], free[C][V];
+	Pairs<V> scale[C], free[C];
 	load_parameters<P, V, C, EDGES>(p.scale, 1.f, t, lanes, offset, p.width, scale);
 	load_parameters<P, V, C, EDGES>(p.free_term, 0.f, t, lanes, offset, p.width, free);
 	const float overWidth = 1.f / static_cast<float>(p.width);
+	// the elements that this group of lanes holds of a row
+	float count = 0.f;
+#pragma unroll
+	for(int c = 0; c < C; ++c) {
+		const int first = (c * lanes + t) * V - offset;
+#pragma unroll
+		for(int j = 0; j < V; ++j) count += inside<V, EDGES>(first, j, p.width) ? 1.f : 0.f;
+	}
+	count = lane_sum(count, lanes < 32 ? lanes : 32);
+	const float overCount = count > 0.f ? 1.f / count : 0.f;
+	int phase = 0;
 	uint4 next[C];
 	auto load = [&](int at) {
 		row.p = x + at * p.xRow;
@@ -97,45 +145,52 @@ __global__ void __launch_bounds__(MAX_ROW_WARPS * 32, V * C <= 8 ? 2 : 1) norm_f
 	load(r);
 	// all threads of a warp stay to the end of its last row
 	for(int left = r - (lanes <= 32 ? (threadIdx.x & 31) / lanes : 0); left < p.height; left += p.rowStep, r += p.rowStep) {
-		uint4 raw[C];
+		Pairs<V> v[C];
+		float2 sums = both(0.f);
 #pragma unroll
-		for(int c = 0; c < C; ++c) raw[c] = next[c];
+		for(int c = 0; c < C; ++c) {
+			unit_pairs<T, V, EDGES>(next[c], (c * lanes + t) * V - offset, p.width, v[c]);
+#pragma unroll
+			for(int j = 0; j < Pairs<V>::N; ++j) sums = add2(sums, v[c].v[j]);
+		}
 		load(r + p.rowStep);
-		float sum = 0.f;
+		// the mean of this group of lanes, and the squares around it; a row of several warps joins theirs:
+		// squares around the row's mean = sum over the warps of (their squares + count (their mean - the row's)^2)
+		const float groupMean = lane_sum(sums.x + sums.y, lanes < 32 ? lanes : 32) * overCount;
+		float2 squares = both(0.f);
 #pragma unroll
 		for(int c = 0; c < C; ++c) {
-			float v[V];
-			whole_floats<T, V, EDGES>(raw[c], (c * lanes + t) * V - offset, p.width, v);
 #pragma unroll
-			for(int j = 0; j < V; ++j) sum += v[j];
+			for(int j = 0; j < Pairs<V>::N; ++j) v[c].v[j] = add2(v[c].v[j], both(-groupMean));
+			clear_outside<V, EDGES>((c * lanes + t) * V - offset, p.width, v[c]);
+#pragma unroll
+			for(int j = 0; j < Pairs<V>::N; ++j) squares = fma2(v[c].v[j], v[c].v[j], squares);
 		}
-		const float mean = row_sum(sum, lanes, slots[0]) * overWidth;
-		float square = 0.f;
-#pragma unroll
-		for(int c = 0; c < C; ++c) {
-			const int first = (c * lanes + t) * V - offset;
-			float v[V];
-			unit_floats<T, V>(raw[c], v);
-			if(whole<V, EDGES>(first, p.width)) {
-#pragma unroll
-				for(int j = 0; j < V; ++j) square = fmaf(v[j] - mean, v[j] - mean, square);
-			} else {
-#pragma unroll
-				for(int j = 0; j < V; ++j) {
-					if(inside<V, EDGES>(first, j, p.width)) square = fmaf(v[j] - mean, v[j] - mean, square);
-				}
-			}
+		float mean = groupMean, square = squares.x + squares.y;
+		square = lane_sum(square, lanes < 32 ? lanes : 32);
+		if(lanes > 32) {
+			if((threadIdx.x & 31) == 0) joined[phase][threadIdx.x >> 5] = make_float4(mean, square, count, 0.f);
+			__syncthreads(); // one a row: the slots alternate
+			const int w = threadIdx.x & (MAX_ROW_WARPS - 1);
+			const float4 o = w < (lanes >> 5) ? joined[phase][w] : make_float4(0.f, 0.f, 0.f, 0.f);
+			mean = lane_sum(o.x * o.z, MAX_ROW_WARPS) * overWidth;
+			square = lane_sum(fmaf((o.x - mean) * (o.x - mean), o.z, o.y), MAX_ROW_WARPS);
+			phase ^= 1;
 		}
-		const float inv = rsqrtf(row_sum(square, lanes, slots[1]) * overWidth + p.epsilon);
+		const float inv = rsqrtf(square * overWidth + p.epsilon);
 		if(r < p.height) {
 			T* const out = static_cast<T*>(p.out) + r * p.outRow;
+			const float2 shift = both(groupMean - mean), by = both(inv);
 #pragma unroll
 			for(int c = 0; c < C; ++c) {
-				float v[V];
-				unit_floats<T, V>(raw[c], v);
+				float y[V > 1 ? V : 2];
 #pragma unroll
-				for(int j = 0; j < V; ++j) v[j] = fmaf((v[j] - mean) * inv, scale[c][j], free[c][j]);
-				store_unit<T, V, EDGES>(out, (c * lanes + t) * V - offset, p.width, v);
+				for(int j = 0; j < Pairs<V>::N; ++j) {
+					const float2 f = fma2(mul2(add2(v[c].v[j], shift), by), scale[c].v[j], free[c].v[j]);
+					y[2 * j] = f.x;
+					y[2 * j + 1] = f.y;
+				}
+				store_unit<T, V, EDGES>(out, (c * lanes + t) * V - offset, p.width, y);
 			}
 			if(t == 0) {
 				if(p.mean != nullptr) p.mean[r] = mean;
@@ -180,7 +235,7 @@ __global__ void __launch_bounds__(1024) norm_forward_wide_kernel(const NormParam
 template<typename T, typename P, int V, int C, bool EDGES>
 __global__ void __launch_bounds__(MAX_ROW_WARPS * 32) norm_backward_kernel(const NormParams p)
 {
-	__shared__ float slots[2][2][MAX_WARPS];
+	__shared__ float2 joined[2][MAX_ROW_WARPS];
 	__shared__ float sums[2][SMALL_WIDTH];
 	const int lanes = p.lanes;
 	const int t = threadIdx.x & (lanes <= 32 ? lanes - 1 : 1023);
@@ -194,12 +249,12 @@ __global__ void __launch_bounds__(MAX_ROW_WARPS * 32) norm_backward_kernel(const
 	dr.begin = dy;
 	dr.end = dy + (p.height - 1) * p.dyRow + p.width;
 	const int offset = EDGES ? row_offset<T, V>(x + r * p.xRow) : 0;
-	float scale[C][V], ds[C][V], db[C][V];
+	Pairs<V> scale[C], ds[C], db[C];
 	load_parameters<P, V, C, EDGES>(p.scale, 1.f, t, lanes, offset, p.width, scale);
 #pragma unroll
 	for(int c = 0; c < C; ++c) {
 #pragma unroll
-		for(int j = 0; j < V; ++j) ds[c][j] = db[c][j] = 0.f;
+		for(int j = 0; j < Pairs<V>::N; ++j) ds[c].v[j] = db[c].v[j] = both(0.f);
 	}
 	const float overWidth = 1.f / static_cast<float>(p.width);
 	int phase = 0;
@@ -223,62 +278,49 @@ __global__ void __launch_bounds__(MAX_ROW_WARPS * 32) norm_backward_kernel(const
 	};
 	load(r);
 	for(int left = r - (lanes <= 32 ? (threadIdx.x & 31) / lanes : 0); left < p.height; left += p.rowStep, r += p.rowStep, phase ^= 1) {
-		uint4 rx[C], rd[C];
-#pragma unroll
-		for(int c = 0; c < C; ++c) {
-			rx[c] = nextX[c];
-			rd[c] = nextD[c];
-		}
 		const float mean = nextMean, inv = nextInv;
-		load(r + p.rowStep);
-		float sumG = 0.f, sumGu = 0.f;
+		Pairs<V> u[C], g[C]; // unit rows; gradients times scale
+		float2 sumsG = both(0.f), sumsGu = both(0.f);
 #pragma unroll
 		for(int c = 0; c < C; ++c) {
 			const int first = (c * lanes + t) * V - offset;
-			float u[V], g[V];
-			whole_floats<T, V, EDGES>(rx[c], first, p.width, u); // the neighbours' may be infinite
-			whole_floats<T, V, EDGES>(rd[c], first, p.width, g); // zeros outside, and so is what they are multiplied by
+			unit_pairs<T, V, EDGES>(nextX[c], first, p.width, u[c]); // the neighbours' may be infinite
+			unit_pairs<T, V, EDGES>(nextD[c], first, p.width, g[c]); // zeros outside, and so is what they are multiplied by
 #pragma unroll
-			for(int j = 0; j < V; ++j) {
-				const float unit = (u[j] - mean) * inv;
-				ds[c][j] = fmaf(g[j], unit, ds[c][j]);
-				db[c][j] += g[j];
-				const float by = g[j] * scale[c][j];
-				sumG += by;
-				sumGu = fmaf(by, unit, sumGu);
+			for(int j = 0; j < Pairs<V>::N; ++j) {
+				u[c].v[j] = mul2(add2(u[c].v[j], both(-mean)), both(inv));
+				ds[c].v[j] = fma2(g[c].v[j], u[c].v[j], ds[c].v[j]);
+				db[c].v[j] = add2(db[c].v[j], g[c].v[j]);
+				g[c].v[j] = mul2(g[c].v[j], scale[c].v[j]);
+				sumsG = add2(sumsG, g[c].v[j]);
+				sumsGu = fma2(g[c].v[j], u[c].v[j], sumsGu);
 			}
 		}
-		if(lanes <= 32) {
-			for(int o = lanes >> 1; o > 0; o >>= 1) {
-				sumG += __shfl_xor_sync(0xffffffffu, sumG, o);
-				sumGu += __shfl_xor_sync(0xffffffffu, sumGu, o);
-			}
-		} else {
-			sumG = warp_sum_all(sumG);
-			sumGu = warp_sum_all(sumGu);
-			if((threadIdx.x & 31) == 0) {
-				slots[phase][0][threadIdx.x >> 5] = sumG;
-				slots[phase][1][threadIdx.x >> 5] = sumGu;
-			}
+		load(r + p.rowStep);
+		float sumG = sumsG.x + sumsG.y, sumGu = sumsGu.x + sumsGu.y;
+		sumG = lane_sum(sumG, lanes < 32 ? lanes : 32);
+		sumGu = lane_sum(sumGu, lanes < 32 ? lanes : 32);
+		if(lanes > 32) {
+			if((threadIdx.x & 31) == 0) joined[phase][threadIdx.x >> 5] = make_float2(sumG, sumGu);
 			__syncthreads(); // one a row: the slots alternate
-			const int w = threadIdx.x & 31;
-			sumG = warp_sum_all(w < (lanes >> 5) ? slots[phase][0][w] : 0.f);
-			sumGu = warp_sum_all(w < (lanes >> 5) ? slots[phase][1][w] : 0.f);
+			const int w = threadIdx.x & (MAX_ROW_WARPS - 1);
+			const float2 o = w < (lanes >> 5) ? joined[phase][w] : make_float2(0.f, 0.f);
+			sumG = lane_sum(o.x, MAX_ROW_WARPS);
+			sumGu = lane_sum(o.y, MAX_ROW_WARPS);
 		}
 		if(r < p.height) {
 			const float meanG = sumG * overWidth, meanGu = sumGu * overWidth;
 			T* const out = static_cast<T*>(p.out) + r * p.outRow;
 #pragma unroll
 			for(int c = 0; c < C; ++c) {
-				float u[V], g[V];
-				unit_floats<T, V>(rx[c], u);
-				unit_floats<T, V>(rd[c], g);
+				float y[V > 1 ? V : 2];
 #pragma unroll
-				for(int j = 0; j < V; ++j) {
-					const float unit = (u[j] - mean) * inv;
-					g[j] = (fmaf(g[j], scale[c][j], -meanG) - unit * meanGu) * inv;
+				for(int j = 0; j < Pairs<V>::N; ++j) {
+					const float2 f = mul2(fma2(u[c].v[j], both(-meanGu), add2(g[c].v[j], both(-meanG))), both(inv));
+					y[2 * j] = f.x;
+					y[2 * j + 1] = f.y;
 				}
-				store_unit<T, V, EDGES>(out, (c * lanes + t) * V - offset, p.width, g);
+				store_unit<T, V, EDGES>(out, (c * lanes + t) * V - offset, p.width, y);
 			}
 		}
 	}
@@ -295,11 +337,11 @@ __global__ void __launch_bounds__(MAX_ROW_WARPS * 32) norm_backward_kernel(const
 					if(!inside<V, EDGES>(first, j, p.width)) continue;
 					const int column = first + j;
 					if(rowsAtOnce == 1) {
-						mine[column] = ds[c][j];
-						mine[p.width + column] = db[c][j];
+						mine[column] = j % 2 == 0 ? ds[c].v[j / 2].x : ds[c].v[j / 2].y;
+						mine[p.width + column] = j % 2 == 0 ? db[c].v[j / 2].x : db[c].v[j / 2].y;
 					} else {
-						sums[0][column] = (g > 0 ? sums[0][column] : 0.f) + ds[c][j];
-						sums[1][column] = (g > 0 ? sums[1][column] : 0.f) + db[c][j];
+						sums[0][column] = (g > 0 ? sums[0][column] : 0.f) + (j % 2 == 0 ? ds[c].v[j / 2].x : ds[c].v[j / 2].y);
+						sums[1][column] = (g > 0 ? sums[1][column] : 0.f) + (j % 2 == 0 ? db[c].v[j / 2].x : db[c].v[j / 2].y);
 					}
 				}
 			}
@@ -361,6 +403,7 @@ __global__ void __launch_bounds__(512) norm_parameters_kernel(const float* __res
 	float s = 0.f;
 	if(column < width) {
 		const float* const at = partial + static_cast<long long>(which) * width + column;
+#pragma unroll 8
 		for(int i = lane; i < parts; i += 16) s += at[static_cast<long long>(i) * 2 * width];
 	}
 	sums[lane][threadIdx.x & 31] = s;
@@ -388,7 +431,7 @@ struct Shape {
 	bool wide;      // rows longer than registers hold
 	int unit;       // elements of a unit
 	bool edges;     // rows may begin or end inside a unit
-	int units;      // per thread: 1 to 4, 6 or 8, or 16 units of one element
+	int units;      // per thread: 1 to 4, 6 or 8, or 8 units of one element
 	int lanes;      // threads of a row
 	int threads;    // per block
 	int rowsAtOnce; // of a block
@@ -406,13 +449,13 @@ Shape shape_of(int type, int height, int width, bool alike, bool aligned, bool f
 	s.edges = !aligned || width % s.unit != 0;
 	// a row that begins inside a unit touches one more
 	const int units = alike && !aligned ? (width + 2 * (s.unit - 1)) / s.unit : (width + s.unit - 1) / s.unit;
-	const int most = alike ? 16 / s.unit : 16;
+	const int most = alike ? 16 / s.unit : 8;
 	if(units <= 32 * (forward && alike && size == 2 ? 3 : most) && width <= SMALL_WIDTH) {
 		s.lanes = 32;
 		while(s.lanes > 4 && units <= s.lanes / 2) s.lanes /= 2;
 		s.threads = SMALL_BLOCK;
 		s.rowsAtOnce = SMALL_BLOCK / s.lanes;
-		s.units = alike ? (units + s.lanes - 1) / s.lanes : 16;
+		s.units = alike ? (units + s.lanes - 1) / s.lanes : 8;
 	} else {
 		int hold = units > MAX_ROW_WARPS * 32 * most && forward && alike ? 2 * most : most;
 		auto warps_for = [&](int h) { return (units + 32 * h - 1) / (32 * h); };
@@ -424,23 +467,12 @@ Shape shape_of(int type, int height, int width, bool alike, bool aligned, bool f
 		}
 		s.threads = s.lanes = (s.wide ? MAX_WARPS : warps_for(hold)) * 32;
 		s.rowsAtOnce = 1;
-		s.units = alike ? (units + s.lanes - 1) / s.lanes : 16;
+		s.units = alike ? (units + s.lanes - 1) / s.lanes : 8;
 	}
-	// by the kernels' registers
-	const int residentThreads = s.units * s.unit <= 8 ? (forward ? 1024 : 768) : forward && s.units * s.unit <= 16 ? 640 : 512;
-	if(s.wide) {
-		s.blocks = height < sm_count() * 2 ? height : sm_count() * 2;
-		return s;
-	}
-	// a block's rows are a multiple of a unit's elements apart: all of them begin at the same offset in a unit
+	// at most: the launch goes by what fits (launch_rows)
+	const int most_blocks = sm_count() * (s.wide ? 2 : 1024 / s.threads > 1 ? 1024 / s.threads : 1) + s.unit;
 	const int wanted = (height + s.rowsAtOnce - 1) / s.rowsAtOnce;
-	int resident = sm_count() * (residentThreads / s.threads > 1 ? residentThreads / s.threads : 1);
-	if(wanted > resident) {
-		while(resident * s.rowsAtOnce % s.unit != 0) ++resident;
-		s.blocks = resident;
-	} else {
-		s.blocks = wanted;
-	}
+	s.blocks = wanted < most_blocks ? wanted : most_blocks / s.unit * s.unit;
 	return s;
 }
 
@@ -469,17 +501,49 @@ bool all_aligned(int type, int height, const Operand* o, int n)
 	return true;
 }
 
+using Kernel = void (*)(const NormParams);
+
+// Blocks of a kernel that the device holds at a time; asked once per kernel and block size.
+template<Kernel KERNEL>
+int resident_blocks(int threads)
+{
+	static std::atomic<int> known[MAX_ROW_WARPS + 1];
+	std::atomic<int>& slot = known[threads / 32];
+	int perSm = slot.load(std::memory_order_relaxed);
+	if(perSm == 0) {
+		if(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&perSm, KERNEL, threads, 0) != cudaSuccess || perSm < 1) perSm = 1;
+		slot.store(perSm, std::memory_order_relaxed);
+	}
+	return perSm * sm_count();
+}
+
+// Launches as many blocks of the shape as are resident; returns their number.
+template<Kernel KERNEL>
+int launch_rows(NormParams p, const Shape& s, cudaStream_t stream)
+{
+	int blocks = s.blocks;
+	const int resident = resident_blocks<KERNEL>(s.threads);
+	if(blocks > resident) {
+		// a block's rows are a multiple of a unit's elements apart: all of them begin at the same offset in a unit
+		blocks = resident;
+		while(blocks * s.rowsAtOnce % s.unit != 0) --blocks;
+	}
+	p.rowStep = blocks * s.rowsAtOnce;
+	KERNEL<<<blocks, s.threads, 0, stream>>>(p);
+	return blocks;
+}
+
 template<typename T, typename P, bool EDGES>
 void launch_forward_units(const NormParams& p, const Shape& s, cudaStream_t stream)
 {
 	constexpr int V = Unit16<T>::N;
-	if(s.units <= 1) norm_forward_kernel<T, P, V, 1, EDGES><<<s.blocks, s.threads, 0, stream>>>(p);
-	else if(s.units == 2) norm_forward_kernel<T, P, V, 2, EDGES><<<s.blocks, s.threads, 0, stream>>>(p);
-	else if(s.units == 3) norm_forward_kernel<T, P, V, 3, EDGES><<<s.blocks, s.threads, 0, stream>>>(p);
-	else if(s.units == 4) norm_forward_kernel<T, P, V, 4, EDGES><<<s.blocks, s.threads, 0, stream>>>(p);
+	if(s.units <= 1) launch_rows<norm_forward_kernel<T, P, V, 1, EDGES>>(p, s, stream);
+	else if(s.units == 2) launch_rows<norm_forward_kernel<T, P, V, 2, EDGES>>(p, s, stream);
+	else if(s.units == 3) launch_rows<norm_forward_kernel<T, P, V, 3, EDGES>>(p, s, stream);
+	else if(s.units == 4) launch_rows<norm_forward_kernel<T, P, V, 4, EDGES>>(p, s, stream);
 	else if constexpr(V == 4) {
-		if(s.units <= 6) norm_forward_kernel<T, P, V, 6, EDGES><<<s.blocks, s.threads, 0, stream>>>(p);
-		else norm_forward_kernel<T, P, V, 8, EDGES><<<s.blocks, s.threads, 0, stream>>>(p);
+		if(s.units <= 6) launch_rows<norm_forward_kernel<T, P, V, 6, EDGES>>(p, s, stream);
+		else launch_rows<norm_forward_kernel<T, P, V, 8, EDGES>>(p, s, stream);
 	}
 }
 
@@ -487,35 +551,36 @@ template<typename T, typename P>
 void launch_forward(const NormParams& p, const Shape& s, cudaStream_t stream)
 {
 	if(s.wide) norm_forward_wide_kernel<T, P><<<s.blocks, s.threads, 0, stream>>>(p);
-	else if(s.unit == 1) norm_forward_kernel<T, P, 1, 16, true><<<s.blocks, s.threads, 0, stream>>>(p);
+	else if(s.unit == 1) launch_rows<norm_forward_kernel<T, P, 1, 8, true>>(p, s, stream);
 	else if(s.edges) launch_forward_units<T, P, true>(p, s, stream);
 	else launch_forward_units<T, P, false>(p, s, stream);
 }
 
 template<typename T, typename P, bool EDGES>
-void launch_backward_units(const NormParams& p, const Shape& s, cudaStream_t stream)
+int launch_backward_units(const NormParams& p, const Shape& s, cudaStream_t stream)
 {
 	constexpr int V = Unit16<T>::N;
-	if(s.units <= 1) norm_backward_kernel<T, P, V, 1, EDGES><<<s.blocks, s.threads, 0, stream>>>(p);
-	else if(s.units == 2) norm_backward_kernel<T, P, V, 2, EDGES><<<s.blocks, s.threads, 0, stream>>>(p);
-	else if constexpr(V == 4) {
-		if(s.units == 3) norm_backward_kernel<T, P, V, 3, EDGES><<<s.blocks, s.threads, 0, stream>>>(p);
-		else norm_backward_kernel<T, P, V, 4, EDGES><<<s.blocks, s.threads, 0, stream>>>(p);
+	if(s.units <= 1) return launch_rows<norm_backward_kernel<T, P, V, 1, EDGES>>(p, s, stream);
+	if constexpr(V == 4) {
+		if(s.units == 3) return launch_rows<norm_backward_kernel<T, P, V, 3, EDGES>>(p, s, stream);
+		if(s.units == 4) return launch_rows<norm_backward_kernel<T, P, V, 4, EDGES>>(p, s, stream);
 	}
+	return launch_rows<norm_backward_kernel<T, P, V, 2, EDGES>>(p, s, stream);
 }
 
 template<typename T, typename P>
 void launch_backward(const NormParams& p, const Shape& s, void* scaleDiff, void* freeDiff, cudaStream_t stream)
 {
+	int blocks = s.blocks;
 	if(s.wide) norm_backward_wide_kernel<T, P><<<s.blocks, s.threads, 0, stream>>>(p);
-	else if(s.unit == 1) norm_backward_kernel<T, P, 1, 16, true><<<s.blocks, s.threads, 0, stream>>>(p);
-	else if(s.edges) launch_backward_units<T, P, true>(p, s, stream);
-	else launch_backward_units<T, P, false>(p, s, stream);
+	else if(s.unit == 1) blocks = launch_rows<norm_backward_kernel<T, P, 1, 8, true>>(p, s, stream);
+	else if(s.edges) blocks = launch_backward_units<T, P, true>(p, s, stream);
+	else blocks = launch_backward_units<T, P, false>(p, s, stream);
 	count_launch();
 	if(p.partial != nullptr) {
 		const dim3 grid((p.width + 31) / 32, 2);
 		launch_dependent(true, norm_parameters_kernel<P>, grid, dim3(512), 0, stream, static_cast<const float*>(p.partial),
-			s.blocks, p.width, static_cast<P*>(scaleDiff), static_cast<P*>(freeDiff));
+			blocks, p.width, static_cast<P*>(scaleDiff), static_cast<P*>(freeDiff));
 		count_launch();
 	}
 }
@@ -556,7 +621,7 @@ int nb200_layer_normalization(void* stream, int type, int parameter_type, const 
 	NormParams p = {};
 	p.x = x; p.scale = scale; p.free_term = free_term; p.out = y; p.mean = mean; p.inv = inverse_deviation;
 	p.xRow = x_row_size; p.outRow = y_row_size;
-	p.height = height; p.width = width; p.lanes = s.lanes; p.rowStep = s.blocks * s.rowsAtOnce; p.epsilon = epsilon;
+	p.height = height; p.width = width; p.lanes = s.lanes; p.epsilon = epsilon;
 	with_types(type, parameter_type, [&](auto t, auto q) { launch_forward<decltype(t), decltype(q)>(p, s, as_stream(stream)); });
 	count_launch();
 	return check_launch();
@@ -605,7 +670,7 @@ int nb200_layer_normalization_backward(void* stream, int type, int parameter_typ
 	p.mean = const_cast<float*>(mean); p.inv = const_cast<float*>(inverse_deviation);
 	p.partial = parameters ? scratch : nullptr;
 	p.xRow = x_row_size; p.dyRow = dy_row_size; p.outRow = dx_row_size;
-	p.height = height; p.width = width; p.lanes = s.lanes; p.rowStep = s.blocks * s.rowsAtOnce;
+	p.height = height; p.width = width; p.lanes = s.lanes;
 	with_types(type, parameter_type, [&](auto t, auto q) {
 		launch_backward<decltype(t), decltype(q)>(p, s, scale_diff, free_term_diff, as_stream(stream));
 	});

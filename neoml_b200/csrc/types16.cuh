@@ -173,6 +173,31 @@ __device__ __forceinline__ int row_offset(const T* row)
 	return V == 1 ? 0 : static_cast<int>((reinterpret_cast<uintptr_t>(row) & 15u) / sizeof(T));
 }
 
+// Two fp32 operations in one instruction, each rounded like the scalar one.
+__device__ __forceinline__ unsigned long long as_pair(float2 v)
+{
+	return *reinterpret_cast<unsigned long long*>(&v);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b)
+{
+	float2 r;
+	asm("add.rn.ftz.f32x2 %0, %1, %2;" : "=l"(*reinterpret_cast<unsigned long long*>(&r)) : "l"(as_pair(a)), "l"(as_pair(b)));
+	return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b)
+{
+	float2 r;
+	asm("mul.rn.ftz.f32x2 %0, %1, %2;" : "=l"(*reinterpret_cast<unsigned long long*>(&r)) : "l"(as_pair(a)), "l"(as_pair(b)));
+	return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
+{
+	float2 r;
+	asm("fma.rn.ftz.f32x2 %0, %1, %2, %3;" : "=l"(*reinterpret_cast<unsigned long long*>(&r)) : "l"(as_pair(a)), "l"(as_pair(b)), "l"(as_pair(c)));
+	return r;
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
 __device__ __forceinline__ float warp_sum_all(float v)
 {
 #pragma unroll
