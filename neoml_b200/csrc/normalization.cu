@@ -50,14 +50,28 @@ __device__ __forceinline__ float row_sum(float v, int lanes, float* slots)
 	return warp_sum_all((threadIdx.x & 31) < (lanes >> 5) ? slots[threadIdx.x & 31] : 0.f);
 }
 
-// Sum over groups of `lanes` threads of a warp.
+// Sums over groups of `lanes` threads of a warp (32 and more: over the warp), several side by side.
+template<int N>
+__device__ __forceinline__ void lane_sums(float (&v)[N], int lanes)
+{
+	if(lanes >= 32) {
+#pragma unroll
+		for(int o = 16; o > 0; o >>= 1) {
+#pragma unroll
+			for(int k = 0; k < N; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+		}
+	} else {
+		for(int o = lanes >> 1; o > 0; o >>= 1) {
+#pragma unroll
+			for(int k = 0; k < N; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+		}
+	}
+}
 __device__ __forceinline__ float lane_sum(float v, int lanes)
 {
-#pragma unroll
-	for(int o = 16; o > 0; o >>= 1) {
-		if(o < lanes) v += __shfl_xor_sync(0xffffffffu, v, o);
-	}
-	return v;
+	float one[1] = { v };
+	lane_sums<1>(one, lanes);
+	return one[0];
 }
 
 // A unit's floats in pairs; the second of a unit of one element stays zero.
@@ -104,11 +118,12 @@ __device__ __forceinline__ void load_parameters(const void* from, float missing,
 	}
 }
 
-// C units per thread; the next row is under way while a row is worked on.
-template<typename T, typename P, int V, int C, bool EDGES>
-__global__ void __launch_bounds__(MAX_ROW_WARPS * 32, V * C <= 8 ? 2 : 1) norm_forward_kernel(const NormParams p)
+// C units per thread, ROWS rows at a time (a row's sums are a chain of shuffles that leaves the SM idle: a second row fills it);
+// the rows that follow are under way while these are worked on.
+template<typename T, typename P, int V, int C, bool EDGES, int ROWS>
+__global__ void __launch_bounds__(MAX_ROW_WARPS * 32) norm_forward_kernel(const NormParams p)
 {
-	__shared__ float4 joined[2][MAX_ROW_WARPS];
+	__shared__ float4 joined[2][ROWS][MAX_ROW_WARPS];
 	const int lanes = p.lanes;
 	const int t = threadIdx.x & (lanes <= 32 ? lanes - 1 : 1023);
 	const int rowsAtOnce = lanes <= 32 ? blockDim.x / lanes : 1;
@@ -130,71 +145,101 @@ __global__ void __launch_bounds__(MAX_ROW_WARPS * 32, V * C <= 8 ? 2 : 1) norm_f
 #pragma unroll
 		for(int j = 0; j < V; ++j) count += inside<V, EDGES>(first, j, p.width) ? 1.f : 0.f;
 	}
-	count = lane_sum(count, lanes < 32 ? lanes : 32);
+	count = lane_sum(count, lanes);
 	const float overCount = count > 0.f ? 1.f / count : 0.f;
 	int phase = 0;
-	uint4 next[C];
+	uint4 next[ROWS][C];
 	auto load = [&](int at) {
-		row.p = x + at * p.xRow;
 #pragma unroll
-		for(int c = 0; c < C; ++c) {
-			next[c] = make_uint4(0u, 0u, 0u, 0u);
-			if(at < p.height) load_unit<T, V, EDGES>(row, (c * lanes + t) * V - offset, p.width, next[c]);
+		for(int k = 0; k < ROWS; ++k) {
+			// aligned rows: one behind the last is the last once more, and not stored
+			const int at_k = at + k * p.rowStep;
+			row.p = x + (EDGES ? at_k : min(at_k, p.height - 1)) * p.xRow;
+#pragma unroll
+			for(int c = 0; c < C; ++c) {
+				next[k][c] = make_uint4(0u, 0u, 0u, 0u);
+				if(!EDGES || at_k < p.height) load_unit<T, V, EDGES>(row, (c * lanes + t) * V - offset, p.width, next[k][c]);
+			}
 		}
 	};
 	load(r);
 	// all threads of a warp stay to the end of its last row
-	for(int left = r - (lanes <= 32 ? (threadIdx.x & 31) / lanes : 0); left < p.height; left += p.rowStep, r += p.rowStep) {
-		Pairs<V> v[C];
-		float2 sums = both(0.f);
+	for(int left = r - (lanes <= 32 ? (threadIdx.x & 31) / lanes : 0); left < p.height; left += ROWS * p.rowStep, r += ROWS * p.rowStep) {
+		Pairs<V> v[ROWS][C];
+		float mean[ROWS], square[ROWS], groupMean[ROWS];
 #pragma unroll
-		for(int c = 0; c < C; ++c) {
-			unit_pairs<T, V, EDGES>(next[c], (c * lanes + t) * V - offset, p.width, v[c]);
+		for(int k = 0; k < ROWS; ++k) {
+			float2 sums = both(0.f);
 #pragma unroll
-			for(int j = 0; j < Pairs<V>::N; ++j) sums = add2(sums, v[c].v[j]);
+			for(int c = 0; c < C; ++c) {
+				unit_pairs<T, V, EDGES>(next[k][c], (c * lanes + t) * V - offset, p.width, v[k][c]);
+#pragma unroll
+				for(int j = 0; j < Pairs<V>::N; ++j) sums = add2(sums, v[k][c].v[j]);
+			}
+			mean[k] = sums.x + sums.y;
 		}
-		load(r + p.rowStep);
+		load(r + ROWS * p.rowStep);
 		// the mean of this group of lanes, and the squares around it; a row of several warps joins theirs:
 		// squares around the row's mean = sum over the warps of (their squares + count (their mean - the row's)^2)
-		const float groupMean = lane_sum(sums.x + sums.y, lanes < 32 ? lanes : 32) * overCount;
-		float2 squares = both(0.f);
+		lane_sums<ROWS>(mean, lanes);
 #pragma unroll
-		for(int c = 0; c < C; ++c) {
+		for(int k = 0; k < ROWS; ++k) {
+			groupMean[k] = mean[k] *= overCount;
+			float2 squares = both(0.f);
 #pragma unroll
-			for(int j = 0; j < Pairs<V>::N; ++j) v[c].v[j] = add2(v[c].v[j], both(-groupMean));
-			clear_outside<V, EDGES>((c * lanes + t) * V - offset, p.width, v[c]);
+			for(int c = 0; c < C; ++c) {
 #pragma unroll
-			for(int j = 0; j < Pairs<V>::N; ++j) squares = fma2(v[c].v[j], v[c].v[j], squares);
+				for(int j = 0; j < Pairs<V>::N; ++j) v[k][c].v[j] = add2(v[k][c].v[j], both(-mean[k]));
+				clear_outside<V, EDGES>((c * lanes + t) * V - offset, p.width, v[k][c]);
+#pragma unroll
+				for(int j = 0; j < Pairs<V>::N; ++j) squares = fma2(v[k][c].v[j], v[k][c].v[j], squares);
+			}
+			square[k] = squares.x + squares.y;
 		}
-		float mean = groupMean, square = squares.x + squares.y;
-		square = lane_sum(square, lanes < 32 ? lanes : 32);
+		lane_sums<ROWS>(square, lanes);
 		if(lanes > 32) {
-			if((threadIdx.x & 31) == 0) joined[phase][threadIdx.x >> 5] = make_float4(mean, square, count, 0.f);
-			__syncthreads(); // one a row: the slots alternate
+			if((threadIdx.x & 31) == 0) {
+#pragma unroll
+				for(int k = 0; k < ROWS; ++k) joined[phase][k][threadIdx.x >> 5] = make_float4(mean[k], square[k], count, 0.f);
+			}
+			__syncthreads(); // one for these rows: the slots alternate
 			const int w = threadIdx.x & (MAX_ROW_WARPS - 1);
-			const float4 o = w < (lanes >> 5) ? joined[phase][w] : make_float4(0.f, 0.f, 0.f, 0.f);
-			mean = lane_sum(o.x * o.z, MAX_ROW_WARPS) * overWidth;
-			square = lane_sum(fmaf((o.x - mean) * (o.x - mean), o.z, o.y), MAX_ROW_WARPS);
+			float4 o[ROWS];
+#pragma unroll
+			for(int k = 0; k < ROWS; ++k) {
+				o[k] = w < (lanes >> 5) ? joined[phase][k][w] : make_float4(0.f, 0.f, 0.f, 0.f);
+				mean[k] = o[k].x * o[k].z;
+			}
+			lane_sums<ROWS>(mean, MAX_ROW_WARPS);
+#pragma unroll
+			for(int k = 0; k < ROWS; ++k) {
+				mean[k] *= overWidth;
+				square[k] = fmaf((o[k].x - mean[k]) * (o[k].x - mean[k]), o[k].z, o[k].y);
+			}
+			lane_sums<ROWS>(square, MAX_ROW_WARPS);
 			phase ^= 1;
 		}
-		const float inv = rsqrtf(square * overWidth + p.epsilon);
-		if(r < p.height) {
-			T* const out = static_cast<T*>(p.out) + r * p.outRow;
-			const float2 shift = both(groupMean - mean), by = both(inv);
+#pragma unroll
+		for(int k = 0; k < ROWS; ++k) {
+			const int at = r + k * p.rowStep;
+			if(at >= p.height) continue;
+			const float inv = rsqrtf(square[k] * overWidth + p.epsilon);
+			T* const out = static_cast<T*>(p.out) + at * p.outRow;
+			const float2 shift = both(groupMean[k] - mean[k]), by = both(inv);
 #pragma unroll
 			for(int c = 0; c < C; ++c) {
 				float y[V > 1 ? V : 2];
 #pragma unroll
 				for(int j = 0; j < Pairs<V>::N; ++j) {
-					const float2 f = fma2(mul2(add2(v[c].v[j], shift), by), scale[c].v[j], free[c].v[j]);
+					const float2 f = fma2(mul2(add2(v[k][c].v[j], shift), by), scale[c].v[j], free[c].v[j]);
 					y[2 * j] = f.x;
 					y[2 * j + 1] = f.y;
 				}
 				store_unit<T, V, EDGES>(out, (c * lanes + t) * V - offset, p.width, y);
 			}
 			if(t == 0) {
-				if(p.mean != nullptr) p.mean[r] = mean;
-				if(p.inv != nullptr) p.inv[r] = inv;
+				if(p.mean != nullptr) p.mean[at] = mean[k];
+				if(p.inv != nullptr) p.inv[at] = inv;
 			}
 		}
 	}
@@ -298,15 +343,20 @@ __global__ void __launch_bounds__(MAX_ROW_WARPS * 32) norm_backward_kernel(const
 		}
 		load(r + p.rowStep);
 		float sumG = sumsG.x + sumsG.y, sumGu = sumsGu.x + sumsGu.y;
-		sumG = lane_sum(sumG, lanes < 32 ? lanes : 32);
-		sumGu = lane_sum(sumGu, lanes < 32 ? lanes : 32);
+		float two[2] = { sumG, sumGu };
+		lane_sums<2>(two, lanes);
+		sumG = two[0];
+		sumGu = two[1];
 		if(lanes > 32) {
 			if((threadIdx.x & 31) == 0) joined[phase][threadIdx.x >> 5] = make_float2(sumG, sumGu);
 			__syncthreads(); // one a row: the slots alternate
 			const int w = threadIdx.x & (MAX_ROW_WARPS - 1);
 			const float2 o = w < (lanes >> 5) ? joined[phase][w] : make_float2(0.f, 0.f);
-			sumG = lane_sum(o.x, MAX_ROW_WARPS);
-			sumGu = lane_sum(o.y, MAX_ROW_WARPS);
+			two[0] = o.x;
+			two[1] = o.y;
+			lane_sums<2>(two, MAX_ROW_WARPS);
+			sumG = two[0];
+			sumGu = two[1];
 		}
 		if(r < p.height) {
 			const float meanG = sumG * overWidth, meanGu = sumGu * overWidth;
@@ -533,17 +583,25 @@ int launch_rows(NormParams p, const Shape& s, cudaStream_t stream)
 	return blocks;
 }
 
+// Two rows at a time where a thread has as many; `units` above 16 elements leave no registers for it.
+template<typename T, typename P, int V, int C, bool EDGES>
+void launch_forward_rows(const NormParams& p, const Shape& s, cudaStream_t stream)
+{
+	if(V * C <= 16 && p.height > s.blocks * s.rowsAtOnce) launch_rows<norm_forward_kernel<T, P, V, C, EDGES, V * C <= 16 ? 2 : 1>>(p, s, stream);
+	else launch_rows<norm_forward_kernel<T, P, V, C, EDGES, 1>>(p, s, stream);
+}
+
 template<typename T, typename P, bool EDGES>
 void launch_forward_units(const NormParams& p, const Shape& s, cudaStream_t stream)
 {
 	constexpr int V = Unit16<T>::N;
-	if(s.units <= 1) launch_rows<norm_forward_kernel<T, P, V, 1, EDGES>>(p, s, stream);
-	else if(s.units == 2) launch_rows<norm_forward_kernel<T, P, V, 2, EDGES>>(p, s, stream);
-	else if(s.units == 3) launch_rows<norm_forward_kernel<T, P, V, 3, EDGES>>(p, s, stream);
-	else if(s.units == 4) launch_rows<norm_forward_kernel<T, P, V, 4, EDGES>>(p, s, stream);
+	if(s.units <= 1) launch_forward_rows<T, P, V, 1, EDGES>(p, s, stream);
+	else if(s.units == 2) launch_forward_rows<T, P, V, 2, EDGES>(p, s, stream);
+	else if(s.units == 3) launch_forward_rows<T, P, V, 3, EDGES>(p, s, stream);
+	else if(s.units == 4) launch_forward_rows<T, P, V, 4, EDGES>(p, s, stream);
 	else if constexpr(V == 4) {
-		if(s.units <= 6) launch_rows<norm_forward_kernel<T, P, V, 6, EDGES>>(p, s, stream);
-		else launch_rows<norm_forward_kernel<T, P, V, 8, EDGES>>(p, s, stream);
+		if(s.units <= 6) launch_forward_rows<T, P, V, 6, EDGES>(p, s, stream);
+		else launch_forward_rows<T, P, V, 8, EDGES>(p, s, stream);
 	}
 }
 
@@ -551,7 +609,7 @@ template<typename T, typename P>
 void launch_forward(const NormParams& p, const Shape& s, cudaStream_t stream)
 {
 	if(s.wide) norm_forward_wide_kernel<T, P><<<s.blocks, s.threads, 0, stream>>>(p);
-	else if(s.unit == 1) launch_rows<norm_forward_kernel<T, P, 1, 8, true>>(p, s, stream);
+	else if(s.unit == 1) launch_forward_rows<T, P, 1, 8, true>(p, s, stream);
 	else if(s.edges) launch_forward_units<T, P, true>(p, s, stream);
 	else launch_forward_units<T, P, false>(p, s, stream);
 }
