@@ -19,8 +19,9 @@ namespace nb200 {
 
 namespace {
 
-constexpr int MAX_WARPS = 32;     // of the kernels that loop over a row
-constexpr int MAX_ROW_WARPS = 16; // of those that hold it
+constexpr int MAX_ROW_WARPS = 16; // of a block
+constexpr int WIDE_THREADS = MAX_ROW_WARPS * 32; // of the blocks that loop over a row
+constexpr int WIDE_BYTES = 200 * 1024; // and the shared memory that they stage a row in, at most
 constexpr int SMALL_BLOCK = 128;  // threads of a block whose rows are a warp's or less: several rows at a time
 constexpr int SMALL_WIDTH = 1024; // and what such a row holds at most
 
@@ -39,16 +40,6 @@ struct NormParams {
 	int rowStep;           // rows between two that a thread takes
 	float epsilon;
 };
-
-// Sum over the threads that share a row; every one of them gets it.  `slots` holds a float per warp; the two calls of a
-// row use different ones, so that one barrier each is enough.
-__device__ __forceinline__ float row_sum(float v, int lanes, float* slots)
-{
-	v = warp_sum_all(v);
-	if((threadIdx.x & 31) == 0) slots[threadIdx.x >> 5] = v;
-	__syncthreads();
-	return warp_sum_all((threadIdx.x & 31) < (lanes >> 5) ? slots[threadIdx.x & 31] : 0.f);
-}
 
 // Sums over groups of `lanes` threads of a warp (32 and more: over the warp), several side by side.
 template<int N>
@@ -245,34 +236,112 @@ __global__ void __launch_bounds__(MAX_ROW_WARPS * 32) norm_forward_kernel(const 
 	}
 }
 
-// Rows longer than a block's registers hold: three passes over the row, the second and third out of L2.
-template<typename T, typename P>
-__global__ void __launch_bounds__(1024) norm_forward_wide_kernel(const NormParams p)
+// Sum over a block of WIDE_THREADS threads; every one of them gets it.  Two calls in a row use different slots.
+__device__ __forceinline__ float block_sum(float v, float* slots)
 {
-	__shared__ float slots[2][MAX_WARPS];
+	v = warp_sum_all(v);
+	if((threadIdx.x & 31) == 0) slots[threadIdx.x >> 5] = v;
+	__syncthreads();
+	return warp_sum_all((threadIdx.x & 31) < WIDE_THREADS / 32 ? slots[threadIdx.x & 31] : 0.f);
+}
+
+// Units of a row in shared memory where it fits (STAGED), or read again out of L2.
+template<typename T, int V, bool STAGED>
+struct WideRow {
+	Row<T, V> row;
+	uint4* staged;
+	int offset, width, units;
+	__device__ __forceinline__ void set(const T* x, long long rowSize, int r, uint4* room, int w)
+	{
+		row.p = x + r * rowSize;
+		staged = room;
+		width = w;
+		offset = row_offset<T, V>(row.p);
+		units = (w + offset + V - 1) / V;
+	}
+	// f(first column, the unit's pairs), the first time or again
+	template<bool AGAIN, typename F>
+	__device__ __forceinline__ void each(F&& f) const
+	{
+		constexpr int AHEAD = 4;
+		for(int u0 = threadIdx.x; u0 < units; u0 += WIDE_THREADS * AHEAD) {
+			uint4 raw[AHEAD];
+#pragma unroll
+			for(int k = 0; k < AHEAD; ++k) {
+				const int u = u0 + k * WIDE_THREADS;
+				if(u >= units) continue;
+				if(STAGED && AGAIN) raw[k] = staged[u];
+				else load_unit<T, V>(row, u * V - offset, width, raw[k]);
+			}
+#pragma unroll
+			for(int k = 0; k < AHEAD; ++k) {
+				const int u = u0 + k * WIDE_THREADS;
+				if(u >= units) continue;
+				if(STAGED && !AGAIN) staged[u] = raw[k];
+				Pairs<V> v;
+				unit_pairs<T, V, true>(raw[k], u * V - offset, width, v);
+				f(u * V - offset, v);
+			}
+		}
+	}
+};
+
+// The parameters of a unit's columns: whole vectors where the columns are aligned for it.
+template<typename P, int V>
+__device__ __forceinline__ void unit_parameters(const void* from, int first, int width, float missing, float* v)
+{
+	const P* const at = static_cast<const P*>(from) + first;
+	if(V > 1 && from != nullptr && first >= 0 && first + V <= width && (reinterpret_cast<uintptr_t>(at) & 15u) == 0) {
+#pragma unroll
+		for(int k = 0; k < V / Unit16<P>::N; ++k) Unit16<P>::unpack(reinterpret_cast<const uint4*>(at)[k], v + k * Unit16<P>::N);
+	} else {
+#pragma unroll
+		for(int j = 0; j < V; ++j) v[j] = from != nullptr && first + j >= 0 && first + j < width ? to_float(at[j]) : missing;
+	}
+}
+
+// Rows longer than a block's registers hold.
+template<typename T, typename P, int V, bool STAGED>
+__global__ void __launch_bounds__(WIDE_THREADS) norm_forward_wide_kernel(const NormParams p)
+{
+	extern __shared__ uint4 wideRoom[];
+	__shared__ float slots[2][MAX_ROW_WARPS];
+	const T* const x = static_cast<const T*>(p.x);
+	WideRow<T, V, STAGED> row;
+	row.row.begin = x;
+	row.row.end = x + (p.height - 1) * p.xRow + p.width;
 	const float overWidth = 1.f / static_cast<float>(p.width);
 	for(int r = blockIdx.x; r < p.height; r += gridDim.x) {
-		const T* const x = static_cast<const T*>(p.x) + r * p.xRow;
+		row.set(x, p.xRow, r, wideRoom, p.width);
+		float2 sums = both(0.f), squares = both(0.f);
+		row.template each<false>([&](int, const Pairs<V>& v) {
+#pragma unroll
+			for(int j = 0; j < Pairs<V>::N; ++j) sums = add2(sums, v.v[j]);
+		});
+		const float mean = block_sum(sums.x + sums.y, slots[0]) * overWidth;
+		row.template each<true>([&](int first, const Pairs<V>& v) {
+			Pairs<V> d;
+#pragma unroll
+			for(int j = 0; j < Pairs<V>::N; ++j) d.v[j] = add2(v.v[j], both(-mean));
+			clear_outside<V, true>(first, p.width, d);
+#pragma unroll
+			for(int j = 0; j < Pairs<V>::N; ++j) squares = fma2(d.v[j], d.v[j], squares);
+		});
+		const float inv = rsqrtf(block_sum(squares.x + squares.y, slots[1]) * overWidth + p.epsilon);
 		T* const out = static_cast<T*>(p.out) + r * p.outRow;
-		float sum = 0.f;
-		for(int i = threadIdx.x; i < p.width; i += blockDim.x) sum += to_float(x[i]);
-		const float mean = row_sum(sum, MAX_WARPS * 32, slots[0]) * overWidth;
-		float square = 0.f;
-		for(int i = threadIdx.x; i < p.width; i += blockDim.x) {
-			const float d = to_float(x[i]) - mean;
-			square = fmaf(d, d, square);
-		}
-		const float inv = rsqrtf(row_sum(square, MAX_WARPS * 32, slots[1]) * overWidth + p.epsilon);
-		for(int i = threadIdx.x; i < p.width; i += blockDim.x) {
-			const float s = p.scale != nullptr ? to_float(static_cast<const P*>(p.scale)[i]) : 1.f;
-			const float b = p.free_term != nullptr ? to_float(static_cast<const P*>(p.free_term)[i]) : 0.f;
-			out[i] = from_float<T>(fmaf((to_float(x[i]) - mean) * inv, s, b));
-		}
+		row.template each<true>([&](int first, const Pairs<V>& v) {
+			float y[V > 1 ? V : 2], scale[V], free[V];
+			unit_parameters<P, V>(p.scale, first, p.width, 1.f, scale);
+			unit_parameters<P, V>(p.free_term, first, p.width, 0.f, free);
+#pragma unroll
+			for(int j = 0; j < V; ++j) y[j] = fmaf(((j % 2 == 0 ? v.v[j / 2].x : v.v[j / 2].y) - mean) * inv, scale[j], free[j]);
+			store_unit<T, V>(out, first, p.width, y);
+		});
 		if(threadIdx.x == 0) {
 			if(p.mean != nullptr) p.mean[r] = mean;
 			if(p.inv != nullptr) p.inv[r] = inv;
 		}
-		// every element of this thread's columns has been read by the thread that rewrites it: in place needs no barrier
+		// a unit is staged again, and rewritten in place, by the thread that read it: no barrier
 	}
 }
 
@@ -403,39 +472,117 @@ __global__ void __launch_bounds__(MAX_ROW_WARPS * 32) norm_backward_kernel(const
 	}
 }
 
-// Rows longer than a block's registers hold: sums, then dx, out of L2.
-template<typename T, typename P>
-__global__ void __launch_bounds__(1024) norm_backward_wide_kernel(const NormParams p)
+// Rows longer than a block's registers hold: dx here, the parameters' sums in a kernel of their own (which reads both again).
+template<typename T, typename P, int V, bool STAGED>
+__global__ void __launch_bounds__(WIDE_THREADS) norm_backward_wide_kernel(const NormParams p)
 {
-	__shared__ float slots[2][2][MAX_WARPS];
+	extern __shared__ uint4 wideRoom[];
+	__shared__ float slots[2][2][MAX_ROW_WARPS];
+	const T* const x = static_cast<const T*>(p.x);
+	const T* const dy = static_cast<const T*>(p.dy);
+	WideRow<T, V, STAGED> row, diff;
+	row.row.begin = x;
+	row.row.end = x + (p.height - 1) * p.xRow + p.width;
+	diff.row.begin = dy;
+	diff.row.end = dy + (p.height - 1) * p.dyRow + p.width;
 	const float overWidth = 1.f / static_cast<float>(p.width);
+	const int room = (p.width + 2 * V - 1) / V + 1;
 	int phase = 0;
-	float* const mine = p.partial == nullptr ? nullptr : p.partial + static_cast<long long>(blockIdx.x) * 2 * p.width;
-	bool started = false;
 	for(int r = blockIdx.x; r < p.height; r += gridDim.x, phase ^= 1) {
-		const T* const x = static_cast<const T*>(p.x) + r * p.xRow;
-		const T* const dy = static_cast<const T*>(p.dy) + r * p.dyRow;
-		T* const out = static_cast<T*>(p.out) + r * p.outRow;
+		row.set(x, p.xRow, r, wideRoom, p.width);
+		diff.set(dy, p.dyRow, r, wideRoom + room, p.width);
 		const float mean = __ldg(p.mean + r), inv = __ldg(p.inv + r);
-		float sumG = 0.f, sumGu = 0.f;
-		for(int i = threadIdx.x; i < p.width; i += blockDim.x) {
-			const float unit = (to_float(x[i]) - mean) * inv, d = to_float(dy[i]);
-			const float by = d * (p.scale != nullptr ? to_float(static_cast<const P*>(p.scale)[i]) : 1.f);
-			sumG += by;
-			sumGu = fmaf(by, unit, sumGu);
-			if(mine != nullptr) { // a column belongs to one thread
-				mine[i] = started ? fmaf(d, unit, mine[i]) : d * unit;
-				mine[p.width + i] = started ? mine[p.width + i] + d : d;
+		// both rows are cut alike; f(first column, gradients times scale, unit rows)
+		auto each = [&](bool again, auto f) {
+			constexpr int AHEAD = 2;
+			for(int u0 = threadIdx.x; u0 < row.units; u0 += WIDE_THREADS * AHEAD) {
+				uint4 rx[AHEAD], rd[AHEAD];
+#pragma unroll
+				for(int k = 0; k < AHEAD; ++k) {
+					const int u = u0 + k * WIDE_THREADS;
+					if(u >= row.units) continue;
+					if(STAGED && again) {
+						rx[k] = row.staged[u];
+						rd[k] = diff.staged[u];
+					} else {
+						load_unit<T, V>(row.row, u * V - row.offset, p.width, rx[k]);
+						load_unit<T, V>(diff.row, u * V - row.offset, p.width, rd[k]);
+					}
+				}
+#pragma unroll
+				for(int k = 0; k < AHEAD; ++k) {
+					const int u = u0 + k * WIDE_THREADS, first = u * V - row.offset;
+					if(u >= row.units) continue;
+					if(STAGED && !again) {
+						row.staged[u] = rx[k];
+						diff.staged[u] = rd[k];
+					}
+					Pairs<V> vx, vd;
+					unit_pairs<T, V, true>(rx[k], first, p.width, vx);
+					unit_pairs<T, V, true>(rd[k], first, p.width, vd);
+					float g[V > 1 ? V : 2], unit[V > 1 ? V : 2], scale[V];
+					unit_parameters<P, V>(p.scale, first, p.width, 1.f, scale);
+#pragma unroll
+					for(int j = 0; j < V; ++j) {
+						g[j] = (j % 2 == 0 ? vd.v[j / 2].x : vd.v[j / 2].y) * scale[j];
+						unit[j] = ((j % 2 == 0 ? vx.v[j / 2].x : vx.v[j / 2].y) - mean) * inv;
+					}
+					f(first, g, unit);
+				}
 			}
+		};
+		float sumG = 0.f, sumGu = 0.f;
+		each(false, [&](int, const float* g, const float* unit) {
+#pragma unroll
+			for(int j = 0; j < V; ++j) {
+				sumG += g[j];
+				sumGu = fmaf(g[j], unit[j], sumGu);
+			}
+		});
+		const float meanG = block_sum(sumG, slots[phase][0]) * overWidth;
+		const float meanGu = block_sum(sumGu, slots[phase][1]) * overWidth;
+		T* const out = static_cast<T*>(p.out) + r * p.outRow;
+		each(true, [&](int first, float* g, const float* unit) {
+#pragma unroll
+			for(int j = 0; j < V; ++j) g[j] = ((g[j] - meanG) - unit[j] * meanGu) * inv;
+			store_unit<T, V>(out, first, p.width, g);
+		});
+	}
+}
+
+// The sums of dy u and dy over a slice of the rows, a thread per column (two of 16 bits where rows are aligned for it).
+template<typename T, int W>
+__global__ void __launch_bounds__(256) norm_sums_kernel(const NormParams p)
+{
+	const int column = (blockIdx.x * 256 + threadIdx.x) * W;
+	if(column >= p.width) return;
+	const T* const x = static_cast<const T*>(p.x) + column;
+	const T* const dy = static_cast<const T*>(p.dy) + column;
+	float ds[W], db[W];
+#pragma unroll
+	for(int w = 0; w < W; ++w) ds[w] = db[w] = 0.f;
+#pragma unroll 8
+	for(int r = blockIdx.y; r < p.height; r += gridDim.y) {
+		const float mean = __ldg(p.mean + r), inv = __ldg(p.inv + r);
+		float vx[W], vd[W];
+		if constexpr(W == 2) {
+			const float2 a = unpack2<T>(*reinterpret_cast<const uint32_t*>(x + r * p.xRow)), b = unpack2<T>(*reinterpret_cast<const uint32_t*>(dy + r * p.dyRow));
+			vx[0] = a.x; vx[1] = a.y; vd[0] = b.x; vd[1] = b.y;
+		} else {
+			vx[0] = to_float(x[r * p.xRow]);
+			vd[0] = to_float(dy[r * p.dyRow]);
 		}
-		started = true;
-		const float meanG = row_sum(sumG, MAX_WARPS * 32, slots[phase][0]) * overWidth;
-		const float meanGu = row_sum(sumGu, MAX_WARPS * 32, slots[phase][1]) * overWidth;
-		for(int i = threadIdx.x; i < p.width; i += blockDim.x) {
-			const float unit = (to_float(x[i]) - mean) * inv;
-			const float s = p.scale != nullptr ? to_float(static_cast<const P*>(p.scale)[i]) : 1.f;
-			out[i] = from_float<T>((fmaf(to_float(dy[i]), s, -meanG) - unit * meanGu) * inv);
+#pragma unroll
+		for(int w = 0; w < W; ++w) {
+			ds[w] = fmaf(vd[w], (vx[w] - mean) * inv, ds[w]);
+			db[w] += vd[w];
 		}
+	}
+	float* const mine = p.partial + static_cast<long long>(blockIdx.y) * 2 * p.width;
+#pragma unroll
+	for(int w = 0; w < W; ++w) {
+		mine[column + w] = ds[w];
+		mine[p.width + column + w] = db[w];
 	}
 }
 
@@ -515,12 +662,17 @@ Shape shape_of(int type, int height, int width, bool alike, bool aligned, bool f
 				if(warps_for(h) * h < warps_for(hold) * hold) hold = h;
 			}
 		}
-		s.threads = s.lanes = (s.wide ? MAX_WARPS : warps_for(hold)) * 32;
+		s.threads = s.lanes = (s.wide ? MAX_ROW_WARPS : warps_for(hold)) * 32;
 		s.rowsAtOnce = 1;
 		s.units = alike ? (units + s.lanes - 1) / s.lanes : 8;
 	}
 	// at most: the launch goes by what fits (launch_rows)
-	const int most_blocks = sm_count() * (s.wide ? 2 : 1024 / s.threads > 1 ? 1024 / s.threads : 1) + s.unit;
+	if(s.wide) { // of the parameters' sums: slices of the rows, eight blocks per SM with those side by side
+		const int across = (width + 511) / 512, slices = (sm_count() * 8 + across - 1) / across;
+		s.blocks = height < slices ? height : slices;
+		return s;
+	}
+	const int most_blocks = sm_count() * (1024 / s.threads > 1 ? 1024 / s.threads : 1) + s.unit;
 	const int wanted = (height + s.rowsAtOnce - 1) / s.rowsAtOnce;
 	s.blocks = wanted < most_blocks ? wanted : most_blocks / s.unit * s.unit;
 	return s;
@@ -605,10 +757,48 @@ void launch_forward_units(const NormParams& p, const Shape& s, cudaStream_t stre
 	}
 }
 
+// Blocks of a kernel for long rows: two on an SM where their shared memory allows it.
+template<Kernel STAGED, Kernel AGAIN>
+void launch_wide(const NormParams& p, long long bytes, cudaStream_t stream)
+{
+	const int most = sm_count() * (bytes > 100 * 1024 && bytes <= WIDE_BYTES ? 1 : 2);
+	const int blocks = p.height < most ? p.height : most;
+	if(bytes <= WIDE_BYTES) {
+		cudaFuncSetAttribute(STAGED, cudaFuncAttributeMaxDynamicSharedMemorySize, WIDE_BYTES);
+		STAGED<<<blocks, WIDE_THREADS, static_cast<size_t>(bytes), stream>>>(p);
+	} else {
+		AGAIN<<<blocks, WIDE_THREADS, 0, stream>>>(p);
+	}
+}
+
+template<typename T, typename P, int V>
+void launch_forward_wide(const NormParams& p, cudaStream_t stream)
+{
+	const long long bytes = ((p.width + 2ll * V - 1) / V + 1) * 16;
+	launch_wide<norm_forward_wide_kernel<T, P, V, true>, norm_forward_wide_kernel<T, P, V, false>>(p, bytes, stream);
+}
+
+template<typename T, typename P, int V>
+void launch_backward_wide(const NormParams& p, int slices, cudaStream_t stream)
+{
+	if(p.partial != nullptr) { // first: dx may take the place of dy or x
+		const bool pairs = sizeof(T) == 2 && p.width % 2 == 0 && p.xRow % 2 == 0 && p.dyRow % 2 == 0
+			&& ((reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.dy)) & 3u) == 0;
+		constexpr int W = sizeof(T) == 2 ? 2 : 1;
+		const int perBlock = pairs ? 256 * W : 256;
+		const dim3 grid((p.width + perBlock - 1) / perBlock, slices);
+		if(pairs) norm_sums_kernel<T, W><<<grid, 256, 0, stream>>>(p);
+		else norm_sums_kernel<T, 1><<<grid, 256, 0, stream>>>(p);
+		count_launch();
+	}
+	const long long bytes = 2 * ((p.width + 2ll * V - 1) / V + 1) * 16;
+	launch_wide<norm_backward_wide_kernel<T, P, V, true>, norm_backward_wide_kernel<T, P, V, false>>(p, bytes, stream);
+}
+
 template<typename T, typename P>
 void launch_forward(const NormParams& p, const Shape& s, cudaStream_t stream)
 {
-	if(s.wide) norm_forward_wide_kernel<T, P><<<s.blocks, s.threads, 0, stream>>>(p);
+	if(s.wide) s.unit == 1 ? launch_forward_wide<T, P, 1>(p, stream) : launch_forward_wide<T, P, Unit16<T>::N>(p, stream);
 	else if(s.unit == 1) launch_forward_rows<T, P, 1, 8, true>(p, s, stream);
 	else if(s.edges) launch_forward_units<T, P, true>(p, s, stream);
 	else launch_forward_units<T, P, false>(p, s, stream);
@@ -630,7 +820,7 @@ template<typename T, typename P>
 void launch_backward(const NormParams& p, const Shape& s, void* scaleDiff, void* freeDiff, cudaStream_t stream)
 {
 	int blocks = s.blocks;
-	if(s.wide) norm_backward_wide_kernel<T, P><<<s.blocks, s.threads, 0, stream>>>(p);
+	if(s.wide) s.unit == 1 ? launch_backward_wide<T, P, 1>(p, blocks, stream) : launch_backward_wide<T, P, Unit16<T>::N>(p, blocks, stream);
 	else if(s.unit == 1) blocks = launch_rows<norm_backward_kernel<T, P, 1, 8, true>>(p, s, stream);
 	else if(s.edges) blocks = launch_backward_units<T, P, true>(p, s, stream);
 	else blocks = launch_backward_units<T, P, false>(p, s, stream);
@@ -671,6 +861,7 @@ int nb200_layer_normalization(void* stream, int type, int parameter_type, const 
 {
 	if(!sizes_valid(type, parameter_type, height, width) || x_row_size < width || y_row_size < width) return NB200_EINVAL;
 	if(height == 0) return NB200_OK;
+	if(height > (1 << 30)) return NB200_ETOOBIG;
 	if(x == nullptr || y == nullptr || !type_aligned(x, type) || !type_aligned(y, type)
 		|| !type_aligned(scale, parameter_type) || !type_aligned(free_term, parameter_type)) return NB200_EINVAL;
 	if(device_status_word() == nullptr) return NB200_ENODEVICE;
@@ -711,6 +902,7 @@ int nb200_layer_normalization_backward(void* stream, int type, int parameter_typ
 		|| !type_aligned(x, type) || !type_aligned(dy, type) || !type_aligned(dx, type)
 		|| (parameters && scratch == nullptr))) return NB200_EINVAL;
 	if(height == 0 && !parameters) return NB200_OK;
+	if(height > (1 << 30)) return NB200_ETOOBIG;
 	if(device_status_word() == nullptr) return NB200_ENODEVICE;
 	if(height == 0) { // sums over no rows
 		const int grid = grid_for(width, 256);
