@@ -10,6 +10,7 @@
 #include <torch/csrc/utils/python_arg_parser.h>
 #include <ATen/ATen.h>
 #include <ATen/PythonTorchFunctionTLS.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include "../../include/neoml_b200.h"
 
@@ -265,10 +266,424 @@ PyObject* vector_op(PyObject*, PyObject* const* a, Py_ssize_t count)
 	});
 }
 
+// ---- operators of language models: fp32, fp16 and bf16 data on the device that it is on ------------------------------
+
+const at::Tensor& any_tensor(PyObject* o) // parameters too
+{
+	if(!THPVariable_Check(o) || (!THPVariable_CheckExact(o) && torch::check_has_torch_function(o))) throw NotHere();
+	const at::Tensor& t = THPVariable_Unpack(o);
+	if(!t.has_storage() || !t.is_cuda() || t.is_conj() || t.is_neg()) throw NotHere();
+	return t;
+}
+
+int type_code(const at::Tensor& t)
+{
+	switch(t.scalar_type()) {
+		case at::kFloat: return NB200_TYPE_FP32;
+		case at::kHalf: return NB200_TYPE_FP16;
+		case at::kBFloat16: return NB200_TYPE_BF16;
+		default: throw NotHere();
+	}
+}
+
+struct Matrix {
+	int height, width;
+	long long row;
+};
+Matrix matrix(const at::Tensor& t)
+{
+	const int64_t dims = t.dim();
+	if(dims < 1 || t.size(dims - 1) < 1) throw NotHere();
+	Matrix m;
+	m.width = size_of(t, static_cast<int>(dims) - 1);
+	m.row = m.width;
+	if(dims == 2 && t.size(0) > 1) {
+		if((m.width > 1 && t.stride(1) != 1) || t.stride(0) < m.width) throw NotHere();
+		m.height = size_of(t, 0);
+		m.row = t.stride(0);
+		return m;
+	}
+	if(!t.is_contiguous()) throw NotHere();
+	const int64_t rows = t.numel() / m.width;
+	if(rows > INT32_MAX) throw NotHere();
+	m.height = static_cast<int>(rows);
+	return m;
+}
+
+// An optional contiguous vector of `count` elements of the type, on the device.
+void* vector(PyObject* o, int64_t count, at::ScalarType type, const at::Device& device)
+{
+	if(o == Py_None) return nullptr;
+	const at::Tensor& t = any_tensor(o);
+	if(t.numel() != count || !t.is_contiguous() || t.scalar_type() != type || t.device() != device) throw NotHere();
+	return t.data_ptr();
+}
+template<typename T>
+T* vector_of(PyObject* o, int64_t count, at::ScalarType type, const at::Device& device)
+{
+	return static_cast<T*>(vector(o, count, type, device));
+}
+
+at::Tensor empty(at::IntArrayRef sizes, at::ScalarType type, const at::Device& device)
+{
+	return at::empty(sizes, at::TensorOptions().dtype(type).device(device));
+}
+at::Tensor empty_or(PyObject* given, const at::Tensor& like) // None: a new dense tensor
+{
+	if(given == Py_None) return empty(like.sizes(), like.scalar_type(), like.device());
+	const at::Tensor& t = any_tensor(given);
+	if(t.sizes() != like.sizes() || t.scalar_type() != like.scalar_type() || t.device() != like.device()) throw NotHere();
+	return t;
+}
+
+// The device of the call: current while it lasts, with torch's current stream of that device.
+struct On {
+	c10::cuda::OptionalCUDAGuard guard;
+	void* stream;
+	explicit On(const at::Device& device)
+	{
+		if(c10::cuda::current_device() != device.index()) guard.set_device(device);
+		stream = c10::cuda::getCurrentCUDAStream(device.index()).stream();
+	}
+};
+
+PyObject* answers(int rc, std::initializer_list<const at::Tensor*> results) // null: None
+{
+	if(rc != NB200_OK) return PyLong_FromLong(rc);
+	PyObject* tuple = PyTuple_New(static_cast<Py_ssize_t>(results.size()));
+	if(tuple == nullptr) return nullptr;
+	Py_ssize_t i = 0;
+	for(const at::Tensor* t : results) {
+		PyObject* o = t == nullptr ? Py_NewRef(Py_None) : THPVariable_Wrap(*t);
+		if(o == nullptr) {
+			Py_DECREF(tuple);
+			return nullptr;
+		}
+		PyTuple_SET_ITEM(tuple, i++, o);
+	}
+	return tuple;
+}
+
+at::ScalarType parameter_type(std::initializer_list<PyObject*> parameters, const at::Tensor& x)
+{
+	for(PyObject* o : parameters) {
+		if(o == Py_None) continue;
+		const at::ScalarType type = any_tensor(o).scalar_type();
+		if(type != x.scalar_type() && type != at::kFloat) throw NotHere();
+		return type;
+	}
+	return x.scalar_type();
+}
+int code_of(at::ScalarType type)
+{
+	return type == at::kFloat ? NB200_TYPE_FP32 : type == at::kHalf ? NB200_TYPE_FP16 : NB200_TYPE_BF16;
+}
+
+// source, scale, free_term, epsilon, result
+PyObject* layer_normalization(PyObject*, PyObject* const* a, Py_ssize_t count)
+{
+	return guarded(count, 5, [&]() -> PyObject* {
+		const at::Tensor& x = any_tensor(a[0]);
+		const int type = type_code(x);
+		const Matrix m = matrix(x);
+		const at::Device device = x.device();
+		const at::ScalarType parameter = parameter_type({ a[1], a[2] }, x);
+		const void *scale = vector(a[1], m.width, parameter, device), *free = vector(a[2], m.width, parameter, device);
+		const float epsilon = number(a[3]);
+		at::Tensor y = empty_or(a[4], x);
+		const Matrix my = matrix(y);
+		const at::IntArrayRef rows = x.sizes().slice(0, x.dim() - 1);
+		at::Tensor mean = empty(rows, at::kFloat, device), inverse = empty(rows, at::kFloat, device);
+		const On on(device);
+		const void* xp = x.data_ptr();
+		void* yp = y.data_ptr();
+		float *mp = static_cast<float*>(mean.data_ptr()), *ip = static_cast<float*>(inverse.data_ptr());
+		const int rc = without_gil([&] {
+			return nb200_layer_normalization(on.stream, type, code_of(parameter), xp, m.height, m.width, m.row, scale, free, epsilon, yp, my.row, mp, ip);
+		});
+		return answers(rc, { &y, &mean, &inverse });
+	});
+}
+
+// result_diff, source, mean, inverse_deviation, scale (not None, or parameters False), source_diff, parameters
+PyObject* layer_normalization_backward(PyObject*, PyObject* const* a, Py_ssize_t count)
+{
+	return guarded(count, 7, [&]() -> PyObject* {
+		const at::Tensor &dy = any_tensor(a[0]), &x = any_tensor(a[1]);
+		const int type = type_code(x);
+		if(dy.sizes() != x.sizes() || dy.scalar_type() != x.scalar_type() || dy.device() != x.device()) throw NotHere();
+		const Matrix m = matrix(x), md = matrix(dy);
+		const at::Device device = x.device();
+		const bool parameters = truth(a[6]);
+		if(parameters && a[4] == Py_None) throw NotHere();
+		const at::ScalarType parameter = parameter_type({ a[4] }, x);
+		const float *mean = vector_of<float>(a[2], m.height, at::kFloat, device), *inverse = vector_of<float>(a[3], m.height, at::kFloat, device);
+		if(mean == nullptr || inverse == nullptr) throw NotHere();
+		const void* scale = vector(a[4], m.width, parameter, device);
+		at::Tensor dx = empty_or(a[5], x);
+		const Matrix mx = matrix(dx);
+		const On on(device);
+		at::Tensor ds, db, scratch;
+		void *dsp = nullptr, *dbp = nullptr;
+		float* room = nullptr;
+		if(parameters) {
+			ds = empty({ m.width }, parameter, device);
+			db = empty({ m.width }, parameter, device);
+			scratch = empty({ static_cast<int64_t>(nb200_layer_normalization_backward_scratch_floats(type, m.height, m.width)) }, at::kFloat, device);
+			dsp = ds.data_ptr();
+			dbp = db.data_ptr();
+			room = static_cast<float*>(scratch.data_ptr());
+		}
+		const void *xp = x.data_ptr(), *dyp = dy.data_ptr();
+		void* dxp = dx.data_ptr();
+		const int rc = without_gil([&] {
+			return nb200_layer_normalization_backward(on.stream, type, code_of(parameter), dyp, md.row, xp, m.height, m.width, m.row, scale, mean,
+				inverse, dxp, mx.row, dsp, dbp, room);
+		});
+		return answers(rc, { &dx, parameters ? &ds : nullptr, parameters ? &db : nullptr });
+	});
+}
+
+struct Sequences {
+	nb200_recurrence_desc desc;
+	const at::Tensor* z;
+	const void *zp, *fp, *ip;
+};
+void steps(const at::Tensor& t, const at::Tensor& like, long long* batch, long long* row)
+{
+	if(t.sizes() != like.sizes() || t.scalar_type() != like.scalar_type() || t.device() != like.device()
+		|| (t.size(2) > 1 && t.stride(2) != 1)) throw NotHere();
+	*batch = t.size(0) > 1 ? t.stride(0) : 0;
+	*row = t.size(1) > 1 ? t.stride(1) : 0;
+}
+Sequences sequences(PyObject* update, PyObject* forget, PyObject* input)
+{
+	Sequences s = {};
+	const at::Tensor &z = any_tensor(update), &f = any_tensor(forget);
+	if(z.dim() != 3) throw NotHere();
+	s.z = &z;
+	s.desc.batch = size_of(z, 0); s.desc.length = size_of(z, 1); s.desc.channels = size_of(z, 2);
+	steps(z, z, &s.desc.update_batch, &s.desc.update_row);
+	steps(f, z, &s.desc.forget_batch, &s.desc.forget_row);
+	s.zp = z.data_ptr();
+	s.fp = f.data_ptr();
+	if(input != Py_None) {
+		const at::Tensor& i = any_tensor(input);
+		steps(i, z, &s.desc.input_batch, &s.desc.input_row);
+		s.ip = i.data_ptr();
+		if(s.ip == nullptr) throw NotHere(); // an empty one: the Python code tells it from none
+	}
+	return s;
+}
+
+// update, forget, input, initial_state, lengths, result, final_state
+PyObject* gated_recurrence(PyObject*, PyObject* const* a, Py_ssize_t count)
+{
+	return guarded(count, 7, [&]() -> PyObject* {
+		const Sequences s = sequences(a[0], a[1], a[2]);
+		const at::Tensor& z = *s.z;
+		const int type = type_code(z);
+		const at::Device device = z.device();
+		const int64_t states = z.size(0) * z.size(2);
+		const float* first = vector_of<float>(a[3], states, at::kFloat, device);
+		const int* lengths = vector_of<int>(a[4], z.size(0), at::kInt, device);
+		at::Tensor h = empty_or(a[5], z);
+		if(!h.is_contiguous()) throw NotHere();
+		float* last = vector_of<float>(a[6], states, at::kFloat, device);
+		at::Tensor state = a[6] == Py_None ? empty({ z.size(0), z.size(2) }, at::kFloat, device) : any_tensor(a[6]);
+		if(a[6] == Py_None) last = static_cast<float*>(state.data_ptr());
+		const On on(device);
+		void* hp = h.data_ptr();
+		const int rc = without_gil([&] { return nb200_gated_recurrence(on.stream, type, &s.desc, s.zp, s.fp, s.ip, first, lengths, hp, last); });
+		return answers(rc, { &h, &state });
+	});
+}
+
+// result_diff, result, update, forget, input, initial_state, final_state_diff, lengths
+PyObject* gated_recurrence_backward(PyObject*, PyObject* const* a, Py_ssize_t count)
+{
+	return guarded(count, 8, [&]() -> PyObject* {
+		const Sequences s = sequences(a[2], a[3], a[4]);
+		const at::Tensor &z = *s.z, &dh = any_tensor(a[0]), &h = any_tensor(a[1]);
+		const int type = type_code(z);
+		const at::Device device = z.device();
+		long long dhBatch, dhRow, hBatch, hRow;
+		steps(dh, z, &dhBatch, &dhRow);
+		steps(h, z, &hBatch, &hRow);
+		if(!h.is_contiguous()) throw NotHere();
+		const int64_t states = z.size(0) * z.size(2);
+		const float *first = vector_of<float>(a[5], states, at::kFloat, device), *lastDiff = vector_of<float>(a[6], states, at::kFloat, device);
+		const int* lengths = vector_of<int>(a[7], z.size(0), at::kInt, device);
+		const bool input = a[4] != Py_None;
+		at::Tensor dz = empty(z.sizes(), z.scalar_type(), device), df = empty(z.sizes(), z.scalar_type(), device), di;
+		if(input) di = empty(z.sizes(), z.scalar_type(), device);
+		at::Tensor dfirst = empty({ z.size(0), z.size(2) }, at::kFloat, device);
+		const On on(device);
+		const void *dhp = dh.data_ptr(), *hp = h.data_ptr();
+		void *dzp = dz.data_ptr(), *dfp = df.data_ptr(), *dip = input ? di.data_ptr() : nullptr;
+		float* dfirstp = static_cast<float*>(dfirst.data_ptr());
+		const int rc = without_gil([&] {
+			return nb200_gated_recurrence_backward(on.stream, type, &s.desc, dhp, dhBatch, dhRow, hp, s.zp, s.fp, s.ip, first, lastDiff, lengths, dzp, dfp,
+				dip, dfirstp);
+		});
+		return answers(rc, { &dz, &df, input ? &di : nullptr, &dfirst });
+	});
+}
+
+struct Taught {
+	const at::Tensor* logits;
+	Matrix m;
+	int type, teacherType, kept;
+	const void* teacher;
+	const int* indices;
+	float temperature;
+};
+Taught taught(PyObject* logits, PyObject* teacher, PyObject* indices, PyObject* temperature)
+{
+	Taught t = {};
+	const at::Tensor &x = any_tensor(logits), &top = any_tensor(teacher), &at = any_tensor(indices);
+	t.logits = &x;
+	t.type = type_code(x);
+	t.m = matrix(x);
+	if(top.dim() != x.dim() || top.sizes() != at.sizes() || top.sizes().slice(0, top.dim() - 1) != x.sizes().slice(0, x.dim() - 1)) throw NotHere();
+	t.kept = size_of(top, static_cast<int>(top.dim()) - 1);
+	const at::ScalarType type = parameter_type({ teacher }, x);
+	t.teacherType = code_of(type);
+	t.teacher = vector(teacher, static_cast<int64_t>(t.m.height) * t.kept, type, x.device());
+	t.indices = vector_of<int>(indices, static_cast<int64_t>(t.m.height) * t.kept, at::kInt, x.device());
+	if(!PyFloat_CheckExact(temperature)) throw NotHere();
+	const double tau = PyFloat_AS_DOUBLE(temperature);
+	if(!(tau > 0.0) || !(tau < 1e38)) throw NotHere();
+	t.temperature = static_cast<float>(tau);
+	return t;
+}
+
+// logits, teacher_logits, teacher_indices, temperature
+PyObject* distillation_loss(PyObject*, PyObject* const* a, Py_ssize_t count)
+{
+	return guarded(count, 4, [&]() -> PyObject* {
+		const Taught t = taught(a[0], a[1], a[2], a[3]);
+		const at::Tensor& x = *t.logits;
+		const at::IntArrayRef rows = x.sizes().slice(0, x.dim() - 1);
+		at::Tensor loss = empty(rows, at::kFloat, x.device()), logSum = empty(rows, at::kFloat, x.device());
+		const On on(x.device());
+		const void* xp = x.data_ptr();
+		float *lp = static_cast<float*>(loss.data_ptr()), *sp = static_cast<float*>(logSum.data_ptr());
+		const int rc = without_gil([&] {
+			return nb200_distillation_loss(on.stream, t.type, t.teacherType, xp, t.m.height, t.m.width, t.m.row, t.teacher, t.indices, t.kept,
+				t.temperature, lp, sp);
+		});
+		return answers(rc, { &loss, &logSum });
+	});
+}
+
+// loss_diff, logits, teacher_logits, teacher_indices, log_sum, temperature, result
+PyObject* distillation_loss_backward(PyObject*, PyObject* const* a, Py_ssize_t count)
+{
+	return guarded(count, 7, [&]() -> PyObject* {
+		const Taught t = taught(a[1], a[2], a[3], a[5]);
+		const at::Tensor& x = *t.logits;
+		const float *diff = vector_of<float>(a[0], t.m.height, at::kFloat, x.device()), *logSum = vector_of<float>(a[4], t.m.height, at::kFloat, x.device());
+		if(a[0] == Py_None || a[4] == Py_None) throw NotHere();
+		at::Tensor out = empty_or(a[6], x);
+		const Matrix mo = matrix(out);
+		const On on(x.device());
+		const void* xp = x.data_ptr();
+		void* op = out.data_ptr();
+		const int rc = without_gil([&] {
+			return nb200_distillation_loss_backward(on.stream, t.type, t.teacherType, diff, xp, t.m.height, t.m.width, t.m.row, t.teacher, t.indices,
+				t.kept, t.temperature, logSum, op, mo.row);
+		});
+		return answer(rc, out);
+	});
+}
+
+struct Head {
+	const at::Tensor *x, *w;
+	Matrix m, mw;
+	int type;
+	const int* labels;
+};
+Head head(PyObject* hidden, PyObject* weights, PyObject* labels)
+{
+	Head h = {};
+	const at::Tensor &x = any_tensor(hidden), &w = any_tensor(weights);
+	h.x = &x;
+	h.w = &w;
+	h.type = type_code(x);
+	h.m = matrix(x);
+	if(w.dim() != 2 || w.size(0) < 1 || w.scalar_type() != x.scalar_type() || w.device() != x.device()) throw NotHere();
+	h.mw = matrix(w);
+	if(h.mw.width != h.m.width || any_tensor(labels).sizes() != x.sizes().slice(0, x.dim() - 1)) throw NotHere();
+	h.labels = vector_of<int>(labels, h.m.height, at::kInt, x.device());
+	return h;
+}
+at::Tensor head_scratch(const Head& h, bool backward)
+{
+	const size_t need = nb200_vocabulary_cross_entropy_scratch_bytes(h.type, h.x->data_ptr(), h.m.height, h.m.width, h.m.row, h.w->data_ptr(),
+		h.mw.height, h.mw.row, backward ? 1 : 0);
+	return empty({ static_cast<int64_t>(need) }, at::kByte, h.x->device());
+}
+
+// hidden, weights, labels
+PyObject* vocabulary_cross_entropy(PyObject*, PyObject* const* a, Py_ssize_t count)
+{
+	return guarded(count, 3, [&]() -> PyObject* {
+		const Head h = head(a[0], a[1], a[2]);
+		const at::Device device = h.x->device();
+		const at::IntArrayRef rows = h.x->sizes().slice(0, h.x->dim() - 1);
+		at::Tensor loss = empty(rows, at::kFloat, device), logSum = empty(rows, at::kFloat, device);
+		const On on(device);
+		at::Tensor scratch = head_scratch(h, false);
+		const void *xp = h.x->data_ptr(), *wp = h.w->data_ptr();
+		float *lp = static_cast<float*>(loss.data_ptr()), *sp = static_cast<float*>(logSum.data_ptr());
+		void* room = scratch.data_ptr();
+		const int rc = without_gil([&] {
+			return nb200_vocabulary_cross_entropy(on.stream, h.type, xp, h.m.height, h.m.width, h.m.row, wp, h.mw.height, h.mw.row, h.labels, lp, sp, room);
+		});
+		return answers(rc, { &loss, &logSum });
+	});
+}
+
+// loss_diff, hidden, weights, labels, log_sum, hidden_diff, weights_diff (True, False or a tensor)
+PyObject* vocabulary_cross_entropy_backward(PyObject*, PyObject* const* a, Py_ssize_t count)
+{
+	return guarded(count, 7, [&]() -> PyObject* {
+		const Head h = head(a[1], a[2], a[3]);
+		const at::Device device = h.x->device();
+		if(a[0] == Py_None || a[4] == Py_None) throw NotHere();
+		const float *diff = vector_of<float>(a[0], h.m.height, at::kFloat, device), *logSum = vector_of<float>(a[4], h.m.height, at::kFloat, device);
+		at::Tensor dx, dw;
+		void *dxp = nullptr, *dwp = nullptr;
+		long long dxRow = 0, dwRow = 0;
+		if(a[5] != Py_False) {
+			dx = empty_or(a[5] == Py_True ? Py_None : a[5], *h.x);
+			dxp = dx.data_ptr();
+			dxRow = matrix(dx).row;
+		}
+		if(a[6] != Py_False) {
+			dw = empty_or(a[6] == Py_True ? Py_None : a[6], *h.w);
+			dwp = dw.data_ptr();
+			dwRow = matrix(dw).row;
+		}
+		const On on(device);
+		at::Tensor scratch = head_scratch(h, true);
+		const void *xp = h.x->data_ptr(), *wp = h.w->data_ptr();
+		void* room = scratch.data_ptr();
+		const int rc = without_gil([&] {
+			return nb200_vocabulary_cross_entropy_backward(on.stream, h.type, diff, xp, h.m.height, h.m.width, h.m.row, wp, h.mw.height, h.mw.row,
+				h.labels, logSum, dxp, dxRow, dwp, dwRow, room);
+		});
+		return answers(rc, { a[5] != Py_False ? &dx : nullptr, a[6] != Py_False ? &dw : nullptr });
+	});
+}
+
 PyMethodDef methods[] = {
 #define FAST(name) { #name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr }
 	FAST(blob_convolution), FAST(multiply_by_transposed), FAST(batch_multiply_by_transposed), FAST(multiply_by_matrix),
-	FAST(transpose), FAST(vector_op),
+	FAST(transpose), FAST(vector_op), FAST(layer_normalization), FAST(layer_normalization_backward), FAST(gated_recurrence),
+	FAST(gated_recurrence_backward), FAST(distillation_loss), FAST(distillation_loss_backward), FAST(vocabulary_cross_entropy),
+	FAST(vocabulary_cross_entropy_backward),
 #undef FAST
 	{ nullptr, nullptr, 0, nullptr }
 };

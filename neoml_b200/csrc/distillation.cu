@@ -20,7 +20,8 @@ constexpr int WARPS = THREADS / 32;
 constexpr int KEPT_MAX = NB200_DISTILLATION_KEPT_MAX;
 constexpr int MAX_PARTS = 8;
 constexpr int UNROLL = 4;      // units in flight per thread
-constexpr float LOG2E = 1.4426950408889634f;
+constexpr int ENTRIES = (KEPT_MAX + THREADS - 1) / THREADS; // of the teacher, per thread
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 struct DistillParams {
 	const void* logits;
@@ -36,6 +37,13 @@ struct DistillParams {
 	float temperature;
 };
 
+__device__ __forceinline__ float exp2_fast(float x)
+{
+	float y;
+	asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+	return y;
+}
+
 // Maximum and the sum of 2^(x - maximum).
 struct Running {
 	float top, sum;
@@ -43,75 +51,75 @@ struct Running {
 	{
 		const float t = fmaxf(top, o.top);
 		const float at = t == -INFINITY ? 0.f : t;
-		sum = sum * exp2f(top - at) + o.sum * exp2f(o.top - at);
+		sum = sum * exp2_fast(top - at) + o.sum * exp2_fast(o.top - at);
 		top = t;
 	}
 };
 
-__device__ __forceinline__ float block_sum(float v, float* slots)
-{
-	v = warp_sum_all(v);
-	__syncthreads(); // slots of the call before
-	if((threadIdx.x & 31) == 0) slots[threadIdx.x >> 5] = v;
-	__syncthreads();
-	return warp_sum_all((threadIdx.x & 31) < WARPS ? slots[threadIdx.x & 31] : 0.f);
-}
-__device__ __forceinline__ float block_max(float v, float* slots)
-{
-	v = warp_max_all(v);
-	__syncthreads();
-	if((threadIdx.x & 31) == 0) slots[threadIdx.x >> 5] = v;
-	__syncthreads();
-	return warp_max_all((threadIdx.x & 31) < WARPS ? slots[threadIdx.x & 31] : -INFINITY);
-}
-
-struct Kept {
-	float p[KEPT_MAX];  // the teacher's probabilities; zero for entries that are not used
-	float z[KEPT_MAX];  // the student's logit
-	int at[KEPT_MAX];   // column, -1 for entries that are not used
+// The teacher's side of a row, or of some of its entries: maximum of x = log2(e) teacher / tau, sum of 2^(x - maximum), and the sum of
+// 2^(x - maximum) (ln 2 (x - maximum) - z / tau), z being the student's logit.  The loss is then
+// tau^2 (cross / sum - ln sum + log_sum): no term is larger than the distributions' logarithms, whatever the logits' common offset.
+struct Taught {
+	float top, sum, cross;
+	__device__ __forceinline__ void join(const Taught& o)
+	{
+		const float t = fmaxf(top, o.top);
+		if(t == -INFINITY) return; // neither has an entry
+		const float d1 = top - t, d2 = o.top - t, f1 = exp2_fast(d1), f2 = exp2_fast(d2);
+		// what has vanished adds nothing, not even an infinite loss times zero
+		cross = (f1 == 0.f ? 0.f : f1 * fmaf(d1 * LN2, sum, cross)) + (f2 == 0.f ? 0.f : f2 * fmaf(d2 * LN2, o.sum, o.cross));
+		sum = f1 * sum + f2 * o.sum;
+		top = t;
+	}
 };
 
-// The teacher's probabilities of a row.  An index outside the vocabulary marks an entry that is not used.  False: no entry is.
+// A thread's entries of the teacher.
+struct Entry {
+	float x, z; // x: minus infinity for one that is not used
+	int at;     // column; -1 for one that is not used
+};
+
 template<typename T, typename P>
-__device__ __forceinline__ bool teacher_row(const DistillParams& p, int r, const T* logits, Kept& kept, float* slots)
+__device__ __forceinline__ void load_entries(const DistillParams& p, int r, const T* logits, Entry (&entries)[ENTRIES])
 {
 	const P* const teacher = static_cast<const P*>(p.teacher) + static_cast<long long>(r) * p.kept;
 	const int* const indices = p.indices + static_cast<long long>(r) * p.kept;
 	const float c = LOG2E / p.temperature;
-	float top = -INFINITY, any = 0.f;
-	for(int k = threadIdx.x; k < p.kept; k += THREADS) {
+#pragma unroll
+	for(int e = 0; e < ENTRIES; ++e) {
+		const int k = e * THREADS + threadIdx.x;
+		entries[e] = { -INFINITY, 0.f, -1 };
+		if(k >= p.kept) continue;
 		const int at = __ldg(indices + k);
-		const bool used = at >= 0 && at < p.vocabulary;
-		const float x = used ? to_float(teacher[k]) * c : -INFINITY;
-		kept.at[k] = used ? at : -1;
-		kept.z[k] = used ? to_float(logits[at]) : 0.f;
-		kept.p[k] = x;
-		if(used) any = 1.f;
-		top = fmaxf(top, x);
+		if(at < 0 || at >= p.vocabulary) continue;
+		entries[e].at = at;
+		entries[e].x = to_float(teacher[k]) * c;
+		entries[e].z = to_float(logits[at]);
 	}
-	top = block_max(top, slots);
-	any = block_max(any, slots);
-	const float reference = top == -INFINITY ? 0.f : top;
-	float sum = 0.f;
-	for(int k = threadIdx.x; k < p.kept; k += THREADS) {
-		const float e = exp2f(kept.p[k] - reference);
-		kept.p[k] = e;
-		sum += e;
+}
+
+// The largest of a unit's elements.
+template<typename T>
+__device__ __forceinline__ float unit_top(const uint4& raw)
+{
+	if constexpr(sizeof(T) == 4) {
+		return fmaxf(fmaxf(__uint_as_float(raw.x), __uint_as_float(raw.y)), fmaxf(__uint_as_float(raw.z), __uint_as_float(raw.w)));
+	} else {
+		using T2 = typename PairOf<T>::type;
+		const uint32_t w[4] = { raw.x, raw.y, raw.z, raw.w };
+		const T2 a = __hmax2(__hmax2(*reinterpret_cast<const T2*>(w), *reinterpret_cast<const T2*>(w + 1)),
+			__hmax2(*reinterpret_cast<const T2*>(w + 2), *reinterpret_cast<const T2*>(w + 3)));
+		const float2 f = unpack2<T>(*reinterpret_cast<const uint32_t*>(&a));
+		return fmaxf(f.x, f.y);
 	}
-	sum = block_sum(sum, slots);
-	if(any == 0.f || sum == 0.f) return false; // a row whose teacher kept nothing, or nothing but minus infinity
-	const float over = 1.f / sum;
-	for(int k = threadIdx.x; k < p.kept; k += THREADS) kept.p[k] *= over;
-	return true;
 }
 
 template<typename T, typename P, int V>
 __global__ void __launch_bounds__(THREADS) distillation_forward_kernel(const DistillParams p)
 {
-	__shared__ Kept kept;
-	__shared__ float slots[WARPS];
 	__shared__ Running parts[MAX_PARTS];
 	__shared__ Running warpsOf[WARPS];
+	__shared__ Taught taughtOf[WARPS];
 	const int blocks = p.parts, r = blockIdx.x / blocks, rank = blockIdx.x - r * blocks;
 	if(blocks > 1) cg::this_cluster().sync(); // the others' shared memory exists from here on
 	const T* const x = static_cast<const T*>(p.logits) + r * p.row;
@@ -124,77 +132,100 @@ __global__ void __launch_bounds__(THREADS) distillation_forward_kernel(const Dis
 	row.p = x;
 	row.begin = x;                     // no element of another row is touched
 	row.end = x + p.vocabulary;
+	Entry entries[ENTRIES];
+	if(rank == 0) load_entries<T, P>(p, r, x, entries);
 	Running mine = { -INFINITY, 0.f };
 	for(int u0 = rank * perBlock; u0 < end; u0 += THREADS * UNROLL) {
 		uint4 raw[UNROLL];
+		const int mineFirst = u0 + threadIdx.x, mineLast = mineFirst + (UNROLL - 1) * THREADS;
+		if(mineLast < end && mineFirst * V - offset >= 0 && mineLast * V - offset + V <= p.vocabulary) { // whole units
 #pragma unroll
-		for(int k = 0; k < UNROLL; ++k) {
-			const int u = u0 + k * THREADS + threadIdx.x;
-			raw[k] = make_uint4(0u, 0u, 0u, 0u);
-			if(u < end) load_unit<T, V>(row, u * V - offset, p.vocabulary, raw[k]);
-		}
-		float top = mine.top;
-		float v[UNROLL][V];
+			for(int k = 0; k < UNROLL; ++k) raw[k] = *reinterpret_cast<const uint4*>(x + ((mineFirst + k * THREADS) * V - offset));
+			float top = unit_top<T>(raw[0]);
 #pragma unroll
-		for(int k = 0; k < UNROLL; ++k) {
-			const int u = u0 + k * THREADS + threadIdx.x, first = u * V - offset;
-			unit_floats<T, V>(raw[k], v[k]);
-			const bool whole = u < end && first >= 0 && first + V <= p.vocabulary;
+			for(int k = 1; k < UNROLL; ++k) top = fmaxf(top, unit_top<T>(raw[k]));
+			top = fmaxf(mine.top, top * c);
+			const float at = top == -INFINITY ? 0.f : top;
+			float2 sums = make_float2(mine.sum * exp2_fast(mine.top - at), 0.f);
 #pragma unroll
-			for(int j = 0; j < V; ++j) {
-				v[k][j] = whole || (u < end && inside<V>(first, j, p.vocabulary)) ? v[k][j] * c : -INFINITY;
-				top = fmaxf(top, v[k][j]);
+			for(int k = 0; k < UNROLL; ++k) {
+				float v[V];
+				unit_floats<T, V>(raw[k], v);
+#pragma unroll
+				for(int j = 0; j < V; j += 2) {
+					const float2 e = fma2(make_float2(v[j], v[j + 1]), both(c), both(-at));
+					sums = add2(sums, make_float2(exp2_fast(e.x), exp2_fast(e.y)));
+				}
+			}
+			mine.sum = sums.x + sums.y;
+			mine.top = top;
+		} else {
+			for(int k = 0; k < UNROLL; ++k) {
+				const int u = mineFirst + k * THREADS, first = u * V - offset;
+				if(u >= end) break;
+				uint4 one;
+				load_unit<T, V>(row, first, p.vocabulary, one);
+				float v[V];
+				unit_floats<T, V>(one, v);
+				float top = mine.top;
+#pragma unroll
+				for(int j = 0; j < V; ++j) {
+					v[j] = inside<V>(first, j, p.vocabulary) ? v[j] * c : -INFINITY;
+					top = fmaxf(top, v[j]);
+				}
+				const float at = top == -INFINITY ? 0.f : top;
+				mine.sum *= exp2_fast(mine.top - at);
+#pragma unroll
+				for(int j = 0; j < V; ++j) mine.sum += exp2_fast(v[j] - at);
+				mine.top = top;
 			}
 		}
-		const float at = top == -INFINITY ? 0.f : top;
-		mine.sum *= exp2f(mine.top - at);
+	}
+	Taught taught = { -INFINITY, 0.f, 0.f };
+	if(rank == 0) {
 #pragma unroll
-		for(int k = 0; k < UNROLL; ++k) {
-#pragma unroll
-			for(int j = 0; j < V; ++j) mine.sum += exp2f(v[k][j] - at);
+		for(int e = 0; e < ENTRIES; ++e) {
+			// (not a number counts as an entry)
+			if(entries[e].at >= 0 && entries[e].x != -INFINITY) taught.join({ entries[e].x, 1.f, -entries[e].z / p.temperature });
 		}
-		mine.top = top;
 	}
 #pragma unroll
 	for(int o = 16; o > 0; o >>= 1) {
-		const Running other = { __shfl_xor_sync(0xffffffffu, mine.top, o), __shfl_xor_sync(0xffffffffu, mine.sum, o) };
-		mine.join(other);
+		mine.join({ __shfl_xor_sync(0xffffffffu, mine.top, o), __shfl_xor_sync(0xffffffffu, mine.sum, o) });
+		taught.join({ __shfl_xor_sync(0xffffffffu, taught.top, o), __shfl_xor_sync(0xffffffffu, taught.sum, o),
+			__shfl_xor_sync(0xffffffffu, taught.cross, o) });
 	}
-	if((threadIdx.x & 31) == 0) warpsOf[threadIdx.x >> 5] = mine;
+	if((threadIdx.x & 31) == 0) {
+		warpsOf[threadIdx.x >> 5] = mine;
+		taughtOf[threadIdx.x >> 5] = taught;
+	}
 	__syncthreads();
-	mine = warpsOf[0];
-#pragma unroll
-	for(int w = 1; w < WARPS; ++w) mine.join(warpsOf[w]);
 	if(blocks > 1) {
 		cg::cluster_group cluster = cg::this_cluster();
-		if(threadIdx.x == 0) *cluster.map_shared_rank(&parts[rank], 0) = mine;
-		cluster.sync();
-		if(rank != 0) return;
-		mine = parts[0];
-		for(int k = 1; k < blocks; ++k) mine.join(parts[k]);
-	}
-	// mine.top is in units of log 2
-	const float logSum = mine.top / LOG2E + logf(mine.sum);
-	const bool used = teacher_row<T, P>(p, r, x, kept, slots);
-	float sum = 0.f;
-	if(used) {
-		for(int k = threadIdx.x; k < p.kept; k += THREADS) {
-			const float q = kept.p[k];
-			if(kept.at[k] >= 0 && !(q == 0.f)) sum += q * (logf(q) - (kept.z[k] / p.temperature - logSum));
+		if(threadIdx.x == 0) {
+			for(int w = 1; w < WARPS; ++w) mine.join(warpsOf[w]);
+			*cluster.map_shared_rank(&parts[rank], 0) = mine;
 		}
+		cluster.sync();
 	}
-	sum = block_sum(sum, slots);
-	if(threadIdx.x == 0) {
-		p.logSum[r] = logSum;
-		p.loss[r] = used ? p.temperature * p.temperature * sum : 0.f;
-	}
+	if(rank != 0 || threadIdx.x != 0) return;
+	const Running* const all = blocks > 1 ? parts : warpsOf;
+	mine = all[0];
+	for(int k = 1; k < (blocks > 1 ? blocks : WARPS); ++k) mine.join(all[k]);
+	for(int w = 1; w < WARPS; ++w) taught.join(taughtOf[w]);
+	const float logSum = mine.top * LN2 + logf(mine.sum); // mine.top is in units of log 2
+	p.logSum[r] = logSum;
+	// no entry, or nothing but minus infinity: no loss
+	p.loss[r] = taught.top == -INFINITY && taught.sum == 0.f ? 0.f
+		: p.temperature * p.temperature * (taught.cross / taught.sum - logf(taught.sum) + logSum);
 }
 
 template<typename T, typename P, int V>
 __global__ void __launch_bounds__(THREADS) distillation_backward_kernel(const DistillParams p)
 {
-	__shared__ Kept kept;
-	__shared__ float slots[WARPS];
+	__shared__ int keptAt[KEPT_MAX];
+	__shared__ float keptX[KEPT_MAX];
+	__shared__ Running warpsOf[WARPS];
 	const int blocks = p.parts, r = blockIdx.x / blocks, rank = blockIdx.x - r * blocks;
 	const T* const x = static_cast<const T*>(p.logits) + r * p.row;
 	T* const out = static_cast<T*>(p.out) + r * p.outRow;
@@ -204,10 +235,27 @@ __global__ void __launch_bounds__(THREADS) distillation_backward_kernel(const Di
 	const int begin = rank * perBlock, end = min(units, begin + perBlock);
 	const float c = LOG2E / p.temperature;
 	// the student's kept logits are read here, before anything is written: the gradient may replace the logits
-	const bool used = teacher_row<T, P>(p, r, x, kept, slots);
-	const float by = used ? p.temperature * __ldg(p.lossDiff + r) : 0.f;
-	const float log2Sum = __ldg(p.logSum + r) * LOG2E;
+	Entry entries[ENTRIES];
+	load_entries<T, P>(p, r, x, entries);
+	Running teacher = { -INFINITY, 0.f };
+#pragma unroll
+	for(int e = 0; e < ENTRIES; ++e) {
+		const int k = e * THREADS + threadIdx.x;
+		if(k < p.kept) {
+			keptAt[k] = entries[e].at;
+			keptX[k] = entries[e].x;
+		}
+		if(entries[e].at >= 0 && entries[e].x != -INFINITY) teacher.join({ entries[e].x, 1.f });
+	}
+#pragma unroll
+	for(int o = 16; o > 0; o >>= 1) teacher.join({ __shfl_xor_sync(0xffffffffu, teacher.top, o), __shfl_xor_sync(0xffffffffu, teacher.sum, o) });
+	if((threadIdx.x & 31) == 0) warpsOf[threadIdx.x >> 5] = teacher;
+	const float diff = p.temperature * __ldg(p.lossDiff + r), log2Sum = __ldg(p.logSum + r) * LOG2E;
 	__syncthreads();
+	teacher = warpsOf[0];
+#pragma unroll
+	for(int w = 1; w < WARPS; ++w) teacher.join(warpsOf[w]);
+	const bool used = !(teacher.top == -INFINITY && teacher.sum == 0.f);
 	Row<T, V> row;
 	row.p = x;
 	row.begin = x;
@@ -226,23 +274,24 @@ __global__ void __launch_bounds__(THREADS) distillation_backward_kernel(const Di
 			float v[V];
 			unit_floats<T, V>(raw[k], v);
 #pragma unroll
-			for(int j = 0; j < V; ++j) v[j] = used ? by * exp2f(fmaf(v[j], c, -log2Sum)) : 0.f;
+			for(int j = 0; j < V; ++j) v[j] = used ? diff * exp2_fast(fmaf(v[j], c, -log2Sum)) : 0.f;
 			store_unit<T, V>(out, u * V - offset, p.vocabulary, v);
 		}
 	}
 	if(!used) return;
 	__syncthreads(); // the kept columns of this part have been written, and now get their final value
-	for(int k = threadIdx.x; k < p.kept; k += THREADS) {
-		const int at = kept.at[k];
+#pragma unroll
+	for(int e = 0; e < ENTRIES; ++e) {
+		const int k = e * THREADS + threadIdx.x, at = entries[e].at;
 		if(at < 0 || (at + offset) / V < begin || (at + offset) / V >= end) continue;
 		bool first = true;
 		float sum = 0.f;
 		for(int o = 0; o < p.kept; ++o) { // a column that was kept twice: its first entry adds them up, in order
-			if(kept.at[o] != at) continue;
+			if(keptAt[o] != at) continue;
 			if(o < k) first = false;
-			sum += kept.p[o];
+			sum += exp2_fast(keptX[o] - teacher.top);
 		}
-		if(first) out[at] = from_float<T>(by * (exp2f(fmaf(kept.z[k], c, -log2Sum)) - sum));
+		if(first) out[at] = from_float<T>(diff * (exp2_fast(fmaf(entries[e].z, c, -log2Sum)) - sum / teacher.sum));
 	}
 }
 

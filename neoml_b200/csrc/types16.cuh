@@ -44,6 +44,10 @@ template<> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, flo
 	return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+template<typename T> struct PairOf;
+template<> struct PairOf<__half> { using type = __half2; };
+template<> struct PairOf<__nv_bfloat16> { using type = __nv_bfloat162; };
+
 // 16 bytes as they lie in memory <-> the floats they hold (four or eight).
 template<typename T> struct Unit16 {
 	static constexpr int N = 16 / static_cast<int>(sizeof(T));
