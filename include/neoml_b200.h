@@ -374,22 +374,22 @@ NB200_API int nb200_distillation_loss_backward(void* stream, int type, int teach
  * hidden [rows x width] by weights [vocabulary x width] and the arithmetic of MatrixSoftmaxByRows (NME.h:450) on its rows,
  *   log_sum[r] = log sum_j exp(z[r][j]),   loss[r] = log_sum[r] - z[r][label[r]],   z = hidden * weights^T.
  * A label outside 0..vocabulary-1 marks a row without a target: its loss is zero, and in the backward pass it has no
- * gradient, whatever the row holds.  Both matrices are of `type`; `precision` is that of the products of fp32 matrices, 16-bit ones
- * are multiplied as they are, with fp32 sums.  `scratch` holds nb200_vocabulary_cross_entropy_scratch_bytes(...) bytes, 256-byte
- * aligned: for the logits' partial sums, for copies of operands whose rows do not begin on 16-byte boundaries, and for one piece of
- * the vocabulary's logits (fp32) or of their gradient (backward), 256 MB or 256 columns if that is more. */
+ * gradient, whatever the row holds.  Both matrices are of `type`; sums are fp32.  `scratch` holds nb200_vocabulary_cross_entropy_scratch_bytes(...) bytes, 256-byte
+ * aligned: for the logits' partial sums, for copies of operands whose rows do not begin on 16-byte boundaries (of 16-bit types), for
+ * the hidden rows and one piece of the weights in the tensor core's parts (fp32), and for one piece of the gradient by the logits
+ * (backward); a piece takes 256 MB, or 256 columns if that is more. */
 NB200_API size_t nb200_vocabulary_cross_entropy_scratch_bytes(int type, const void* hidden, int rows, int width,
 	long long hidden_row_size, const void* weights, int vocabulary, long long weights_row_size, int backward);
 NB200_API int nb200_vocabulary_cross_entropy(void* stream, int type, const void* hidden, int rows, int width,
 	long long hidden_row_size, const void* weights, int vocabulary, long long weights_row_size, const int* labels, float* loss,
-	float* log_sum, void* scratch, int precision);
+	float* log_sum, void* scratch);
 /* Its gradients by hidden and weights, each NULL where not wanted: with dz = loss_diff[r] * (softmax(z) - [j = label[r]]) the
  * products dz * weights and dz^T * hidden (NME.h:529-532, NME.h:580-582).  log_sum is the forward pass's.  No atomics: the
  * same bits from run to run. */
 NB200_API int nb200_vocabulary_cross_entropy_backward(void* stream, int type, const float* loss_diff, const void* hidden,
 	int rows, int width, long long hidden_row_size, const void* weights, int vocabulary, long long weights_row_size,
 	const int* labels, const float* log_sum, void* hidden_diff, long long hidden_diff_row_size, void* weights_diff,
-	long long weights_diff_row_size, void* scratch, int precision);
+	long long weights_diff_row_size, void* scratch);
 
 #ifdef __cplusplus
 }

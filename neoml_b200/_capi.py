@@ -117,9 +117,9 @@ SIGNATURES = {
     "nb200_gated_recurrence_backward": (_i, [_vp, _i, _RD, _vp, _ll, _ll, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
                                              _vp]),
     "nb200_vocabulary_cross_entropy_scratch_bytes": (C.c_size_t, [_i, _vp, _i, _i, _ll, _vp, _i, _ll, _i]),
-    "nb200_vocabulary_cross_entropy": (_i, [_vp, _i, _vp, _i, _i, _ll, _vp, _i, _ll, _vp, _vp, _vp, _vp, _i]),
+    "nb200_vocabulary_cross_entropy": (_i, [_vp, _i, _vp, _i, _i, _ll, _vp, _i, _ll, _vp, _vp, _vp, _vp]),
     "nb200_vocabulary_cross_entropy_backward": (_i, [_vp, _i, _vp, _vp, _i, _i, _ll, _vp, _i, _ll, _vp, _vp, _vp, _ll, _vp, _ll,
-                                                     _vp, _i]),
+                                                     _vp]),
     "nb200_distillation_loss": (_i, [_vp, _i, _i, _vp, _i, _i, _ll, _vp, _vp, _i, _f, _vp, _vp]),
     "nb200_distillation_loss_backward": (_i, [_vp, _i, _i, _vp, _vp, _i, _i, _ll, _vp, _vp, _i, _f, _vp, _vp, _ll]),
 }

@@ -268,9 +268,11 @@ PyObject* vector_op(PyObject*, PyObject* const* a, Py_ssize_t count)
 
 // ---- operators of language models: fp32, fp16 and bf16 data on the device that it is on ------------------------------
 
+PyObject* g_parameter = nullptr; // torch.nn.Parameter, held for as long as the process lives
+
 const at::Tensor& any_tensor(PyObject* o) // parameters too
 {
-	if(!THPVariable_Check(o) || (!THPVariable_CheckExact(o) && torch::check_has_torch_function(o))) throw NotHere();
+	if(!THPVariable_CheckExact(o) && reinterpret_cast<PyObject*>(Py_TYPE(o)) != g_parameter) throw NotHere();
 	const at::Tensor& t = THPVariable_Unpack(o);
 	if(!t.has_storage() || !t.is_cuda() || t.is_conj() || t.is_neg()) throw NotHere();
 	return t;
@@ -694,5 +696,10 @@ PyModuleDef module = { PyModuleDef_HEAD_INIT, "_ops_native", nullptr, -1, method
 
 PyMODINIT_FUNC PyInit__ops_native()
 {
+	PyObject* const nn = PyImport_ImportModule("torch.nn.parameter");
+	if(nn == nullptr) return nullptr;
+	g_parameter = PyObject_GetAttrString(nn, "Parameter");
+	Py_DECREF(nn);
+	if(g_parameter == nullptr) return nullptr;
 	return PyModule_Create(&module);
 }

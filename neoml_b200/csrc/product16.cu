@@ -7,6 +7,11 @@
 // Operands whose m or n is adjacent in memory need no transposition: the tensor core reads them MN-major.  A box of 64 adjacent
 // indices x 64 k lands as 64 rows of 128 bytes; eight rows are a swizzle atom of 1024 bytes (stride byte offset), the next 64
 // indices lie 8192 bytes further (leading byte offset).  Every wait is bounded (common.cuh).
+//
+// The tensor core's own additions cut off rather than round: a running sum loses about 3e-9 of itself with each MMA, always towards zero
+// (measured: 1.3e-6 after 384 of them, 3.5e-5 after 11250).  16-bit results do not show it.  For fp32 operands the K loop
+// is cut into chunks of 1024 whose sums the epilogue warps add up in registers, and within a chunk the small products go first, so that
+// only the 64 MMAs of hi hi work on a sum of full size: 1e-7.
 #include "product16.cuh"
 
 #include <cuda.h>
@@ -34,12 +39,9 @@ __device__ __forceinline__ float exp2_fast(float x)
 	return y;
 }
 
-__device__ __forceinline__ void tma_load_2d(uint32_t dst, const void* map, uint64_t* bar, int x, int y)
-{
-	asm volatile(
-		"cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-		::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y) : "memory");
-}
+// The products of planes in the order of their MMAs, small ones first: 0 hi, 1 mid, 2 lo.
+__device__ constexpr int PLANE_A[6] = { 2, 0, 1, 1, 0, 0 }, PLANE_B[6] = { 0, 2, 1, 0, 1, 0 };
+constexpr int CHUNK = 1024 / BK; // K blocks of fp32 operands that are summed in tensor memory
 
 // MN-major operand of 16-bit elements: see the head of this file.
 __device__ __forceinline__ uint64_t desc_across(uint32_t smemAddr)
@@ -102,10 +104,11 @@ __device__ __forceinline__ uint32_t pack16(float a, float b, int bf16)
 	return bf16 ? pack2<__nv_bfloat16>(a, b) : pack2<__half>(a, b);
 }
 
-template<int EPILOGUE, bool A_ACROSS, bool B_ACROSS>
+template<int EPILOGUE, bool A_ACROSS, bool B_ACROSS, bool FP32>
 __global__ void __launch_bounds__(THREADS, 1) product16_kernel(const Product16Params p, const __grid_constant__ CUtensorMap mapA,
 	const __grid_constant__ CUtensorMap mapB)
 {
+	constexpr int TERMS = FP32 ? 6 : 1;
 	extern __shared__ uint8_t smemRaw[];
 	uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smemRaw) + 1023) & ~static_cast<uintptr_t>(1023));
 	uint64_t* const bars = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE_BYTES);
@@ -143,29 +146,35 @@ __global__ void __launch_bounds__(THREADS, 1) product16_kernel(const Product16Pa
 		if(elect_one()) {
 			int it = 0;
 			bool ok = true;
+			auto load = [&](const Tile& t, int kb, int planeA, int planeB) {
+				const int s = it % STAGES;
+				if(it >= STAGES && !mbar_wait_bounded(bars + B_EMPTY + s, (it / STAGES - 1) & 1, abortFlag, p.status, (KERNEL_ID << 8) | SITE_LOAD)) return false;
+				uint64_t* const full = bars + B_FULL + s;
+				const uint32_t a = smemBase + s * STAGE_BYTES, b = a + A_BYTES;
+				mbar_arrive_expect_tx(full, STAGE_BYTES);
+				const int ka = p.akOffset + kb * BK, kbB = p.bkOffset + kb * BK;
+				if constexpr(A_ACROSS) {
+#pragma unroll
+					for(int i = 0; i < BM / 64; ++i) tma_load_3d(a + i * 8192, &mapA, full, p.aOffset + t.m0 + i * 64, ka, planeA);
+				} else {
+					tma_load_3d(a, &mapA, full, ka, p.aOffset + t.m0, planeA);
+				}
+				if constexpr(B_ACROSS) {
+#pragma unroll
+					for(int i = 0; i < BN / 64; ++i) tma_load_3d(b + i * 8192, &mapB, full, p.bOffset + t.n0 + i * 64, kbB, planeB);
+				} else {
+					tma_load_3d(b, &mapB, full, kbB, p.bOffset + t.n0, planeB);
+				}
+				++it;
+				return true;
+			};
 			for(int tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x) {
 				const Tile t = tile_of(p, tile);
-				for(int kb = t.kBegin; kb < t.kEnd; ++kb, ++it) {
-					const int s = it % STAGES;
-					if(it >= STAGES && !mbar_wait_bounded(bars + B_EMPTY + s, (it / STAGES - 1) & 1, abortFlag, p.status, (KERNEL_ID << 8) | SITE_LOAD)) {
-						ok = false;
-						break;
-					}
-					uint64_t* const full = bars + B_FULL + s;
-					const uint32_t a = smemBase + s * STAGE_BYTES, b = a + A_BYTES;
-					mbar_arrive_expect_tx(full, STAGE_BYTES);
-					const int ka = p.akOffset + kb * BK, kbB = p.bkOffset + kb * BK;
-					if constexpr(A_ACROSS) {
-#pragma unroll
-						for(int i = 0; i < BM / 64; ++i) tma_load_2d(a + i * 8192, &mapA, full, p.aOffset + t.m0 + i * 64, ka);
-					} else {
-						tma_load_2d(a, &mapA, full, ka, p.aOffset + t.m0);
-					}
-					if constexpr(B_ACROSS) {
-#pragma unroll
-						for(int i = 0; i < BN / 64; ++i) tma_load_2d(b + i * 8192, &mapB, full, p.bOffset + t.n0 + i * 64, kbB);
-					} else {
-						tma_load_2d(b, &mapB, full, kbB, p.bOffset + t.n0);
+				const int chunk = FP32 ? CHUNK : p.kBlocks;
+				for(int k0 = t.kBegin; ok && k0 < t.kEnd; k0 += chunk) {
+					const int k1 = min(t.kEnd, k0 + chunk);
+					for(int term = 0; ok && term < TERMS; ++term) {
+						for(int kb = k0; ok && kb < k1; ++kb) ok = load(t, kb, FP32 ? PLANE_A[term] : 0, FP32 ? PLANE_B[term] : 0);
 					}
 				}
 			}
@@ -183,29 +192,39 @@ __global__ void __launch_bounds__(THREADS, 1) product16_kernel(const Product16Pa
 			const uint32_t idesc = umma_idesc_f16(BM, BN) | format | (A_ACROSS ? 1u << 15 : 0u) | (B_ACROSS ? 1u << 16 : 0u);
 			int it = 0, n = 0;
 			bool ok = true;
-			for(int tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x, ++n) {
+			for(int tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x) {
 				const Tile t = tile_of(p, tile);
-				const int acc = n & 1;
-				if(n >= 2 && !mbar_wait_bounded(bars + B_ACCEMPTY + acc, (n / 2 - 1) & 1, abortFlag, p.status, (KERNEL_ID << 8) | SITE_MMA_ACC)) break;
-				tc_fence_after_sync();
-				const uint32_t d = tmemBase + acc * BN;
-				for(int kb = t.kBegin; kb < t.kEnd; ++kb, ++it) {
-					const int s = it % STAGES;
-					if(!mbar_wait_bounded(bars + B_FULL + s, (it / STAGES) & 1, abortFlag, p.status, (KERNEL_ID << 8) | SITE_MMA)) {
+				const int chunk = FP32 ? CHUNK : p.kBlocks;
+				int k0 = t.kBegin;
+				do { // a part of K without steps takes its turn too
+					const int acc = n & 1;
+					if(n >= 2 && !mbar_wait_bounded(bars + B_ACCEMPTY + acc, (n / 2 - 1) & 1, abortFlag, p.status, (KERNEL_ID << 8) | SITE_MMA_ACC)) {
 						ok = false;
 						break;
 					}
 					tc_fence_after_sync();
-					const uint32_t a = smemBase + s * STAGE_BYTES, b = a + A_BYTES;
+					const uint32_t d = tmemBase + acc * BN;
+					const int steps = (min(t.kEnd, k0 + chunk) - k0) * TERMS;
+					for(int i = 0; i < steps; ++i, ++it) {
+						const int s = it % STAGES;
+						if(!mbar_wait_bounded(bars + B_FULL + s, (it / STAGES) & 1, abortFlag, p.status, (KERNEL_ID << 8) | SITE_MMA)) {
+							ok = false;
+							break;
+						}
+						tc_fence_after_sync();
+						const uint32_t a = smemBase + s * STAGE_BYTES, b = a + A_BYTES;
 #pragma unroll
-					for(int k = 0; k < BK / 16; ++k) {
-						const uint64_t da = A_ACROSS ? desc_across(a + k * 2048) : umma_desc_k128(a + k * 32);
-						const uint64_t db = B_ACROSS ? desc_across(b + k * 2048) : umma_desc_k128(b + k * 32);
-						umma_f16_ss(d, da, db, idesc, kb > t.kBegin || k > 0 ? 1u : 0u);
+						for(int k = 0; k < BK / 16; ++k) {
+							const uint64_t da = A_ACROSS ? desc_across(a + k * 2048) : umma_desc_k128(a + k * 32);
+							const uint64_t db = B_ACROSS ? desc_across(b + k * 2048) : umma_desc_k128(b + k * 32);
+							umma_f16_ss(d, da, db, idesc, i > 0 || k > 0 ? 1u : 0u);
+						}
+						umma_commit(bars + B_EMPTY + s);
 					}
-					umma_commit(bars + B_EMPTY + s);
-				}
-				if(ok) umma_commit(bars + B_ACCFULL + acc);
+					if(ok) umma_commit(bars + B_ACCFULL + acc);
+					++n;
+					k0 += chunk;
+				} while(ok && k0 < t.kEnd);
 			}
 			if(*abortFlag != 0) { // nothing may still write tensor memory when it is freed
 				int ignored = 0;
@@ -217,13 +236,13 @@ __global__ void __launch_bounds__(THREADS, 1) product16_kernel(const Product16Pa
 	} else if(warp >= 4) {
 		const int quarter = warp & 3, half = (warp - 4) >> 2;
 		int n = 0;
-		for(int tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++n) {
+		bool ok = true;
+		for(int tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x) {
 			const Tile t = tile_of(p, tile);
-			const int acc = n & 1;
 			const int row = t.m0 + quarter * 32 + lane;
 			const bool on = row < p.m;
 			const int col0 = t.n0 + half * 128;
-			const uint32_t at = tmemBase + (static_cast<uint32_t>(quarter * 32) << 16) + acc * BN + half * 128;
+			const uint32_t tmemRow = tmemBase + (static_cast<uint32_t>(quarter * 32) << 16) + half * 128;
 			int label = -1;
 			float logSum2 = 0.f, by = 0.f;
 			if(on && (EPILOGUE == PRODUCT16_STATS || EPILOGUE == PRODUCT16_DIFF)) {
@@ -237,75 +256,79 @@ __global__ void __launch_bounds__(THREADS, 1) product16_kernel(const Product16Pa
 			}
 			if(EPILOGUE == PRODUCT16_STORE) by = __ldg(p.resultScale);
 			const int own = label - p.firstColumn - col0; // the label's place in this thread's columns, if it is there
-			if(!mbar_wait_bounded_warp(bars + B_ACCFULL + acc, (n >> 1) & 1, abortFlag, p.status, (KERNEL_ID << 8) | SITE_EPILOGUE)) break;
-			tc_fence_after_sync();
 			float top = -INFINITY, sum = 0.f;
-#pragma unroll 1
-			for(int c = 0; c < 128; c += 32) {
-				uint32_t r[32];
-				tmem_ld32_issue(at + c, r);
-				tmem_ld_wait();
-				if(EPILOGUE == PRODUCT16_SUM && t.kBegin >= t.kEnd) { // a part of K without steps: nothing was multiplied
-#pragma unroll
-					for(int i = 0; i < 32; ++i) r[i] = 0u;
-				}
-				if(c == 96) { // the accumulator is free
-					tc_fence_before_sync();
-					if(lane == 0) mbar_arrive(bars + B_ACCEMPTY + acc);
-				}
+			// what becomes of 32 columns of the thread's row, from col0 + c
+			auto finish = [&](int c, float (&r)[32]) __attribute__((always_inline)) {
 				if constexpr(EPILOGUE == PRODUCT16_STATS) {
 					const int left = p.columns - p.firstColumn - col0 - c; // valid ones of these 32
 					if(left < 32) {
 #pragma unroll
 						for(int i = 0; i < 32; ++i) {
-							if(i >= left) r[i] = 0xff800000u;
+							if(i >= left) r[i] = -INFINITY;
 						}
 					}
-					const bool here = own >= c && own < c + 32;
-					if(__any_sync(0xffffffffu, here)) {
-						float value = 0.f;
+					const uint32_t hot = own >= c && own < c + 32 ? 1u << (own - c) : 0u;
+					if(__any_sync(0xffffffffu, hot != 0u)) {
+						uint32_t value = 0u; // (written so that the row stays in registers)
 #pragma unroll
-						for(int i = 0; i < 32; ++i) {
-							if(own - c == i) value = __uint_as_float(r[i]);
-						}
-						if(here && left > own - c) p.labelled[row] = value;
+						for(int i = 0; i < 32; ++i) value |= (hot >> i & 1u) != 0u ? __float_as_uint(r[i]) : 0u;
+						if(hot != 0u && left > own - c) p.labelled[row] = __uint_as_float(value);
 					}
-					float newTop = top;
+					float most = r[0];
 #pragma unroll
-					for(int i = 0; i < 32; ++i) newTop = fmaxf(newTop, __uint_as_float(r[i]) * LOG2E);
+					for(int i = 1; i < 32; ++i) most = fmaxf(most, r[i]);
+					const float newTop = fmaxf(top, most * LOG2E);
 					const float reference = newTop == -INFINITY ? 0.f : newTop;
-					float part[4] = { 0.f, 0.f, 0.f, 0.f };
+					float2 part[2] = { both(0.f), both(0.f) };
 #pragma unroll
-					for(int i = 0; i < 32; ++i) part[i & 3] += exp2_fast(fmaf(__uint_as_float(r[i]), LOG2E, -reference));
-					sum = sum * exp2_fast(top - reference) + ((part[0] + part[1]) + (part[2] + part[3]));
+					for(int i = 0; i < 32; i += 2) {
+						const float2 e = fma2(make_float2(r[i], r[i + 1]), both(LOG2E), both(-reference));
+						part[(i >> 1) & 1] = add2(part[(i >> 1) & 1], make_float2(exp2_fast(e.x), exp2_fast(e.y)));
+					}
+					const float2 parts = add2(part[0], part[1]);
+					sum = sum * exp2_fast(top - reference) + (parts.x + parts.y);
 					top = newTop;
 				} else if constexpr(EPILOGUE == PRODUCT16_DIFF) {
 					const int left = p.columns - p.firstColumn - col0 - c;
-					float v[32];
 #pragma unroll
-					for(int i = 0; i < 32; ++i) v[i] = by * exp2_fast(fmaf(__uint_as_float(r[i]), LOG2E, -logSum2));
-					if(__any_sync(0xffffffffu, own >= c && own < c + 32)) {
+					for(int i = 0; i < 32; i += 2) {
+						const float2 e = fma2(make_float2(r[i], r[i + 1]), both(LOG2E), both(-logSum2));
+						const float2 v = mul2(make_float2(exp2_fast(e.x), exp2_fast(e.y)), both(by));
+						r[i] = v.x;
+						r[i + 1] = v.y;
+					}
+					const uint32_t hot = own >= c && own < c + 32 ? 1u << (own - c) : 0u;
+					if(__any_sync(0xffffffffu, hot != 0u)) {
 #pragma unroll
-						for(int i = 0; i < 32; ++i) {
-							if(own - c == i) v[i] -= by;
-						}
+						for(int i = 0; i < 32; ++i) r[i] -= (hot >> i & 1u) != 0u ? by : 0.f;
 					}
 					// a row without a target has no gradient, whatever its logits; columns behind the vocabulary are zeros,
 					// which the products that read them count on
 					if(by == 0.f || left < 32) {
 #pragma unroll
 						for(int i = 0; i < 32; ++i) {
-							if(by == 0.f || i >= left) v[i] = 0.f;
+							if(by == 0.f || i >= left) r[i] = 0.f;
 						}
 					}
 					if(on) {
-						uint16_t* const out = static_cast<uint16_t*>(p.out16) + row * p.ldOut + col0 + c;
+						uint16_t* const out = static_cast<uint16_t*>(p.out) + row * p.ldOut + col0 + c;
 #pragma unroll
-						for(int j = 0; j < 2; ++j) {
-							uint32_t w[8];
+						for(int plane = 0; plane < (FP32 ? 3 : 1); ++plane) {
 #pragma unroll
-							for(int i = 0; i < 8; ++i) w[i] = pack16(v[j * 16 + 2 * i], v[j * 16 + 2 * i + 1], p.bf16);
-							store32(out + j * 16, w);
+							for(int j = 0; j < 2; ++j) {
+								uint32_t w[8];
+#pragma unroll
+								for(int i = 0; i < 8; ++i) {
+									float &v0 = r[j * 16 + 2 * i], &v1 = r[j * 16 + 2 * i + 1];
+									w[i] = FP32 ? pack2<__nv_bfloat16>(v0, v1) : pack16(v0, v1, p.bf16);
+									if(FP32) { // the rest, for the next plane
+										const float2 taken = unpack2<__nv_bfloat16>(w[i]);
+										v0 -= taken.x;
+										v1 -= taken.y;
+									}
+								}
+								store32(out + plane * p.outPlane + j * 16, w);
+							}
 						}
 					}
 				} else if constexpr(EPILOGUE == PRODUCT16_SUM) {
@@ -314,27 +337,45 @@ __global__ void __launch_bounds__(THREADS, 1) product16_kernel(const Product16Pa
 #pragma unroll
 						for(int j = 0; j < 4; ++j) {
 							if(col0 + c + j * 8 < p.n) { // ldPlane is a multiple of 8
+								uint32_t w[8];
 								if(p.accumulate) {
-									uint32_t before[8];
-									load32(out + j * 8, before);
+									load32(out + j * 8, w);
 #pragma unroll
-									for(int i = 0; i < 8; ++i) r[j * 8 + i] = __float_as_uint(__uint_as_float(r[j * 8 + i]) + __uint_as_float(before[i]));
+									for(int i = 0; i < 8; ++i) w[i] = __float_as_uint(r[j * 8 + i] + __uint_as_float(w[i]));
+								} else {
+#pragma unroll
+									for(int i = 0; i < 8; ++i) w[i] = __float_as_uint(r[j * 8 + i]);
 								}
-								store32(out + j * 8, r + j * 8);
+								store32(out + j * 8, w);
+							}
+						}
+					}
+				} else if constexpr(FP32) {
+					if(on) {
+						float* const out = static_cast<float*>(p.out) + row * p.ldOut + col0 + c;
+						const bool aligned = (p.ldOut & 3) == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15u) == 0;
+#pragma unroll
+						for(int j = 0; j < 8; ++j) {
+							const int left = p.n - (col0 + c + j * 4);
+							if(aligned && left >= 4) {
+								*reinterpret_cast<float4*>(out + j * 4) = make_float4(r[j * 4] * by, r[j * 4 + 1] * by, r[j * 4 + 2] * by, r[j * 4 + 3] * by);
+							} else {
+#pragma unroll
+								for(int i = 0; i < 4; ++i) {
+									if(i < left) out[j * 4 + i] = r[j * 4 + i] * by;
+								}
 							}
 						}
 					}
 				} else {
 					if(on) {
-						uint16_t* const out = static_cast<uint16_t*>(p.out16) + row * p.ldOut + col0 + c;
-						const bool aligned = (p.ldOut & 7) == 0 && (reinterpret_cast<uintptr_t>(p.out16) & 15u) == 0;
+						uint16_t* const out = static_cast<uint16_t*>(p.out) + row * p.ldOut + col0 + c;
+						const bool aligned = (p.ldOut & 7) == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15u) == 0;
 #pragma unroll
 						for(int j = 0; j < 4; ++j) {
 							uint32_t w[4];
 #pragma unroll
-							for(int i = 0; i < 4; ++i) {
-								w[i] = pack16(__uint_as_float(r[j * 8 + 2 * i]) * by, __uint_as_float(r[j * 8 + 2 * i + 1]) * by, p.bf16);
-							}
+							for(int i = 0; i < 4; ++i) w[i] = pack16(r[j * 8 + 2 * i] * by, r[j * 8 + 2 * i + 1] * by, p.bf16);
 							const int left = p.n - (col0 + c + j * 8);
 							if(aligned && left >= 8) {
 								*reinterpret_cast<uint4*>(out + j * 8) = make_uint4(w[0], w[1], w[2], w[3]);
@@ -346,6 +387,52 @@ __global__ void __launch_bounds__(THREADS, 1) product16_kernel(const Product16Pa
 							}
 						}
 					}
+				}
+			};
+			const bool empty = t.kBegin >= t.kEnd; // a part of K without steps: nothing was multiplied
+			if constexpr(FP32) {
+				float total[4][32];
+				int k0 = t.kBegin;
+				do {
+					const int acc = n & 1;
+					ok = mbar_wait_bounded_warp(bars + B_ACCFULL + acc, (n >> 1) & 1, abortFlag, p.status, (KERNEL_ID << 8) | SITE_EPILOGUE);
+					if(!ok) break;
+					tc_fence_after_sync();
+#pragma unroll
+					for(int c = 0; c < 4; ++c) {
+						uint32_t r[32];
+						tmem_ld32_issue(tmemRow + acc * BN + c * 32, r);
+						tmem_ld_wait();
+#pragma unroll
+						for(int i = 0; i < 32; ++i) total[c][i] = (k0 == t.kBegin ? 0.f : total[c][i]) + (empty ? 0.f : __uint_as_float(r[i]));
+					}
+					tc_fence_before_sync();
+					if(lane == 0) mbar_arrive(bars + B_ACCEMPTY + acc);
+					++n;
+					k0 += CHUNK;
+				} while(k0 < t.kEnd);
+				if(!ok) break;
+#pragma unroll
+				for(int c = 0; c < 4; ++c) finish(c * 32, total[c]);
+			} else {
+				const int acc = n & 1;
+				ok = mbar_wait_bounded_warp(bars + B_ACCFULL + acc, (n >> 1) & 1, abortFlag, p.status, (KERNEL_ID << 8) | SITE_EPILOGUE);
+				if(!ok) break;
+				++n;
+				tc_fence_after_sync();
+#pragma unroll 1
+				for(int c = 0; c < 128; c += 32) {
+					uint32_t r[32];
+					tmem_ld32_issue(tmemRow + acc * BN + c, r);
+					tmem_ld_wait();
+					if(c == 96) { // the accumulator is free
+						tc_fence_before_sync();
+						if(lane == 0) mbar_arrive(bars + B_ACCEMPTY + acc);
+					}
+					float v[32];
+#pragma unroll
+					for(int i = 0; i < 32; ++i) v[i] = EPILOGUE == PRODUCT16_SUM && empty ? 0.f : __uint_as_float(r[i]);
+					finish(c, v);
 				}
 			}
 			if(EPILOGUE == PRODUCT16_STATS && on) {
@@ -380,15 +467,15 @@ using Kernel = void (*)(const Product16Params, const CUtensorMap, const CUtensor
 
 } // namespace
 
-bool product16_map(void* map, const void* base, bool bf16, long long inner, long long rows, long long rowSize, int boxRows)
+bool product16_map(void* map, const void* base, bool bf16, long long inner, long long rows, long long rowSize, int boxRows, long long planeSize)
 {
 	const EncodeTiledFn encode = encoder();
-	if(encode == nullptr || !aligned16(base) || rowSize % 8 != 0 || rowSize * 2 >= (1ll << 40)) return false;
-	const cuuint64_t dims[2] = { static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(rows) };
-	const cuuint64_t strides[1] = { static_cast<cuuint64_t>(rowSize) * 2 };
-	const cuuint32_t box[2] = { 64, static_cast<cuuint32_t>(boxRows) };
-	const cuuint32_t steps[2] = { 1, 1 };
-	return encode(static_cast<CUtensorMap*>(map), bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
+	if(encode == nullptr || !aligned16(base) || rowSize % 8 != 0 || planeSize % 8 != 0 || rowSize * 2 >= (1ll << 40) || planeSize * 2 >= (1ll << 40)) return false;
+	const cuuint64_t dims[3] = { static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(rows), planeSize > 0 ? 3u : 1u };
+	const cuuint64_t strides[2] = { static_cast<cuuint64_t>(rowSize) * 2, static_cast<cuuint64_t>(planeSize > 0 ? planeSize : rowSize) * 2 };
+	const cuuint32_t box[3] = { 64, static_cast<cuuint32_t>(boxRows), 1 };
+	const cuuint32_t steps[3] = { 1, 1, 1 };
+	return encode(static_cast<CUtensorMap*>(map), bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
 		const_cast<void*>(base), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
 		CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -397,11 +484,11 @@ int product16(Product16Epilogue epilogue, bool aAcross, bool bAcross, const Prod
 	cudaStream_t stream)
 {
 	Kernel kernel = nullptr;
-	if(epilogue == PRODUCT16_STATS && !aAcross && !bAcross) kernel = product16_kernel<PRODUCT16_STATS, false, false>;
-	else if(epilogue == PRODUCT16_DIFF && !aAcross && !bAcross) kernel = product16_kernel<PRODUCT16_DIFF, false, false>;
-	else if(epilogue == PRODUCT16_SUM && !aAcross && bAcross) kernel = product16_kernel<PRODUCT16_SUM, false, true>;
-	else if(epilogue == PRODUCT16_SUM && aAcross && bAcross) kernel = product16_kernel<PRODUCT16_SUM, true, true>;
-	else if(epilogue == PRODUCT16_STORE && aAcross && bAcross) kernel = product16_kernel<PRODUCT16_STORE, true, true>;
+	if(epilogue == PRODUCT16_STATS && !aAcross && !bAcross) kernel = p.fp32 ? product16_kernel<PRODUCT16_STATS, false, false, true> : product16_kernel<PRODUCT16_STATS, false, false, false>;
+	else if(epilogue == PRODUCT16_DIFF && !aAcross && !bAcross) kernel = p.fp32 ? product16_kernel<PRODUCT16_DIFF, false, false, true> : product16_kernel<PRODUCT16_DIFF, false, false, false>;
+	else if(epilogue == PRODUCT16_SUM && !aAcross && bAcross) kernel = p.fp32 ? product16_kernel<PRODUCT16_SUM, false, true, true> : product16_kernel<PRODUCT16_SUM, false, true, false>;
+	else if(epilogue == PRODUCT16_SUM && aAcross && bAcross) kernel = p.fp32 ? product16_kernel<PRODUCT16_SUM, true, true, true> : product16_kernel<PRODUCT16_SUM, true, true, false>;
+	else if(epilogue == PRODUCT16_STORE && aAcross && bAcross) kernel = p.fp32 ? product16_kernel<PRODUCT16_STORE, true, true, true> : product16_kernel<PRODUCT16_STORE, true, true, false>;
 	else return NB200_EINVAL;
 	const long long tiles = static_cast<long long>(p.mTiles) * p.nTiles * p.splits;
 	if(tiles > 0x7fffffffLL - 1024) return NB200_ETOOBIG;

@@ -1,6 +1,10 @@
 // Products of 16-bit matrices on the tensor core (fp16 or bf16 in, fp32 accumulators), with the epilogues of the cross entropy over a
 // vocabulary (vocabulary_loss.cu).  D[m][n] = sum_k A[m][k] B[n][k]; either operand may lie with its k adjacent (rows of k) or with
 // its m or n adjacent (rows per k, as a gradient's product meets what the forward pass stored).
+//
+// fp32 operands come as three bf16 matrices each ("planes"), x = hi + mid + lo with eight bits of x in each: all 24.  Of the nine
+// products of planes six are formed (hi hi, hi mid, mid hi, mid mid, hi lo, lo hi); what is left out is below 2^-26 of the product of
+// the largest.  bf16 rather than fp16 parts, since softmax gradients reach from 1 to far below what a half holds.
 #pragma once
 #include "types16.cuh"
 
@@ -8,9 +12,9 @@ namespace nb200 {
 
 enum Product16Epilogue {
 	PRODUCT16_STATS, // per row and 128 columns: maximum and sum of exponentials, and the labelled column's value
-	PRODUCT16_DIFF,  // 16-bit gradient by the logits: coefficient[row] * (softmax - [column is the label])
+	PRODUCT16_DIFF,  // gradient by the logits, 16-bit or three planes: coefficient[row] * (softmax - [column is the label])
 	PRODUCT16_SUM,   // fp32 planes, one per part of K; added to what is there where `accumulate` is set
-	PRODUCT16_STORE  // 16-bit result times *resultScale
+	PRODUCT16_STORE  // result times *resultScale, of the operands' type
 };
 
 struct Product16Params {
@@ -21,6 +25,7 @@ struct Product16Params {
 	int aOffset, bOffset;   // added to the m and n coordinates of the loads
 	int akOffset, bkOffset; // and to their k coordinates
 	int bf16;            // operands are bf16 rather than fp16
+	int fp32;            // operands are three bf16 planes
 	int* status;
 	// STATS
 	float2* partial;     // [2 * nTiles][m]: maximum in units of log 2, sum of 2^(x - maximum)
@@ -34,8 +39,9 @@ struct Product16Params {
 	const float* rowScale; // [m], times *scale
 	const float* scale;
 	// DIFF, STORE
-	void* out16;
+	void* out;           // STORE: 16-bit or fp32
 	long long ldOut;
+	long long outPlane;  // DIFF with planes: elements between them
 	// STORE
 	const float* resultScale;
 	// SUM
@@ -48,8 +54,10 @@ struct Product16Params {
 int product16(Product16Epilogue epilogue, bool aAcross, bool bAcross, const Product16Params& p, const void* mapA, const void* mapB,
 	cudaStream_t stream);
 // Map of a matrix of 16-bit elements, `inner` adjacent ones in each of `rows` rows; boxes of 64 x boxRows land as 128-byte rows
-// with the 128-byte swizzle.  False where TMA cannot describe it (base or rows off a 16-byte boundary).
-bool product16_map(void* map, const void* base, bool bf16, long long inner, long long rows, long long rowSize, int boxRows);
+// with the 128-byte swizzle.  planeSize > 0: three such matrices that many elements apart.  False where TMA cannot describe it (base
+// or rows off a 16-byte boundary).
+bool product16_map(void* map, const void* base, bool bf16, long long inner, long long rows, long long rowSize, int boxRows,
+	long long planeSize = 0);
 
 constexpr int PRODUCT16_M = 128, PRODUCT16_N = 256, PRODUCT16_K = 64; // of a tile
 constexpr int PRODUCT16_BOX_A = 128, PRODUCT16_BOX_B = 256, PRODUCT16_BOX_ACROSS = 64; // boxRows of the operands' maps

@@ -466,6 +466,9 @@ def LayerNormalization(source, scale=None, free_term=None, *, epsilon=1e-5, resu
     (result, mean, inverse_deviation); the last two are what the backward pass takes, fp32, one per row.  scale and
     free_term have `width` elements, both of the source's type or both fp32; None stands for ones and zeros.  `result` may
     be `source`."""
+    done = _native().layer_normalization(source, scale, free_term, epsilon, result)
+    if done is not None:
+        return _checked("LayerNormalization", done)
     height, width, row = _matrix(source)
     code, parameter = _typed(source), next((p.dtype for p in (scale, free_term) if p is not None), source.dtype)
     assert parameter in (source.dtype, torch.float32), "parameters of the rows' type or fp32"
@@ -487,6 +490,10 @@ def LayerNormalizationBackward(result_diff, source, mean, inverse_deviation, sca
     """The gradients of LayerNormalization: (source_diff, scale_diff, free_term_diff) from the result's, what went in and
     the two vectors that the forward pass returned.  The parameters' gradients are of the scale's type (without a scale
     `parameter_type`, or the source's); None with parameters=False.  `source_diff` may be `result_diff`."""
+    done = _native().layer_normalization_backward(result_diff, source, mean, inverse_deviation, scale, source_diff,
+                                                   parameters)
+    if done is not None:
+        return _checked("LayerNormalizationBackward", done)
     height, width, row = _matrix(source)
     code = _typed(source)
     parameter = scale.dtype if scale is not None else parameter_type or source.dtype
@@ -533,6 +540,9 @@ def GatedRecurrence(update, forget, input=None, *, initial_state=None, lengths=N
     (None: zeros); `final_state` may be the same tensor, as when tokens are served one at a time.  lengths (int32 [batch])
     ends sequences early: behind their end the result is zero and the state stays.  The three inputs may be strided views or
     expanded; channels are adjacent."""
+    done = _native().gated_recurrence(update, forget, input, initial_state, lengths, result, final_state)
+    if done is not None:
+        return _checked("GatedRecurrence", done)
     desc, code = _recurrence_desc(update, forget, input), _typed(update)
     batch, length, channels = update.shape
     if result is None:
@@ -556,6 +566,9 @@ def GatedRecurrenceBackward(result_diff, result, update, forget, input=None, *, 
     without input gates.  `result` is what the forward pass returned; final_state_diff (fp32, None: zeros) is the gradient
     of the last state.  Gradients are dense, one for every element that an expanded input stands for, and zero behind a
     sequence's end."""
+    done = _native().gated_recurrence_backward(result_diff, result, update, forget, input, initial_state, final_state_diff, lengths)
+    if done is not None:
+        return _checked("GatedRecurrenceBackward", done)
     desc, code = _recurrence_desc(update, forget, input), _typed(update)
     batch, length, channels = update.shape
     diff_strides = _steps(result_diff, update.shape, update.dtype)
@@ -588,6 +601,9 @@ def DistillationLoss(logits, teacher_logits, teacher_indices, *, temperature=1.0
     kept some top logits: teacher_logits and teacher_indices (int32) [..., kept], at most 1024 of them, renormalised among
     themselves.  An index outside the vocabulary marks an entry that is not used; rows without one have loss zero.
     Returns (loss, log_sum), fp32, one per row; log_sum, of logits / temperature, is what the backward pass takes."""
+    done = _native().distillation_loss(logits, teacher_logits, teacher_indices, temperature)
+    if done is not None:
+        return _checked("DistillationLoss", done)
     rows, vocabulary, row = _matrix(logits)
     code = _typed(logits)
     kept, teacher_at, indices_at = _teacher(logits, teacher_logits, teacher_indices, rows, temperature)
@@ -603,6 +619,9 @@ def DistillationLoss(logits, teacher_logits, teacher_indices, *, temperature=1.0
 def DistillationLossBackward(loss_diff, logits, teacher_logits, teacher_indices, log_sum, *, temperature=1.0, result=None):
     """The gradient of DistillationLoss by the logits, from that of each row's loss (fp32) and the log_sum of the forward
     pass.  `result` may be `logits`, which the gradient then replaces."""
+    done = _native().distillation_loss_backward(loss_diff, logits, teacher_logits, teacher_indices, log_sum, temperature, result)
+    if done is not None:
+        return _checked("DistillationLossBackward", done)
     rows, vocabulary, row = _matrix(logits)
     code = _typed(logits)
     kept, teacher_at, indices_at = _teacher(logits, teacher_logits, teacher_indices, rows, temperature)
@@ -634,11 +653,13 @@ def _head_scratch(code, hidden, rows, width, row, weights, vocabulary, weights_r
     return torch.empty(need, dtype=torch.uint8, device=hidden.device)
 
 
-def VocabularyCrossEntropy(hidden, weights, labels, *, precision=PREC_3XTF32):
+def VocabularyCrossEntropy(hidden, weights, labels):
     """Softmax cross entropy of the logits hidden @ weights^T against labels (int32), without keeping the logits: hidden
     [..., width], weights [vocabulary, width], labels [...].  Returns (loss, log_sum), fp32, one per row; log_sum is what the
-    backward pass takes.  A label outside the vocabulary marks a row without a target (padding, a prompt): loss zero.
-    `precision` is that of the products of fp32 matrices."""
+    backward pass takes.  A label outside the vocabulary marks a row without a target (padding, a prompt): loss zero."""
+    done = _native().vocabulary_cross_entropy(hidden, weights, labels)
+    if done is not None:
+        return _checked("VocabularyCrossEntropy", done)
     code, rows, width, row, vocabulary, weights_row = _head(hidden, weights, labels)
     device = _device_of(hidden, weights, labels)
     labels_at = _vector(labels, rows, torch.int32)
@@ -647,15 +668,17 @@ def VocabularyCrossEntropy(hidden, weights, labels, *, precision=PREC_3XTF32):
         scratch = _head_scratch(code, hidden, rows, width, row, weights, vocabulary, weights_row, False)
         capi.check("VocabularyCrossEntropy", capi.load().nb200_vocabulary_cross_entropy(
             _current(device), code, hidden.data_ptr(), rows, width, row, weights.data_ptr(), vocabulary, weights_row, labels_at,
-            loss.data_ptr(), log_sum.data_ptr(), scratch.data_ptr(), precision))
+            loss.data_ptr(), log_sum.data_ptr(), scratch.data_ptr()))
     return loss, log_sum
 
 
-def VocabularyCrossEntropyBackward(loss_diff, hidden, weights, labels, log_sum, *, hidden_diff=True, weights_diff=True,
-                                   precision=PREC_3XTF32):
+def VocabularyCrossEntropyBackward(loss_diff, hidden, weights, labels, log_sum, *, hidden_diff=True, weights_diff=True):
     """The gradients of VocabularyCrossEntropy by hidden and weights, from that of each row's loss (fp32) and the forward
     pass's log_sum.  hidden_diff and weights_diff: True for a new tensor, False where that gradient is not wanted (None comes
     back), or the tensor to write.  Rows without a target have no gradient."""
+    done = _native().vocabulary_cross_entropy_backward(loss_diff, hidden, weights, labels, log_sum, hidden_diff, weights_diff)
+    if done is not None:
+        return _checked("VocabularyCrossEntropyBackward", done)
     code, rows, width, row, vocabulary, weights_row = _head(hidden, weights, labels)
     device = _device_of(loss_diff, hidden, weights, labels, log_sum)
     pointers = (_vector(loss_diff, rows, torch.float32), _vector(labels, rows, torch.int32), _vector(log_sum, rows, torch.float32))
@@ -670,5 +693,5 @@ def VocabularyCrossEntropyBackward(loss_diff, hidden, weights, labels, log_sum, 
         scratch = _head_scratch(code, hidden, rows, width, row, weights, vocabulary, weights_row, True)
         capi.check("VocabularyCrossEntropyBackward", capi.load().nb200_vocabulary_cross_entropy_backward(
             _current(device), code, pointers[0], hidden.data_ptr(), rows, width, row, weights.data_ptr(), vocabulary, weights_row,
-            pointers[1], pointers[2], *places, scratch.data_ptr(), precision))
+            pointers[1], pointers[2], *places, scratch.data_ptr()))
     return tuple(diffs)
