@@ -10,8 +10,9 @@
 //
 // The tensor core's own additions cut off rather than round: a running sum loses about 3e-9 of itself with each MMA, always towards zero
 // (measured: 1.3e-6 after 384 of them, 3.5e-5 after 11250).  16-bit results do not show it.  For fp32 operands the K loop
-// is cut into chunks of 1024 whose sums the epilogue warps add up in registers, and within a chunk the small products go first, so that
-// only the 64 MMAs of hi hi work on a sum of full size: 1e-7.
+// is cut into chunks of 256 whose sums the epilogue warps add up in registers, and within a chunk the small products go first, so that
+// only the 16 MMAs of hi hi work on a sum of full size.  Gradients of 1023 x 768 rows over 30011 entries are 3.7e-7 off then
+// (1.3e-6 with chunks of 1024, 6.7e-7 of 512, fp32 arithmetic 5.7e-7), and take as long: the additions hide behind the MMAs.
 #include "product16.cuh"
 
 #include <cuda.h>
@@ -41,7 +42,7 @@ __device__ __forceinline__ float exp2_fast(float x)
 
 // The products of planes in the order of their MMAs, small ones first: 0 hi, 1 mid, 2 lo.
 __device__ constexpr int PLANE_A[6] = { 2, 0, 1, 1, 0, 0 }, PLANE_B[6] = { 0, 2, 1, 0, 1, 0 };
-constexpr int CHUNK = 1024 / BK; // K blocks of fp32 operands that are summed in tensor memory
+constexpr int CHUNK = 256 / BK; // K blocks of fp32 operands that are summed in tensor memory
 
 // MN-major operand of 16-bit elements: see the head of this file.
 __device__ __forceinline__ uint64_t desc_across(uint32_t smemAddr)
