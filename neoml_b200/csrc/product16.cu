@@ -371,19 +371,28 @@ __global__ void __launch_bounds__(THREADS, 1) product16_kernel(const Product16Pa
 				} else {
 					if(on) {
 						uint16_t* const out = static_cast<uint16_t*>(p.out) + row * p.ldOut + col0 + c;
+						// whole sectors where rows allow it: a thread's row is 32 bytes at a time
+						const bool sectors = (p.ldOut & 15) == 0 && (reinterpret_cast<uintptr_t>(p.out) & 31u) == 0;
 						const bool aligned = (p.ldOut & 7) == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15u) == 0;
 #pragma unroll
-						for(int j = 0; j < 4; ++j) {
-							uint32_t w[4];
+						for(int j = 0; j < 2; ++j) {
+							uint32_t w[8];
 #pragma unroll
-							for(int i = 0; i < 4; ++i) w[i] = pack16(r[j * 8 + 2 * i] * by, r[j * 8 + 2 * i + 1] * by, p.bf16);
-							const int left = p.n - (col0 + c + j * 8);
-							if(aligned && left >= 8) {
-								*reinterpret_cast<uint4*>(out + j * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+							for(int i = 0; i < 8; ++i) w[i] = pack16(r[j * 16 + 2 * i] * by, r[j * 16 + 2 * i + 1] * by, p.bf16);
+							const int left = p.n - (col0 + c + j * 16);
+							if(sectors && left >= 16) {
+								store32(out + j * 16, w);
 							} else {
 #pragma unroll
-								for(int i = 0; i < 8; ++i) {
-									if(i < left) out[j * 8 + i] = static_cast<uint16_t>(i & 1 ? w[i >> 1] >> 16 : w[i >> 1] & 0xffffu);
+								for(int h = 0; h < 2; ++h) {
+									if(aligned && left >= 8 * h + 8) {
+										*reinterpret_cast<uint4*>(out + j * 16 + h * 8) = make_uint4(w[4 * h], w[4 * h + 1], w[4 * h + 2], w[4 * h + 3]);
+									} else {
+#pragma unroll
+										for(int i = 8 * h; i < 8 * h + 8; ++i) {
+											if(i < left) out[j * 16 + i] = static_cast<uint16_t>(i & 1 ? w[i >> 1] >> 16 : w[i >> 1] & 0xffffu);
+										}
+									}
 								}
 							}
 						}
