@@ -153,8 +153,12 @@ __global__ void __launch_bounds__(256) sum_planes_kernel(const float* __restrict
 		}
 		T* const to = out + row * outRow + col;
 		if constexpr(sizeof(T) == 4) {
-			const float f[4] = { v.x, v.y, v.z, v.w };
-			for(int j = 0; j < 4 && col + j < width; ++j) to[j] = f[j] * scale;
+			const float f[4] = { v.x * scale, v.y * scale, v.z * scale, v.w * scale };
+			if((outRow & 3) == 0 && (reinterpret_cast<uintptr_t>(out) & 15u) == 0 && col + 4 <= width) {
+				*reinterpret_cast<float4*>(to) = make_float4(f[0], f[1], f[2], f[3]);
+			} else {
+				for(int j = 0; j < 4 && col + j < width; ++j) to[j] = f[j];
+			}
 		} else if(vector && col + 4 <= width) {
 			*reinterpret_cast<uint2*>(to) = make_uint2(pack2<T>(v.x * scale, v.y * scale), pack2<T>(v.z * scale, v.w * scale));
 		} else {
@@ -226,14 +230,20 @@ int round_up(long long v, int to) { return static_cast<int>((v + to - 1) / to * 
 
 bool rows_for_tma(const void* p, long long row) { return aligned16(p) && row % 8 == 0; }
 
-// Columns of the vocabulary that are handled at a time: dz of a piece, and for fp32 the planes of a piece of the weights, take at most
-// PIECE_BYTES.  The 16-bit forward pass needs neither.
+// Rows of weights_diff that do not begin on 16-byte boundaries: a tile's threads, which have a row each, would store element by element.
+// They are written by the pass that adds up the parts of K then, along the rows (gradient of 5000 x 1030 fp16 weights by 1000 rows: 100
+// us in all, 177 when the tiles' threads stored it).
+bool by_planes(const Problem& q) { return q.width % (q.type == NB200_TYPE_FP32 ? 4 : 8) != 0; }
+
+// Columns of the vocabulary that are handled at a time: dz of a piece, for fp32 the planes of a piece of the weights, and the fp32 sums
+// of by_planes() take at most PIECE_BYTES each.  The 16-bit forward pass needs none of them.
 int piece_of(const Problem& q, bool backward)
 {
 	const bool fp32 = q.type == NB200_TYPE_FP32;
 	long long perColumn = fp32 ? 6ll * round_up(q.width, 8) : 0;
 	const long long diff = backward ? (fp32 ? 6ll : 2ll) * q.rows : 0;
 	if(diff > perColumn) perColumn = diff;
+	if(backward && by_planes(q) && 4ll * round_up(q.width, 8) > perColumn) perColumn = 4ll * round_up(q.width, 8);
 	const long long whole = round_up(q.vocabulary, PRODUCT16_N);
 	if(perColumn == 0) return static_cast<int>(whole);
 	long long piece = PIECE_BYTES / perColumn / PRODUCT16_N * PRODUCT16_N;
@@ -297,7 +307,7 @@ struct Backward {
 		weights = fp32 ? room.take<uint16_t>(3 * piece * ld) : rows_for_tma(q.weights, q.weightsRow) ? nullptr : room.take<uint16_t>(q.vocabulary * ld);
 		diff = room.take<uint16_t>(planes * q.rows * piece);
 		hiddenPlanes = room.take<float>(static_cast<size_t>(hiddenSplits) * q.rows * ld);
-		weightsPlanes = weightsSplits > 1 ? room.take<float>(static_cast<size_t>(weightsSplits) * piece * ld) : nullptr;
+		weightsPlanes = weightsSplits > 1 || by_planes(q) ? room.take<float>(static_cast<size_t>(weightsSplits) * piece * ld) : nullptr;
 	}
 };
 
@@ -438,7 +448,7 @@ int backward(const Problem& q, const float* lossDiff, const int* labels, const f
 		if(weightsDiff != nullptr) {
 			void* const out = static_cast<uint8_t*>(weightsDiff) + first * weightsDiffRow * type_size(q.type);
 			p = params_of(q, columns, q.width, w.weightsSplits, q.rows, false);
-			if(p.splits > 1) {
+			if(w.weightsPlanes != nullptr) {
 				p.plane = w.weightsPlanes; p.ldPlane = ld;
 				rc = product16(PRODUCT16_SUM, true, true, p, &diffAcross, &hiddenAcross, stream);
 				if(rc != NB200_OK) return rc;
