@@ -43,9 +43,26 @@ struct RecurrenceParams {
 	int* status;
 };
 
-struct Gate {
-	float keep, take; // sigmoid(x), 1 - sigmoid(x)
-};
+// The one or two channels of a thread.
+template<int W> struct Num;
+template<> struct Num<1> { float v; };
+template<> struct Num<2> { float2 v; };
+__device__ __forceinline__ Num<1> add(Num<1> a, Num<1> b) { return { a.v + b.v }; }
+__device__ __forceinline__ Num<1> mul(Num<1> a, Num<1> b) { return { a.v * b.v }; }
+__device__ __forceinline__ Num<1> fma(Num<1> a, Num<1> b, Num<1> c) { return { fmaf(a.v, b.v, c.v) }; }
+__device__ __forceinline__ Num<2> add(Num<2> a, Num<2> b) { return { add2(a.v, b.v) }; }
+__device__ __forceinline__ Num<2> mul(Num<2> a, Num<2> b) { return { mul2(a.v, b.v) }; }
+__device__ __forceinline__ Num<2> fma(Num<2> a, Num<2> b, Num<2> c) { return { fma2(a.v, b.v, c.v) }; }
+template<int W> __device__ __forceinline__ Num<W> all(float v)
+{
+	if constexpr(W == 1) return { v };
+	else return { both(v) };
+}
+template<int W> __device__ __forceinline__ Num<W> pick(bool yes, Num<W> a, Num<W> b)
+{
+	if constexpr(W == 1) return { yes ? a.v : b.v };
+	else return { make_float2(yes ? a.v.x : b.v.x, yes ? a.v.y : b.v.y) };
+}
 
 __device__ __forceinline__ float exp2_fast(float x)
 {
@@ -59,17 +76,10 @@ __device__ __forceinline__ float inverse_fast(float x)
 	asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
 	return y;
 }
-// Both without cancellation; the exponential never overflows.
-__device__ __forceinline__ Gate gate(float x)
-{
-	const float e = exp2_fast(fabsf(x) * -1.4426950408889634f);
-	const float large = inverse_fast(1.f + e), small = e * large;
-	return x >= 0.f ? Gate{ large, small } : Gate{ small, large };
-}
-__device__ __forceinline__ float sigmoid(float x)
-{
-	return inverse_fast(1.f + exp2_fast(x * -1.4426950408889634f)); // of infinity: zero
-}
+__device__ __forceinline__ Num<1> exp2_of(Num<1> x) { return { exp2_fast(x.v) }; }
+__device__ __forceinline__ Num<2> exp2_of(Num<2> x) { return { make_float2(exp2_fast(x.v.x), exp2_fast(x.v.y)) }; }
+__device__ __forceinline__ Num<1> inverse_of(Num<1> x) { return { inverse_fast(x.v) }; }
+__device__ __forceinline__ Num<2> inverse_of(Num<2> x) { return { make_float2(inverse_fast(x.v.x), inverse_fast(x.v.y)) }; }
 
 // W channels of one step as they lie in memory: one register
 template<typename T, int W>
@@ -79,22 +89,55 @@ __device__ __forceinline__ uint32_t load_raw(const T* p)
 	else return *reinterpret_cast<const unsigned short*>(p);
 }
 template<typename T, int W>
-__device__ __forceinline__ float2 floats(uint32_t raw)
+__device__ __forceinline__ Num<W> number(uint32_t raw)
 {
-	if constexpr(sizeof(T) == 4) return make_float2(__uint_as_float(raw), 0.f);
-	else return unpack2<T>(raw);
+	if constexpr(sizeof(T) == 4) return { __uint_as_float(raw) };
+	else if constexpr(W == 1) return { unpack2<T>(raw).x };
+	else return { unpack2<T>(raw) };
 }
 template<typename T, int W>
-__device__ __forceinline__ void store_raw(T* p, float a, float b)
+__device__ __forceinline__ void store_raw(T* p, Num<W> v)
 {
-	if constexpr(sizeof(T) == 4) *p = a;
-	else if constexpr(W == 2) *reinterpret_cast<uint32_t*>(p) = pack2<T>(a, b);
-	else *p = from_float<T>(a);
+	if constexpr(sizeof(T) == 4) *p = v.v;
+	else if constexpr(W == 2) *reinterpret_cast<uint32_t*>(p) = pack2<T>(v.v.x, v.v.y);
+	else *p = from_float<T>(v.v);
+}
+
+template<int W>
+struct Gate {
+	Num<W> keep, take; // sigmoid(x), 1 - sigmoid(x)
+};
+
+constexpr float MINUS_LOG2E = -1.4426950408889634f;
+
+// Both without cancellation: with e = 2^(-x log2 e), keep = 1 / (1 + e) and take = e keep.  In fp32, where e may overflow, of |x|,
+// and exchanged for a negative x.  16-bit gates are held at -80 instead (not a number stays one): 1.8e-35 is no other gate than zero there.
+template<typename T, int W>
+__device__ __forceinline__ Gate<W> gate(uint32_t raw)
+{
+	if constexpr(sizeof(T) == 4) {
+		const float x = __uint_as_float(raw);
+		const float e = exp2_fast(fabsf(x) * MINUS_LOG2E);
+		const float large = inverse_fast(1.f + e), small = e * large;
+		return x >= 0.f ? Gate<W>{ { large }, { small } } : Gate<W>{ { small }, { large } };
+	} else {
+		using T2 = typename PairOf<T>::type;
+		const uint32_t floor = pack2<T>(-80.f, -80.f);
+		const T2 held = __hmax2_nan(*reinterpret_cast<const T2*>(&raw), *reinterpret_cast<const T2*>(&floor));
+		const Num<W> e = exp2_of(mul(number<T, W>(*reinterpret_cast<const uint32_t*>(&held)), all<W>(MINUS_LOG2E)));
+		const Num<W> keep = inverse_of(add(e, all<W>(1.f)));
+		return { keep, mul(e, keep) };
+	}
+}
+template<typename T, int W>
+__device__ __forceinline__ Num<W> sigmoid(uint32_t raw)
+{
+	return inverse_of(add(exp2_of(mul(number<T, W>(raw), all<W>(MINUS_LOG2E))), all<W>(1.f))); // 2^infinity: zero
 }
 
 template<int W>
 struct Fold {
-	float a[W], h[W];
+	Num<W> a, h;
 };
 
 // What a block's threads share: their folds, and those of the cluster's blocks (two sets, for alternating rounds).
@@ -113,7 +156,7 @@ __device__ __forceinline__ void send(const Fold<1>& f, Fold<1>* at, uint64_t* ba
 		"mapa.shared::cluster.u32 a, %0, %2;\n\t"
 		"mapa.shared::cluster.u32 m, %1, %2;\n\t"
 		"st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.b32 [a], {%3, %4}, [m];\n\t}"
-		::"r"(smem_u32(at)), "r"(smem_u32(bar)), "r"(rank), "r"(__float_as_uint(f.a[0])), "r"(__float_as_uint(f.h[0])) : "memory");
+		::"r"(smem_u32(at)), "r"(smem_u32(bar)), "r"(rank), "r"(__float_as_uint(f.a.v)), "r"(__float_as_uint(f.h.v)) : "memory");
 }
 __device__ __forceinline__ void send(const Fold<2>& f, Fold<2>* at, uint64_t* bar, int rank)
 {
@@ -121,8 +164,8 @@ __device__ __forceinline__ void send(const Fold<2>& f, Fold<2>* at, uint64_t* ba
 		"mapa.shared::cluster.u32 a, %0, %2;\n\t"
 		"mapa.shared::cluster.u32 m, %1, %2;\n\t"
 		"st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [a], {%3, %4, %5, %6}, [m];\n\t}"
-		::"r"(smem_u32(at)), "r"(smem_u32(bar)), "r"(rank), "r"(__float_as_uint(f.a[0])), "r"(__float_as_uint(f.a[1])),
-		  "r"(__float_as_uint(f.h[0])), "r"(__float_as_uint(f.h[1])) : "memory");
+		::"r"(smem_u32(at)), "r"(smem_u32(bar)), "r"(rank), "r"(__float_as_uint(f.a.v.x)), "r"(__float_as_uint(f.a.v.y)),
+		  "r"(__float_as_uint(f.h.v.x)), "r"(__float_as_uint(f.h.v.y)) : "memory");
 }
 
 template<int W>
@@ -145,21 +188,13 @@ __device__ __forceinline__ void begin_sharing(Shared<W>& s, int blocks)
 // the set of the round before, and nobody sends the round after next without having received that fold.
 template<int W>
 __device__ __forceinline__ void join(Shared<W>& s, const Fold<W>& mine, int round, int rank, int blocks, int warps, int* status,
-	float* carry, float* state)
+	Num<W>& carry, Num<W>& state)
 {
 	const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, set = round & 1;
-	Fold<W> before;
-#pragma unroll
-	for(int w = 0; w < W; ++w) {
-		before.a[w] = 1.f;
-		before.h[w] = 0.f;
-	}
+	Fold<W> before = { all<W>(1.f), all<W>(0.f) };
 	auto after = [](Fold<W>& f, const Fold<W>& next) {
-#pragma unroll
-		for(int w = 0; w < W; ++w) {
-			f.h[w] = fmaf(next.a[w], f.h[w], next.h[w]);
-			f.a[w] *= next.a[w];
-		}
+		f.h = fma(next.a, f.h, next.h);
+		f.a = mul(f.a, next.a);
 	};
 	if(warps > 1) {
 		if(warp < warps - 1) s.warps[set][warp][lane] = mine;
@@ -167,31 +202,45 @@ __device__ __forceinline__ void join(Shared<W>& s, const Fold<W>& mine, int roun
 		for(int k = 0; k < warp; ++k) after(before, s.warps[set][k][lane]);
 	}
 	if(warp == warps - 1) { // the block's fold, to every block of the cluster, this one too
-		Fold<W> all = before;
-		after(all, mine);
+		Fold<W> whole = before;
+		after(whole, mine);
 		if(blocks == 1) { // launched without a cluster: st.async is not an instruction of such a kernel
-			s.blocks[set][0][lane] = all;
+			s.blocks[set][0][lane] = whole;
 			__syncwarp();
 			if(lane == 0) mbar_arrive(s.arrived + set);
 		} else {
 			if(lane == 0) mbar_arrive_expect_tx(s.arrived + set, static_cast<uint32_t>(blocks * 32 * sizeof(Fold<W>)));
-			for(int k = 0; k < blocks; ++k) send(all, &s.blocks[set][rank][lane], s.arrived + set, k);
+			for(int k = 0; k < blocks; ++k) send(whole, &s.blocks[set][rank][lane], s.arrived + set, k);
 		}
 	}
 	// should the wait give up, the rounds go on with what is there: every block has to reach the end
 	mbar_wait_bounded_warp(s.arrived + set, (round >> 1) & 1, &s.abortFlag, status, (KERNEL_ID << 8) | 1);
-	float start[W];
+	Num<W> start = carry;
 	for(int k = 0; k < blocks; ++k) {
-		if(k == rank) {
-#pragma unroll
-			for(int w = 0; w < W; ++w) start[w] = carry[w];
-		}
+		if(k == rank) start = carry;
 		const Fold<W> next = s.blocks[set][k][lane];
-#pragma unroll
-		for(int w = 0; w < W; ++w) carry[w] = fmaf(next.a[w], carry[w], next.h[w]);
+		carry = fma(next.a, carry, next.h);
 	}
-#pragma unroll
-	for(int w = 0; w < W; ++w) state[w] = fmaf(before.a[w], start[w], before.h[w]);
+	state = fma(before.a, start, before.h);
+}
+
+// A state or its gradient, fp32; null: zeros.
+template<int W>
+__device__ __forceinline__ Num<W> load_state(const float* from, long long at)
+{
+	if(from == nullptr) return all<W>(0.f);
+	if constexpr(W == 1) return { from[at] };
+	else return { make_float2(from[at], from[at + 1]) };
+}
+template<int W>
+__device__ __forceinline__ void store_state(float* to, long long at, Num<W> v)
+{
+	if constexpr(W == 1) {
+		to[at] = v.v;
+	} else {
+		to[at] = v.v.x;
+		to[at + 1] = v.v.y;
+	}
 }
 
 __device__ __forceinline__ int sequence_length(const RecurrenceParams& p, int b)
@@ -241,9 +290,7 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, W == 1 ? 3 : 2) recurrence_for
 #pragma unroll
 	for(int k = 0; k < STEPS; ++k) offset[k] = (static_cast<uint32_t>(first + k) * p.channels + c) * static_cast<uint32_t>(sizeof(T));
 	const long long state0 = static_cast<long long>(b) * p.channels + c;
-	float carry[W];
-#pragma unroll
-	for(int w = 0; w < W; ++w) carry[w] = p.first != nullptr ? p.first[state0 + w] : 0.f;
+	Num<W> carry = load_state<W>(p.first, state0);
 
 	uint32_t rz[STEPS], rf[STEPS], ri[STEPS];
 	auto load = [&](int t, auto full) {
@@ -260,29 +307,19 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, W == 1 ? 3 : 2) recurrence_for
 	else load(t, No());
 	// the whole cluster agrees on n, and on the number of rounds
 	for(; round * stride < n; ++round) {
-		float a[STEPS][W], h[STEPS][W];
-		Fold<W> mine;
-#pragma unroll
-		for(int w = 0; w < W; ++w) {
-			mine.a[w] = 1.f;
-			mine.h[w] = 0.f;
-		}
+		Num<W> a[STEPS], h[STEPS];
+		Fold<W> mine = { all<W>(1.f), all<W>(0.f) };
 		auto fold = [&](auto full) {
 #pragma unroll
 			for(int k = 0; k < STEPS; ++k) {
-				const float2 vz = floats<T, W>(rz[k]), vf = floats<T, W>(rf[k]);
-				float2 vi = make_float2(0.f, 0.f);
-				if constexpr(INPUT) vi = floats<T, W>(ri[k]);
 				const bool in = decltype(full)::value || t + k < n;
-#pragma unroll
-				for(int w = 0; w < W; ++w) {
-					const Gate forget = gate(w == 0 ? vf.x : vf.y);
-					const float take = INPUT ? sigmoid(w == 0 ? vi.x : vi.y) : forget.take;
-					a[k][w] = in ? forget.keep : 1.f;
-					h[k][w] = in ? take * (w == 0 ? vz.x : vz.y) : 0.f;
-					mine.h[w] = fmaf(a[k][w], mine.h[w], h[k][w]);
-					mine.a[w] *= a[k][w];
-				}
+				const Gate<W> forget = gate<T, W>(rf[k]);
+				Num<W> take = forget.take;
+				if constexpr(INPUT) take = sigmoid<T, W>(ri[k]);
+				a[k] = pick<W>(in, forget.keep, all<W>(1.f));
+				h[k] = pick<W>(in, mul(take, number<T, W>(rz[k])), all<W>(0.f));
+				mine.h = fma(a[k], mine.h, h[k]);
+				mine.a = mul(mine.a, a[k]);
 			}
 		};
 		const bool whole = t + STEPS <= n;
@@ -295,15 +332,14 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, W == 1 ? 3 : 2) recurrence_for
 		}
 		if(t + stride + STEPS <= n) load(t + stride, Yes());
 		else load(t + stride, No());
-		float state[W];
+		Num<W> state;
 		join<W>(s, mine, round, rank, blocks, warps, p.status, carry, state);
 		auto apply = [&](auto full) {
 #pragma unroll
 			for(int k = 0; k < STEPS; ++k) {
-#pragma unroll
-				for(int w = 0; w < W; ++w) state[w] = fmaf(a[k][w], state[w], h[k][w]);
+				state = fma(a[k], state, h[k]);
 				T* const to = DENSE ? reinterpret_cast<T*>(outRound + offset[k]) : out + static_cast<long long>(t + k) * p.channels + c;
-				if(on && (decltype(full)::value || t + k < n)) store_raw<T, W>(to, state[0], state[W - 1]);
+				if(on && (decltype(full)::value || t + k < n)) store_raw<T, W>(to, state);
 			}
 		};
 		if(whole) apply(Yes());
@@ -313,12 +349,9 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, W == 1 ? 3 : 2) recurrence_for
 	}
 	// behind the sequence the results are zeros
 	for(int k = n + rank * warps + warp; k < p.length; k += blocks * warps) {
-		if(on) store_raw<T, W>(out + static_cast<long long>(k) * p.channels + c, 0.f, 0.f);
+		if(on) store_raw<T, W>(out + static_cast<long long>(k) * p.channels + c, all<W>(0.f));
 	}
-	if(on && p.last != nullptr && rank == 0 && warp == 0) {
-#pragma unroll
-		for(int w = 0; w < W; ++w) p.last[state0 + w] = carry[w];
-	}
+	if(on && p.last != nullptr && rank == 0 && warp == 0) store_state<W>(p.last, state0, carry);
 	if(blocks > 1) cg::this_cluster().sync(); // nobody leaves while its shared memory may be written
 }
 
@@ -355,19 +388,15 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 2) recurrence_backward_kernel(
 #pragma unroll
 	for(int k = 0; k < STEPS; ++k) offset[k] = (static_cast<uint32_t>(stride - 1 - back - k) * p.channels + c) * static_cast<uint32_t>(sizeof(T));
 	const long long state0 = static_cast<long long>(b) * p.channels + c;
-	float carry[W], first[W]; // carry: what step t + 1 hands back, a_{t+1} S_{t+1}
-#pragma unroll
-	for(int w = 0; w < W; ++w) {
-		carry[w] = p.lastDiff != nullptr ? p.lastDiff[state0 + w] : 0.f;
-		first[w] = p.first != nullptr ? p.first[state0 + w] : 0.f;
-	}
+	Num<W> carry = load_state<W>(p.lastDiff, state0); // what step t + 1 hands back, a_{t+1} S_{t+1}
+	const Num<W> first = load_state<W>(p.first, state0);
 	// behind the sequence the gradients are zeros
 	for(int k = n + rank * warps + warp; k < p.length; k += blocks * warps) {
 		const long long at = static_cast<long long>(k) * p.channels + c;
 		if(!on) break;
-		store_raw<T, W>(dz + at, 0.f, 0.f);
-		store_raw<T, W>(df + at, 0.f, 0.f);
-		if constexpr(INPUT) store_raw<T, W>(di + at, 0.f, 0.f);
+		store_raw<T, W>(dz + at, all<W>(0.f));
+		store_raw<T, W>(df + at, all<W>(0.f));
+		if constexpr(INPUT) store_raw<T, W>(di + at, all<W>(0.f));
 	}
 	// The gates and the gradients are wanted when a round begins, the rest only when its state has arrived: the former are
 	// loaded a whole round ahead, the latter while the round before them ends.
@@ -398,28 +427,19 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 2) recurrence_backward_kernel(
 		load_rest(t, No());
 	}
 	for(; round * stride < n; ++round) {
-		float a[STEPS][W], u[STEPS][W];
-		Fold<W> mine;
-#pragma unroll
-		for(int w = 0; w < W; ++w) {
-			mine.a[w] = 1.f;
-			mine.h[w] = 0.f;
-		}
+		Num<W> a[STEPS], u[STEPS];
+		Fold<W> mine = { all<W>(1.f), all<W>(0.f) };
 		auto fold = [&](auto full) {
 #pragma unroll
 			for(int k = 0; k < STEPS; ++k) {
 				rd[k] = nd[k];
-				const float2 vf = floats<T, W>(rf[k]), vd = floats<T, W>(rd[k]);
 				const bool in = decltype(full)::value || t - k >= 0;
-#pragma unroll
-				for(int w = 0; w < W; ++w) {
-					const Gate forget = gate(w == 0 ? vf.x : vf.y);
-					a[k][w] = in ? forget.keep : 1.f;
-					u[k][w] = forget.take;
-					// a (dh + s): this step's own part is a dh
-					mine.h[w] = a[k][w] * (mine.h[w] + (w == 0 ? vd.x : vd.y));
-					mine.a[w] *= a[k][w];
-				}
+				const Gate<W> forget = gate<T, W>(rf[k]);
+				a[k] = pick<W>(in, forget.keep, all<W>(1.f));
+				u[k] = forget.take;
+				// a (dh + s): this step's own part is a dh
+				mine.h = mul(a[k], add(mine.h, number<T, W>(rd[k])));
+				mine.a = mul(mine.a, a[k]);
 			}
 		};
 		const bool whole = t - STEPS >= 0, nextWhole = t - stride - STEPS >= 0;
@@ -431,37 +451,32 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 2) recurrence_backward_kernel(
 		}
 		if(nextWhole) load_gates(t - stride, Yes());
 		else load_gates(t - stride, No());
-		float state[W];
+		Num<W> state;
 		join<W>(s, mine, round, rank, blocks, warps, p.status, carry, state);
 		auto apply = [&](auto full) {
 #pragma unroll
 			for(int k = 0; k < STEPS; ++k) {
-				const float2 vd = floats<T, W>(rd[k]), vz = floats<T, W>(rz[k]);
-				float2 vh = floats<T, W>(rh[k]), vi = make_float2(0.f, 0.f);
-				if(!decltype(full)::value && t - k == 0) vh = make_float2(first[0], first[W - 1]);
-				if constexpr(INPUT) vi = floats<T, W>(ri[k]);
-				float oz[W], of[W], oi[W];
-#pragma unroll
-				for(int w = 0; w < W; ++w) {
-					const float S = state[w] + (w == 0 ? vd.x : vd.y), zz = w == 0 ? vz.x : vz.y, before = w == 0 ? vh.x : vh.y;
-					const float slope = a[k][w] * u[k][w];
-					if constexpr(INPUT) {
-						const Gate take = gate(w == 0 ? vi.x : vi.y);
-						oz[w] = S * take.keep;
-						of[w] = S * before * slope;
-						oi[w] = oz[w] * zz * take.take;
-					} else {
-						oz[w] = S * u[k][w];
-						of[w] = S * (before - zz) * slope;
-					}
-					state[w] = a[k][w] * S;
+				const Num<W> S = add(state, number<T, W>(rd[k])), value = number<T, W>(rz[k]);
+				Num<W> before = number<T, W>(rh[k]);
+				if(!decltype(full)::value && t - k == 0) before = first;
+				const Num<W> slope = mul(a[k], u[k]);
+				Num<W> oz, of, oi = S;
+				if constexpr(INPUT) {
+					const Gate<W> take = gate<T, W>(ri[k]);
+					oz = mul(S, take.keep);
+					of = mul(mul(S, before), slope);
+					oi = mul(mul(oz, value), take.take);
+				} else {
+					oz = mul(S, u[k]);
+					of = mul(mul(S, fma(value, all<W>(-1.f), before)), slope);
 				}
+				state = mul(a[k], S);
 				if(on && (decltype(full)::value || t - k >= 0)) {
 					const long long step = DENSE ? 0 : static_cast<long long>(t - k) * p.channels + c;
-					store_raw<T, W>(DENSE ? reinterpret_cast<T*>(reinterpret_cast<uint8_t*>(dz) + outRound + offset[k]) : dz + step, oz[0], oz[W - 1]);
-					store_raw<T, W>(DENSE ? reinterpret_cast<T*>(reinterpret_cast<uint8_t*>(df) + outRound + offset[k]) : df + step, of[0], of[W - 1]);
+					store_raw<T, W>(DENSE ? reinterpret_cast<T*>(reinterpret_cast<uint8_t*>(dz) + outRound + offset[k]) : dz + step, oz);
+					store_raw<T, W>(DENSE ? reinterpret_cast<T*>(reinterpret_cast<uint8_t*>(df) + outRound + offset[k]) : df + step, of);
 					if constexpr(INPUT) {
-						store_raw<T, W>(DENSE ? reinterpret_cast<T*>(reinterpret_cast<uint8_t*>(di) + outRound + offset[k]) : di + step, oi[0], oi[W - 1]);
+						store_raw<T, W>(DENSE ? reinterpret_cast<T*>(reinterpret_cast<uint8_t*>(di) + outRound + offset[k]) : di + step, oi);
 					}
 				}
 			}
@@ -478,10 +493,7 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 2) recurrence_backward_kernel(
 		outRound -= roundBytes;
 		t -= stride;
 	}
-	if(on && p.last != nullptr && rank == 0 && warp == 0) {
-#pragma unroll
-		for(int w = 0; w < W; ++w) p.last[state0 + w] = carry[w];
-	}
+	if(on && p.last != nullptr && rank == 0 && warp == 0) store_state<W>(p.last, state0, carry);
 	if(blocks > 1) cg::this_cluster().sync();
 }
 
