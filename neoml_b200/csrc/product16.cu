@@ -490,6 +490,22 @@ bool product16_map(void* map, const void* base, bool bf16, long long inner, long
 		CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+bool sequence_map(void* map, const void* base, int type, long long channels, long long length, long long batch, long long row,
+	long long batchStride, int steps)
+{
+	const EncodeTiledFn encode = encoder();
+	const long long size = type_size(type);
+	if(encode == nullptr || !aligned16(base) || row <= 0 || batchStride <= 0 || row * size % 16 != 0 || batchStride * size % 16 != 0
+		|| row * size >= (1ll << 40) || batchStride * size >= (1ll << 40)) return false;
+	const cuuint64_t dims[3] = { static_cast<cuuint64_t>(channels), static_cast<cuuint64_t>(length), static_cast<cuuint64_t>(batch) };
+	const cuuint64_t strides[2] = { static_cast<cuuint64_t>(row * size), static_cast<cuuint64_t>(batchStride * size) };
+	const cuuint32_t box[3] = { static_cast<cuuint32_t>(128 / size), static_cast<cuuint32_t>(steps), 1 };
+	const cuuint32_t each[3] = { 1, 1, 1 };
+	return encode(static_cast<CUtensorMap*>(map), type == NB200_TYPE_FP32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : type == NB200_TYPE_FP16
+		? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, each,
+		CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 int product16(Product16Epilogue epilogue, bool aAcross, bool bAcross, const Product16Params& p, const void* mapA, const void* mapB,
 	cudaStream_t stream)
 {

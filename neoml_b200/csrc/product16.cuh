@@ -59,6 +59,11 @@ int product16(Product16Epilogue epilogue, bool aAcross, bool bAcross, const Prod
 bool product16_map(void* map, const void* base, bool bf16, long long inner, long long rows, long long rowSize, int boxRows,
 	long long planeSize = 0);
 
+// Map of [batch][length][channels] in the operator types: boxes of `steps` steps x 128 bytes of channels, dense.  False as above, and where
+// a stride is zero.
+bool sequence_map(void* map, const void* base, int type, long long channels, long long length, long long batch, long long row,
+	long long batchStride, int steps);
+
 constexpr int PRODUCT16_M = 128, PRODUCT16_N = 256, PRODUCT16_K = 64; // of a tile
 constexpr int PRODUCT16_BOX_A = 128, PRODUCT16_BOX_B = 256, PRODUCT16_BOX_ACROSS = 64; // boxRows of the operands' maps
 

@@ -16,8 +16,9 @@
 //            mbarrier: a cluster-wide barrier would wait for the results' stores to global memory too, every round
 // The next round's loads are issued before this one is folded.
 // The gates' pre-activations are the inputs: a gate of 0.999 rounded to bf16 is 1 and would never forget.
-#include "types16.cuh"
+#include "product16.cuh"
 #include <cooperative_groups.h>
+#include <cuda.h>
 
 namespace nb200 {
 
@@ -497,6 +498,254 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 2) recurrence_backward_kernel(
 	if(blocks > 1) cg::this_cluster().sync();
 }
 
+// ---- the same fed by TMA ----------------------------------------------------------------------------------------------
+// Long sequences whose rows begin on 16-byte boundaries: a warp's stretches come as boxes of S steps x 128 bytes into a ring of its
+// own in shared memory, several rounds ahead, by one lane's instructions; steps and channels that do not exist come as zeros.  Loads into
+// registers are one round ahead at most, and that held the kernels above to 55 - 70 % of the memory's rate.  A ring needs no
+// barrier for free stages: its warp has read a stage when it asks for the next round in its place.
+
+struct Maps {
+	CUtensorMap z, f, i, dh, h;
+};
+
+// One warp's ring: `arrays` boxes a stage.
+template<int S>
+struct Ring {
+	static constexpr int BOX_BYTES = S * 128;
+	uint8_t* stages;
+	uint64_t* full;
+	int arrays, depth;
+	__device__ __forceinline__ const uint32_t* box(int round, int array) const
+	{
+		return reinterpret_cast<const uint32_t*>(stages + ((round % depth) * arrays + array) * BOX_BYTES);
+	}
+	__device__ __forceinline__ uint32_t begin(int round) const // by one lane
+	{
+		mbar_arrive_expect_tx(full + round % depth, arrays * BOX_BYTES);
+		return smem_u32(stages + (round % depth) * arrays * BOX_BYTES);
+	}
+	__device__ __forceinline__ void wait(int round, volatile int* abortFlag, int* status) const
+	{
+		mbar_wait_bounded_warp(full + round % depth, (round / depth) & 1, abortFlag, status, (KERNEL_ID << 8) | 2);
+	}
+};
+
+template<int S, int DEPTH>
+__device__ __forceinline__ Ring<S> make_ring(uint8_t* room, uint64_t (&bars)[MAX_WARPS][DEPTH], int arrays)
+{
+	const int warp = threadIdx.x >> 5;
+	Ring<S> ring = { room + warp * DEPTH * arrays * Ring<S>::BOX_BYTES, bars[warp], arrays, DEPTH };
+	if((threadIdx.x & 31) == 0) {
+		for(int k = 0; k < DEPTH; ++k) mbar_init(ring.full + k, 1);
+		mbar_init_fence();
+	}
+	return ring; // begin_sharing() is the barrier behind this
+}
+
+// The stage has been read by the whole warp: its next round may be asked for.
+__device__ __forceinline__ void stage_read()
+{
+	__syncwarp();
+	fence_proxy_async_smem();
+}
+
+template<typename T, int W, bool INPUT, int S, int DEPTH>
+__global__ void __launch_bounds__(MAX_WARPS * 32, S == 8 ? 3 : 2) recurrence_forward_stream_kernel(const RecurrenceParams p, const __grid_constant__ Maps maps)
+{
+	extern __shared__ __align__(128) uint8_t streamRoom[];
+	__shared__ Shared<W> s;
+	__shared__ uint64_t bars[MAX_WARPS][DEPTH];
+	constexpr int ARRAYS = INPUT ? 3 : 2;
+	const int blocks = gridDim.y, rank = blockIdx.y;
+	const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+	constexpr int BOX_BYTES = Ring<S>::BOX_BYTES;
+	const Ring<S> ring = make_ring<S, DEPTH>(streamRoom, bars, ARRAYS);
+	begin_sharing<W>(s, blocks);
+	const int b = blockIdx.z;
+	const int tile = blockIdx.x * 32 * W;
+	const int c = tile + lane * W;
+	const bool on = c < p.channels;
+	const int n = sequence_length(p, b);
+	const int span = warps * S, stride = span * blocks;
+	const int first = rank * span + warp * S;
+	T* const out = static_cast<T*>(p.out) + static_cast<long long>(b) * p.length * p.channels;
+	uint8_t* outRound = reinterpret_cast<uint8_t*>(out);
+	const long long roundBytes = static_cast<long long>(stride) * p.channels * sizeof(T);
+	uint32_t offset[S];
+#pragma unroll
+	for(int k = 0; k < S; ++k) offset[k] = (static_cast<uint32_t>(first + k) * p.channels + c) * static_cast<uint32_t>(sizeof(T));
+	const long long state0 = static_cast<long long>(b) * p.channels + c;
+	Num<W> carry = all<W>(0.f);
+	if(on) carry = load_state<W>(p.first, state0);
+	auto ask = [&](int round) {
+		const int t = first + round * stride;
+		if(t >= n || lane != 0) return;
+		const uint32_t at = ring.begin(round);
+		uint64_t* const bar = ring.full + round % DEPTH;
+		tma_load_3d(at, &maps.z, bar, tile, t, b);
+		tma_load_3d(at + BOX_BYTES, &maps.f, bar, tile, t, b);
+		if constexpr(INPUT) tma_load_3d(at + 2 * BOX_BYTES, &maps.i, bar, tile, t, b);
+	};
+	for(int k = 0; k < DEPTH; ++k) ask(k);
+	int t = first;
+	for(int round = 0; round * stride < n; ++round, t += stride) {
+		Num<W> a[S], h[S];
+		Fold<W> mine = { all<W>(1.f), all<W>(0.f) };
+		auto fold = [&](auto full) {
+			const uint32_t *z = ring.box(round, 0) + lane, *f = ring.box(round, 1) + lane, *i = ring.box(round, INPUT ? 2 : 0) + lane;
+#pragma unroll
+			for(int k = 0; k < S; ++k) {
+				const bool in = decltype(full)::value || t + k < n;
+				const Gate<W> forget = gate<T, W>(f[k * 32]);
+				Num<W> take = forget.take;
+				if constexpr(INPUT) take = sigmoid<T, W>(i[k * 32]);
+				a[k] = pick<W>(in, forget.keep, all<W>(1.f));
+				h[k] = pick<W>(in, mul(take, number<T, W>(z[k * 32])), all<W>(0.f));
+				mine.h = fma(a[k], mine.h, h[k]);
+				mine.a = mul(mine.a, a[k]);
+			}
+		};
+		const bool whole = t + S <= n;
+		if(t < n) ring.wait(round, &s.abortFlag, p.status);
+		if(whole) fold(Yes());
+		else if(t < n) fold(No());
+		stage_read();
+		ask(round + DEPTH);
+		Num<W> state;
+		join<W>(s, mine, round, rank, blocks, warps, p.status, carry, state);
+		auto apply = [&](auto full) {
+#pragma unroll
+			for(int k = 0; k < S; ++k) {
+				state = fma(a[k], state, h[k]);
+				if(on && (decltype(full)::value || t + k < n)) store_raw<T, W>(reinterpret_cast<T*>(outRound + offset[k]), state);
+			}
+		};
+		if(whole) apply(Yes());
+		else if(t < n) apply(No());
+		outRound += roundBytes;
+	}
+	// behind the sequence the results are zeros
+	for(int k = n + rank * warps + warp; k < p.length; k += blocks * warps) {
+		if(on) store_raw<T, W>(out + static_cast<long long>(k) * p.channels + c, all<W>(0.f));
+	}
+	if(on && p.last != nullptr && rank == 0 && warp == 0) store_state<W>(p.last, state0, carry);
+	if(blocks > 1) cg::this_cluster().sync(); // nobody leaves while its shared memory may be written
+}
+
+template<typename T, int W, bool INPUT, int S, int DEPTH>
+__global__ void __launch_bounds__(MAX_WARPS * 32, 2) recurrence_backward_stream_kernel(const RecurrenceParams p, const __grid_constant__ Maps maps)
+{
+	extern __shared__ __align__(128) uint8_t streamRoom[];
+	__shared__ Shared<W> s;
+	__shared__ uint64_t bars[MAX_WARPS][DEPTH];
+	constexpr int ARRAYS = INPUT ? 5 : 4;
+	const int blocks = gridDim.y, rank = blockIdx.y;
+	const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+	constexpr int BOX_BYTES = Ring<S>::BOX_BYTES;
+	const Ring<S> ring = make_ring<S, DEPTH>(streamRoom, bars, ARRAYS);
+	begin_sharing<W>(s, blocks);
+	const int b = blockIdx.z;
+	const int tile = blockIdx.x * 32 * W;
+	const int c = tile + lane * W;
+	const bool on = c < p.channels;
+	const int n = sequence_length(p, b);
+	const int span = warps * S, stride = span * blocks;
+	const int back = rank * span + warp * S; // steps between the round's last one and this thread's first
+	const long long roundBytes = static_cast<long long>(stride) * p.channels * sizeof(T);
+	const long long sequence = static_cast<long long>(b) * p.length * p.channels;
+	long long outRound = static_cast<long long>(n - stride) * p.channels * static_cast<long long>(sizeof(T));
+	uint8_t* const dz = reinterpret_cast<uint8_t*>(static_cast<T*>(p.out) + sequence);
+	uint8_t* const df = reinterpret_cast<uint8_t*>(static_cast<T*>(p.df) + sequence);
+	uint8_t* const di = INPUT ? reinterpret_cast<uint8_t*>(static_cast<T*>(p.di) + sequence) : nullptr;
+	uint32_t offset[S];
+#pragma unroll
+	for(int k = 0; k < S; ++k) offset[k] = (static_cast<uint32_t>(stride - 1 - back - k) * p.channels + c) * static_cast<uint32_t>(sizeof(T));
+	const long long state0 = static_cast<long long>(b) * p.channels + c;
+	Num<W> carry = all<W>(0.f), first = all<W>(0.f);
+	if(on) {
+		carry = load_state<W>(p.lastDiff, state0);
+		first = load_state<W>(p.first, state0);
+	}
+	auto ask = [&](int round) {
+		const int t = n - 1 - back - round * stride, from = t - S + 1; // a box may begin in front of step 0
+		if(t < 0 || lane != 0) return;
+		const uint32_t at = ring.begin(round);
+		uint64_t* const bar = ring.full + round % DEPTH;
+		tma_load_3d(at, &maps.f, bar, tile, from, b);
+		tma_load_3d(at + BOX_BYTES, &maps.dh, bar, tile, from, b);
+		tma_load_3d(at + 2 * BOX_BYTES, &maps.z, bar, tile, from, b);
+		tma_load_3d(at + 3 * BOX_BYTES, &maps.h, bar, tile, from - 1, b); // the step before
+		if constexpr(INPUT) tma_load_3d(at + 4 * BOX_BYTES, &maps.i, bar, tile, from, b);
+	};
+	for(int k = 0; k < DEPTH; ++k) ask(k);
+	// behind the sequence the gradients are zeros
+	for(int k = n + rank * warps + warp; k < p.length; k += blocks * warps) {
+		const long long at = (static_cast<long long>(k) * p.channels + c) * static_cast<long long>(sizeof(T));
+		if(!on) break;
+		store_raw<T, W>(reinterpret_cast<T*>(dz + at), all<W>(0.f));
+		store_raw<T, W>(reinterpret_cast<T*>(df + at), all<W>(0.f));
+		if constexpr(INPUT) store_raw<T, W>(reinterpret_cast<T*>(di + at), all<W>(0.f));
+	}
+	int t = n - 1 - back;
+	for(int round = 0; round * stride < n; ++round, t -= stride) {
+		Num<W> a[S], u[S];
+		Fold<W> mine = { all<W>(1.f), all<W>(0.f) };
+		const uint32_t *f = ring.box(round, 0) + lane, *d = ring.box(round, 1) + lane, *z = ring.box(round, 2) + lane,
+			*h = ring.box(round, 3) + lane, *i = ring.box(round, INPUT ? 4 : 0) + lane;
+		auto fold = [&](auto full) {
+#pragma unroll
+			for(int k = 0; k < S; ++k) {
+				const int row = (S - 1 - k) * 32;
+				const bool in = decltype(full)::value || t - k >= 0;
+				const Gate<W> forget = gate<T, W>(f[row]);
+				a[k] = pick<W>(in, forget.keep, all<W>(1.f));
+				u[k] = forget.take;
+				mine.h = mul(a[k], add(mine.h, number<T, W>(d[row]))); // this step's own part is a dh
+				mine.a = mul(mine.a, a[k]);
+			}
+		};
+		const bool whole = t - S >= 0;
+		if(t >= 0) ring.wait(round, &s.abortFlag, p.status);
+		if(whole) fold(Yes());
+		else if(t >= 0) fold(No());
+		Num<W> state;
+		join<W>(s, mine, round, rank, blocks, warps, p.status, carry, state);
+		auto apply = [&](auto full) {
+#pragma unroll
+			for(int k = 0; k < S; ++k) {
+				const int row = (S - 1 - k) * 32;
+				const Num<W> S = add(state, number<T, W>(d[row])), value = number<T, W>(z[row]);
+				Num<W> before = number<T, W>(h[row]);
+				if(!decltype(full)::value && t - k == 0) before = first;
+				const Num<W> slope = mul(a[k], u[k]);
+				Num<W> oz, of, oi = S;
+				if constexpr(INPUT) {
+					const Gate<W> take = gate<T, W>(i[row]);
+					oz = mul(S, take.keep);
+					of = mul(mul(S, before), slope);
+					oi = mul(mul(oz, value), take.take);
+				} else {
+					oz = mul(S, u[k]);
+					of = mul(mul(S, fma(value, all<W>(-1.f), before)), slope);
+				}
+				state = mul(a[k], S);
+				if(on && (decltype(full)::value || t - k >= 0)) {
+					store_raw<T, W>(reinterpret_cast<T*>(dz + outRound + offset[k]), oz);
+					store_raw<T, W>(reinterpret_cast<T*>(df + outRound + offset[k]), of);
+					if constexpr(INPUT) store_raw<T, W>(reinterpret_cast<T*>(di + outRound + offset[k]), oi);
+				}
+			}
+		};
+		if(whole) apply(Yes());
+		else if(t >= 0) apply(No());
+		stage_read();
+		ask(round + DEPTH);
+		outRound -= roundBytes;
+	}
+	if(on && p.last != nullptr && rank == 0 && warp == 0) store_state<W>(p.last, state0, carry);
+	if(blocks > 1) cg::this_cluster().sync();
+}
+
 using Kernel = void (*)(const RecurrenceParams);
 
 template<typename T, int W, bool BACKWARD>
@@ -518,6 +767,40 @@ Kernel kernel_for(int type, bool pair, bool input, bool dense)
 	return pair ? kernel_of<__nv_bfloat16, 2, BACKWARD>(input, dense) : kernel_of<__nv_bfloat16, 1, BACKWARD>(input, dense);
 }
 
+// Rounds that a warp's loads are ahead of its work, by what fits beside one another in 16 or more warps' shared memory.
+constexpr int FORWARD_STEPS = 16, FORWARD_DEPTH = 2, FORWARD_INPUT_DEPTH = 2, BACKWARD_STEPS = 8, BACKWARD_DEPTH = 3, BACKWARD_INPUT_DEPTH = 2;
+
+using StreamKernel = void (*)(const RecurrenceParams, const Maps);
+
+template<bool BACKWARD, typename T, int W>
+StreamKernel stream_of(bool input)
+{
+	if(BACKWARD) return input ? recurrence_backward_stream_kernel<T, W, true, BACKWARD_STEPS, BACKWARD_INPUT_DEPTH>
+		: recurrence_backward_stream_kernel<T, W, false, BACKWARD_STEPS, BACKWARD_DEPTH>;
+	return input ? recurrence_forward_stream_kernel<T, W, true, FORWARD_STEPS, FORWARD_INPUT_DEPTH>
+		: recurrence_forward_stream_kernel<T, W, false, FORWARD_STEPS, FORWARD_DEPTH>;
+}
+template<bool BACKWARD>
+StreamKernel stream_for(int type, bool input)
+{
+	return type == NB200_TYPE_FP32 ? stream_of<BACKWARD, float, 1>(input)
+		: type == NB200_TYPE_FP16 ? stream_of<BACKWARD, __half, 2>(input) : stream_of<BACKWARD, __nv_bfloat16, 2>(input);
+}
+
+// Maps of the operands; false where one of them does not lie as TMA takes it (or a step's distance does not fit 32 bits of a round's offsets).
+bool make_maps(Maps& maps, int type, bool backward, const RecurrenceParams& p, int batch)
+{
+	const int size = type_size(type);
+	const long long dense = p.channels;
+	if(dense * size % 16 != 0 || dense * size * (MAX_CLUSTER + 1) * MAX_WARPS * FORWARD_STEPS >= (1ll << 32)) return false;
+	const int steps = backward ? BACKWARD_STEPS : FORWARD_STEPS;
+	auto one = [&](CUtensorMap& map, const void* base, long long batchStride, long long row) {
+		return sequence_map(&map, base, type, p.channels, p.length, batch, row, batch > 1 ? batchStride : row * p.length, steps);
+	};
+	return one(maps.z, p.z, p.zBatch, p.zRow) && one(maps.f, p.f, p.fBatch, p.fRow) && (p.i == nullptr || one(maps.i, p.i, p.iBatch, p.iRow))
+		&& (!backward || (one(maps.dh, p.dh, p.dhBatch, p.dhRow) && one(maps.h, p.h, dense * p.length, dense)));
+}
+
 // How many warps and blocks share a sequence's time axis: the fewest that fill three quarters of the warps that the SMs hold
 // (16, or 24 in the kernels of fewer registers).  Blocks of four warps: 16 x 2048 x 2048 bf16 took 98 us in blocks of four, 102
 // in blocks of eight and 146 of two, in clusters of two (of four, eight) of the first 102 (109, 125); 64 x 100 x 4096 fp16, where a
@@ -531,8 +814,8 @@ int launch(int type, bool pair, bool backward, RecurrenceParams p, int batch, cu
 		&& (p.length <= 1 || (p.zRow == row && p.fRow == row && (!input || p.iRow == row) && (!backward || p.dhRow == row)));
 	const Kernel kernel = backward ? kernel_for<true>(type, pair, input, dense) : kernel_for<false>(type, pair, input, dense);
 	p.status = device_status_word();
-	const int perWarp = pair ? 64 : 32;
-	const int tiles = (p.channels + perWarp - 1) / perWarp;
+	const int perTile = pair ? 64 : 32;
+	const int tiles = (p.channels + perTile - 1) / perTile;
 	const int stretches = (p.length + STEPS - 1) / STEPS;
 	const long long groups = static_cast<long long>(tiles) * batch;
 	const long long wanted = static_cast<long long>(sm_count()) * (backward || pair ? 12 : 18);
@@ -541,6 +824,13 @@ int launch(int type, bool pair, bool backward, RecurrenceParams p, int batch, cu
 	while(warps < 4 && more(warps, blocks)) warps *= 2;
 	while(blocks < MAX_CLUSTER && more(warps, blocks)) blocks *= 2;
 	while(warps < MAX_WARPS && more(warps, blocks)) warps *= 2;
+	Maps maps = {};
+	StreamKernel stream_kernel = nullptr;
+	int depth = 0;
+	if(p.length >= 2 * warps * blocks * (backward ? BACKWARD_STEPS : FORWARD_STEPS) && make_maps(maps, type, backward, p, batch)) {
+		stream_kernel = backward ? stream_for<true>(type, input) : stream_for<false>(type, input);
+		depth = backward ? (input ? BACKWARD_INPUT_DEPTH : BACKWARD_DEPTH) : (input ? FORWARD_INPUT_DEPTH : FORWARD_DEPTH);
+	}
 	cudaLaunchConfig_t config = {};
 	config.blockDim = dim3(warps * 32);
 	config.gridDim = dim3(tiles, blocks, batch);
@@ -552,7 +842,15 @@ int launch(int type, bool pair, bool backward, RecurrenceParams p, int batch, cu
 	attribute[0].val.clusterDim.z = 1;
 	config.attrs = attribute;
 	config.numAttrs = blocks > 1 ? 1 : 0;
-	cudaLaunchKernelEx(&config, kernel, p);
+	if(stream_kernel != nullptr) {
+		const int arrays = (backward ? 4 : 2) + (input ? 1 : 0);
+		const int perWarp = depth * arrays * (backward ? BACKWARD_STEPS : FORWARD_STEPS) * 128;
+		config.dynamicSmemBytes = static_cast<size_t>(warps) * perWarp;
+		cudaFuncSetAttribute(stream_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_WARPS * perWarp);
+		cudaLaunchKernelEx(&config, stream_kernel, static_cast<const RecurrenceParams&>(p), static_cast<const Maps&>(maps));
+	} else {
+		cudaLaunchKernelEx(&config, kernel, static_cast<const RecurrenceParams&>(p));
+	}
 	count_launch();
 	return check_launch();
 }
