@@ -657,9 +657,10 @@ Shape shape_of(int type, int height, int width, bool alike, bool aligned, bool f
 		int hold = units > MAX_ROW_WARPS * 32 * most && forward && alike ? 2 * most : most;
 		auto warps_for = [&](int h) { return (units + 32 * h - 1) / (32 * h); };
 		s.wide = warps_for(hold) > MAX_ROW_WARPS;
-		if(alike && !s.wide) {
+		if(alike && !s.wide) { // a thread's share of a row's sums costs about as much as 1.7 units; more than 24 elements do not stay in registers
+			auto cost = [&](int h) { return warps_for(h) * (17 + 10 * h) * (h * s.unit > 24 ? 3 : 2); };
 			for(int h = hold - 1; h >= 1 && warps_for(h) <= MAX_ROW_WARPS; --h) {
-				if(warps_for(h) * h < warps_for(hold) * hold) hold = h;
+				if(cost(h) < cost(hold)) hold = h;
 			}
 		}
 		s.threads = s.lanes = (s.wide ? MAX_ROW_WARPS : warps_for(hold)) * 32;

@@ -8,7 +8,7 @@
 // The work is bound by memory as long as every element is read once and both gates are formed once, so a chunk of the time
 // axis is read into registers, folded there, joined with the chunks around it, and its states are written out of the
 // same registers:
-//   thread   one channel (two 16-bit channels where rows are aligned for it) times STEPS steps: loads them all at once,
+//   thread   one channel (two 16-bit channels) times STEPS steps: loads them all at once,
 //            folds them to one (A, H)
 //   block    its warps hold consecutive stretches of time for the same 32 or 64 channels; the folds meet in shared memory
 //   cluster  up to 8 blocks hold consecutive stretches again; a cluster walks its channels' whole time axis, carrying the state
@@ -82,26 +82,31 @@ __device__ __forceinline__ Num<2> exp2_of(Num<2> x) { return { make_float2(exp2_
 __device__ __forceinline__ Num<1> inverse_of(Num<1> x) { return { inverse_fast(x.v) }; }
 __device__ __forceinline__ Num<2> inverse_of(Num<2> x) { return { make_float2(inverse_fast(x.v.x), inverse_fast(x.v.y)) }; }
 
-// W channels of one step as they lie in memory: one register
-template<typename T, int W>
-__device__ __forceinline__ uint32_t load_raw(const T* p)
+// The channels of one step as they lie in memory: one register.  SPLIT: two 16-bit channels that are not one aligned word; `second`
+// is 1, or 0 where the thread has the last channel alone.
+template<typename T, bool SPLIT>
+__device__ __forceinline__ uint32_t load_raw(const T* p, int second)
 {
-	if constexpr(sizeof(T) * W == 4) return *reinterpret_cast<const uint32_t*>(p);
-	else return *reinterpret_cast<const unsigned short*>(p);
+	if constexpr(!SPLIT) return *reinterpret_cast<const uint32_t*>(p);
+	else return reinterpret_cast<const unsigned short*>(p)[0] | static_cast<uint32_t>(reinterpret_cast<const unsigned short*>(p)[second]) << 16;
 }
 template<typename T, int W>
 __device__ __forceinline__ Num<W> number(uint32_t raw)
 {
 	if constexpr(sizeof(T) == 4) return { __uint_as_float(raw) };
-	else if constexpr(W == 1) return { unpack2<T>(raw).x };
 	else return { unpack2<T>(raw) };
 }
-template<typename T, int W>
-__device__ __forceinline__ void store_raw(T* p, Num<W> v)
+template<typename T, int W, bool SPLIT>
+__device__ __forceinline__ void store_raw(T* p, Num<W> v, int second)
 {
-	if constexpr(sizeof(T) == 4) *p = v.v;
-	else if constexpr(W == 2) *reinterpret_cast<uint32_t*>(p) = pack2<T>(v.v.x, v.v.y);
-	else *p = from_float<T>(v.v);
+	if constexpr(sizeof(T) == 4) {
+		*p = v.v;
+	} else if constexpr(!SPLIT) {
+		*reinterpret_cast<uint32_t*>(p) = pack2<T>(v.v.x, v.v.y);
+	} else {
+		p[0] = from_float<T>(v.v.x);
+		if(second != 0) p[1] = from_float<T>(v.v.y);
+	}
 }
 
 template<int W>
@@ -141,14 +146,21 @@ struct Fold {
 	Num<W> a, h;
 };
 
-// What a block's threads share: their folds, and those of the cluster's blocks (two sets, for alternating rounds).
+// What a block's threads share: their folds, and those of the cluster's blocks, each in two sets for alternating rounds; laid out at the
+// head of the dynamic shared memory, alike in all blocks of the cluster.
 template<int W>
 struct Shared {
-	Fold<W> warps[2][MAX_WARPS][32];
-	Fold<W> blocks[2][MAX_CLUSTER][32];
-	uint64_t arrived[2];
-	int abortFlag;
+	Fold<W>* folds; // [2][warps][32], then [2][blocks][32]
+	int warpCount, blockCount;
+	uint64_t* arrived;  // [2]
+	int* abortFlag;
+	__device__ __forceinline__ Fold<W>& warp(int set, int k, int lane) const { return folds[(set * warpCount + k) * 32 + lane]; }
+	__device__ __forceinline__ Fold<W>& block(int set, int k, int lane) const { return folds[(2 * warpCount + set * blockCount + k) * 32 + lane]; }
 };
+__host__ __device__ __forceinline__ constexpr int shared_bytes(int warps, int blocks, int w) // a multiple of 128
+{
+	return 2 * (warps + blocks) * 32 * 8 * w;
+}
 
 // Stores a fold in the shared memory of block `rank` of the cluster and counts its bytes on that block's barrier.
 __device__ __forceinline__ void send(const Fold<1>& f, Fold<1>* at, uint64_t* bar, int rank)
@@ -170,16 +182,17 @@ __device__ __forceinline__ void send(const Fold<2>& f, Fold<2>* at, uint64_t* ba
 }
 
 template<int W>
-__device__ __forceinline__ void begin_sharing(Shared<W>& s, int blocks)
+__device__ __forceinline__ Shared<W> begin_sharing(uint8_t* room, uint64_t* arrived, int* abortFlag, int warps, int blocks)
 {
 	if(threadIdx.x == 0) {
-		mbar_init(s.arrived, 1);
-		mbar_init(s.arrived + 1, 1);
+		mbar_init(arrived, 1);
+		mbar_init(arrived + 1, 1);
 		mbar_init_fence();
-		s.abortFlag = 0;
+		*abortFlag = 0;
 	}
 	if(blocks > 1) cg::this_cluster().sync(); // the others' shared memory and barriers exist from here on
 	else __syncthreads();
+	return { reinterpret_cast<Fold<W>*>(room), warps, blocks, arrived, abortFlag };
 }
 
 // Joins the folds of a round: `mine` is this thread's stretch; the state before it is returned in `state`, and `carry` moves on by
@@ -188,7 +201,7 @@ __device__ __forceinline__ void begin_sharing(Shared<W>& s, int blocks)
 // behind the readers.  Between blocks: a block sends its fold of a round after its own barrier, when all its warps have read
 // the set of the round before, and nobody sends the round after next without having received that fold.
 template<int W>
-__device__ __forceinline__ void join(Shared<W>& s, const Fold<W>& mine, int round, int rank, int blocks, int warps, int* status,
+__device__ __forceinline__ void join(const Shared<W>& s, const Fold<W>& mine, int round, int rank, int blocks, int warps, int* status,
 	Num<W>& carry, Num<W>& state)
 {
 	const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, set = round & 1;
@@ -198,28 +211,28 @@ __device__ __forceinline__ void join(Shared<W>& s, const Fold<W>& mine, int roun
 		f.a = mul(f.a, next.a);
 	};
 	if(warps > 1) {
-		if(warp < warps - 1) s.warps[set][warp][lane] = mine;
+		if(warp < warps - 1) s.warp(set, warp, lane) = mine;
 		__syncthreads();
-		for(int k = 0; k < warp; ++k) after(before, s.warps[set][k][lane]);
+		for(int k = 0; k < warp; ++k) after(before, s.warp(set, k, lane));
 	}
 	if(warp == warps - 1) { // the block's fold, to every block of the cluster, this one too
 		Fold<W> whole = before;
 		after(whole, mine);
 		if(blocks == 1) { // launched without a cluster: st.async is not an instruction of such a kernel
-			s.blocks[set][0][lane] = whole;
+			s.block(set, 0, lane) = whole;
 			__syncwarp();
 			if(lane == 0) mbar_arrive(s.arrived + set);
 		} else {
 			if(lane == 0) mbar_arrive_expect_tx(s.arrived + set, static_cast<uint32_t>(blocks * 32 * sizeof(Fold<W>)));
-			for(int k = 0; k < blocks; ++k) send(whole, &s.blocks[set][rank][lane], s.arrived + set, k);
+			for(int k = 0; k < blocks; ++k) send(whole, &s.block(set, rank, lane), s.arrived + set, k);
 		}
 	}
 	// should the wait give up, the rounds go on with what is there: every block has to reach the end
-	mbar_wait_bounded_warp(s.arrived + set, (round >> 1) & 1, &s.abortFlag, status, (KERNEL_ID << 8) | 1);
+	mbar_wait_bounded_warp(s.arrived + set, (round >> 1) & 1, s.abortFlag, status, (KERNEL_ID << 8) | 1);
 	Num<W> start = carry;
 	for(int k = 0; k < blocks; ++k) {
 		if(k == rank) start = carry;
-		const Fold<W> next = s.blocks[set][k][lane];
+		const Fold<W> next = s.block(set, k, lane);
 		carry = fma(next.a, carry, next.h);
 	}
 	state = fma(before.a, start, before.h);
@@ -227,20 +240,20 @@ __device__ __forceinline__ void join(Shared<W>& s, const Fold<W>& mine, int roun
 
 // A state or its gradient, fp32; null: zeros.
 template<int W>
-__device__ __forceinline__ Num<W> load_state(const float* from, long long at)
+__device__ __forceinline__ Num<W> load_state(const float* from, long long at, int second)
 {
 	if(from == nullptr) return all<W>(0.f);
 	if constexpr(W == 1) return { from[at] };
-	else return { make_float2(from[at], from[at + 1]) };
+	else return { make_float2(from[at], from[at + second]) };
 }
 template<int W>
-__device__ __forceinline__ void store_state(float* to, long long at, Num<W> v)
+__device__ __forceinline__ void store_state(float* to, long long at, Num<W> v, int second)
 {
 	if constexpr(W == 1) {
 		to[at] = v.v;
 	} else {
 		to[at] = v.v.x;
-		to[at + 1] = v.v.y;
+		if(second != 0) to[at + 1] = v.v.y;
 	}
 }
 
@@ -267,17 +280,20 @@ struct Operand {
 struct Yes { static constexpr bool value = true; };
 struct No { static constexpr bool value = false; };
 
-template<typename T, int W, bool INPUT, bool DENSE>
+template<typename T, int W, bool INPUT, bool DENSE, bool SPLIT>
 __global__ void __launch_bounds__(MAX_WARPS * 32, W == 1 ? 3 : 2) recurrence_forward_kernel(const RecurrenceParams p)
 {
-	__shared__ Shared<W> s;
+	extern __shared__ __align__(128) uint8_t sharedRoom[];
+	__shared__ uint64_t arrived[2];
+	__shared__ int abortFlag;
 	const int blocks = gridDim.y, rank = blockIdx.y; // the blocks of a cluster
 	const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5;
-	begin_sharing<W>(s, blocks);
+	const Shared<W> s = begin_sharing<W>(sharedRoom, arrived, &abortFlag, warps, blocks);
 	const int b = blockIdx.z;
 	const int own = (blockIdx.x * 32 + (threadIdx.x & 31)) * W;
 	const bool on = own < p.channels;
-	const int c = on ? own : p.channels - W; // lanes behind the last channel read what others read, and write nothing
+	const int c = on ? own : 0; // lanes behind the last channel read what others read, and write nothing
+	const int second = c + 1 < p.channels ? 1 : 0;
 	const int n = sequence_length(p, b);
 	const int span = warps * STEPS, stride = span * blocks;
 	const int first = rank * span + warp * STEPS;
@@ -291,16 +307,16 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, W == 1 ? 3 : 2) recurrence_for
 #pragma unroll
 	for(int k = 0; k < STEPS; ++k) offset[k] = (static_cast<uint32_t>(first + k) * p.channels + c) * static_cast<uint32_t>(sizeof(T));
 	const long long state0 = static_cast<long long>(b) * p.channels + c;
-	Num<W> carry = load_state<W>(p.first, state0);
+	Num<W> carry = load_state<W>(p.first, state0, second);
 
 	uint32_t rz[STEPS], rf[STEPS], ri[STEPS];
 	auto load = [&](int t, auto full) {
 #pragma unroll
 		for(int k = 0; k < STEPS; ++k) {
 			const bool in = decltype(full)::value || t + k < n;
-			rz[k] = in ? load_raw<T, W>(z.at(offset[k], t + k, c)) : 0u;
-			rf[k] = in ? load_raw<T, W>(f.at(offset[k], t + k, c)) : 0u;
-			if constexpr(INPUT) ri[k] = in ? load_raw<T, W>(i.at(offset[k], t + k, c)) : 0u;
+			rz[k] = in ? load_raw<T, SPLIT>(z.at(offset[k], t + k, c), second) : 0u;
+			rf[k] = in ? load_raw<T, SPLIT>(f.at(offset[k], t + k, c), second) : 0u;
+			if constexpr(INPUT) ri[k] = in ? load_raw<T, SPLIT>(i.at(offset[k], t + k, c), second) : 0u;
 		}
 	};
 	int round = 0, t = first;
@@ -340,7 +356,7 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, W == 1 ? 3 : 2) recurrence_for
 			for(int k = 0; k < STEPS; ++k) {
 				state = fma(a[k], state, h[k]);
 				T* const to = DENSE ? reinterpret_cast<T*>(outRound + offset[k]) : out + static_cast<long long>(t + k) * p.channels + c;
-				if(on && (decltype(full)::value || t + k < n)) store_raw<T, W>(to, state);
+				if(on && (decltype(full)::value || t + k < n)) store_raw<T, W, SPLIT>(to, state, second);
 			}
 		};
 		if(whole) apply(Yes());
@@ -350,24 +366,27 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, W == 1 ? 3 : 2) recurrence_for
 	}
 	// behind the sequence the results are zeros
 	for(int k = n + rank * warps + warp; k < p.length; k += blocks * warps) {
-		if(on) store_raw<T, W>(out + static_cast<long long>(k) * p.channels + c, all<W>(0.f));
+		if(on) store_raw<T, W, SPLIT>(out + static_cast<long long>(k) * p.channels + c, all<W>(0.f), second);
 	}
-	if(on && p.last != nullptr && rank == 0 && warp == 0) store_state<W>(p.last, state0, carry);
+	if(on && p.last != nullptr && rank == 0 && warp == 0) store_state<W>(p.last, state0, carry, second);
 	if(blocks > 1) cg::this_cluster().sync(); // nobody leaves while its shared memory may be written
 }
 
 // Time runs backwards: step k of a stretch is t - k.
-template<typename T, int W, bool INPUT, bool DENSE>
+template<typename T, int W, bool INPUT, bool DENSE, bool SPLIT>
 __global__ void __launch_bounds__(MAX_WARPS * 32, 2) recurrence_backward_kernel(const RecurrenceParams p)
 {
-	__shared__ Shared<W> s;
+	extern __shared__ __align__(128) uint8_t sharedRoom[];
+	__shared__ uint64_t arrived[2];
+	__shared__ int abortFlag;
 	const int blocks = gridDim.y, rank = blockIdx.y;
 	const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5;
-	begin_sharing<W>(s, blocks);
+	const Shared<W> s = begin_sharing<W>(sharedRoom, arrived, &abortFlag, warps, blocks);
 	const int b = blockIdx.z;
 	const int own = (blockIdx.x * 32 + (threadIdx.x & 31)) * W;
 	const bool on = own < p.channels;
-	const int c = on ? own : p.channels - W;
+	const int c = on ? own : 0;
+	const int second = c + 1 < p.channels ? 1 : 0;
 	const int n = sequence_length(p, b);
 	const int span = warps * STEPS, stride = span * blocks;
 	const int back = rank * span + warp * STEPS; // steps between the round's last one and this thread's first
@@ -389,15 +408,15 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 2) recurrence_backward_kernel(
 #pragma unroll
 	for(int k = 0; k < STEPS; ++k) offset[k] = (static_cast<uint32_t>(stride - 1 - back - k) * p.channels + c) * static_cast<uint32_t>(sizeof(T));
 	const long long state0 = static_cast<long long>(b) * p.channels + c;
-	Num<W> carry = load_state<W>(p.lastDiff, state0); // what step t + 1 hands back, a_{t+1} S_{t+1}
-	const Num<W> first = load_state<W>(p.first, state0);
+	Num<W> carry = load_state<W>(p.lastDiff, state0, second); // what step t + 1 hands back, a_{t+1} S_{t+1}
+	const Num<W> first = load_state<W>(p.first, state0, second);
 	// behind the sequence the gradients are zeros
 	for(int k = n + rank * warps + warp; k < p.length; k += blocks * warps) {
 		const long long at = static_cast<long long>(k) * p.channels + c;
 		if(!on) break;
-		store_raw<T, W>(dz + at, all<W>(0.f));
-		store_raw<T, W>(df + at, all<W>(0.f));
-		if constexpr(INPUT) store_raw<T, W>(di + at, all<W>(0.f));
+		store_raw<T, W, SPLIT>(dz + at, all<W>(0.f), second);
+		store_raw<T, W, SPLIT>(df + at, all<W>(0.f), second);
+		if constexpr(INPUT) store_raw<T, W, SPLIT>(di + at, all<W>(0.f), second);
 	}
 	// The gates and the gradients are wanted when a round begins, the rest only when its state has arrived: the former are
 	// loaded a whole round ahead, the latter while the round before them ends.
@@ -406,17 +425,17 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 2) recurrence_backward_kernel(
 #pragma unroll
 		for(int k = 0; k < STEPS; ++k) {
 			const bool in = decltype(full)::value || t - k >= 0;
-			rf[k] = in ? load_raw<T, W>(f.at(offset[k], t - k, c)) : 0u;
-			nd[k] = in ? load_raw<T, W>(dh.at(offset[k], t - k, c)) : 0u;
+			rf[k] = in ? load_raw<T, SPLIT>(f.at(offset[k], t - k, c), second) : 0u;
+			nd[k] = in ? load_raw<T, SPLIT>(dh.at(offset[k], t - k, c), second) : 0u;
 		}
 	};
 	auto load_rest = [&](int t, auto full) {
 #pragma unroll
 		for(int k = 0; k < STEPS; ++k) {
 			const bool in = decltype(full)::value || t - k >= 0;
-			rz[k] = in ? load_raw<T, W>(z.at(offset[k], t - k, c)) : 0u;
-			rh[k] = decltype(full)::value || t - k > 0 ? load_raw<T, W>(h.at(offset[k], t - k, c)) : 0u;
-			if constexpr(INPUT) ri[k] = in ? load_raw<T, W>(i.at(offset[k], t - k, c)) : 0u;
+			rz[k] = in ? load_raw<T, SPLIT>(z.at(offset[k], t - k, c), second) : 0u;
+			rh[k] = decltype(full)::value || t - k > 0 ? load_raw<T, SPLIT>(h.at(offset[k], t - k, c), second) : 0u;
+			if constexpr(INPUT) ri[k] = in ? load_raw<T, SPLIT>(i.at(offset[k], t - k, c), second) : 0u;
 		}
 	};
 	int round = 0, t = n - 1 - back;
@@ -474,10 +493,10 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 2) recurrence_backward_kernel(
 				state = mul(a[k], S);
 				if(on && (decltype(full)::value || t - k >= 0)) {
 					const long long step = DENSE ? 0 : static_cast<long long>(t - k) * p.channels + c;
-					store_raw<T, W>(DENSE ? reinterpret_cast<T*>(reinterpret_cast<uint8_t*>(dz) + outRound + offset[k]) : dz + step, oz);
-					store_raw<T, W>(DENSE ? reinterpret_cast<T*>(reinterpret_cast<uint8_t*>(df) + outRound + offset[k]) : df + step, of);
+					store_raw<T, W, SPLIT>(DENSE ? reinterpret_cast<T*>(reinterpret_cast<uint8_t*>(dz) + outRound + offset[k]) : dz + step, oz, second);
+					store_raw<T, W, SPLIT>(DENSE ? reinterpret_cast<T*>(reinterpret_cast<uint8_t*>(df) + outRound + offset[k]) : df + step, of, second);
 					if constexpr(INPUT) {
-						store_raw<T, W>(DENSE ? reinterpret_cast<T*>(reinterpret_cast<uint8_t*>(di) + outRound + offset[k]) : di + step, oi);
+						store_raw<T, W, SPLIT>(DENSE ? reinterpret_cast<T*>(reinterpret_cast<uint8_t*>(di) + outRound + offset[k]) : di + step, oi, second);
 					}
 				}
 			}
@@ -494,7 +513,7 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 2) recurrence_backward_kernel(
 		outRound -= roundBytes;
 		t -= stride;
 	}
-	if(on && p.last != nullptr && rank == 0 && warp == 0) store_state<W>(p.last, state0, carry);
+	if(on && p.last != nullptr && rank == 0 && warp == 0) store_state<W>(p.last, state0, carry, second);
 	if(blocks > 1) cg::this_cluster().sync();
 }
 
@@ -552,15 +571,16 @@ __device__ __forceinline__ void stage_read()
 template<typename T, int W, bool INPUT, int S, int DEPTH>
 __global__ void __launch_bounds__(MAX_WARPS * 32, S == 8 ? 3 : 2) recurrence_forward_stream_kernel(const RecurrenceParams p, const __grid_constant__ Maps maps)
 {
-	extern __shared__ __align__(128) uint8_t streamRoom[];
-	__shared__ Shared<W> s;
+	extern __shared__ __align__(128) uint8_t sharedRoom[];
+	__shared__ uint64_t arrived[2];
+	__shared__ int abortFlag;
 	__shared__ uint64_t bars[MAX_WARPS][DEPTH];
 	constexpr int ARRAYS = INPUT ? 3 : 2;
 	const int blocks = gridDim.y, rank = blockIdx.y;
 	const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 	constexpr int BOX_BYTES = Ring<S>::BOX_BYTES;
-	const Ring<S> ring = make_ring<S, DEPTH>(streamRoom, bars, ARRAYS);
-	begin_sharing<W>(s, blocks);
+	const Ring<S> ring = make_ring<S, DEPTH>(sharedRoom + shared_bytes(warps, blocks, W), bars, ARRAYS);
+	const Shared<W> s = begin_sharing<W>(sharedRoom, arrived, &abortFlag, warps, blocks);
 	const int b = blockIdx.z;
 	const int tile = blockIdx.x * 32 * W;
 	const int c = tile + lane * W;
@@ -576,7 +596,7 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, S == 8 ? 3 : 2) recurrence_for
 	for(int k = 0; k < S; ++k) offset[k] = (static_cast<uint32_t>(first + k) * p.channels + c) * static_cast<uint32_t>(sizeof(T));
 	const long long state0 = static_cast<long long>(b) * p.channels + c;
 	Num<W> carry = all<W>(0.f);
-	if(on) carry = load_state<W>(p.first, state0);
+	if(on) carry = load_state<W>(p.first, state0, 1);
 	auto ask = [&](int round) {
 		const int t = first + round * stride;
 		if(t >= n || lane != 0) return;
@@ -606,7 +626,7 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, S == 8 ? 3 : 2) recurrence_for
 			}
 		};
 		const bool whole = t + S <= n;
-		if(t < n) ring.wait(round, &s.abortFlag, p.status);
+		if(t < n) ring.wait(round, s.abortFlag, p.status);
 		if(whole) fold(Yes());
 		else if(t < n) fold(No());
 		stage_read();
@@ -617,7 +637,7 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, S == 8 ? 3 : 2) recurrence_for
 #pragma unroll
 			for(int k = 0; k < S; ++k) {
 				state = fma(a[k], state, h[k]);
-				if(on && (decltype(full)::value || t + k < n)) store_raw<T, W>(reinterpret_cast<T*>(outRound + offset[k]), state);
+				if(on && (decltype(full)::value || t + k < n)) store_raw<T, W, false>(reinterpret_cast<T*>(outRound + offset[k]), state, 1);
 			}
 		};
 		if(whole) apply(Yes());
@@ -626,24 +646,25 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, S == 8 ? 3 : 2) recurrence_for
 	}
 	// behind the sequence the results are zeros
 	for(int k = n + rank * warps + warp; k < p.length; k += blocks * warps) {
-		if(on) store_raw<T, W>(out + static_cast<long long>(k) * p.channels + c, all<W>(0.f));
+		if(on) store_raw<T, W, false>(out + static_cast<long long>(k) * p.channels + c, all<W>(0.f), 1);
 	}
-	if(on && p.last != nullptr && rank == 0 && warp == 0) store_state<W>(p.last, state0, carry);
+	if(on && p.last != nullptr && rank == 0 && warp == 0) store_state<W>(p.last, state0, carry, 1);
 	if(blocks > 1) cg::this_cluster().sync(); // nobody leaves while its shared memory may be written
 }
 
 template<typename T, int W, bool INPUT, int S, int DEPTH>
 __global__ void __launch_bounds__(MAX_WARPS * 32, 2) recurrence_backward_stream_kernel(const RecurrenceParams p, const __grid_constant__ Maps maps)
 {
-	extern __shared__ __align__(128) uint8_t streamRoom[];
-	__shared__ Shared<W> s;
+	extern __shared__ __align__(128) uint8_t sharedRoom[];
+	__shared__ uint64_t arrived[2];
+	__shared__ int abortFlag;
 	__shared__ uint64_t bars[MAX_WARPS][DEPTH];
 	constexpr int ARRAYS = INPUT ? 5 : 4;
 	const int blocks = gridDim.y, rank = blockIdx.y;
 	const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 	constexpr int BOX_BYTES = Ring<S>::BOX_BYTES;
-	const Ring<S> ring = make_ring<S, DEPTH>(streamRoom, bars, ARRAYS);
-	begin_sharing<W>(s, blocks);
+	const Ring<S> ring = make_ring<S, DEPTH>(sharedRoom + shared_bytes(warps, blocks, W), bars, ARRAYS);
+	const Shared<W> s = begin_sharing<W>(sharedRoom, arrived, &abortFlag, warps, blocks);
 	const int b = blockIdx.z;
 	const int tile = blockIdx.x * 32 * W;
 	const int c = tile + lane * W;
@@ -663,8 +684,8 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 2) recurrence_backward_stream_
 	const long long state0 = static_cast<long long>(b) * p.channels + c;
 	Num<W> carry = all<W>(0.f), first = all<W>(0.f);
 	if(on) {
-		carry = load_state<W>(p.lastDiff, state0);
-		first = load_state<W>(p.first, state0);
+		carry = load_state<W>(p.lastDiff, state0, 1);
+		first = load_state<W>(p.first, state0, 1);
 	}
 	auto ask = [&](int round) {
 		const int t = n - 1 - back - round * stride, from = t - S + 1; // a box may begin in front of step 0
@@ -682,9 +703,9 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 2) recurrence_backward_stream_
 	for(int k = n + rank * warps + warp; k < p.length; k += blocks * warps) {
 		const long long at = (static_cast<long long>(k) * p.channels + c) * static_cast<long long>(sizeof(T));
 		if(!on) break;
-		store_raw<T, W>(reinterpret_cast<T*>(dz + at), all<W>(0.f));
-		store_raw<T, W>(reinterpret_cast<T*>(df + at), all<W>(0.f));
-		if constexpr(INPUT) store_raw<T, W>(reinterpret_cast<T*>(di + at), all<W>(0.f));
+		store_raw<T, W, false>(reinterpret_cast<T*>(dz + at), all<W>(0.f), 1);
+		store_raw<T, W, false>(reinterpret_cast<T*>(df + at), all<W>(0.f), 1);
+		if constexpr(INPUT) store_raw<T, W, false>(reinterpret_cast<T*>(di + at), all<W>(0.f), 1);
 	}
 	int t = n - 1 - back;
 	for(int round = 0; round * stride < n; ++round, t -= stride) {
@@ -705,7 +726,7 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 2) recurrence_backward_stream_
 			}
 		};
 		const bool whole = t - S >= 0;
-		if(t >= 0) ring.wait(round, &s.abortFlag, p.status);
+		if(t >= 0) ring.wait(round, s.abortFlag, p.status);
 		if(whole) fold(Yes());
 		else if(t >= 0) fold(No());
 		Num<W> state;
@@ -730,9 +751,9 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 2) recurrence_backward_stream_
 				}
 				state = mul(a[k], S);
 				if(on && (decltype(full)::value || t - k >= 0)) {
-					store_raw<T, W>(reinterpret_cast<T*>(dz + outRound + offset[k]), oz);
-					store_raw<T, W>(reinterpret_cast<T*>(df + outRound + offset[k]), of);
-					if constexpr(INPUT) store_raw<T, W>(reinterpret_cast<T*>(di + outRound + offset[k]), oi);
+					store_raw<T, W, false>(reinterpret_cast<T*>(dz + outRound + offset[k]), oz, 1);
+					store_raw<T, W, false>(reinterpret_cast<T*>(df + outRound + offset[k]), of, 1);
+					if constexpr(INPUT) store_raw<T, W, false>(reinterpret_cast<T*>(di + outRound + offset[k]), oi, 1);
 				}
 			}
 		};
@@ -742,40 +763,41 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 2) recurrence_backward_stream_
 		ask(round + DEPTH);
 		outRound -= roundBytes;
 	}
-	if(on && p.last != nullptr && rank == 0 && warp == 0) store_state<W>(p.last, state0, carry);
+	if(on && p.last != nullptr && rank == 0 && warp == 0) store_state<W>(p.last, state0, carry, 1);
 	if(blocks > 1) cg::this_cluster().sync();
 }
 
 using Kernel = void (*)(const RecurrenceParams);
 
-template<typename T, int W, bool BACKWARD>
+template<typename T, int W, bool SPLIT, bool BACKWARD>
 Kernel kernel_of(bool input, bool dense)
 {
 	if(BACKWARD) {
-		if(dense) return input ? recurrence_backward_kernel<T, W, true, true> : recurrence_backward_kernel<T, W, false, true>;
-		return input ? recurrence_backward_kernel<T, W, true, false> : recurrence_backward_kernel<T, W, false, false>;
+		if(dense) return input ? recurrence_backward_kernel<T, W, true, true, SPLIT> : recurrence_backward_kernel<T, W, false, true, SPLIT>;
+		return input ? recurrence_backward_kernel<T, W, true, false, SPLIT> : recurrence_backward_kernel<T, W, false, false, SPLIT>;
 	}
-	if(dense) return input ? recurrence_forward_kernel<T, W, true, true> : recurrence_forward_kernel<T, W, false, true>;
-	return input ? recurrence_forward_kernel<T, W, true, false> : recurrence_forward_kernel<T, W, false, false>;
+	if(dense) return input ? recurrence_forward_kernel<T, W, true, true, SPLIT> : recurrence_forward_kernel<T, W, false, true, SPLIT>;
+	return input ? recurrence_forward_kernel<T, W, true, false, SPLIT> : recurrence_forward_kernel<T, W, false, false, SPLIT>;
 }
 
 template<bool BACKWARD>
 Kernel kernel_for(int type, bool pair, bool input, bool dense)
 {
-	if(type == NB200_TYPE_FP32) return kernel_of<float, 1, BACKWARD>(input, dense);
-	if(type == NB200_TYPE_FP16) return pair ? kernel_of<__half, 2, BACKWARD>(input, dense) : kernel_of<__half, 1, BACKWARD>(input, dense);
-	return pair ? kernel_of<__nv_bfloat16, 2, BACKWARD>(input, dense) : kernel_of<__nv_bfloat16, 1, BACKWARD>(input, dense);
+	if(type == NB200_TYPE_FP32) return kernel_of<float, 1, false, BACKWARD>(input, dense);
+	if(type == NB200_TYPE_FP16) return pair ? kernel_of<__half, 2, false, BACKWARD>(input, dense) : kernel_of<__half, 2, true, BACKWARD>(input, dense);
+	return pair ? kernel_of<__nv_bfloat16, 2, false, BACKWARD>(input, dense) : kernel_of<__nv_bfloat16, 2, true, BACKWARD>(input, dense);
 }
 
 // Rounds that a warp's loads are ahead of its work, by what fits beside one another in 16 or more warps' shared memory.
-constexpr int FORWARD_STEPS = 16, FORWARD_DEPTH = 2, FORWARD_INPUT_DEPTH = 2, BACKWARD_STEPS = 8, BACKWARD_DEPTH = 3, BACKWARD_INPUT_DEPTH = 2;
+constexpr int FORWARD_STEPS = 16, FORWARD_DEPTH = 2, FORWARD_INPUT_DEPTH = 2, BACKWARD_STEPS = 8, BACKWARD_DEPTH = 2,
+	BACKWARD_INPUT_STEPS = 16, BACKWARD_INPUT_DEPTH = 2;
 
 using StreamKernel = void (*)(const RecurrenceParams, const Maps);
 
 template<bool BACKWARD, typename T, int W>
 StreamKernel stream_of(bool input)
 {
-	if(BACKWARD) return input ? recurrence_backward_stream_kernel<T, W, true, BACKWARD_STEPS, BACKWARD_INPUT_DEPTH>
+	if(BACKWARD) return input ? recurrence_backward_stream_kernel<T, W, true, BACKWARD_INPUT_STEPS, BACKWARD_INPUT_DEPTH>
 		: recurrence_backward_stream_kernel<T, W, false, BACKWARD_STEPS, BACKWARD_DEPTH>;
 	return input ? recurrence_forward_stream_kernel<T, W, true, FORWARD_STEPS, FORWARD_INPUT_DEPTH>
 		: recurrence_forward_stream_kernel<T, W, false, FORWARD_STEPS, FORWARD_DEPTH>;
@@ -788,12 +810,11 @@ StreamKernel stream_for(int type, bool input)
 }
 
 // Maps of the operands; false where one of them does not lie as TMA takes it (or a step's distance does not fit 32 bits of a round's offsets).
-bool make_maps(Maps& maps, int type, bool backward, const RecurrenceParams& p, int batch)
+bool make_maps(Maps& maps, int type, bool backward, const RecurrenceParams& p, int batch, int steps)
 {
 	const int size = type_size(type);
 	const long long dense = p.channels;
 	if(dense * size % 16 != 0 || dense * size * (MAX_CLUSTER + 1) * MAX_WARPS * FORWARD_STEPS >= (1ll << 32)) return false;
-	const int steps = backward ? BACKWARD_STEPS : FORWARD_STEPS;
 	auto one = [&](CUtensorMap& map, const void* base, long long batchStride, long long row) {
 		return sequence_map(&map, base, type, p.channels, p.length, batch, row, batch > 1 ? batchStride : row * p.length, steps);
 	};
@@ -814,11 +835,11 @@ int launch(int type, bool pair, bool backward, RecurrenceParams p, int batch, cu
 		&& (p.length <= 1 || (p.zRow == row && p.fRow == row && (!input || p.iRow == row) && (!backward || p.dhRow == row)));
 	const Kernel kernel = backward ? kernel_for<true>(type, pair, input, dense) : kernel_for<false>(type, pair, input, dense);
 	p.status = device_status_word();
-	const int perTile = pair ? 64 : 32;
-	const int tiles = (p.channels + perTile - 1) / perTile;
+	const int channelsPerLane = type == NB200_TYPE_FP32 ? 1 : 2;
+	const int tiles = (p.channels + 32 * channelsPerLane - 1) / (32 * channelsPerLane);
 	const int stretches = (p.length + STEPS - 1) / STEPS;
 	const long long groups = static_cast<long long>(tiles) * batch;
-	const long long wanted = static_cast<long long>(sm_count()) * (backward || pair ? 12 : 18);
+	const long long wanted = static_cast<long long>(sm_count()) * (backward || channelsPerLane == 2 ? 12 : 18);
 	int warps = stretches < 2 ? 1 : 2, blocks = 1;
 	auto more = [&](int w, int n) { return groups * w * n < wanted && w * n < stretches; };
 	while(warps < 4 && more(warps, blocks)) warps *= 2;
@@ -827,13 +848,15 @@ int launch(int type, bool pair, bool backward, RecurrenceParams p, int batch, cu
 	Maps maps = {};
 	StreamKernel stream_kernel = nullptr;
 	int depth = 0;
-	if(p.length >= 2 * warps * blocks * (backward ? BACKWARD_STEPS : FORWARD_STEPS) && make_maps(maps, type, backward, p, batch)) {
+	const int steps = !backward ? FORWARD_STEPS : input ? BACKWARD_INPUT_STEPS : BACKWARD_STEPS;
+	if(p.length >= 2 * warps * blocks * steps && make_maps(maps, type, backward, p, batch, steps)) {
 		stream_kernel = backward ? stream_for<true>(type, input) : stream_for<false>(type, input);
 		depth = backward ? (input ? BACKWARD_INPUT_DEPTH : BACKWARD_DEPTH) : (input ? FORWARD_INPUT_DEPTH : FORWARD_DEPTH);
 	}
 	cudaLaunchConfig_t config = {};
 	config.blockDim = dim3(warps * 32);
 	config.gridDim = dim3(tiles, blocks, batch);
+	config.dynamicSmemBytes = shared_bytes(warps, blocks, channelsPerLane);
 	config.stream = stream;
 	cudaLaunchAttribute attribute[1];
 	attribute[0].id = cudaLaunchAttributeClusterDimension;
@@ -844,9 +867,9 @@ int launch(int type, bool pair, bool backward, RecurrenceParams p, int batch, cu
 	config.numAttrs = blocks > 1 ? 1 : 0;
 	if(stream_kernel != nullptr) {
 		const int arrays = (backward ? 4 : 2) + (input ? 1 : 0);
-		const int perWarp = depth * arrays * (backward ? BACKWARD_STEPS : FORWARD_STEPS) * 128;
-		config.dynamicSmemBytes = static_cast<size_t>(warps) * perWarp;
-		cudaFuncSetAttribute(stream_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_WARPS * perWarp);
+		const int perWarp = depth * arrays * steps * 128;
+		config.dynamicSmemBytes += static_cast<size_t>(warps) * perWarp;
+		cudaFuncSetAttribute(stream_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(config.dynamicSmemBytes));
 		cudaLaunchKernelEx(&config, stream_kernel, static_cast<const RecurrenceParams&>(p), static_cast<const Maps&>(maps));
 	} else {
 		cudaLaunchKernelEx(&config, kernel, static_cast<const RecurrenceParams&>(p));
