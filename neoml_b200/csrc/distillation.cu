@@ -360,7 +360,7 @@ int nb200_distillation_loss(void* stream, int type, int teacher_type, const void
 	if(logits == nullptr || loss == nullptr || log_sum == nullptr || !type_aligned(logits, type)
 		|| !type_aligned(teacher_logits, teacher_type)) return NB200_EINVAL;
 	if(kept > 0 && (teacher_logits == nullptr || teacher_indices == nullptr)) return NB200_EINVAL;
-	if(kept > KEPT_MAX) return NB200_ETOOBIG;
+	if(kept > KEPT_MAX || vocabulary > (1 << 30)) return NB200_ETOOBIG;
 	if(device_status_word() == nullptr) return NB200_ENODEVICE;
 	DistillParams p = {};
 	p.logits = logits; p.teacher = teacher_logits; p.indices = teacher_indices; p.logSum = log_sum; p.loss = loss;
@@ -380,7 +380,7 @@ int nb200_distillation_loss_backward(void* stream, int type, int teacher_type, c
 	if(logits == nullptr || loss_diff == nullptr || log_sum == nullptr || logits_diff == nullptr || !type_aligned(logits, type)
 		|| !type_aligned(logits_diff, type) || !type_aligned(teacher_logits, teacher_type)) return NB200_EINVAL;
 	if(kept > 0 && (teacher_logits == nullptr || teacher_indices == nullptr)) return NB200_EINVAL;
-	if(kept > KEPT_MAX) return NB200_ETOOBIG;
+	if(kept > KEPT_MAX || vocabulary > (1 << 30)) return NB200_ETOOBIG;
 	if(device_status_word() == nullptr) return NB200_ENODEVICE;
 	DistillParams p = {};
 	p.logits = logits; p.teacher = teacher_logits; p.indices = teacher_indices; p.lossDiff = loss_diff;

@@ -862,7 +862,7 @@ int nb200_layer_normalization(void* stream, int type, int parameter_type, const 
 {
 	if(!sizes_valid(type, parameter_type, height, width) || x_row_size < width || y_row_size < width) return NB200_EINVAL;
 	if(height == 0) return NB200_OK;
-	if(height > (1 << 30)) return NB200_ETOOBIG;
+	if(height > (1 << 30) || width > (1 << 30)) return NB200_ETOOBIG;
 	if(x == nullptr || y == nullptr || !type_aligned(x, type) || !type_aligned(y, type)
 		|| !type_aligned(scale, parameter_type) || !type_aligned(free_term, parameter_type)) return NB200_EINVAL;
 	if(device_status_word() == nullptr) return NB200_ENODEVICE;
@@ -879,7 +879,7 @@ int nb200_layer_normalization(void* stream, int type, int parameter_type, const 
 
 size_t nb200_layer_normalization_backward_scratch_floats(int type, int height, int width)
 {
-	if(!type_valid(type) || height <= 0 || width <= 0) return 0;
+	if(!type_valid(type) || height <= 0 || width <= 0 || height > (1 << 30) || width > (1 << 30)) return 0;
 	// whichever form the operands' alignment selects
 	int blocks = 0;
 	for(int form = 0; form < 3; ++form) {
@@ -903,7 +903,7 @@ int nb200_layer_normalization_backward(void* stream, int type, int parameter_typ
 		|| !type_aligned(x, type) || !type_aligned(dy, type) || !type_aligned(dx, type)
 		|| (parameters && scratch == nullptr))) return NB200_EINVAL;
 	if(height == 0 && !parameters) return NB200_OK;
-	if(height > (1 << 30)) return NB200_ETOOBIG;
+	if(height > (1 << 30) || width > (1 << 30)) return NB200_ETOOBIG;
 	if(device_status_word() == nullptr) return NB200_ENODEVICE;
 	if(height == 0) { // sums over no rows
 		const int grid = grid_for(width, 256);

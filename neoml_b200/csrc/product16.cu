@@ -521,7 +521,7 @@ int product16(Product16Epilogue epilogue, bool aAcross, bool bAcross, const Prod
 	if(tiles == 0) return NB200_OK;
 	if(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES) != cudaSuccess) return check_launch();
 	const int grid = tiles < sm_count() ? static_cast<int>(tiles) : sm_count();
-	launch_dependent(false, kernel, dim3(grid), dim3(THREADS), SMEM_BYTES, stream, p, *static_cast<const CUtensorMap*>(mapA),
+	launch_dependent(true, kernel, dim3(grid), dim3(THREADS), SMEM_BYTES, stream, p, *static_cast<const CUtensorMap*>(mapA),
 		*static_cast<const CUtensorMap*>(mapB));
 	count_launch();
 	return check_launch();

@@ -869,7 +869,9 @@ int launch(int type, bool pair, bool backward, RecurrenceParams p, int batch, cu
 		const int arrays = (backward ? 4 : 2) + (input ? 1 : 0);
 		const int perWarp = depth * arrays * steps * 128;
 		config.dynamicSmemBytes += static_cast<size_t>(warps) * perWarp;
-		cudaFuncSetAttribute(stream_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(config.dynamicSmemBytes));
+		// the most that the kernel is ever launched with: another thread may be between this and its own launch
+		cudaFuncSetAttribute(stream_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+			MAX_WARPS * perWarp + shared_bytes(MAX_WARPS, MAX_CLUSTER, channelsPerLane));
 		cudaLaunchKernelEx(&config, stream_kernel, static_cast<const RecurrenceParams&>(p), static_cast<const Maps&>(maps));
 	} else {
 		cudaLaunchKernelEx(&config, kernel, static_cast<const RecurrenceParams&>(p));

@@ -32,53 +32,98 @@ __device__ __forceinline__ bool has_target(const int* labels, int row, int vocab
 
 // ---- 16-bit types ---------------------------------------------------------------------------------------------------
 
-// Rows of 16-bit elements copied to aligned rows.  With labels: a row without a target or with a loss_diff of zero becomes
-// zeros -- it has no gradient, whatever it holds -- and the first block finds the scale of dz.
-__global__ void __launch_bounds__(256) copy_rows16_kernel(const uint16_t* __restrict__ src, long long srcRow, int rows, int width,
-	uint16_t* __restrict__ dst, int dstRow, const int* __restrict__ labels, const float* __restrict__ lossDiff, int vocabulary,
-	float* scale, int fp16)
+// Eight 16-bit elements from any address: 32-bit words around them, shifted by half a word where they begin inside one.
+__device__ __forceinline__ uint4 gather8(const uint16_t* p)
 {
-	int block = blockIdx.x, blocks = gridDim.x;
-	if(scale != nullptr) {
-		if(block == 0) {
-			__shared__ float slots[8];
-			float most = 0.f;
-			for(int r = threadIdx.x; r < rows; r += blockDim.x) {
-				if(has_target(labels, r, vocabulary)) most = fmaxf(most, fabsf(lossDiff[r]));
-			}
-			most = warp_max_all(most);
-			if((threadIdx.x & 31) == 0) slots[threadIdx.x >> 5] = most;
-			__syncthreads();
-			if(threadIdx.x == 0) {
-				for(int i = 1; i < 8; ++i) most = fmaxf(most, slots[i]);
-				int e = 0;
-				if(fp16 && most > 0.f && most < INFINITY) {
-					e = 14 - ilogbf(most);
-					e = e > 100 ? 100 : e < -100 ? -100 : e;
-				}
-				scale[0] = ldexpf(1.f, e);
-				scale[1] = ldexpf(1.f, -e);
-			}
-			return;
+	const uintptr_t a = reinterpret_cast<uintptr_t>(p);
+	if((a & 15u) == 0) return *reinterpret_cast<const uint4*>(p);
+	const uint32_t* const w = reinterpret_cast<const uint32_t*>(a & ~static_cast<uintptr_t>(3));
+	if((a & 3u) == 0) return make_uint4(w[0], w[1], w[2], w[3]);
+	const uint32_t v[5] = { w[0], w[1], w[2], w[3], w[4] };
+	return make_uint4(__funnelshift_r(v[0], v[1], 16), __funnelshift_r(v[1], v[2], 16), __funnelshift_r(v[2], v[3], 16), __funnelshift_r(v[3], v[4], 16));
+}
+
+// Row and unit of a flat index.
+__device__ __forceinline__ void row_unit(long long i, int perRow, int* row, int* unit)
+{
+	const int r = i <= 0xffffffffll ? static_cast<int>(static_cast<uint32_t>(i) / static_cast<uint32_t>(perRow)) : static_cast<int>(i / perRow);
+	*row = r;
+	*unit = static_cast<int>(i - static_cast<long long>(r) * perRow);
+}
+
+// The scale of dz (the head of this file) and its inverse: one block.
+__global__ void __launch_bounds__(256) diff_scale_kernel(int rows, const int* __restrict__ labels, const float* __restrict__ lossDiff,
+	int vocabulary, float* scale, int fp16)
+{
+	__shared__ float slots[8];
+	dependent_wait();
+	float most = 0.f;
+	if(fp16) {
+		for(int r = threadIdx.x; r < rows; r += blockDim.x) {
+			if(has_target(labels, r, vocabulary)) most = fmaxf(most, fabsf(lossDiff[r]));
 		}
-		--block;
-		--blocks;
 	}
-	const bool vector = (srcRow & 7) == 0 && (reinterpret_cast<uintptr_t>(src) & 15u) == 0;
-	for(long long r = block; r < rows; r += blocks) {
-		const bool keep = labels == nullptr || (has_target(labels, static_cast<int>(r), vocabulary) && !(lossDiff[r] == 0.f));
-		const uint16_t* const from = src + r * srcRow;
-		uint16_t* const to = dst + r * dstRow;
-		if(vector) {
-			for(int i = threadIdx.x * 8; i < width; i += blockDim.x * 8) {
-				if(i + 8 <= width) {
-					*reinterpret_cast<uint4*>(to + i) = keep ? *reinterpret_cast<const uint4*>(from + i) : make_uint4(0u, 0u, 0u, 0u);
-				} else {
-					for(int j = i; j < dstRow; ++j) to[j] = keep && j < width ? from[j] : 0;
-				}
+	most = warp_max_all(most);
+	if((threadIdx.x & 31) == 0) slots[threadIdx.x >> 5] = most;
+	__syncthreads();
+	if(threadIdx.x == 0) {
+		for(int i = 1; i < 8; ++i) most = fmaxf(most, slots[i]);
+		int e = 0;
+		if(most > 0.f && most < INFINITY) {
+			e = 14 - ilogbf(most);
+			e = e > 100 ? 100 : e < -100 ? -100 : e;
+		}
+		scale[0] = ldexpf(1.f, e);
+		scale[1] = ldexpf(1.f, -e);
+	}
+}
+
+// Rows of 16-bit elements copied to aligned rows of dstRow (a multiple of 8) elements, zeros behind the width.  With labels: a row without a
+// target or with a loss_diff of zero becomes zeros -- it has no gradient, whatever it holds.
+__global__ void __launch_bounds__(256) copy_rows16_kernel(const uint16_t* __restrict__ src, long long srcRow, int rows, int width,
+	uint16_t* __restrict__ dst, int dstRow, const int* __restrict__ labels, const float* __restrict__ lossDiff, int vocabulary)
+{
+	dependent_wait();
+	const int perRow = dstRow / 8;
+	const long long total = static_cast<long long>(rows) * perRow;
+	for(long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += static_cast<long long>(gridDim.x) * blockDim.x) {
+		int r, u;
+		row_unit(i, perRow, &r, &u);
+		const uint16_t* const from = src + r * srcRow + u * 8;
+		uint4 v = make_uint4(0u, 0u, 0u, 0u);
+		if(labels == nullptr || (has_target(labels, r, vocabulary) && !(lossDiff[r] == 0.f))) {
+			// a word around the first or the last element of all may reach outside
+			const bool inside = u * 8 + 8 <= width && (i != 0 || (reinterpret_cast<uintptr_t>(from) & 3u) == 0) && (r != rows - 1 || u * 8 + 8 < width);
+			if(inside || (u * 8 + 8 <= width && (reinterpret_cast<uintptr_t>(from) & 3u) == 0)) {
+				v = gather8(from);
+			} else {
+				uint32_t e[8];
+#pragma unroll
+				for(int j = 0; j < 8; ++j) e[j] = u * 8 + j < width ? from[j] : 0u;
+				v = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
 			}
+		}
+		*reinterpret_cast<uint4*>(dst + static_cast<long long>(r) * dstRow + u * 8) = v;
+	}
+}
+
+// The way back: aligned rows of srcRow > width elements to rows that begin anywhere.
+__global__ void __launch_bounds__(256) spread_rows16_kernel(const uint16_t* __restrict__ src, int srcRow, int rows, int width, uint16_t* __restrict__ dst,
+	long long dstRow)
+{
+	dependent_wait();
+	const int perRow = (width + 14) / 8;
+	const long long total = static_cast<long long>(rows) * perRow;
+	for(long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += static_cast<long long>(gridDim.x) * blockDim.x) {
+		int r, u;
+		row_unit(i, perRow, &r, &u);
+		uint16_t* const to = dst + r * dstRow;
+		const int first = u * 8 - static_cast<int>((reinterpret_cast<uintptr_t>(to) & 15u) / 2);
+		const uint16_t* const from = src + static_cast<long long>(r) * srcRow;
+		if(first >= 0 && first + 8 <= width) {
+			*reinterpret_cast<uint4*>(to + first) = gather8(from + first);
 		} else {
-			for(int i = threadIdx.x; i < dstRow; i += blockDim.x) to[i] = keep && i < width ? from[i] : 0;
+			for(int j = first < 0 ? 0 : first; j < first + 8 && j < width; ++j) to[j] = from[j];
 		}
 	}
 }
@@ -172,28 +217,38 @@ __global__ void __launch_bounds__(256) sum_planes_kernel(const float* __restrict
 __global__ void __launch_bounds__(256) split_rows_kernel(const float* __restrict__ src, long long srcRow, int rows, int width,
 	__nv_bfloat16* __restrict__ dst, int dstRow, long long plane, const int* __restrict__ labels, const float* __restrict__ lossDiff, int vocabulary)
 {
+	dependent_wait();
+	const int perRow = dstRow / 8;
+	const long long total = static_cast<long long>(rows) * perRow;
 	const bool vector = (srcRow & 3) == 0 && (reinterpret_cast<uintptr_t>(src) & 15u) == 0;
-	for(long long r = blockIdx.x; r < rows; r += gridDim.x) {
-		const bool keep = labels == nullptr || (has_target(labels, static_cast<int>(r), vocabulary) && !(lossDiff[r] == 0.f));
-		const float* const from = src + r * srcRow;
-		__nv_bfloat16* const to = dst + r * dstRow;
-		for(int i = threadIdx.x * 4; i < dstRow; i += blockDim.x * 4) { // dstRow is a multiple of 8
-			float v[4];
-			if(vector && i + 4 <= width) {
-				const float4 f = *reinterpret_cast<const float4*>(from + i);
-				v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
+	for(long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += static_cast<long long>(gridDim.x) * blockDim.x) {
+		int r, u;
+		row_unit(i, perRow, &r, &u);
+		const float* const from = src + r * srcRow + u * 8;
+		float v[8];
+#pragma unroll
+		for(int j = 0; j < 8; ++j) v[j] = 0.f;
+		if(labels == nullptr || (has_target(labels, r, vocabulary) && !(lossDiff[r] == 0.f))) {
+			if(vector && u * 8 + 8 <= width) {
+				Unit16<float>::unpack(reinterpret_cast<const uint4*>(from)[0], v);
+				Unit16<float>::unpack(reinterpret_cast<const uint4*>(from)[1], v + 4);
 			} else {
 #pragma unroll
-				for(int j = 0; j < 4; ++j) v[j] = i + j < width ? from[i + j] : 0.f;
+				for(int j = 0; j < 8; ++j) v[j] = u * 8 + j < width ? from[j] : 0.f;
 			}
+		}
+		__nv_bfloat16* const to = dst + static_cast<long long>(r) * dstRow + u * 8;
 #pragma unroll
-			for(int k = 0; k < 3; ++k) {
-				const uint32_t a = keep ? pack2<__nv_bfloat16>(v[0], v[1]) : 0u, b = keep ? pack2<__nv_bfloat16>(v[2], v[3]) : 0u;
-				*reinterpret_cast<uint2*>(to + k * plane + i) = make_uint2(a, b);
-				const float2 fa = unpack2<__nv_bfloat16>(a), fb = unpack2<__nv_bfloat16>(b);
-				// (an infinite or undefined element stays one in every plane)
-				v[0] -= fa.x; v[1] -= fa.y; v[2] -= fb.x; v[3] -= fb.y;
+		for(int k = 0; k < 3; ++k) {
+			uint32_t w[4];
+#pragma unroll
+			for(int j = 0; j < 4; ++j) {
+				w[j] = pack2<__nv_bfloat16>(v[2 * j], v[2 * j + 1]);
+				const float2 taken = unpack2<__nv_bfloat16>(w[j]); // (an infinite or undefined element stays one in every plane)
+				v[2 * j] -= taken.x;
+				v[2 * j + 1] -= taken.y;
 			}
+			*reinterpret_cast<uint4*>(to + k * plane) = make_uint4(w[0], w[1], w[2], w[3]);
 		}
 	}
 }
@@ -230,20 +285,21 @@ int round_up(long long v, int to) { return static_cast<int>((v + to - 1) / to * 
 
 bool rows_for_tma(const void* p, long long row) { return aligned16(p) && row % 8 == 0; }
 
-// Rows of weights_diff that do not begin on 16-byte boundaries: a tile's threads, which have a row each, would store element by element.
-// They are written by the pass that adds up the parts of K then, along the rows (gradient of 5000 x 1030 fp16 weights by 1000 rows: 100
-// us in all, 177 when the tiles' threads stored it).
-bool by_planes(const Problem& q) { return q.width % (q.type == NB200_TYPE_FP32 ? 4 : 8) != 0; }
+// Rows of weights_diff that do not begin on 16-byte boundaries: a tile's threads, which have a row each, would store element by element
+// (gradient of 5000 x 1030 fp16 weights by 1000 rows: 177 us).  16-bit ones go to aligned rows first, fp32 ones to the planes that
+// parts of K are added up from.
+bool odd_rows(const Problem& q) { return q.width % (q.type == NB200_TYPE_FP32 ? 4 : 8) != 0; }
 
-// Columns of the vocabulary that are handled at a time: dz of a piece, for fp32 the planes of a piece of the weights, and the fp32 sums
-// of by_planes() take at most PIECE_BYTES each.  The 16-bit forward pass needs none of them.
+// Columns of the vocabulary that are handled at a time: dz of a piece, for fp32 the planes of a piece of the weights, and the aligned
+// rows of odd_rows() take at most PIECE_BYTES each.  The 16-bit forward pass needs none of them.
 int piece_of(const Problem& q, bool backward)
 {
 	const bool fp32 = q.type == NB200_TYPE_FP32;
 	long long perColumn = fp32 ? 6ll * round_up(q.width, 8) : 0;
 	const long long diff = backward ? (fp32 ? 6ll : 2ll) * q.rows : 0;
 	if(diff > perColumn) perColumn = diff;
-	if(backward && by_planes(q) && 4ll * round_up(q.width, 8) > perColumn) perColumn = 4ll * round_up(q.width, 8);
+	const long long odd = backward && odd_rows(q) ? type_size(q.type) * static_cast<long long>(round_up(q.width, 8)) : 0;
+	if(odd > perColumn) perColumn = odd;
 	const long long whole = round_up(q.vocabulary, PRODUCT16_N);
 	if(perColumn == 0) return static_cast<int>(whole);
 	long long piece = PIECE_BYTES / perColumn / PRODUCT16_N * PRODUCT16_N;
@@ -293,6 +349,7 @@ struct Backward {
 	float* scale;
 	uint16_t *hidden, *weights, *diff;
 	float *hiddenPlanes, *weightsPlanes;
+	uint16_t* weightsRows; // weights_diff in aligned rows; null: straight to the caller
 	Backward(const Problem& q, Room& room)
 	{
 		const bool fp32 = q.type == NB200_TYPE_FP32;
@@ -307,7 +364,8 @@ struct Backward {
 		weights = fp32 ? room.take<uint16_t>(3 * piece * ld) : rows_for_tma(q.weights, q.weightsRow) ? nullptr : room.take<uint16_t>(q.vocabulary * ld);
 		diff = room.take<uint16_t>(planes * q.rows * piece);
 		hiddenPlanes = room.take<float>(static_cast<size_t>(hiddenSplits) * q.rows * ld);
-		weightsPlanes = weightsSplits > 1 || by_planes(q) ? room.take<float>(static_cast<size_t>(weightsSplits) * piece * ld) : nullptr;
+		weightsPlanes = weightsSplits > 1 || (fp32 && odd_rows(q)) ? room.take<float>(static_cast<size_t>(weightsSplits) * piece * ld) : nullptr;
+		weightsRows = weightsPlanes == nullptr && odd_rows(q) ? room.take<uint16_t>(piece * ld) : nullptr;
 	}
 };
 
@@ -323,19 +381,23 @@ bool too_big(const Problem& q)
 
 // ---- launches -----------------------------------------------------------------------------------------------------------
 
-void copy_rows(const void* src, long long srcRow, int rows, int width, uint16_t* dst, const int* labels, const float* lossDiff,
-	int vocabulary, float* scale, int fp16, cudaStream_t stream)
+dim3 units_grid(int rows, int perRow) { return dim3(grid_for(static_cast<long long>(rows) * perRow, 256, 8)); }
+
+void copy_rows(const void* src, long long srcRow, int rows, int width, uint16_t* dst, const int* labels, const float* lossDiff, int vocabulary,
+	cudaStream_t stream)
 {
-	copy_rows16_kernel<<<grid_for(rows, 1, 16) + (scale != nullptr ? 1 : 0), 256, 0, stream>>>(static_cast<const uint16_t*>(src), srcRow, rows, width, dst,
-		round_up(width, 8), labels, lossDiff, vocabulary, scale, fp16);
+	const int ld = round_up(width, 8);
+	launch_dependent(true, copy_rows16_kernel, units_grid(rows, ld / 8), dim3(256), 0, stream, static_cast<const uint16_t*>(src), srcRow, rows, width, dst,
+		ld, labels, lossDiff, vocabulary);
 	count_launch();
 }
 
 void split_rows(const void* src, long long srcRow, int rows, int width, uint16_t* dst, long long plane, const int* labels, const float* lossDiff,
 	int vocabulary, cudaStream_t stream)
 {
-	split_rows_kernel<<<grid_for(rows, 1, 16), 256, 0, stream>>>(static_cast<const float*>(src), srcRow, rows, width,
-		reinterpret_cast<__nv_bfloat16*>(dst), round_up(width, 8), plane, labels, lossDiff, vocabulary);
+	const int ld = round_up(width, 8);
+	launch_dependent(true, split_rows_kernel, units_grid(rows, ld / 8), dim3(256), 0, stream, static_cast<const float*>(src), srcRow, rows, width,
+		reinterpret_cast<__nv_bfloat16*>(dst), ld, plane, labels, lossDiff, vocabulary);
 	count_launch();
 }
 
@@ -375,8 +437,8 @@ int forward(const Problem& q, const int* labels, float* loss, float* logSum, voi
 	const bool fp32 = q.type == NB200_TYPE_FP32, bf16 = q.type != NB200_TYPE_FP16;
 	const long long ld = round_up(q.width, 8);
 	if(fp32) split_rows(q.hidden, q.hiddenRow, q.rows, q.width, f.hidden, q.rows * ld, nullptr, nullptr, 0, stream);
-	else if(f.hidden != nullptr) copy_rows(q.hidden, q.hiddenRow, q.rows, q.width, f.hidden, nullptr, nullptr, 0, nullptr, 0, stream);
-	if(!fp32 && f.weights != nullptr) copy_rows(q.weights, q.weightsRow, q.vocabulary, q.width, f.weights, nullptr, nullptr, 0, nullptr, 0, stream);
+	else if(f.hidden != nullptr) copy_rows(q.hidden, q.hiddenRow, q.rows, q.width, f.hidden, nullptr, nullptr, 0, stream);
+	if(!fp32 && f.weights != nullptr) copy_rows(q.weights, q.weightsRow, q.vocabulary, q.width, f.weights, nullptr, nullptr, 0, stream);
 	CUtensorMap a, b;
 	if(!product16_map(&a, f.hidden ? f.hidden : q.hidden, bf16, q.width, q.rows, f.hidden ? ld : q.hiddenRow, PRODUCT16_BOX_A, fp32 ? q.rows * ld : 0)) return NB200_EINVAL;
 	for(int first = 0; first < q.vocabulary; first += f.piece) {
@@ -418,10 +480,10 @@ int backward(const Problem& q, const float* lossDiff, const int* labels, const f
 	const bool fp32 = q.type == NB200_TYPE_FP32, bf16 = q.type != NB200_TYPE_FP16;
 	const long long ld = round_up(q.width, 8), hiddenPlane = fp32 ? q.rows * ld : 0, diffPlane = fp32 ? static_cast<long long>(q.rows) * w.piece : 0;
 	if(fp32) split_rows(q.hidden, q.hiddenRow, q.rows, q.width, w.hidden, hiddenPlane, labels, lossDiff, q.vocabulary, stream);
-	// (for fp32 only the scale, which is one then)
-	copy_rows(fp32 ? nullptr : q.hidden, q.hiddenRow, fp32 ? 0 : q.rows, q.width, w.hidden, labels, lossDiff, q.vocabulary, w.scale,
-		q.type == NB200_TYPE_FP16 ? 1 : 0, stream);
-	if(!fp32 && w.weights != nullptr) copy_rows(q.weights, q.weightsRow, q.vocabulary, q.width, w.weights, nullptr, nullptr, 0, nullptr, 0, stream);
+	else copy_rows(q.hidden, q.hiddenRow, q.rows, q.width, w.hidden, labels, lossDiff, q.vocabulary, stream);
+	launch_dependent(true, diff_scale_kernel, dim3(1), dim3(256), 0, stream, q.rows, labels, lossDiff, q.vocabulary, w.scale, q.type == NB200_TYPE_FP16 ? 1 : 0);
+	count_launch();
+	if(!fp32 && w.weights != nullptr) copy_rows(q.weights, q.weightsRow, q.vocabulary, q.width, w.weights, nullptr, nullptr, 0, stream);
 	CUtensorMap hidden, hiddenAcross, rows, across, diff, diffAcross;
 	if(!product16_map(&hidden, w.hidden, bf16, q.width, q.rows, ld, PRODUCT16_BOX_A, hiddenPlane)
 		|| !product16_map(&hiddenAcross, w.hidden, bf16, q.width, q.rows, ld, PRODUCT16_BOX_ACROSS, hiddenPlane)
@@ -454,9 +516,16 @@ int backward(const Problem& q, const float* lossDiff, const int* labels, const f
 				if(rc != NB200_OK) return rc;
 				sum_planes(q, w.weightsPlanes, p.splits, columns, w.scale + 1, out, weightsDiffRow, stream);
 			} else {
-				p.out = out; p.ldOut = weightsDiffRow; p.resultScale = w.scale + 1;
+				p.out = w.weightsRows != nullptr ? w.weightsRows : out;
+				p.ldOut = w.weightsRows != nullptr ? ld : weightsDiffRow;
+				p.resultScale = w.scale + 1;
 				rc = product16(PRODUCT16_STORE, true, true, p, &diffAcross, &hiddenAcross, stream);
 				if(rc != NB200_OK) return rc;
+				if(w.weightsRows != nullptr) {
+					launch_dependent(true, spread_rows16_kernel, units_grid(columns, (q.width + 14) / 8), dim3(256), 0, stream,
+						static_cast<const uint16_t*>(w.weightsRows), static_cast<int>(ld), columns, q.width, static_cast<uint16_t*>(out), weightsDiffRow);
+					count_launch();
+				}
 			}
 		}
 	}

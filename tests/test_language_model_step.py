@@ -143,3 +143,34 @@ def test_tokens_one_at_a_time(t):
     step = torch.finfo(t).eps
     assert (torch.cat(logs, 1) - want).abs().max() <= 16 * step * want.abs().max() + 1e-5
     assert (state - last).abs().max() <= 2.0 ** -18 * last.abs().max()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", TYPES)
+def test_same_bits_without_the_native_half(monkeypatch, t):
+    m, d = _model(t)
+    want = _step(m, d)
+    monkeypatch.setattr(ops, "_native_module", ops._DeclinesAll())
+    got = _step(m, d)
+    for a, b in zip((*got[:3], *got[3].values()), (*want[:3], *want[3].values())):
+        assert a.shape == b.shape and a.dtype == b.dtype and torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_parameters_and_other_streams():
+    """torch's parameters are taken like tensors, nothing is recorded for its automatic gradients, and a call runs on the stream
+    that is current where it is made."""
+    m, d = _model(torch.bfloat16)
+    want = _step(m, d)
+    p = {k: torch.nn.Parameter(v) for k, v in m.items()}
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        y, mean, inv = ops.LayerNormalization(p["x"], p["scale1"], p["free1"])
+        h, last = ops.GatedRecurrence(y, p["gates"], p["inputs"], initial_state=p["state"], lengths=d["lengths"])
+        z, _, _ = ops.LayerNormalization(h, p["scale2"], p["free2"])
+        inside = torch.arange(L, device="cuda") < d["lengths"][:, None]
+        loss, log_sum = ops.VocabularyCrossEntropy(z, p["head"], torch.where(inside, d["labels"], -1).int())
+    side.synchronize()
+    assert torch.equal(loss, want[0]) and torch.equal(last, want[2])
+    assert not any(t.requires_grad for t in (y, mean, inv, h, last, loss, log_sum))
