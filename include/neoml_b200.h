@@ -375,9 +375,9 @@ NB200_API int nb200_distillation_loss_backward(void* stream, int type, int teach
  *   log_sum[r] = log sum_j exp(z[r][j]),   loss[r] = log_sum[r] - z[r][label[r]],   z = hidden * weights^T.
  * A label outside 0..vocabulary-1 marks a row without a target: its loss is zero, and in the backward pass it has no
  * gradient, whatever the row holds.  Both matrices are of `type`; sums are fp32.  `scratch` holds nb200_vocabulary_cross_entropy_scratch_bytes(...) bytes, 256-byte
- * aligned: for the logits' partial sums, for copies of operands whose rows do not begin on 16-byte boundaries (of 16-bit types), for
- * the hidden rows and one piece of the weights in the tensor core's parts (fp32), and for one piece of the gradient by the logits
- * (backward); a piece takes 256 MB, or 256 columns if that is more. */
+ * aligned: for the logits' partial sums (8 bytes per row and 128 entries), for copies of operands whose rows do not begin on 16-byte boundaries
+ * (of 16-bit types), for the hidden rows and up to 1 GB of the weights in the tensor core's parts (fp32), and for one piece of the
+ * gradient by the logits (backward), 256 MB or 256 columns if that is more. */
 NB200_API size_t nb200_vocabulary_cross_entropy_scratch_bytes(int type, const void* hidden, int rows, int width,
 	long long hidden_row_size, const void* weights, int vocabulary, long long weights_row_size, int backward);
 NB200_API int nb200_vocabulary_cross_entropy(void* stream, int type, const void* hidden, int rows, int width,

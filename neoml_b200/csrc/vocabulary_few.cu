@@ -1,0 +1,349 @@
+// The cross entropy over a vocabulary for up to eight rows of fp32: a token or a few of each text that is scored or decoded.
+//
+// The weights are then read for less arithmetic than reading them takes; what counts is that they come once, as they lie, without the
+// planes that the tensor core wants of fp32 (vocabulary_loss.cu), and that nothing but fp32 multiply-adds stands between.  A block has
+// a stretch of the vocabulary:
+//   logits     tiles of 64 entries x 64 elements go through shared memory; four neighbouring threads share an entry, each taking
+//              every fourth element for all the rows, two rows per instruction
+//   forward    every thread keeps a running maximum and sum for its entries and a quarter of the rows; a block's join in the end
+//   backward   dz of the stretch stays in shared memory; then a thread takes columns of the weights down the stretch, reading them once
+//              more (out of L2 while they fit), and gives weights_diff as it goes and its part of hidden_diff at the end
+// 4 x 203 rows over 106779 entries: loss 38 us, gradients 75 us; by planes 118 and 316.  Eight rows of 1031 over 30011: 70 + 183 us against 128
+// + 315; sixteen 190 + 347 against 127 + 322.  16-bit rows are faster on the tensor core from the first on (one row of 1024 over
+// 32000 bf16: 20 us there, 57 by this kernel).
+#include "vocabulary_few.cuh"
+
+namespace nb200 {
+
+namespace {
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr int THREADS = 256, WARPS = THREADS / 32;
+constexpr int TILE = FEW_TILE;       // vocabulary entries
+constexpr int CHUNK = 64;            // elements of them at a time
+constexpr int PITCH = CHUNK + 4;     // 8 entries x 4 elements of a warp's read lie in 32 different banks
+
+__device__ __forceinline__ float exp2_fast(float x)
+{
+	float y;
+	asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+	return y;
+}
+
+// What a warp has in hand of a chunk: its eight entries' elements lane and lane + 32.
+struct Staged {
+	static constexpr int ROWS = TILE / WARPS;
+	float v[ROWS][2];
+	__device__ __forceinline__ void load(const FewParams& p, int entry0, int k0)
+	{
+		const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+#pragma unroll
+		for(int i = 0; i < ROWS; ++i) {
+			const int entry = entry0 + warp + i * WARPS;
+			const float* const row = p.weights + static_cast<long long>(entry) * p.weightsRow;
+#pragma unroll
+			for(int j = 0; j < 2; ++j) {
+				const int k = k0 + lane + 32 * j;
+				v[i][j] = entry < p.vocabulary && k < p.width ? row[k] : 0.f;
+			}
+		}
+	}
+	__device__ __forceinline__ void store(float* tile) const
+	{
+		const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+#pragma unroll
+		for(int i = 0; i < ROWS; ++i) {
+			float* const to = tile + (warp + i * WARPS) * PITCH;
+			to[lane] = v[i][0];
+			to[lane + 32] = v[i][1];
+		}
+	}
+};
+
+// The rows' elements k0 .. k0 + 63, rows without data as zeros; stored as [element][row].
+template<int NT>
+struct StagedHidden {
+	static constexpr int N = CHUNK * NT / THREADS;
+	float v[N];
+	__device__ __forceinline__ void load(const FewParams& p, int k0)
+	{
+#pragma unroll
+		for(int i = 0; i < N; ++i) {
+			const int at = threadIdx.x + i * THREADS, t = at / CHUNK, k = at % CHUNK;
+			v[i] = t < p.rows && k0 + k < p.width ? p.hidden[t * p.hiddenRow + k0 + k] : 0.f;
+		}
+	}
+	__device__ __forceinline__ void store(float* to) const
+	{
+#pragma unroll
+		for(int i = 0; i < N; ++i) {
+			const int at = threadIdx.x + i * THREADS;
+			to[at % CHUNK * NT + at / CHUNK] = v[i];
+		}
+	}
+};
+
+template<int NT>
+struct Tiles {
+	float weights[2][TILE * PITCH];
+	float hidden[2][CHUNK * NT];
+};
+
+// The logits of the entries entry0 .. entry0 + 63: this thread's entry is threadIdx.x / 4, and all four threads of an entry get them.
+template<int NT>
+__device__ __forceinline__ void tile_logits(const FewParams& p, Tiles<NT>& s, Staged& staged, StagedHidden<NT>& hidden, int entry0, int next0, float2 (&z)[NT / 2], int& phase)
+{
+	const int entry = threadIdx.x >> 2, part = threadIdx.x & 3;
+#pragma unroll
+	for(int t = 0; t < NT / 2; ++t) z[t] = both(0.f);
+	for(int k0 = 0; k0 < p.width; k0 += CHUNK, phase ^= 1) {
+		staged.store(s.weights[phase]);
+		hidden.store(s.hidden[phase]);
+		__syncthreads(); // one a chunk: the buffers alternate
+		if(k0 + CHUNK < p.width || next0 >= 0) { // under way while this chunk is worked on
+			const int k1 = k0 + CHUNK < p.width ? k0 + CHUNK : 0;
+			staged.load(p, k1 > 0 ? entry0 : next0, k1);
+			hidden.load(p, k1);
+		}
+		const float* const w = s.weights[phase] + entry * PITCH + part;
+		const float* const h = s.hidden[phase] + part * NT;
+#pragma unroll
+		for(int k = 0; k < CHUNK / 4; ++k) {
+			const float2 x = both(w[4 * k]);
+#pragma unroll
+			for(int t = 0; t < NT / 4; ++t) {
+				const float4 y = *reinterpret_cast<const float4*>(h + 4 * k * NT + 4 * t);
+				z[2 * t] = fma2(x, make_float2(y.x, y.y), z[2 * t]);
+				z[2 * t + 1] = fma2(x, make_float2(y.z, y.w), z[2 * t + 1]);
+			}
+		}
+	}
+#pragma unroll
+	for(int o = 1; o < 4; o <<= 1) {
+#pragma unroll
+		for(int t = 0; t < NT / 2; ++t) {
+			z[t] = add2(z[t], make_float2(__shfl_xor_sync(0xffffffffu, z[t].x, o), __shfl_xor_sync(0xffffffffu, z[t].y, o)));
+		}
+	}
+}
+
+__device__ __forceinline__ bool has_target(const FewParams& p, int row, int* label)
+{
+	*label = row < p.rows ? __ldg(p.labels + row) : -1;
+	return *label >= 0 && *label < p.vocabulary;
+}
+
+__device__ __forceinline__ float2 join(float2 a, float2 b)
+{
+	const float t = fmaxf(a.x, b.x), at = t == -INFINITY ? 0.f : t;
+	return make_float2(t, a.y * exp2_fast(a.x - at) + b.y * exp2_fast(b.x - at));
+}
+
+template<int NT>
+__global__ void __launch_bounds__(THREADS) few_forward_kernel(const FewParams p)
+{
+	extern __shared__ __align__(16) uint8_t room[];
+	Tiles<NT>& s = *reinterpret_cast<Tiles<NT>*>(room);
+	__shared__ float2 joined[WARPS][NT];
+	const int begin = blockIdx.x * p.perBlock, end = min(p.vocabulary, begin + p.perBlock);
+	const int part = threadIdx.x & 3;
+	float2 running[NT / 4]; // of rows 4 i + part
+	int label[NT / 4];
+#pragma unroll
+	for(int i = 0; i < NT / 4; ++i) {
+		running[i] = make_float2(-INFINITY, 0.f);
+		if(!has_target(p, 4 * i + part, &label[i])) label[i] = -1;
+	}
+	Staged staged;
+	StagedHidden<NT> hidden;
+	staged.load(p, begin, 0);
+	hidden.load(p, 0);
+	int phase = 0;
+	for(int entry0 = begin; entry0 < end; entry0 += TILE) {
+		float2 z[NT / 2];
+		tile_logits<NT>(p, s, staged, hidden, entry0, entry0 + TILE < end ? entry0 + TILE : -1, z, phase);
+		const int entry = entry0 + (threadIdx.x >> 2);
+		if(entry < end) {
+#pragma unroll
+			for(int i = 0; i < NT / 4; ++i) {
+				const float own = part == 0 ? z[2 * i].x : part == 1 ? z[2 * i].y : part == 2 ? z[2 * i + 1].x : z[2 * i + 1].y;
+				if(entry == label[i]) p.labelled[4 * i + part] = own;
+				running[i] = join(running[i], make_float2(own * LOG2E, 1.f));
+			}
+		}
+	}
+#pragma unroll
+	for(int i = 0; i < NT / 4; ++i) {
+#pragma unroll
+		for(int o = 4; o < 32; o <<= 1) {
+			running[i] = join(running[i], make_float2(__shfl_xor_sync(0xffffffffu, running[i].x, o), __shfl_xor_sync(0xffffffffu, running[i].y, o)));
+		}
+		if((threadIdx.x & 31) < 4) joined[threadIdx.x >> 5][4 * i + part] = running[i];
+	}
+	__syncthreads();
+	const int row = threadIdx.x;
+	if(row < p.rows) {
+		float2 all = joined[0][row];
+		for(int w = 1; w < WARPS; ++w) all = join(all, joined[w][row]);
+		p.partial[static_cast<long long>(blockIdx.x) * p.rows + row] = all;
+	}
+}
+
+template<int NT>
+__global__ void __launch_bounds__(THREADS) few_backward_kernel(const FewParams p)
+{
+	extern __shared__ __align__(16) uint8_t room[];
+	Tiles<NT>& s = *reinterpret_cast<Tiles<NT>*>(room);
+	float* const dz = reinterpret_cast<float*>(room + sizeof(Tiles<NT>)); // [perBlock][NT]
+	const int begin = blockIdx.x * p.perBlock, end = min(p.vocabulary, begin + p.perBlock);
+	const int part = threadIdx.x & 3;
+	float logSum2[NT / 4], by[NT / 4];
+	int label[NT / 4];
+#pragma unroll
+	for(int i = 0; i < NT / 4; ++i) {
+		const bool used = has_target(p, 4 * i + part, &label[i]);
+		by[i] = used ? __ldg(p.lossDiff + 4 * i + part) : 0.f;
+		logSum2[i] = used ? __ldg(p.logSum + 4 * i + part) * LOG2E : 0.f;
+	}
+	Staged staged;
+	StagedHidden<NT> hidden;
+	staged.load(p, begin, 0);
+	hidden.load(p, 0);
+	int phase = 0;
+	for(int entry0 = begin; entry0 < end; entry0 += TILE) {
+		float2 z[NT / 2];
+		tile_logits<NT>(p, s, staged, hidden, entry0, entry0 + TILE < end ? entry0 + TILE : -1, z, phase);
+		const int entry = entry0 + (threadIdx.x >> 2);
+#pragma unroll
+		for(int i = 0; i < NT / 4; ++i) {
+			const float own = part == 0 ? z[2 * i].x : part == 1 ? z[2 * i].y : part == 2 ? z[2 * i + 1].x : z[2 * i + 1].y;
+			// a row without a target has no gradient, whatever its logits
+			const float q = exp2_fast(fmaf(own, LOG2E, -logSum2[i])) - (entry == label[i] ? 1.f : 0.f);
+			if(entry < end) dz[(entry - begin) * NT + 4 * i + part] = by[i] == 0.f ? 0.f : by[i] * q;
+		}
+	}
+	__syncthreads();
+	const float* const weights = p.weights + static_cast<long long>(begin) * p.weightsRow;
+	float* const out = p.weightsDiff == nullptr ? nullptr : p.weightsDiff + static_cast<long long>(begin) * p.weightsDiffRow;
+	const int count = end - begin;
+	for(int c = threadIdx.x; c < p.width; c += THREADS) {
+		float2 h[NT / 2], dx[NT / 2]; // pairs of rows
+#pragma unroll
+		for(int t = 0; t < NT; ++t) {
+			int unused;
+			const float v = has_target(p, t, &unused) && !(__ldg(p.lossDiff + t) == 0.f) ? p.hidden[t * p.hiddenRow + c] : 0.f;
+			(t % 2 == 0 ? h[t / 2].x : h[t / 2].y) = v;
+			dx[t / 2] = both(0.f);
+		}
+		constexpr int AHEAD = 8;
+		for(int e0 = 0; e0 < count; e0 += AHEAD) {
+			float w[AHEAD];
+#pragma unroll
+			for(int k = 0; k < AHEAD; ++k) w[k] = p.hiddenPart != nullptr && e0 + k < count ? weights[static_cast<long long>(e0 + k) * p.weightsRow + c] : 0.f;
+#pragma unroll
+			for(int k = 0; k < AHEAD; ++k) {
+				if(e0 + k >= count) break;
+				float2 sums = both(0.f);
+				const float2 x = both(w[k]);
+#pragma unroll
+				for(int t = 0; t < NT / 4; ++t) {
+					const float4 d = *reinterpret_cast<const float4*>(dz + (e0 + k) * NT + 4 * t);
+					const float2 d0 = make_float2(d.x, d.y), d1 = make_float2(d.z, d.w);
+					sums = fma2(d1, h[2 * t + 1], fma2(d0, h[2 * t], sums));
+					dx[2 * t] = fma2(d0, x, dx[2 * t]);
+					dx[2 * t + 1] = fma2(d1, x, dx[2 * t + 1]);
+				}
+				if(out != nullptr) out[static_cast<long long>(e0 + k) * p.weightsDiffRow + c] = sums.x + sums.y;
+			}
+		}
+		if(p.hiddenPart != nullptr) {
+			float* const mine = p.hiddenPart + static_cast<long long>(blockIdx.x) * p.rows * p.width + c;
+#pragma unroll
+			for(int t = 0; t < NT; ++t) {
+				if(t < p.rows) mine[static_cast<long long>(t) * p.width] = t % 2 == 0 ? dx[t / 2].x : dx[t / 2].y;
+			}
+		}
+	}
+}
+
+// hidden_diff from the blocks' parts, added in order: 32 columns of a row per block, eight threads a column take every eighth part.
+__global__ void __launch_bounds__(256) few_hidden_kernel(const FewParams p, int parts, float* __restrict__ out, long long outRow)
+{
+	__shared__ float sums[8][32];
+	dependent_wait();
+	const int lane = threadIdx.x & 31, group = threadIdx.x >> 5;
+	const int c = blockIdx.x * 32 + lane, t = blockIdx.y;
+	float s = 0.f;
+	if(c < p.width) {
+		const float* const at = p.hiddenPart + static_cast<long long>(t) * p.width + c;
+		constexpr int AHEAD = 8;
+		for(int i = group; i < parts; i += 8 * AHEAD) {
+			float v[AHEAD];
+#pragma unroll
+			for(int k = 0; k < AHEAD; ++k) v[k] = i + 8 * k < parts ? at[static_cast<long long>(i + 8 * k) * p.rows * p.width] : 0.f;
+#pragma unroll
+			for(int k = 0; k < AHEAD; ++k) s += v[k];
+		}
+	}
+	sums[group][lane] = s;
+	__syncthreads();
+	if(group != 0 || c >= p.width) return;
+	s = 0.f;
+#pragma unroll
+	for(int g = 0; g < 8; ++g) s += sums[g][lane];
+	out[t * outRow + c] = s;
+}
+
+template<int NT>
+void launch_forward(const FewParams& p, cudaStream_t stream)
+{
+	few_forward_kernel<NT><<<few_blocks(p.vocabulary), THREADS, sizeof(Tiles<NT>), stream>>>(p);
+	count_launch();
+}
+
+template<int NT>
+void launch_backward(const FewParams& p, cudaStream_t stream)
+{
+	constexpr size_t each = NT * sizeof(float), most = sizeof(Tiles<NT>) + FEW_MOST_ENTRIES * each;
+	cudaFuncSetAttribute(few_backward_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(most));
+	few_backward_kernel<NT><<<few_blocks(p.vocabulary), THREADS, sizeof(Tiles<NT>) + p.perBlock * each, stream>>>(p);
+	count_launch();
+}
+
+static_assert(sizeof(Tiles<8>) <= 48 * 1024, "more shared memory than a kernel may have without asking");
+
+} // namespace
+
+int few_forward(const FewParams& p, cudaStream_t stream)
+{
+	if(p.rows <= 4) launch_forward<4>(p, stream);
+	else launch_forward<8>(p, stream);
+	return check_launch();
+}
+
+int few_backward(const FewParams& p, float* hiddenDiff, long long hiddenDiffRow, cudaStream_t stream)
+{
+	if(p.rows <= 4) launch_backward<4>(p, stream);
+	else launch_backward<8>(p, stream);
+	if(hiddenDiff != nullptr) {
+		launch_dependent(true, few_hidden_kernel, dim3((p.width + 31) / 32, p.rows), dim3(256), 0, stream, p, few_blocks(p.vocabulary), hiddenDiff,
+			hiddenDiffRow);
+		count_launch();
+	}
+	return check_launch();
+}
+
+// Blocks of a stretch each: four on an SM, or as many more as keep a stretch's dz within a block's shared memory; whole tiles.
+int few_entries(int vocabulary)
+{
+	const int tiles = (vocabulary + TILE - 1) / TILE, wanted = sm_count() * 4;
+	int perBlock = (tiles + wanted - 1) / wanted * TILE;
+	return perBlock > FEW_MOST_ENTRIES ? FEW_MOST_ENTRIES : perBlock;
+}
+int few_blocks(int vocabulary)
+{
+	const int perBlock = few_entries(vocabulary);
+	return (vocabulary + perBlock - 1) / perBlock;
+}
+
+} // namespace nb200

@@ -12,8 +12,9 @@
 //   of two that puts the largest loss_diff at 2^14, because softmax values of 1e-7 are below what a half holds; dz between 1
 //   and 2^-38 of the largest then keeps some or all of its bits.  hidden_diff is summed in fp32 over the pieces.
 // fp32: the same with three bf16 planes of each operand (product16.cuh), a piece of the weights split at a time: six times the
-// multiply-adds, and results as exact as fp32 sums in order give them.
+// multiply-adds, and results as exact as fp32 sums in order give them.  Up to eight rows of fp32: vocabulary_few.cu.
 #include "product16.cuh"
+#include "vocabulary_few.cuh"
 
 #include <cuda.h>
 
@@ -22,7 +23,7 @@ namespace nb200 {
 namespace {
 
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr long long PIECE_BYTES = 256ll << 20;
+constexpr long long DIFF_BYTES = 256ll << 20, PIECE_BYTES = 1ll << 30;
 
 __device__ __forceinline__ bool has_target(const int* labels, int row, int vocabulary)
 {
@@ -290,21 +291,25 @@ bool rows_for_tma(const void* p, long long row) { return aligned16(p) && row % 8
 // parts of K are added up from.
 bool odd_rows(const Problem& q) { return q.width % (q.type == NB200_TYPE_FP32 ? 4 : 8) != 0; }
 
-// Columns of the vocabulary that are handled at a time: dz of a piece, for fp32 the planes of a piece of the weights, and the aligned
-// rows of odd_rows() take at most PIECE_BYTES each.  The 16-bit forward pass needs none of them.
+// Columns of the vocabulary that are handled at a time: dz of a piece takes at most DIFF_BYTES; the planes of its weights (fp32) and the
+// aligned rows of odd_rows() take at most PIECE_BYTES each, which leaves a tile per SM for 128 rows of 4096 elements (with a
+// quarter of it, 75 x 4043 rows over 35434 entries ran on 35 of 148 SMs).  The 16-bit forward pass needs none of them.
 int piece_of(const Problem& q, bool backward)
 {
 	const bool fp32 = q.type == NB200_TYPE_FP32;
-	long long perColumn = fp32 ? 6ll * round_up(q.width, 8) : 0;
-	const long long diff = backward ? (fp32 ? 6ll : 2ll) * q.rows : 0;
-	if(diff > perColumn) perColumn = diff;
-	const long long odd = backward && odd_rows(q) ? type_size(q.type) * static_cast<long long>(round_up(q.width, 8)) : 0;
-	if(odd > perColumn) perColumn = odd;
-	const long long whole = round_up(q.vocabulary, PRODUCT16_N);
-	if(perColumn == 0) return static_cast<int>(whole);
-	long long piece = PIECE_BYTES / perColumn / PRODUCT16_N * PRODUCT16_N;
-	if(piece < PRODUCT16_N) piece = PRODUCT16_N;
+	const long long whole = round_up(q.vocabulary, PRODUCT16_N), ld = round_up(q.width, 8);
+	long long piece = whole;
+	auto limit = [&](long long bytes, long long perColumn) {
+		if(perColumn > 0 && bytes / perColumn < piece) piece = bytes / perColumn;
+	};
+	if(fp32) limit(PIECE_BYTES, 6 * ld);
+	if(backward) {
+		limit(DIFF_BYTES, (fp32 ? 6ll : 2ll) * q.rows);
+		if(odd_rows(q)) limit(PIECE_BYTES, type_size(q.type) * ld);
+	}
 	if(piece >= whole) return static_cast<int>(whole);
+	piece = piece / PRODUCT16_N * PRODUCT16_N;
+	if(piece < PRODUCT16_N) piece = PRODUCT16_N;
 	const long long pieces = (whole + piece - 1) / piece;   // of equal size
 	return round_up((whole + pieces - 1) / pieces, PRODUCT16_N);
 }
@@ -324,6 +329,22 @@ int splits_of(long long tiles, int kBlocks)
 struct Aligned {
 	const void* p;
 	long long row, plane;
+};
+
+// Few rows of fp32 go to kernels of their own, whose blocks have stretches of the vocabulary: not where it is shorter than the rows (6 x
+// 4007 rows over 119 entries, two blocks: 240 us).
+bool few_rows(const Problem& q) { return q.type == NB200_TYPE_FP32 && q.rows <= FEW_ROWS && q.vocabulary >= q.width; }
+
+struct FewRoom {
+	float2* partial;
+	float *labelled, *hiddenPart;
+	FewRoom(const Problem& q, bool backward, Room& room)
+	{
+		const size_t blocks = few_blocks(q.vocabulary);
+		partial = backward ? nullptr : room.take<float2>(blocks * q.rows);
+		labelled = backward ? nullptr : room.take<float>(q.rows);
+		hiddenPart = backward ? room.take<float>(blocks * q.rows * q.width) : nullptr;
+	}
 };
 
 struct Forward {
@@ -430,9 +451,35 @@ Product16Params params_of(const Problem& q, int m, int n, int splits, int k, boo
 	return p;
 }
 
+FewParams few_params(const Problem& q, const int* labels)
+{
+	FewParams p = {};
+	p.hidden = static_cast<const float*>(q.hidden); p.weights = static_cast<const float*>(q.weights); p.hiddenRow = q.hiddenRow; p.weightsRow = q.weightsRow;
+	p.rows = q.rows; p.width = q.width; p.vocabulary = q.vocabulary; p.perBlock = few_entries(q.vocabulary);
+	p.labels = labels;
+	return p;
+}
+
+void join_partials(const Problem& q, const float2* partial, int parts, const float* labelled, const int* labels, float* loss, float* logSum,
+	cudaStream_t stream)
+{
+	launch_dependent(true, join_partials_kernel, dim3((q.rows + 31) / 32), dim3(JOIN_WARPS * 32), 0, stream, partial, parts, q.rows, labelled, labels,
+		q.vocabulary, loss, logSum);
+	count_launch();
+}
+
 int forward(const Problem& q, const int* labels, float* loss, float* logSum, void* scratch, cudaStream_t stream)
 {
 	Room room = { static_cast<uint8_t*>(scratch) };
+	if(few_rows(q)) {
+		const FewRoom w(q, false, room);
+		FewParams p = few_params(q, labels);
+		p.partial = w.partial; p.labelled = w.labelled;
+		const int rc = few_forward(p, stream);
+		if(rc != NB200_OK) return rc;
+		join_partials(q, w.partial, few_blocks(q.vocabulary), w.labelled, labels, loss, logSum, stream);
+		return check_launch();
+	}
 	const Forward f(q, room);
 	const bool fp32 = q.type == NB200_TYPE_FP32, bf16 = q.type != NB200_TYPE_FP16;
 	const long long ld = round_up(q.width, 8);
@@ -451,9 +498,7 @@ int forward(const Problem& q, const int* labels, float* loss, float* logSum, voi
 		const int rc = product16(PRODUCT16_STATS, false, false, p, &a, &b, stream);
 		if(rc != NB200_OK) return rc;
 	}
-	launch_dependent(true, join_partials_kernel, dim3((q.rows + 31) / 32), dim3(JOIN_WARPS * 32), 0, stream, static_cast<const float2*>(f.partial),
-		(q.vocabulary + PRODUCT16_N - 1) / PRODUCT16_N * 2, q.rows, static_cast<const float*>(f.labelled), labels, q.vocabulary, loss, logSum);
-	count_launch();
+	join_partials(q, f.partial, (q.vocabulary + PRODUCT16_N - 1) / PRODUCT16_N * 2, f.labelled, labels, loss, logSum, stream);
 	return check_launch();
 }
 
@@ -476,6 +521,14 @@ int backward(const Problem& q, const float* lossDiff, const int* labels, const f
 	void* weightsDiff, long long weightsDiffRow, void* scratch, cudaStream_t stream)
 {
 	Room room = { static_cast<uint8_t*>(scratch) };
+	if(few_rows(q)) {
+		const FewRoom few(q, true, room);
+		FewParams p = few_params(q, labels);
+		p.logSum = logSum; p.lossDiff = lossDiff;
+		p.weightsDiff = static_cast<float*>(weightsDiff); p.weightsDiffRow = weightsDiffRow;
+		p.hiddenPart = hiddenDiff != nullptr ? few.hiddenPart : nullptr;
+		return few_backward(p, static_cast<float*>(hiddenDiff), hiddenDiffRow, stream);
+	}
 	const Backward w(q, room);
 	const bool fp32 = q.type == NB200_TYPE_FP32, bf16 = q.type != NB200_TYPE_FP16;
 	const long long ld = round_up(q.width, 8), hiddenPlane = fp32 ? q.rows * ld : 0, diffPlane = fp32 ? static_cast<long long>(q.rows) * w.piece : 0;
@@ -549,7 +602,8 @@ size_t nb200_vocabulary_cross_entropy_scratch_bytes(int type, const void* hidden
 	const Problem q = { type, rows, width, vocabulary, hidden, weights, hidden_row_size, weights_row_size };
 	if(!valid(q) || rows == 0 || too_big(q)) return 0;
 	Room room = { nullptr };
-	if(backward) Backward(q, room);
+	if(few_rows(q)) FewRoom(q, backward != 0, room);
+	else if(backward) Backward(q, room);
 	else Forward(q, room);
 	return room.used;
 }

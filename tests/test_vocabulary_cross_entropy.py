@@ -80,7 +80,8 @@ def _check(x, w, labels, dloss=None, got_forward=None, **kw):
 @pytest.mark.gpu
 @pytest.mark.parametrize("t", TYPES)
 @pytest.mark.parametrize("rows,width,v", [(1, 1, 1), (1, 8, 2), (3, 64, 256), (128, 64, 256), (129, 72, 300), (7, 129, 1000), (200, 1031, 515),
-                                          (48, 256, 32000), (1, 512, 5003), (1000, 96, 257), (300, 640, 1500), (2049, 33, 77), (130, 2048, 700)])
+                                          (48, 256, 32000), (1, 512, 5003), (1000, 96, 257), (300, 640, 1500), (2049, 33, 77), (130, 2048, 700), (4, 203, 70001), (8, 31, 300), (9, 1001, 2000),
+                                          (16, 130, 5000), (16, 4100, 64), (17, 203, 3000), (2, 3, 150000)])
 def test_against_64_bits(t, rows, width, v):
     _check(*_case(t, rows, width, v))
 
@@ -278,4 +279,6 @@ def test_argument_validation_needs_no_device():
     # one piece of the gradient by the logits, however large the vocabulary
     assert 250e6 < need(2, 256, 8192, 64, 64, 256, 10 ** 7, 64, 1) < 300e6
     # a copy of weights that do not begin on a 16-byte boundary
-    assert need(2, 256, 4, 64, 64, 258, 10 ** 6, 64, 0) - need(2, 256, 4, 64, 64, 256, 10 ** 6, 64, 0) == 128 * 10 ** 6
+    assert need(2, 256, 40, 64, 64, 258, 10 ** 6, 64, 0) - need(2, 256, 40, 64, 64, 256, 10 ** 6, 64, 0) == 128 * 10 ** 6
+    # a few rows of fp32 take the weights as they lie
+    assert need(0, 260, 4, 64, 64, 260, 10 ** 6, 64, 0) < 10 ** 5
