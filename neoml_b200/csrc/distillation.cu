@@ -15,12 +15,12 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int THREADS = 256;
-constexpr int WARPS = THREADS / 32;
+constexpr int BLOCK = 256;     // threads of a row's block; a warp where the row and the teacher's entries are short
 constexpr int KEPT_MAX = NB200_DISTILLATION_KEPT_MAX;
 constexpr int MAX_PARTS = 8;
 constexpr int UNROLL = 4;      // units in flight per thread
-constexpr int ENTRIES = (KEPT_MAX + THREADS - 1) / THREADS; // of the teacher, per thread
+constexpr int ENTRIES = KEPT_MAX / BLOCK; // of the teacher, per thread
+static_assert(ENTRIES * BLOCK == KEPT_MAX, "every entry has a thread");
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 struct DistillParams {
@@ -79,7 +79,7 @@ struct Entry {
 	int at;     // column; -1 for one that is not used
 };
 
-template<typename T, typename P>
+template<typename T, typename P, int THREADS>
 __device__ __forceinline__ void load_entries(const DistillParams& p, int r, const T* logits, Entry (&entries)[ENTRIES])
 {
 	const P* const teacher = static_cast<const P*>(p.teacher) + static_cast<long long>(r) * p.kept;
@@ -114,9 +114,10 @@ __device__ __forceinline__ float unit_top(const uint4& raw)
 	}
 }
 
-template<typename T, typename P, int V>
+template<typename T, typename P, int V, int THREADS>
 __global__ void __launch_bounds__(THREADS) distillation_forward_kernel(const DistillParams p)
 {
+	constexpr int WARPS = THREADS / 32;
 	__shared__ Running parts[MAX_PARTS];
 	__shared__ Running warpsOf[WARPS];
 	__shared__ Taught taughtOf[WARPS];
@@ -133,7 +134,7 @@ __global__ void __launch_bounds__(THREADS) distillation_forward_kernel(const Dis
 	row.begin = x;                     // no element of another row is touched
 	row.end = x + p.vocabulary;
 	Entry entries[ENTRIES];
-	if(rank == 0) load_entries<T, P>(p, r, x, entries);
+	if(rank == 0) load_entries<T, P, THREADS>(p, r, x, entries);
 	Running mine = { -INFINITY, 0.f };
 	for(int u0 = rank * perBlock; u0 < end; u0 += THREADS * UNROLL) {
 		uint4 raw[UNROLL];
@@ -220,11 +221,12 @@ __global__ void __launch_bounds__(THREADS) distillation_forward_kernel(const Dis
 		: p.temperature * p.temperature * (taught.cross / taught.sum - logf(taught.sum) + logSum);
 }
 
-template<typename T, typename P, int V>
+template<typename T, typename P, int V, int THREADS>
 __global__ void __launch_bounds__(THREADS) distillation_backward_kernel(const DistillParams p)
 {
-	__shared__ int keptAt[KEPT_MAX];
-	__shared__ float keptX[KEPT_MAX];
+	constexpr int WARPS = THREADS / 32;
+	__shared__ int keptAt[ENTRIES * THREADS];
+	__shared__ float keptX[ENTRIES * THREADS];
 	__shared__ Running warpsOf[WARPS];
 	const int blocks = p.parts, r = blockIdx.x / blocks, rank = blockIdx.x - r * blocks;
 	const T* const x = static_cast<const T*>(p.logits) + r * p.row;
@@ -236,7 +238,7 @@ __global__ void __launch_bounds__(THREADS) distillation_backward_kernel(const Di
 	const float c = LOG2E / p.temperature;
 	// the student's kept logits are read here, before anything is written: the gradient may replace the logits
 	Entry entries[ENTRIES];
-	load_entries<T, P>(p, r, x, entries);
+	load_entries<T, P, THREADS>(p, r, x, entries);
 	Running teacher = { -INFINITY, 0.f };
 #pragma unroll
 	for(int e = 0; e < ENTRIES; ++e) {
@@ -314,7 +316,7 @@ int parts_of(int type, int rows, int vocabulary)
 {
 	const int units = (vocabulary + 16 / type_size(type) - 1) / (16 / type_size(type));
 	int parts = 1;
-	while(parts < MAX_PARTS && static_cast<long long>(rows) * parts < sm_count() * 2 && units > parts * THREADS) parts *= 2;
+	while(parts < MAX_PARTS && static_cast<long long>(rows) * parts < sm_count() * 2 && units > parts * BLOCK) parts *= 2;
 	return parts;
 }
 
@@ -322,7 +324,6 @@ int run(const DistillParams& p, int type, int teacherType, int rows, bool backwa
 {
 	cudaLaunchConfig_t config = {};
 	config.gridDim = dim3(static_cast<unsigned>(rows) * p.parts);
-	config.blockDim = dim3(THREADS);
 	config.stream = stream;
 	cudaLaunchAttribute attribute[1];
 	attribute[0].id = cudaLaunchAttributeClusterDimension;
@@ -331,13 +332,19 @@ int run(const DistillParams& p, int type, int teacherType, int rows, bool backwa
 	attribute[0].val.clusterDim.z = 1;
 	config.attrs = attribute;
 	config.numAttrs = p.parts > 1 && !backward ? 1 : 0;
+	// a warp per row: the loss of 8000 rows of 1000 bf16 took 41 us with blocks of 256 and takes 14, its gradient 50 and 13
+	const bool small = p.parts == 1 && p.kept <= ENTRIES * 32 && p.vocabulary <= 32 * 8 * (16 / type_size(type)) && rows >= sm_count();
+	config.blockDim = dim3(small ? 32 : BLOCK);
 	with_types(type, teacherType, [&](auto t, auto q) {
 		using T = decltype(t);
 		using P = decltype(q);
 		constexpr int V = Unit16<T>::N;
-		if(!backward) cudaLaunchKernelEx(&config, distillation_forward_kernel<T, P, V>, p);
-		else if(alike) cudaLaunchKernelEx(&config, distillation_backward_kernel<T, P, V>, p);
-		else cudaLaunchKernelEx(&config, distillation_backward_kernel<T, P, 1>, p);
+		if(!backward) cudaLaunchKernelEx(&config, small ? distillation_forward_kernel<T, P, V, 32> : distillation_forward_kernel<T, P, V, BLOCK>, p);
+		else if(alike) cudaLaunchKernelEx(&config, small ? distillation_backward_kernel<T, P, V, 32> : distillation_backward_kernel<T, P, V, BLOCK>, p);
+		else {
+			config.blockDim = dim3(BLOCK);
+			cudaLaunchKernelEx(&config, distillation_backward_kernel<T, P, 1, BLOCK>, p);
+		}
 	});
 	count_launch();
 	return check_launch();

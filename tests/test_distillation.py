@@ -69,7 +69,7 @@ def _check(z, top, index, tau, **kw):
 @pytest.mark.gpu
 @pytest.mark.parametrize("t", TYPES)
 @pytest.mark.parametrize("rows,v,k", [(1, 1, 1), (3, 2, 2), (5, 100, 7), (1, 50257, 64), (17, 32003, 100), (300, 1001, 33), (2, 4096, 1024),
-                                      (4, 130001, 256), (601, 513, 5)])
+                                      (4, 130001, 256), (601, 513, 5), (700, 2049, 128), (200, 1024, 129), (500, 3, 2)])
 def test_against_64_bits(t, rows, v, k):
     for seed, tau in ((1, 1.0), (2, 2.5)):
         _check(_made(t, rows, v, seed=seed), _made(t, rows, k, seed=seed + 10), _indices(rows, v, k, seed + 20), tau)
@@ -79,8 +79,9 @@ def test_against_64_bits(t, rows, v, k):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("t", TYPES)
-def test_unused_repeated_and_masked_entries(t):
-    rows, v, k = 40, 777, 12
+@pytest.mark.parametrize("rows", [40, 300])   # a block per row, a warp per row
+def test_unused_repeated_and_masked_entries(t, rows):
+    v, k = 777, 12
     z, top, index = _made(t, rows, v, seed=1), _made(t, rows, k, seed=2), _indices(rows, v, k, 3)
     index[0] = -1                        # a row without a teacher
     index[1, 3:] = v                     # behind the vocabulary: not used
@@ -116,8 +117,9 @@ def test_a_kept_column_that_the_student_excludes():
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("t", TYPES)
-def test_views_in_place_and_repeats(t):
-    rows, v, k = 37, 1003, 20
+@pytest.mark.parametrize("rows", [37, 411])
+def test_views_in_place_and_repeats(t, rows):
+    v, k = 1003, 20
     wide, top, index = _made(t, rows, v + 30, seed=1), _made(t, rows, k, seed=2), _indices(rows, v, k, 3)
     dloss = _made(torch.float32, rows, seed=4)
     for first in (0, 3, 8):
