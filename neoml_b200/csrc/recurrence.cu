@@ -849,7 +849,8 @@ int launch(int type, bool pair, bool backward, RecurrenceParams p, int batch, cu
 	StreamKernel stream_kernel = nullptr;
 	int depth = 0;
 	const int steps = !backward ? FORWARD_STEPS : input ? BACKWARD_INPUT_STEPS : BACKWARD_STEPS;
-	if(p.length >= 2 * warps * blocks * steps && make_maps(maps, type, backward, p, batch, steps)) {
+	// (their stores go by whole words; maps ask more of what is read)
+	if((pair || channelsPerLane == 1) && p.length >= 2 * warps * blocks * steps && make_maps(maps, type, backward, p, batch, steps)) {
 		stream_kernel = backward ? stream_for<true>(type, input) : stream_for<false>(type, input);
 		depth = backward ? (input ? BACKWARD_INPUT_DEPTH : BACKWARD_DEPTH) : (input ? FORWARD_INPUT_DEPTH : FORWARD_DEPTH);
 	}

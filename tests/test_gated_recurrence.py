@@ -1,5 +1,7 @@
 """GatedRecurrence and its backward pass against a step-by-step 64-bit recurrence, with bounds that follow each state's own
 rounding errors through time."""
+import ctypes
+
 import pytest
 import torch
 
@@ -243,6 +245,33 @@ def test_graph_stream_and_repeats():
     graph.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(x, y) for x, y in zip(got, step())) and not torch.equal(got[0], first[0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("gate", [False, True])
+def test_long_results_off_word_boundaries(t, gate):
+    """Long sequences whose operands are aligned and whose results begin one element further."""
+    b, n, c = 2, 2100, 64
+    z, f, i, h0, _ = _case(t, b, n, c, gate)
+    dh = _made(t, b, n, c, seed=7)
+
+    def off():
+        return torch.empty(b * n * c + 1, dtype=t, device="cuda")[1:].view(b, n, c)
+    h, last = ops.GatedRecurrence(z, f, i, initial_state=h0, result=off())
+    want = _reference(z, f, i, h0, None, dh, None)
+    _close(h, want["h"], "h")
+    _close(last, want["last"], "last")
+    h = h.clone()
+    dz, df, di, dh0 = off(), off(), off() if gate else None, torch.empty_like(h0)
+    desc = capi.RecurrenceDesc(b, n, c, *(n * c, c) * 3)
+    at = lambda x: None if x is None else x.data_ptr()  # noqa: E731
+    assert capi.load().nb200_gated_recurrence_backward(
+        torch.cuda.current_stream().cuda_stream, ops._TYPES[t], ctypes.byref(desc), at(dh), n * c, c, at(h), at(z), at(f), at(i), at(h0), None,
+        None, at(dz), at(df), at(di), at(dh0)) == capi.OK
+    for name, got in (("dz", dz), ("df", df), ("di", di), ("dh0", dh0)):
+        if got is not None:
+            _close(got, want[name], name)
 
 
 def test_refusals():
