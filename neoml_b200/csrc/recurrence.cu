@@ -368,8 +368,9 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, W == 1 ? 3 : 2) recurrence_for
 	for(int k = n + rank * warps + warp; k < p.length; k += blocks * warps) {
 		if(on) store_raw<T, W, SPLIT>(out + static_cast<long long>(k) * p.channels + c, all<W>(0.f), second);
 	}
-	if(on && p.last != nullptr && rank == 0 && warp == 0) store_state<W>(p.last, state0, carry, second);
 	if(blocks > 1) cg::this_cluster().sync(); // nobody leaves while its shared memory may be written
+	// behind it: the initial state, which all blocks read, may lie in the same place
+	if(on && p.last != nullptr && rank == 0 && warp == 0) store_state<W>(p.last, state0, carry, second);
 }
 
 // Time runs backwards: step k of a stretch is t - k.
@@ -513,8 +514,8 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 2) recurrence_backward_kernel(
 		outRound -= roundBytes;
 		t -= stride;
 	}
-	if(on && p.last != nullptr && rank == 0 && warp == 0) store_state<W>(p.last, state0, carry, second);
 	if(blocks > 1) cg::this_cluster().sync();
+	if(on && p.last != nullptr && rank == 0 && warp == 0) store_state<W>(p.last, state0, carry, second);
 }
 
 // ---- the same fed by TMA ----------------------------------------------------------------------------------------------
@@ -648,8 +649,9 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, S == 8 ? 3 : 2) recurrence_for
 	for(int k = n + rank * warps + warp; k < p.length; k += blocks * warps) {
 		if(on) store_raw<T, W, false>(out + static_cast<long long>(k) * p.channels + c, all<W>(0.f), 1);
 	}
-	if(on && p.last != nullptr && rank == 0 && warp == 0) store_state<W>(p.last, state0, carry, 1);
 	if(blocks > 1) cg::this_cluster().sync(); // nobody leaves while its shared memory may be written
+	// behind it: the initial state, which all blocks read, may lie in the same place
+	if(on && p.last != nullptr && rank == 0 && warp == 0) store_state<W>(p.last, state0, carry, 1);
 }
 
 template<typename T, int W, bool INPUT, int S, int DEPTH>
@@ -763,8 +765,8 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 2) recurrence_backward_stream_
 		ask(round + DEPTH);
 		outRound -= roundBytes;
 	}
-	if(on && p.last != nullptr && rank == 0 && warp == 0) store_state<W>(p.last, state0, carry, 1);
 	if(blocks > 1) cg::this_cluster().sync();
+	if(on && p.last != nullptr && rank == 0 && warp == 0) store_state<W>(p.last, state0, carry, 1);
 }
 
 using Kernel = void (*)(const RecurrenceParams);

@@ -192,6 +192,20 @@ def test_tokens_one_at_a_time(t, gate):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("n", [24, 300, 2100])
+def test_state_in_place_over_many_steps(t, n):
+    """Few channels: several blocks share a sequence and read the state that one of them replaces."""
+    b, c = 1, 64
+    z, f, i, h0, _ = _case(t, b, n, c, True)
+    want, last = ops.GatedRecurrence(z, f, i, initial_state=h0)
+    for _ in range(20):
+        state = h0.clone()
+        got, same = ops.GatedRecurrence(z, f, i, initial_state=state, final_state=state)
+        assert same is state and torch.equal(got, want) and torch.equal(state, last)
+
+
+@pytest.mark.gpu
 def test_extreme_gates():
     inf = float("inf")
     z = torch.full((1, 4, 3), 2.0, device="cuda")
