@@ -365,7 +365,7 @@ int nb200_distillation_loss(void* stream, int type, int teacher_type, const void
 	if(!arguments_valid(type, teacher_type, rows, vocabulary, row_size, kept, temperature)) return NB200_EINVAL;
 	if(rows == 0) return NB200_OK;
 	if(logits == nullptr || loss == nullptr || log_sum == nullptr || !type_aligned(logits, type)
-		|| !type_aligned(teacher_logits, teacher_type)) return NB200_EINVAL;
+		|| !type_aligned(teacher_logits, teacher_type) || !words_aligned(teacher_indices, loss, log_sum)) return NB200_EINVAL;
 	if(kept > 0 && (teacher_logits == nullptr || teacher_indices == nullptr)) return NB200_EINVAL;
 	if(kept > KEPT_MAX || vocabulary > (1 << 30)) return NB200_ETOOBIG;
 	if(device_status_word() == nullptr) return NB200_ENODEVICE;
@@ -385,7 +385,8 @@ int nb200_distillation_loss_backward(void* stream, int type, int teacher_type, c
 	}
 	if(rows == 0) return NB200_OK;
 	if(logits == nullptr || loss_diff == nullptr || log_sum == nullptr || logits_diff == nullptr || !type_aligned(logits, type)
-		|| !type_aligned(logits_diff, type) || !type_aligned(teacher_logits, teacher_type)) return NB200_EINVAL;
+		|| !type_aligned(logits_diff, type) || !type_aligned(teacher_logits, teacher_type)
+		|| !words_aligned(loss_diff, teacher_indices, log_sum)) return NB200_EINVAL;
 	if(kept > 0 && (teacher_logits == nullptr || teacher_indices == nullptr)) return NB200_EINVAL;
 	if(kept > KEPT_MAX || vocabulary > (1 << 30)) return NB200_ETOOBIG;
 	if(device_status_word() == nullptr) return NB200_ENODEVICE;

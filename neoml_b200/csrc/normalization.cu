@@ -864,7 +864,8 @@ int nb200_layer_normalization(void* stream, int type, int parameter_type, const 
 	if(height == 0) return NB200_OK;
 	if(height > (1 << 30) || width > (1 << 30)) return NB200_ETOOBIG;
 	if(x == nullptr || y == nullptr || !type_aligned(x, type) || !type_aligned(y, type)
-		|| !type_aligned(scale, parameter_type) || !type_aligned(free_term, parameter_type)) return NB200_EINVAL;
+		|| !type_aligned(scale, parameter_type) || !type_aligned(free_term, parameter_type)
+		|| !words_aligned(mean, inverse_deviation)) return NB200_EINVAL;
 	if(device_status_word() == nullptr) return NB200_ENODEVICE;
 	const Operand operands[] = { { x, x_row_size }, { y, y_row_size } };
 	const Shape s = shape_of(type, height, width, aligned_alike(type, height, operands, 2), all_aligned(type, height, operands, 2), true);
@@ -898,7 +899,7 @@ int nb200_layer_normalization_backward(void* stream, int type, int parameter_typ
 	}
 	const bool parameters = scale_diff != nullptr || free_term_diff != nullptr;
 	if(!type_aligned(scale, parameter_type) || !type_aligned(scale_diff, parameter_type)
-		|| !type_aligned(free_term_diff, parameter_type)) return NB200_EINVAL;
+		|| !type_aligned(free_term_diff, parameter_type) || !words_aligned(mean, inverse_deviation, scratch)) return NB200_EINVAL;
 	if(height > 0 && (x == nullptr || dy == nullptr || dx == nullptr || mean == nullptr || inverse_deviation == nullptr
 		|| !type_aligned(x, type) || !type_aligned(dy, type) || !type_aligned(dx, type)
 		|| (parameters && scratch == nullptr))) return NB200_EINVAL;

@@ -910,8 +910,6 @@ bool desc_valid(int type, const nb200_recurrence_desc* d)
 	return true;
 }
 
-bool floats_aligned(const float* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
-
 } // namespace
 
 } // namespace nb200
@@ -927,7 +925,7 @@ int nb200_gated_recurrence(void* stream, int type, const nb200_recurrence_desc* 
 	if(d->batch == 0 || d->channels == 0) return NB200_OK;
 	if(d->length > 0 && (update == nullptr || forget == nullptr || result == nullptr)) return NB200_EINVAL;
 	if(!type_aligned(update, type) || !type_aligned(forget, type) || !type_aligned(input, type) || !type_aligned(result, type)
-		|| !floats_aligned(initial_state) || !floats_aligned(final_state)) return NB200_EINVAL;
+		|| !words_aligned(initial_state, final_state, lengths)) return NB200_EINVAL;
 	if(d->batch > 65535 || d->length > (1 << 30)) return NB200_ETOOBIG;
 	if(device_status_word() == nullptr) return NB200_ENODEVICE;
 	RecurrenceParams p = {};
@@ -954,7 +952,7 @@ int nb200_gated_recurrence_backward(void* stream, int type, const nb200_recurren
 	for(const void* t : typed) {
 		if(!type_aligned(t, type)) return NB200_EINVAL;
 	}
-	if(!floats_aligned(initial_state) || !floats_aligned(final_state_diff) || !floats_aligned(initial_state_diff)) return NB200_EINVAL;
+	if(!words_aligned(initial_state, final_state_diff, lengths, initial_state_diff)) return NB200_EINVAL;
 	if(d->batch > 65535 || d->length > (1 << 30)) return NB200_ETOOBIG;
 	if(device_status_word() == nullptr) return NB200_ENODEVICE;
 	RecurrenceParams p = {};

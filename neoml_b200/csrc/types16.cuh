@@ -11,6 +11,8 @@ inline int type_size(int type) { return type == NB200_TYPE_FP32 ? 4 : 2; }
 inline bool type_valid(int type) { return type == NB200_TYPE_FP32 || type == NB200_TYPE_FP16 || type == NB200_TYPE_BF16; }
 // every address of a row-addressed operand is a multiple of its element's size
 inline bool type_aligned(const void* p, int type) { return (reinterpret_cast<uintptr_t>(p) & (type_size(type) - 1)) == 0; }
+// and so is that of fp32 and int32 vectors; null is one that is not given
+template<typename... P> bool words_aligned(const P*... p) { return ((reinterpret_cast<uintptr_t>(p) | ... | 0u) & 3u) == 0; }
 
 #ifdef __CUDACC__
 

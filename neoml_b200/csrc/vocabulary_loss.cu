@@ -614,7 +614,8 @@ int nb200_vocabulary_cross_entropy(void* stream, int type, const void* hidden, i
 	const Problem q = { type, rows, width, vocabulary, hidden, weights, hidden_row_size, weights_row_size };
 	if(!valid(q)) return NB200_EINVAL;
 	if(rows == 0) return NB200_OK;
-	if(hidden == nullptr || weights == nullptr || labels == nullptr || loss == nullptr || log_sum == nullptr || !scratch_valid(scratch)) return NB200_EINVAL;
+	if(hidden == nullptr || weights == nullptr || labels == nullptr || loss == nullptr || log_sum == nullptr || !scratch_valid(scratch)
+		|| !words_aligned(labels, loss, log_sum)) return NB200_EINVAL;
 	if(too_big(q)) return NB200_ETOOBIG;
 	if(device_status_word() == nullptr) return NB200_ENODEVICE;
 	return forward(q, labels, loss, log_sum, scratch, as_stream(stream));
@@ -630,7 +631,7 @@ int nb200_vocabulary_cross_entropy_backward(void* stream, int type, const float*
 		|| !type_aligned(hidden_diff, type) || !type_aligned(weights_diff, type)) return NB200_EINVAL;
 	if(hidden_diff == nullptr && weights_diff == nullptr) return NB200_OK;
 	if(rows > 0 && (hidden == nullptr || weights == nullptr || labels == nullptr || loss_diff == nullptr || log_sum == nullptr
-		|| !scratch_valid(scratch))) return NB200_EINVAL;
+		|| !scratch_valid(scratch) || !words_aligned(loss_diff, labels, log_sum))) return NB200_EINVAL;
 	if(too_big(q)) return NB200_ETOOBIG;
 	if(rows == 0 && weights_diff == nullptr) return NB200_OK;
 	if(device_status_word() == nullptr) return NB200_ENODEVICE;

@@ -203,3 +203,14 @@ def test_argument_validation_needs_no_device():
         bad = list(backward)
         bad[at] = value
         assert lib.nb200_distillation_loss_backward(*bad) == capi.EINVAL, (at, value)
+
+
+def test_vectors_off_word_boundaries_are_refused():
+    lib = capi.load()
+    calls = ((lib.nb200_distillation_loss, [None, 1, 1, 64, 4, 8, 8, 64, 64, 2, 1.0, 64, 64], (8, 11, 12)),
+             (lib.nb200_distillation_loss_backward, [None, 1, 1, 64, 64, 4, 8, 8, 64, 64, 2, 1.0, 64, 64, 8], (3, 9, 12)))
+    for function, good, places in calls:
+        for at in places:
+            bad = list(good)
+            bad[at] = 66
+            assert function(*bad) == capi.EINVAL, (function, at)

@@ -327,3 +327,15 @@ def test_argument_validation_needs_no_device():
         bad = list(backward)
         bad[at] = value
         assert lib.nb200_gated_recurrence_backward(*bad) == capi.EINVAL, (at, value)
+
+
+def test_vectors_off_word_boundaries_are_refused():
+    lib = capi.load()
+    desc = ctypes.byref(capi.RecurrenceDesc(2, 3, 4, 0, 0, 0, 0, 0, 0))
+    calls = ((lib.nb200_gated_recurrence, [None, 1, desc, 64, 64, None, None, None, 64, None], (6, 7, 9)),
+             (lib.nb200_gated_recurrence_backward, [None, 1, desc, 64, 0, 0, 64, 64, 64, None, None, None, None, 64, 64, None, None], (10, 11, 12, 16)))
+    for function, good, places in calls:
+        for at in places:
+            bad = list(good)
+            bad[at] = 66
+            assert function(*bad) == capi.EINVAL, (function, at)

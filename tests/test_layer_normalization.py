@@ -219,3 +219,14 @@ def test_argument_validation_needs_no_device():
         assert lib.nb200_layer_normalization_backward(*bad) == capi.EINVAL, (at, value)
     assert lib.nb200_layer_normalization_backward_scratch_floats(0, 0, 8) == 0
     assert lib.nb200_layer_normalization_backward_scratch_floats(0, 5, 8) >= 16
+
+
+def test_vectors_off_word_boundaries_are_refused():
+    lib = capi.load()
+    calls = ((lib.nb200_layer_normalization, [None, 1, 1, 64, 4, 8, 8, None, None, 1e-5, 64, 8, None, None], (12, 13)),
+             (lib.nb200_layer_normalization_backward, [None, 1, 1, 64, 8, 64, 4, 8, 8, None, 64, 64, 64, 8, 64, 64, 64], (10, 11, 16)))
+    for function, good, places in calls:
+        for at in places:
+            bad = list(good)
+            bad[at] = 66
+            assert function(*bad) == capi.EINVAL, (function, at)

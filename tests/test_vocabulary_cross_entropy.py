@@ -282,3 +282,14 @@ def test_argument_validation_needs_no_device():
     assert need(2, 256, 40, 64, 64, 258, 10 ** 6, 64, 0) - need(2, 256, 40, 64, 64, 256, 10 ** 6, 64, 0) == 128 * 10 ** 6
     # a few rows of fp32 take the weights as they lie
     assert need(0, 260, 4, 64, 64, 260, 10 ** 6, 64, 0) < 10 ** 5
+
+
+def test_vectors_off_word_boundaries_are_refused():
+    lib = capi.load()
+    calls = ((lib.nb200_vocabulary_cross_entropy, [None, 2, 64, 4, 8, 8, 64, 10, 8, 64, 64, 64, 256], (9, 10, 11)),
+             (lib.nb200_vocabulary_cross_entropy_backward, [None, 2, 64, 64, 4, 8, 8, 64, 10, 8, 64, 64, 64, 8, 64, 8, 256], (2, 10, 11)))
+    for function, good, places in calls:
+        for at in places:
+            bad = list(good)
+            bad[at] = 66
+            assert function(*bad) == capi.EINVAL, (function, at)
