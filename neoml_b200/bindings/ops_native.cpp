@@ -647,7 +647,7 @@ PyObject* vocabulary_cross_entropy(PyObject*, PyObject* const* a, Py_ssize_t cou
 	});
 }
 
-// loss_diff, hidden, weights, labels, log_sum, hidden_diff, weights_diff (True, False or a tensor)
+// loss_diff, hidden, weights, labels, log_sum, hidden_diff, weights_diff (True, a tensor, or False or None: not wanted)
 PyObject* vocabulary_cross_entropy_backward(PyObject*, PyObject* const* a, Py_ssize_t count)
 {
 	return guarded(count, 7, [&]() -> PyObject* {
@@ -658,12 +658,13 @@ PyObject* vocabulary_cross_entropy_backward(PyObject*, PyObject* const* a, Py_ss
 		at::Tensor dx, dw;
 		void *dxp = nullptr, *dwp = nullptr;
 		long long dxRow = 0, dwRow = 0;
-		if(a[5] != Py_False) {
+		const bool wantsX = a[5] != Py_False && a[5] != Py_None, wantsW = a[6] != Py_False && a[6] != Py_None;
+		if(wantsX) {
 			dx = empty_or(a[5] == Py_True ? Py_None : a[5], *h.x);
 			dxp = dx.data_ptr();
 			dxRow = matrix(dx).row;
 		}
-		if(a[6] != Py_False) {
+		if(wantsW) {
 			dw = empty_or(a[6] == Py_True ? Py_None : a[6], *h.w);
 			dwp = dw.data_ptr();
 			dwRow = matrix(dw).row;
@@ -676,7 +677,7 @@ PyObject* vocabulary_cross_entropy_backward(PyObject*, PyObject* const* a, Py_ss
 			return nb200_vocabulary_cross_entropy_backward(on.stream, h.type, diff, xp, h.m.height, h.m.width, h.m.row, wp, h.mw.height, h.mw.row,
 				h.labels, logSum, dxp, dxRow, dwp, dwRow, room);
 		});
-		return answers(rc, { a[5] != Py_False ? &dx : nullptr, a[6] != Py_False ? &dw : nullptr });
+		return answers(rc, { wantsX ? &dx : nullptr, wantsW ? &dw : nullptr });
 	});
 }
 

@@ -432,6 +432,7 @@ def _typed(t: torch.Tensor) -> int:
 
 def _device_of(*tensors) -> torch.device:
     """The one device that all of them (None left out) are on."""
+    assert not any(t is not None and t.is_neg() for t in tensors), "tensors that hold their own values, no negated views"
     devices = {t.device for t in tensors if t is not None}
     assert len(devices) == 1 and next(iter(devices)).type == "cuda", "tensors on one CUDA device only"
     return next(iter(devices))
@@ -674,8 +675,8 @@ def VocabularyCrossEntropy(hidden, weights, labels):
 
 def VocabularyCrossEntropyBackward(loss_diff, hidden, weights, labels, log_sum, *, hidden_diff=True, weights_diff=True):
     """The gradients of VocabularyCrossEntropy by hidden and weights, from that of each row's loss (fp32) and the forward
-    pass's log_sum.  hidden_diff and weights_diff: True for a new tensor, False where that gradient is not wanted (None comes
-    back), or the tensor to write.  Rows without a target have no gradient."""
+    pass's log_sum.  hidden_diff and weights_diff: True for a new tensor, the tensor to write, or False or None where that
+    gradient is not wanted (None comes back).  Rows without a target have no gradient."""
     done = _native().vocabulary_cross_entropy_backward(loss_diff, hidden, weights, labels, log_sum, hidden_diff, weights_diff)
     if done is not None:
         return _checked("VocabularyCrossEntropyBackward", done)
@@ -687,7 +688,8 @@ def VocabularyCrossEntropyBackward(loss_diff, hidden, weights, labels, log_sum, 
         diff = torch.empty(like.shape, dtype=like.dtype, device=device) if wanted is True else None if wanted is False else wanted
         diffs.append(diff)
         if diff is not None:
-            assert diff.shape == like.shape and diff.dtype == like.dtype and diff.device == device, "gradients like their operands"
+            assert diff.shape == like.shape and diff.dtype == like.dtype and diff.device == device and not diff.is_neg(), \
+                "gradients like their operands"
         places += (None, 0) if diff is None else (diff.data_ptr(), _matrix(diff)[2])
     with torch.cuda.device(device):
         scratch = _head_scratch(code, hidden, rows, width, row, weights, vocabulary, weights_row, True)

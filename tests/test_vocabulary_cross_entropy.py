@@ -293,3 +293,28 @@ def test_vectors_off_word_boundaries_are_refused():
             bad = list(good)
             bad[at] = 66
             assert function(*bad) == capi.EINVAL, (function, at)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", TYPES)
+def test_none_is_not_wanted(t):
+    x, w, labels = _case(t, 30, 24, 100)
+    dloss = _made(torch.float32, 30, seed=9)
+    _, log_sum = ops.VocabularyCrossEntropy(x, w, labels)
+    dx, dw = ops.VocabularyCrossEntropyBackward(dloss, x, w, labels, log_sum)
+    only, none = ops.VocabularyCrossEntropyBackward(dloss, x, w, labels, log_sum, weights_diff=None)
+    assert none is None and torch.equal(only, dx)
+    none, only = ops.VocabularyCrossEntropyBackward(dloss, x, w, labels, log_sum, hidden_diff=None)
+    assert none is None and torch.equal(only, dw)
+
+
+def test_negated_views_are_refused():
+    x, w, labels = torch.zeros(4, 8), torch.zeros(10, 8), torch.zeros(4, dtype=torch.int32)
+    with pytest.raises(AssertionError, match="negated"):
+        ops.VocabularyCrossEntropy(torch._neg_view(x), w, labels)
+    with pytest.raises(AssertionError, match="negated"):
+        ops.LayerNormalization(torch._neg_view(x))
+    with pytest.raises(AssertionError, match="negated"):
+        ops.GatedRecurrence(x[None], torch._neg_view(x[None]))
+    with pytest.raises(AssertionError, match="negated"):
+        ops.DistillationLoss(torch._neg_view(x), torch.zeros(4, 2), torch.zeros(4, 2, dtype=torch.int32))
