@@ -153,18 +153,18 @@ __global__ void __launch_bounds__(THREADS, 1) product16_kernel(const Product16Pa
 				uint64_t* const full = bars + B_FULL + s;
 				const uint32_t a = smemBase + s * STAGE_BYTES, b = a + A_BYTES;
 				mbar_arrive_expect_tx(full, STAGE_BYTES);
-				const int ka = p.akOffset + kb * BK, kbB = p.bkOffset + kb * BK;
+				const int k = kb * BK;
 				if constexpr(A_ACROSS) {
 #pragma unroll
-					for(int i = 0; i < BM / 64; ++i) tma_load_3d(a + i * 8192, &mapA, full, p.aOffset + t.m0 + i * 64, ka, planeA);
+					for(int i = 0; i < BM / 64; ++i) tma_load_3d(a + i * 8192, &mapA, full, t.m0 + i * 64, k, planeA);
 				} else {
-					tma_load_3d(a, &mapA, full, ka, p.aOffset + t.m0, planeA);
+					tma_load_3d(a, &mapA, full, k, t.m0, planeA);
 				}
 				if constexpr(B_ACROSS) {
 #pragma unroll
-					for(int i = 0; i < BN / 64; ++i) tma_load_3d(b + i * 8192, &mapB, full, p.bOffset + t.n0 + i * 64, kbB, planeB);
+					for(int i = 0; i < BN / 64; ++i) tma_load_3d(b + i * 8192, &mapB, full, t.n0 + i * 64, k, planeB);
 				} else {
-					tma_load_3d(b, &mapB, full, kbB, p.bOffset + t.n0, planeB);
+					tma_load_3d(b, &mapB, full, k, t.n0, planeB);
 				}
 				++it;
 				return true;

@@ -22,8 +22,6 @@ struct Product16Params {
 	int mTiles, nTiles, splits;
 	int kBlocks, kBlocksPerSplit;
 	int mFast;           // consecutive tiles go down the rows (A stays near) rather than along the columns
-	int aOffset, bOffset;   // added to the m and n coordinates of the loads
-	int akOffset, bkOffset; // and to their k coordinates
 	int bf16;            // operands are bf16 rather than fp16
 	int fp32;            // operands are three bf16 planes
 	int* status;
