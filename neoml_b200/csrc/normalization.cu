@@ -10,7 +10,8 @@
 // A row is cut into 16-byte units of memory, whatever its first address: the units at both ends hold elements of the
 // neighbouring rows too, which are left out of sums and stores (and a unit that would reach outside the matrix is read by
 // elements).  A block's rows are a multiple of a whole unit's elements apart, so that all of them have the same
-// alignment and a thread's columns never change.  This is why rows of odd width run at the same rate as even ones.
+// alignment and a thread's columns never change.  Loads and stores of rows of odd width are whole units too then; what bounds
+// those is the tests of every unit against the row's ends (16384 x 4096 bf16: 49 us forward, 5.5 TB/s; 40000 x 1031: 86 us, 1.9 TB/s).
 // Operands whose rows are aligned differently from one another (a view of some columns) take the form with units of one element.
 #include "types16.cuh"
 #include <atomic>

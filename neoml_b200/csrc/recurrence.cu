@@ -521,7 +521,7 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 2) recurrence_backward_kernel(
 // ---- the same fed by TMA ----------------------------------------------------------------------------------------------
 // Long sequences whose rows begin on 16-byte boundaries: a warp's stretches come as boxes of S steps x 128 bytes into a ring of its
 // own in shared memory, several rounds ahead, by one lane's instructions; steps and channels that do not exist come as zeros.  Loads into
-// registers are one round ahead at most, and that held the kernels above to 55 - 70 % of the memory's rate.  A ring needs no
+// registers are one round ahead at most: the kernels above take 1.1 to 1.5 times as long (launch()'s comment).  A ring needs no
 // barrier for free stages: its warp has read a stage when it asks for the next round in its place.
 
 struct Maps {
@@ -825,10 +825,11 @@ bool make_maps(Maps& maps, int type, bool backward, const RecurrenceParams& p, i
 }
 
 // How many warps and blocks share a sequence's time axis: the fewest that fill three quarters of the warps that the SMs hold
-// (16, or 24 in the kernels of fewer registers).  Blocks of four warps: 16 x 2048 x 2048 bf16 took 98 us in blocks of four, 102
-// in blocks of eight and 146 of two, in clusters of two (of four, eight) of the first 102 (109, 125); 64 x 100 x 4096 fp16, where a
-// warp per sequence is enough, 47 us in blocks of two and 63 of eight.  Where there are few channels (2 x 16384 x 2048) clusters
-// of eight blocks of four are fastest: 113 us, 159 in clusters of four, 477 without.
+// (16, or 24 in the kernels of fewer registers); up to four warps before more blocks, which exchange folds through the cluster.  Measured,
+// forward + backward by TMA: 16 x 2048 x 2048 bf16 73 + 141 us in blocks of four, 100 + 170 of two, 78 + 140 of eight, 80 + 144 in clusters of
+// two; 64 x 100 x 4096 fp16 39 + 57 in blocks of two, 60 + 94 of eight.  Where there are few channels (2 x 16384 x 2048 bf16) clusters of eight
+// blocks of four: 84 + 141, in clusters of four 116 + 199, without 352 + 617.  By loads into registers the three take 93 + 181, 43 + 77 and
+// 104 + 213 in the same shapes.
 int launch(int type, bool pair, bool backward, RecurrenceParams p, int batch, cudaStream_t stream)
 {
 	const bool input = p.i != nullptr;
