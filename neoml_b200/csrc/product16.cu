@@ -3,6 +3,7 @@
 //   warp 0      loads: tiles of A (128 x 64) and B (256 x 64) by TMA into a ring of four stages
 //   warp 1      issues the MMAs (128 x 256 x 16) into one of two accumulators of 256 tensor-memory columns
 //   warps 4-11  epilogue: two warps per lane quarter, 128 columns each, while the next tile is multiplied
+// NARROW: tiles of 64 columns, eight stages, 32 columns per epilogue warp, for products that have few tiles and no K to split.
 //
 // Operands whose m or n is adjacent in memory need no transposition: the tensor core reads them MN-major.  A box of 64 adjacent
 // indices x 64 k lands as 64 rows of 128 bytes; eight rows are a swizzle atom of 1024 bytes (stride byte offset), the next 64
@@ -22,16 +23,15 @@ namespace nb200 {
 
 namespace {
 
-constexpr int BM = PRODUCT16_M, BN = PRODUCT16_N, BK = PRODUCT16_K;
-constexpr int STAGES = 4;
-constexpr int A_BYTES = BM * BK * 2, B_BYTES = BN * BK * 2, STAGE_BYTES = A_BYTES + B_BYTES;
+constexpr int BM = PRODUCT16_M, BK = PRODUCT16_K;
+constexpr int RING_BYTES = 192 * 1024; // four stages, or eight narrow ones
+constexpr int A_BYTES = BM * BK * 2;
 constexpr int EPILOGUE_WARPS = 8;
 constexpr int THREADS = (4 + EPILOGUE_WARPS) * 32;
-constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 + 256;
+constexpr int SMEM_BYTES = RING_BYTES + 1024 + 256;
 constexpr int KERNEL_ID = 0x70;       // in the status word: (KERNEL_ID << 8) | site
 constexpr float LOG2E = 1.4426950408889634f;
 enum { SITE_LOAD = 1, SITE_MMA = 2, SITE_MMA_ACC = 3, SITE_EPILOGUE = 4 };
-enum { B_FULL = 0, B_EMPTY = STAGES, B_ACCFULL = 2 * STAGES, B_ACCEMPTY = 2 * STAGES + 2, B_DONE = 2 * STAGES + 4, BARS };
 
 __device__ __forceinline__ float exp2_fast(float x)
 {
@@ -80,6 +80,7 @@ struct Tile {
 	int m0, n0, mTile, nTile, split, kBegin, kEnd;
 };
 
+template<int BN>
 __device__ __forceinline__ Tile tile_of(const Product16Params& p, int tile)
 {
 	Tile t;
@@ -105,14 +106,18 @@ __device__ __forceinline__ uint32_t pack16(float a, float b, int bf16)
 	return bf16 ? pack2<__nv_bfloat16>(a, b) : pack2<__half>(a, b);
 }
 
-template<int EPILOGUE, bool A_ACROSS, bool B_ACROSS, bool FP32>
+template<int EPILOGUE, bool A_ACROSS, bool B_ACROSS, bool FP32, bool NARROW>
 __global__ void __launch_bounds__(THREADS, 1) product16_kernel(const Product16Params p, const __grid_constant__ CUtensorMap mapA,
 	const __grid_constant__ CUtensorMap mapB)
 {
 	constexpr int TERMS = FP32 ? 6 : 1;
+	constexpr int BN = NARROW ? PRODUCT16_NARROW : PRODUCT16_N, COLUMNS = BN / 2; // of a tile, and of an epilogue warp
+	constexpr int STAGE_BYTES = A_BYTES + BN * BK * 2, STAGES = RING_BYTES / STAGE_BYTES;
+	static_assert(STAGES * STAGE_BYTES == RING_BYTES && STAGE_BYTES % 1024 == 0, "stages fill the ring");
+	enum { B_FULL = 0, B_EMPTY = STAGES, B_ACCFULL = 2 * STAGES, B_ACCEMPTY = 2 * STAGES + 2, B_DONE = 2 * STAGES + 4, BARS };
 	extern __shared__ uint8_t smemRaw[];
 	uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smemRaw) + 1023) & ~static_cast<uintptr_t>(1023));
-	uint64_t* const bars = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE_BYTES);
+	uint64_t* const bars = reinterpret_cast<uint64_t*>(smem + RING_BYTES);
 	uint32_t* const tmemSlot = reinterpret_cast<uint32_t*>(bars + BARS);
 	volatile int* const abortFlag = reinterpret_cast<volatile int*>(tmemSlot + 1);
 	const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -152,17 +157,18 @@ __global__ void __launch_bounds__(THREADS, 1) product16_kernel(const Product16Pa
 				if(it >= STAGES && !mbar_wait_bounded(bars + B_EMPTY + s, (it / STAGES - 1) & 1, abortFlag, p.status, (KERNEL_ID << 8) | SITE_LOAD)) return false;
 				uint64_t* const full = bars + B_FULL + s;
 				const uint32_t a = smemBase + s * STAGE_BYTES, b = a + A_BYTES;
-				mbar_arrive_expect_tx(full, STAGE_BYTES);
+				// boxes and rows that nothing of the result needs are left out: what their place in the stage holds reaches no other row
+				// or column of the accumulator
+				const int boxesA = A_ACROSS ? min(BM / 64, (p.m - t.m0 + 63) / 64) : 1, boxesB = B_ACROSS ? min(BN / 64, (p.n - t.n0 + 63) / 64) : 1;
+				mbar_arrive_expect_tx(full, (A_ACROSS ? boxesA * 8192 : p.boxA * BK * 2) + (B_ACROSS ? boxesB * 8192 : BN * BK * 2));
 				const int k = kb * BK;
 				if constexpr(A_ACROSS) {
-#pragma unroll
-					for(int i = 0; i < BM / 64; ++i) tma_load_3d(a + i * 8192, &mapA, full, t.m0 + i * 64, k, planeA);
+					for(int i = 0; i < boxesA; ++i) tma_load_3d(a + i * 8192, &mapA, full, t.m0 + i * 64, k, planeA);
 				} else {
 					tma_load_3d(a, &mapA, full, k, t.m0, planeA);
 				}
 				if constexpr(B_ACROSS) {
-#pragma unroll
-					for(int i = 0; i < BN / 64; ++i) tma_load_3d(b + i * 8192, &mapB, full, t.n0 + i * 64, k, planeB);
+					for(int i = 0; i < boxesB; ++i) tma_load_3d(b + i * 8192, &mapB, full, t.n0 + i * 64, k, planeB);
 				} else {
 					tma_load_3d(b, &mapB, full, k, t.n0, planeB);
 				}
@@ -170,7 +176,7 @@ __global__ void __launch_bounds__(THREADS, 1) product16_kernel(const Product16Pa
 				return true;
 			};
 			for(int tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x) {
-				const Tile t = tile_of(p, tile);
+				const Tile t = tile_of<BN>(p, tile);
 				const int chunk = FP32 ? CHUNK : p.kBlocks;
 				for(int k0 = t.kBegin; ok && k0 < t.kEnd; k0 += chunk) {
 					const int k1 = min(t.kEnd, k0 + chunk);
@@ -194,7 +200,7 @@ __global__ void __launch_bounds__(THREADS, 1) product16_kernel(const Product16Pa
 			int it = 0, n = 0;
 			bool ok = true;
 			for(int tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x) {
-				const Tile t = tile_of(p, tile);
+				const Tile t = tile_of<BN>(p, tile);
 				const int chunk = FP32 ? CHUNK : p.kBlocks;
 				int k0 = t.kBegin;
 				do { // a part of K without steps takes its turn too
@@ -239,11 +245,11 @@ __global__ void __launch_bounds__(THREADS, 1) product16_kernel(const Product16Pa
 		int n = 0;
 		bool ok = true;
 		for(int tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x) {
-			const Tile t = tile_of(p, tile);
+			const Tile t = tile_of<BN>(p, tile);
 			const int row = t.m0 + quarter * 32 + lane;
 			const bool on = row < p.m;
-			const int col0 = t.n0 + half * 128;
-			const uint32_t tmemRow = tmemBase + (static_cast<uint32_t>(quarter * 32) << 16) + half * 128;
+			const int col0 = t.n0 + half * COLUMNS;
+			const uint32_t tmemRow = tmemBase + (static_cast<uint32_t>(quarter * 32) << 16) + half * COLUMNS;
 			int label = -1;
 			float logSum2 = 0.f, by = 0.f;
 			if(on && (EPILOGUE == PRODUCT16_STATS || EPILOGUE == PRODUCT16_DIFF)) {
@@ -401,7 +407,7 @@ __global__ void __launch_bounds__(THREADS, 1) product16_kernel(const Product16Pa
 			};
 			const bool empty = t.kBegin >= t.kEnd; // a part of K without steps: nothing was multiplied
 			if constexpr(FP32) {
-				float total[4][32];
+				float total[COLUMNS / 32][32];
 				int k0 = t.kBegin;
 				do {
 					const int acc = n & 1;
@@ -409,7 +415,7 @@ __global__ void __launch_bounds__(THREADS, 1) product16_kernel(const Product16Pa
 					if(!ok) break;
 					tc_fence_after_sync();
 #pragma unroll
-					for(int c = 0; c < 4; ++c) {
+					for(int c = 0; c < COLUMNS / 32; ++c) {
 						uint32_t r[32];
 						tmem_ld32_issue(tmemRow + acc * BN + c * 32, r);
 						tmem_ld_wait();
@@ -423,7 +429,7 @@ __global__ void __launch_bounds__(THREADS, 1) product16_kernel(const Product16Pa
 				} while(k0 < t.kEnd);
 				if(!ok) break;
 #pragma unroll
-				for(int c = 0; c < 4; ++c) finish(c * 32, total[c]);
+				for(int c = 0; c < COLUMNS / 32; ++c) finish(c * 32, total[c]);
 			} else {
 				const int acc = n & 1;
 				ok = mbar_wait_bounded_warp(bars + B_ACCFULL + acc, (n >> 1) & 1, abortFlag, p.status, (KERNEL_ID << 8) | SITE_EPILOGUE);
@@ -431,11 +437,11 @@ __global__ void __launch_bounds__(THREADS, 1) product16_kernel(const Product16Pa
 				++n;
 				tc_fence_after_sync();
 #pragma unroll 1
-				for(int c = 0; c < 128; c += 32) {
+				for(int c = 0; c < COLUMNS; c += 32) {
 					uint32_t r[32];
 					tmem_ld32_issue(tmemRow + acc * BN + c, r);
 					tmem_ld_wait();
-					if(c == 96) { // the accumulator is free
+					if(c == COLUMNS - 32) { // the accumulator is free
 						tc_fence_before_sync();
 						if(lane == 0) mbar_arrive(bars + B_ACCEMPTY + acc);
 					}
@@ -475,6 +481,13 @@ EncodeTiledFn encoder()
 
 using Kernel = void (*)(const Product16Params, const CUtensorMap, const CUtensorMap);
 
+template<int EPILOGUE>
+Kernel rows_kernel(const Product16Params& p)
+{
+	if(p.narrow) return p.fp32 ? product16_kernel<EPILOGUE, false, false, true, true> : product16_kernel<EPILOGUE, false, false, false, true>;
+	return p.fp32 ? product16_kernel<EPILOGUE, false, false, true, false> : product16_kernel<EPILOGUE, false, false, false, false>;
+}
+
 } // namespace
 
 bool product16_map(void* map, const void* base, bool bf16, long long inner, long long rows, long long rowSize, int boxRows, long long planeSize)
@@ -510,11 +523,11 @@ int product16(Product16Epilogue epilogue, bool aAcross, bool bAcross, const Prod
 	cudaStream_t stream)
 {
 	Kernel kernel = nullptr;
-	if(epilogue == PRODUCT16_STATS && !aAcross && !bAcross) kernel = p.fp32 ? product16_kernel<PRODUCT16_STATS, false, false, true> : product16_kernel<PRODUCT16_STATS, false, false, false>;
-	else if(epilogue == PRODUCT16_DIFF && !aAcross && !bAcross) kernel = p.fp32 ? product16_kernel<PRODUCT16_DIFF, false, false, true> : product16_kernel<PRODUCT16_DIFF, false, false, false>;
-	else if(epilogue == PRODUCT16_SUM && !aAcross && bAcross) kernel = p.fp32 ? product16_kernel<PRODUCT16_SUM, false, true, true> : product16_kernel<PRODUCT16_SUM, false, true, false>;
-	else if(epilogue == PRODUCT16_SUM && aAcross && bAcross) kernel = p.fp32 ? product16_kernel<PRODUCT16_SUM, true, true, true> : product16_kernel<PRODUCT16_SUM, true, true, false>;
-	else if(epilogue == PRODUCT16_STORE && aAcross && bAcross) kernel = p.fp32 ? product16_kernel<PRODUCT16_STORE, true, true, true> : product16_kernel<PRODUCT16_STORE, true, true, false>;
+	if(epilogue == PRODUCT16_STATS && !aAcross && !bAcross) kernel = rows_kernel<PRODUCT16_STATS>(p);
+	else if(epilogue == PRODUCT16_DIFF && !aAcross && !bAcross) kernel = rows_kernel<PRODUCT16_DIFF>(p);
+	else if(epilogue == PRODUCT16_SUM && !aAcross && bAcross && !p.narrow) kernel = p.fp32 ? product16_kernel<PRODUCT16_SUM, false, true, true, false> : product16_kernel<PRODUCT16_SUM, false, true, false, false>;
+	else if(epilogue == PRODUCT16_SUM && aAcross && bAcross && !p.narrow) kernel = p.fp32 ? product16_kernel<PRODUCT16_SUM, true, true, true, false> : product16_kernel<PRODUCT16_SUM, true, true, false, false>;
+	else if(epilogue == PRODUCT16_STORE && aAcross && bAcross && !p.narrow) kernel = p.fp32 ? product16_kernel<PRODUCT16_STORE, true, true, true, false> : product16_kernel<PRODUCT16_STORE, true, true, false, false>;
 	else return NB200_EINVAL;
 	const long long tiles = static_cast<long long>(p.mTiles) * p.nTiles * p.splits;
 	if(tiles > 0x7fffffffLL - 1024) return NB200_ETOOBIG;

@@ -11,7 +11,7 @@
 namespace nb200 {
 
 enum Product16Epilogue {
-	PRODUCT16_STATS, // per row and 128 columns: maximum and sum of exponentials, and the labelled column's value
+	PRODUCT16_STATS, // per row and half a tile of columns: maximum and sum of exponentials, and the labelled column's value
 	PRODUCT16_DIFF,  // gradient by the logits, 16-bit or three planes: coefficient[row] * (softmax - [column is the label])
 	PRODUCT16_SUM,   // fp32 planes, one per part of K; added to what is there where `accumulate` is set
 	PRODUCT16_STORE  // result times *resultScale, of the operands' type
@@ -21,6 +21,8 @@ struct Product16Params {
 	int m, n;            // rows and columns of the result
 	int mTiles, nTiles, splits;
 	int kBlocks, kBlocksPerSplit;
+	int narrow;          // tiles of PRODUCT16_NARROW columns, B's box likewise: STATS and DIFF
+	int boxA;            // rows of A's box where A lies in rows: product16_box_a(m)
 	int mFast;           // consecutive tiles go down the rows (A stays near) rather than along the columns
 	int bf16;            // operands are bf16 rather than fp16
 	int fp32;            // operands are three bf16 planes
@@ -62,7 +64,9 @@ bool product16_map(void* map, const void* base, bool bf16, long long inner, long
 bool sequence_map(void* map, const void* base, int type, long long channels, long long length, long long batch, long long row,
 	long long batchStride, int steps);
 
-constexpr int PRODUCT16_M = 128, PRODUCT16_N = 256, PRODUCT16_K = 64; // of a tile
-constexpr int PRODUCT16_BOX_A = 128, PRODUCT16_BOX_B = 256, PRODUCT16_BOX_ACROSS = 64; // boxRows of the operands' maps
+constexpr int PRODUCT16_M = 128, PRODUCT16_N = 256, PRODUCT16_NARROW = 64, PRODUCT16_K = 64; // of a tile
+// boxRows of the operands' maps: across, and in rows; of B in rows the tile's columns
+constexpr int PRODUCT16_BOX_ACROSS = 64;
+inline int product16_box_a(int m) { return m >= PRODUCT16_M ? PRODUCT16_M : (m + 7) / 8 * 8; } // no more rows than there are
 
 } // namespace nb200

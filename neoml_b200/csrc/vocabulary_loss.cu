@@ -169,33 +169,46 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) join_partials_kernel(const fl
 	}
 }
 
-// out[row][col] = sum of the planes, in order, times *by
+// out[row][col] = sum of the planes times *by: `group` neighbouring threads (1 or 8) share four columns, each adds every group-th plane in
+// order, and their sums meet in a tree.
 template<typename T>
 __global__ void __launch_bounds__(256) sum_planes_kernel(const float* __restrict__ planes, int count, long long planeSize, long long ldPlane,
-	int rows, int width, const float* __restrict__ by, T* __restrict__ out, long long outRow)
+	int rows, int width, int group, const float* __restrict__ by, T* __restrict__ out, long long outRow)
 {
 	dependent_wait();
 	const float scale = __ldg(by);
+	const int member = threadIdx.x & (group - 1);
 	const int quads = (width + 3) / 4;
 	const bool vector = (outRow & 3) == 0 && (reinterpret_cast<uintptr_t>(out) & 7u) == 0;
 	const long long total = static_cast<long long>(rows) * quads;
-	const long long step = static_cast<long long>(gridDim.x) * blockDim.x;
-	for(long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += step) {
+	const long long step = static_cast<long long>(gridDim.x) * blockDim.x / group;
+	for(long long i = (static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) / group; i < total; i += step) {
 		const long long row = i / quads;
 		const int col = static_cast<int>(i - row * quads) * 4;
 		float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 		constexpr int AHEAD = 8;
-		for(int k = 0; k < count; k += AHEAD) {
+		for(int k = member; k < count; k += AHEAD * group) {
 			float4 w[AHEAD];
 #pragma unroll
 			for(int j = 0; j < AHEAD; ++j) {
 				w[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-				if(k + j < count) w[j] = *reinterpret_cast<const float4*>(planes + (k + j) * planeSize + row * ldPlane + col);
+				if(k + j * group < count) w[j] = *reinterpret_cast<const float4*>(planes + (k + j * group) * planeSize + row * ldPlane + col);
 			}
 #pragma unroll
 			for(int j = 0; j < AHEAD; ++j) {
 				v.x += w[j].x; v.y += w[j].y; v.z += w[j].z; v.w += w[j].w;
 			}
+		}
+		if(group > 1) {
+			const unsigned mask = 0xffu << (threadIdx.x & 24u); // the eight of them
+#pragma unroll
+			for(int o = 4; o > 0; o >>= 1) {
+				v.x += __shfl_xor_sync(mask, v.x, o);
+				v.y += __shfl_xor_sync(mask, v.y, o);
+				v.z += __shfl_xor_sync(mask, v.z, o);
+				v.w += __shfl_xor_sync(mask, v.w, o);
+			}
+			if(member != 0) continue;
 		}
 		T* const to = out + row * outRow + col;
 		if constexpr(sizeof(T) == 4) {
@@ -314,16 +327,26 @@ int piece_of(const Problem& q, bool backward)
 	return round_up((whole + pieces - 1) / pieces, PRODUCT16_N);
 }
 
-// Parts of K where a product has few tiles: enough for one tile per SM, none shorter than 8 steps of 64.
+// Parts of K where a product has few tiles: enough for one tile per SM, none shorter than 8 steps of 64.  (26 x 207 fp32 by 78703: 34 us in 148
+// parts, 52 in 64.)
 int splits_of(long long tiles, int kBlocks)
 {
 	const int sms = sm_count();
 	if(tiles * 2 > sms) return 1;
 	long long splits = sms / tiles;
 	if(splits > kBlocks / 8) splits = kBlocks / 8;
-	if(splits > 64) splits = 64;
 	return splits < 1 ? 1 : static_cast<int>(splits);
 }
+
+// Tiles of 64 columns for the products with the weights' rows where all of them find an SM at once: a step of such a tile takes two thirds
+// of one of 256 columns (59 x 3596 fp32 rows over 6319 entries, 99 tiles: 76 us against 137 with 25; 11 x 334 over 16431, 257 tiles in two
+// rounds: 36 us against 23 with 65).
+bool narrow(const Problem& q, int piece)
+{
+	const long long columns = q.vocabulary < piece ? q.vocabulary : piece;
+	return static_cast<long long>((q.rows + PRODUCT16_M - 1) / PRODUCT16_M) * ((columns + PRODUCT16_NARROW - 1) / PRODUCT16_NARROW) <= sm_count();
+}
+int tile_columns(bool narrow) { return narrow ? PRODUCT16_NARROW : PRODUCT16_N; }
 
 // An operand as TMA takes it: where it lies, and how far its rows and planes are apart.
 struct Aligned {
@@ -348,7 +371,7 @@ struct FewRoom {
 };
 
 struct Forward {
-	int piece;
+	int piece, tileColumns, parts; // parts: of a row's sums
 	float2* partial;
 	float* labelled;
 	uint16_t *hidden, *weights; // copies in aligned rows, or planes; null: as they are
@@ -357,8 +380,9 @@ struct Forward {
 		const bool fp32 = q.type == NB200_TYPE_FP32;
 		const size_t ld = round_up(q.width, 8);
 		piece = piece_of(q, false);
-		const int nTiles = (q.vocabulary + PRODUCT16_N - 1) / PRODUCT16_N;
-		partial = room.take<float2>(static_cast<size_t>(nTiles) * 2 * q.rows);
+		tileColumns = tile_columns(narrow(q, piece));
+		parts = (q.vocabulary + tileColumns - 1) / tileColumns * 2;
+		partial = room.take<float2>(static_cast<size_t>(parts) * q.rows);
 		labelled = room.take<float>(q.rows);
 		hidden = fp32 ? room.take<uint16_t>(3 * q.rows * ld) : rows_for_tma(q.hidden, q.hiddenRow) ? nullptr : room.take<uint16_t>(q.rows * ld);
 		weights = fp32 ? room.take<uint16_t>(3 * piece * ld) : rows_for_tma(q.weights, q.weightsRow) ? nullptr : room.take<uint16_t>(q.vocabulary * ld);
@@ -366,7 +390,7 @@ struct Forward {
 };
 
 struct Backward {
-	int piece, hiddenSplits, weightsSplits;
+	int piece, tileColumns, hiddenSplits, weightsSplits;
 	float* scale;
 	uint16_t *hidden, *weights, *diff;
 	float *hiddenPlanes, *weightsPlanes;
@@ -376,6 +400,7 @@ struct Backward {
 		const bool fp32 = q.type == NB200_TYPE_FP32;
 		const size_t ld = round_up(q.width, 8), planes = fp32 ? 3 : 1;
 		piece = piece_of(q, true);
+		tileColumns = tile_columns(narrow(q, piece));
 		const long long mTiles = (q.rows + PRODUCT16_M - 1) / PRODUCT16_M, dTiles = (q.width + PRODUCT16_N - 1) / PRODUCT16_N;
 		hiddenSplits = splits_of(mTiles * dTiles, piece / PRODUCT16_K);
 		// its result goes straight to the caller where K is not split
@@ -435,12 +460,14 @@ Aligned weights_piece(const Problem& q, uint16_t* room, int first, int columns, 
 	return { all + first * row, row, 0 };
 }
 
-Product16Params params_of(const Problem& q, int m, int n, int splits, int k, bool mFast)
+Product16Params params_of(const Problem& q, int m, int n, int splits, int k, bool mFast, int tileColumns = PRODUCT16_N)
 {
 	Product16Params p = {};
 	p.m = m; p.n = n;
 	p.mTiles = (m + PRODUCT16_M - 1) / PRODUCT16_M;
-	p.nTiles = (n + PRODUCT16_N - 1) / PRODUCT16_N;
+	p.nTiles = (n + tileColumns - 1) / tileColumns;
+	p.narrow = tileColumns == PRODUCT16_N ? 0 : 1;
+	p.boxA = product16_box_a(m);
 	p.splits = splits;
 	p.kBlocks = (k + PRODUCT16_K - 1) / PRODUCT16_K;
 	p.kBlocksPerSplit = (p.kBlocks + splits - 1) / splits;
@@ -487,18 +514,18 @@ int forward(const Problem& q, const int* labels, float* loss, float* logSum, voi
 	else if(f.hidden != nullptr) copy_rows(q.hidden, q.hiddenRow, q.rows, q.width, f.hidden, nullptr, nullptr, 0, stream);
 	if(!fp32 && f.weights != nullptr) copy_rows(q.weights, q.weightsRow, q.vocabulary, q.width, f.weights, nullptr, nullptr, 0, stream);
 	CUtensorMap a, b;
-	if(!product16_map(&a, f.hidden ? f.hidden : q.hidden, bf16, q.width, q.rows, f.hidden ? ld : q.hiddenRow, PRODUCT16_BOX_A, fp32 ? q.rows * ld : 0)) return NB200_EINVAL;
+	if(!product16_map(&a, f.hidden ? f.hidden : q.hidden, bf16, q.width, q.rows, f.hidden ? ld : q.hiddenRow, product16_box_a(q.rows), fp32 ? q.rows * ld : 0)) return NB200_EINVAL;
 	for(int first = 0; first < q.vocabulary; first += f.piece) {
 		const int columns = q.vocabulary - first < f.piece ? q.vocabulary - first : f.piece;
 		const Aligned w = weights_piece(q, f.weights, first, columns, f.piece, stream);
-		if(!product16_map(&b, w.p, bf16, q.width, columns, w.row, PRODUCT16_BOX_B, w.plane)) return NB200_EINVAL;
-		Product16Params p = params_of(q, q.rows, columns, 1, q.width, true);
-		p.partial = f.partial + static_cast<long long>(first / PRODUCT16_N) * 2 * q.rows;
+		if(!product16_map(&b, w.p, bf16, q.width, columns, w.row, f.tileColumns, w.plane)) return NB200_EINVAL;
+		Product16Params p = params_of(q, q.rows, columns, 1, q.width, true, f.tileColumns);
+		p.partial = f.partial + static_cast<long long>(first / f.tileColumns) * 2 * q.rows;
 		p.labelled = f.labelled; p.labels = labels; p.firstColumn = first; p.columns = q.vocabulary;
 		const int rc = product16(PRODUCT16_STATS, false, false, p, &a, &b, stream);
 		if(rc != NB200_OK) return rc;
 	}
-	join_partials(q, f.partial, (q.vocabulary + PRODUCT16_N - 1) / PRODUCT16_N * 2, f.labelled, labels, loss, logSum, stream);
+	join_partials(q, f.partial, f.parts, f.labelled, labels, loss, logSum, stream);
 	return check_launch();
 }
 
@@ -506,8 +533,11 @@ template<typename T>
 void sum_planes_of(const Problem& q, const float* planes, int count, int rows, const float* by, void* out, long long outRow, cudaStream_t stream)
 {
 	const long long ld = round_up(q.width, 8);
-	const dim3 grid(grid_for(static_cast<long long>(rows) * ((q.width + 3) / 4), 256, 16));
-	launch_dependent(true, sum_planes_kernel<T>, grid, dim3(256), 0, stream, planes, count, rows * ld, ld, rows, q.width, by, static_cast<T*>(out), outRow);
+	const long long quads = static_cast<long long>(rows) * ((q.width + 3) / 4);
+	// few results of many planes: 11 x 334 of 64 planes took 11 us with one thread, 4.5 with eight
+	const int group = count > 8 && quads * 8 <= sm_count() * 2048ll ? 8 : 1;
+	const dim3 grid(grid_for(quads * group, 256, 16));
+	launch_dependent(true, sum_planes_kernel<T>, grid, dim3(256), 0, stream, planes, count, rows * ld, ld, rows, q.width, group, by, static_cast<T*>(out), outRow);
 	count_launch();
 }
 void sum_planes(const Problem& q, const float* planes, int count, int rows, const float* by, void* out, long long outRow, cudaStream_t stream)
@@ -538,23 +568,23 @@ int backward(const Problem& q, const float* lossDiff, const int* labels, const f
 	count_launch();
 	if(!fp32 && w.weights != nullptr) copy_rows(q.weights, q.weightsRow, q.vocabulary, q.width, w.weights, nullptr, nullptr, 0, stream);
 	CUtensorMap hidden, hiddenAcross, rows, across, diff, diffAcross;
-	if(!product16_map(&hidden, w.hidden, bf16, q.width, q.rows, ld, PRODUCT16_BOX_A, hiddenPlane)
+	if(!product16_map(&hidden, w.hidden, bf16, q.width, q.rows, ld, product16_box_a(q.rows), hiddenPlane)
 		|| !product16_map(&hiddenAcross, w.hidden, bf16, q.width, q.rows, ld, PRODUCT16_BOX_ACROSS, hiddenPlane)
-		|| !product16_map(&diff, w.diff, bf16, w.piece, q.rows, w.piece, PRODUCT16_BOX_A, diffPlane)
+		|| !product16_map(&diff, w.diff, bf16, w.piece, q.rows, w.piece, product16_box_a(q.rows), diffPlane)
 		|| !product16_map(&diffAcross, w.diff, bf16, w.piece, q.rows, w.piece, PRODUCT16_BOX_ACROSS, diffPlane)) return NB200_EINVAL;
 	for(int first = 0; first < q.vocabulary; first += w.piece) {
 		const int columns = q.vocabulary - first < w.piece ? q.vocabulary - first : w.piece;
 		const Aligned piece = weights_piece(q, w.weights, first, columns, w.piece, stream);
-		if(!product16_map(&rows, piece.p, bf16, q.width, columns, piece.row, PRODUCT16_BOX_B, piece.plane)
+		if(!product16_map(&rows, piece.p, bf16, q.width, columns, piece.row, w.tileColumns, piece.plane)
 			|| !product16_map(&across, piece.p, bf16, q.width, columns, piece.row, PRODUCT16_BOX_ACROSS, piece.plane)) return NB200_EINVAL;
-		Product16Params p = params_of(q, q.rows, columns, 1, q.width, true);
+		Product16Params p = params_of(q, q.rows, columns, 1, q.width, true, w.tileColumns);
 		p.labels = labels; p.firstColumn = first; p.columns = q.vocabulary;
 		p.logSum = logSum; p.rowScale = lossDiff; p.scale = w.scale;
 		p.out = w.diff; p.ldOut = w.piece; p.outPlane = diffPlane;
 		int rc = product16(PRODUCT16_DIFF, false, false, p, &hidden, &rows, stream);
 		if(rc != NB200_OK) return rc;
 		if(hiddenDiff != nullptr) {
-			// dz ends in zeros behind the vocabulary, up to a whole tile's columns
+			// dz ends in zeros behind the vocabulary, up to whole K blocks
 			p = params_of(q, q.rows, q.width, w.hiddenSplits, columns, false);
 			p.plane = w.hiddenPlanes; p.ldPlane = ld; p.accumulate = first > 0;
 			rc = product16(PRODUCT16_SUM, false, true, p, &diff, &across, stream);
