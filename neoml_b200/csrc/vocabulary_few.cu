@@ -1,4 +1,5 @@
-// The cross entropy over a vocabulary for up to eight rows of fp32: a token or a few of each text that is scored or decoded.
+// The cross entropy over a vocabulary for up to eight rows of fp32 (its loss for up to 32): a token or a few of each text that is scored or
+// decoded.
 //
 // The weights are then read for less arithmetic than reading them takes; what counts is that they come once, as they lie, without the
 // planes that the tensor core wants of fp32 (vocabulary_loss.cu), and that nothing but fp32 multiply-adds stands between.  A block has
@@ -294,10 +295,162 @@ __global__ void __launch_bounds__(256) few_hidden_kernel(const FewParams p, int 
 	out[t * outRow + c] = s;
 }
 
+// ---- nine to 32 rows, forward --------------------------------------------------------------------------------------------
+// A tile is 128 entries and all the rows.  A warp has eight rows and every KS-th stretch of the elements, a lane four entries 32 apart:
+// 32 sums, each of an even and an odd half that one paired multiply-add serves.  Four elements take four 16-byte loads of weights, eight of
+// rows (which all lanes share) and 64 paired multiply-adds.  Chunks of 32 elements come by asynchronous copies, two ahead, V elements
+// each; 36 words from row to row keep 16-byte loads free of conflicts.  The KS warps' sums meet in shared memory, each warp ends some of the rows.
+//   One block per SM: 16 x 4096 rows over 50257 entries 306 us (2.7 TB/s; by planes 667), 16 x 1024 over 32000 58 us (110), 32 x 1024 84 (111);
+// with two blocks per SM 407, 61 and 87.  Widths that are odd come by 4-byte copies: 16 x 1861 over 66524 307 us, 1862 222 (419 by planes).
+constexpr int GROUP_ROWS = 8, GROUP_TILE = 128, GROUP_CHUNK = 32, GROUP_PITCH = GROUP_CHUNK + 4, GROUP_STAGES = 3;
+
+template<int G, int KS>
+struct GroupRoom {
+	struct {
+		float weights[GROUP_TILE * GROUP_PITCH];
+		float hidden[GROUP_ROWS * G * GROUP_PITCH];
+	} stages[GROUP_STAGES];
+	float logits[KS][GROUP_ROWS * G][GROUP_TILE];
+};
+
+template<int V>
+__device__ __forceinline__ void copy_words(float* to, const float* from, bool there) // zeros where it is not
+{
+	if constexpr(V < 4) asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(smem_u32(to)), "l"(from), "r"(there ? 4 * V : 0), "n"(4 * V) : "memory");
+	else asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(to)), "l"(from), "r"(there ? 16 : 0) : "memory");
+}
+
+template<int G, int KS, int V>
+__global__ void __launch_bounds__(G * KS * 32) group_forward_kernel(const FewParams p)
+{
+	extern __shared__ __align__(16) uint8_t room[];
+	GroupRoom<G, KS>& s = *reinterpret_cast<GroupRoom<G, KS>*>(room);
+	constexpr int WARPS_ALL = G * KS, OWN = GROUP_ROWS / KS; // rows that a warp ends
+	const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+	const int group = warp % G, part = warp / G;
+	const int own0 = group * GROUP_ROWS + part * OWN;
+	const int begin = blockIdx.x * p.perBlock, end = min(p.vocabulary, begin + p.perBlock);
+	int label[OWN]; // -1: not in these rows
+#pragma unroll
+	for(int r = 0; r < OWN; ++r) {
+		if(!has_target(p, own0 + r, &label[r])) label[r] = -1;
+	}
+	// the chunk that is asked for next, and its stage
+	int nextEntry = begin, nextK = 0, nextStage = 0;
+	auto load = [&] {
+		if(nextEntry < end) {
+			constexpr int PER_ROW = GROUP_CHUNK / V, AT_ONCE = 32 / PER_ROW; // lanes of an entry, entries of a warp's copy
+			const int k = nextK + lane % PER_ROW * V;
+			const bool in = k < p.width; // the width is a multiple of V
+			float* const weights = s.stages[nextStage].weights + lane % PER_ROW * V;
+#pragma unroll 4
+			for(int e = warp * AT_ONCE + lane / PER_ROW; e < GROUP_TILE; e += WARPS_ALL * AT_ONCE) {
+				const bool there = in && nextEntry + e < p.vocabulary;
+				copy_words<V>(weights + e * GROUP_PITCH, there ? p.weights + static_cast<long long>(nextEntry + e) * p.weightsRow + k : p.weights, there);
+			}
+			float* const hidden = s.stages[nextStage].hidden + lane;
+#pragma unroll
+			for(int i = 0; i < OWN; ++i) {
+				const bool there = nextK + lane < p.width && own0 + i < p.rows;
+				copy_words<1>(hidden + (own0 + i) * GROUP_PITCH, there ? p.hidden + (own0 + i) * p.hiddenRow + nextK + lane : p.hidden, there);
+			}
+			nextK += GROUP_CHUNK;
+			if(nextK >= p.width) {
+				nextK = 0;
+				nextEntry += GROUP_TILE;
+			}
+			nextStage = nextStage + 1 == GROUP_STAGES ? 0 : nextStage + 1;
+		}
+		asm volatile("cp.async.commit_group;" ::: "memory"); // an empty one counts too
+	};
+	float2 running[OWN];
+#pragma unroll
+	for(int r = 0; r < OWN; ++r) running[r] = make_float2(-INFINITY, 0.f);
+	for(int i = 0; i < GROUP_STAGES - 1; ++i) load();
+	int stage = 0;
+	for(int entry0 = begin; entry0 < end; entry0 += GROUP_TILE) {
+		float2 z[4][GROUP_ROWS];
+#pragma unroll
+		for(int j = 0; j < 4; ++j) {
+#pragma unroll
+			for(int r = 0; r < GROUP_ROWS; ++r) z[j][r] = both(0.f);
+		}
+		for(int k0 = 0; k0 < p.width; k0 += GROUP_CHUNK) {
+			asm volatile("cp.async.wait_group %0;" ::"n"(GROUP_STAGES - 2) : "memory");
+			__syncthreads(); // this chunk is there, and everyone is done with the one before, whose stage is asked for again
+			load();
+			const float* const w = s.stages[stage].weights + lane * GROUP_PITCH + part * (GROUP_CHUNK / KS);
+			const float* const h = s.stages[stage].hidden + group * GROUP_ROWS * GROUP_PITCH + part * (GROUP_CHUNK / KS);
+			stage = stage + 1 == GROUP_STAGES ? 0 : stage + 1;
+#pragma unroll 2
+			for(int k = 0; k < GROUP_CHUNK / KS; k += 4) {
+				float4 x[4];
+#pragma unroll
+				for(int j = 0; j < 4; ++j) x[j] = *reinterpret_cast<const float4*>(w + 32 * j * GROUP_PITCH + k);
+#pragma unroll
+				for(int r = 0; r < GROUP_ROWS; ++r) {
+					const float4 y = *reinterpret_cast<const float4*>(h + r * GROUP_PITCH + k);
+#pragma unroll
+					for(int j = 0; j < 4; ++j) {
+						z[j][r] = fma2(make_float2(x[j].x, x[j].y), make_float2(y.x, y.y), z[j][r]);
+						z[j][r] = fma2(make_float2(x[j].z, x[j].w), make_float2(y.z, y.w), z[j][r]);
+					}
+				}
+			}
+		}
+		// (the logits of the tile before were read in front of the chunks' barriers)
+#pragma unroll
+		for(int j = 0; j < 4; ++j) {
+#pragma unroll
+			for(int r = 0; r < GROUP_ROWS; ++r) s.logits[part][group * GROUP_ROWS + r][lane + 32 * j] = z[j][r].x + z[j][r].y;
+		}
+		__syncthreads();
+#pragma unroll
+		for(int r = 0; r < OWN; ++r) {
+			float v[4], top = running[r].x;
+#pragma unroll
+			for(int j = 0; j < 4; ++j) {
+				const int entry = entry0 + lane + 32 * j;
+				float value = s.logits[0][own0 + r][lane + 32 * j];
+#pragma unroll
+				for(int k = 1; k < KS; ++k) value += s.logits[k][own0 + r][lane + 32 * j];
+				if(entry == label[r]) p.labelled[own0 + r] = value;
+				v[j] = entry < end ? value * LOG2E : -INFINITY;
+				top = fmaxf(top, v[j]);
+			}
+			const float at = top == -INFINITY ? 0.f : top;
+			running[r].y *= exp2_fast(running[r].x - at);
+#pragma unroll
+			for(int j = 0; j < 4; ++j) running[r].y += exp2_fast(v[j] - at);
+			running[r].x = top;
+		}
+	}
+#pragma unroll
+	for(int r = 0; r < OWN; ++r) {
+#pragma unroll
+		for(int o = 16; o > 0; o >>= 1) {
+			running[r] = join(running[r], make_float2(__shfl_xor_sync(0xffffffffu, running[r].x, o), __shfl_xor_sync(0xffffffffu, running[r].y, o)));
+		}
+		if(lane == 0 && own0 + r < p.rows) p.partial[static_cast<long long>(blockIdx.x) * p.rows + own0 + r] = running[r];
+	}
+}
+
+template<int G, int KS>
+void launch_group(const FewParams& p, cudaStream_t stream)
+{
+	constexpr int BYTES = static_cast<int>(sizeof(GroupRoom<G, KS>));
+	const bool quads = p.width % 4 == 0 && p.weightsRow % 4 == 0 && aligned16(p.weights);
+	const bool pairs = p.width % 2 == 0 && p.weightsRow % 2 == 0 && (reinterpret_cast<uintptr_t>(p.weights) & 7u) == 0;
+	const auto kernel = quads ? group_forward_kernel<G, KS, 4> : pairs ? group_forward_kernel<G, KS, 2> : group_forward_kernel<G, KS, 1>;
+	cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES);
+	kernel<<<few_blocks(p.rows, p.vocabulary), G * KS * 32, BYTES, stream>>>(p);
+	count_launch();
+}
+
 template<int NT>
 void launch_forward(const FewParams& p, cudaStream_t stream)
 {
-	few_forward_kernel<NT><<<few_blocks(p.vocabulary), THREADS, sizeof(Tiles<NT>), stream>>>(p);
+	few_forward_kernel<NT><<<few_blocks(p.rows, p.vocabulary), THREADS, sizeof(Tiles<NT>), stream>>>(p);
 	count_launch();
 }
 
@@ -306,7 +459,7 @@ void launch_backward(const FewParams& p, cudaStream_t stream)
 {
 	constexpr size_t each = NT * sizeof(float), most = sizeof(Tiles<NT>) + FEW_MOST_ENTRIES * each;
 	cudaFuncSetAttribute(few_backward_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(most));
-	few_backward_kernel<NT><<<few_blocks(p.vocabulary), THREADS, sizeof(Tiles<NT>) + p.perBlock * each, stream>>>(p);
+	few_backward_kernel<NT><<<few_blocks(p.rows, p.vocabulary), THREADS, sizeof(Tiles<NT>) + p.perBlock * each, stream>>>(p);
 	count_launch();
 }
 
@@ -317,7 +470,10 @@ static_assert(sizeof(Tiles<8>) <= 48 * 1024, "more shared memory than a kernel m
 int few_forward(const FewParams& p, cudaStream_t stream)
 {
 	if(p.rows <= 4) launch_forward<4>(p, stream);
-	else launch_forward<8>(p, stream);
+	else if(p.rows <= 8) launch_forward<8>(p, stream);
+	else if(p.rows <= 16) launch_group<2, 4>(p, stream);
+	else if(p.rows <= 24) launch_group<3, 4>(p, stream);
+	else launch_group<4, 2>(p, stream);
 	return check_launch();
 }
 
@@ -326,23 +482,24 @@ int few_backward(const FewParams& p, float* hiddenDiff, long long hiddenDiffRow,
 	if(p.rows <= 4) launch_backward<4>(p, stream);
 	else launch_backward<8>(p, stream);
 	if(hiddenDiff != nullptr) {
-		launch_dependent(true, few_hidden_kernel, dim3((p.width + 31) / 32, p.rows), dim3(256), 0, stream, p, few_blocks(p.vocabulary), hiddenDiff,
+		launch_dependent(true, few_hidden_kernel, dim3((p.width + 31) / 32, p.rows), dim3(256), 0, stream, p, few_blocks(p.rows, p.vocabulary), hiddenDiff,
 			hiddenDiffRow);
 		count_launch();
 	}
 	return check_launch();
 }
 
-// Blocks of a stretch each: four on an SM, or as many more as keep a stretch's dz within a block's shared memory; whole tiles.
-int few_entries(int vocabulary)
+// Blocks of a stretch each: four on an SM (one of more than eight rows), or as many more as keep a stretch's dz within a
+// block's shared memory; whole tiles.
+int few_entries(int rows, int vocabulary)
 {
-	const int tiles = (vocabulary + TILE - 1) / TILE, wanted = sm_count() * 4;
-	int perBlock = (tiles + wanted - 1) / wanted * TILE;
-	return perBlock > FEW_MOST_ENTRIES ? FEW_MOST_ENTRIES : perBlock;
+	const int tile = rows > FEW_ROWS ? GROUP_TILE : TILE, tiles = (vocabulary + tile - 1) / tile, wanted = sm_count() * (rows > FEW_ROWS ? 1 : 4);
+	const int perBlock = (tiles + wanted - 1) / wanted * tile;
+	return rows <= FEW_ROWS && perBlock > FEW_MOST_ENTRIES ? FEW_MOST_ENTRIES : perBlock;
 }
-int few_blocks(int vocabulary)
+int few_blocks(int rows, int vocabulary)
 {
-	const int perBlock = few_entries(vocabulary);
+	const int perBlock = few_entries(rows, vocabulary);
 	return (vocabulary + perBlock - 1) / perBlock;
 }
 

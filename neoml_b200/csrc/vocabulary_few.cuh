@@ -5,6 +5,7 @@
 namespace nb200 {
 
 constexpr int FEW_ROWS = 8;             // at most
+constexpr int FEW_FORWARD_ROWS = 32;    // and of the forward pass
 constexpr int FEW_TILE = 64;            // vocabulary entries of a tile
 constexpr int FEW_MOST_ENTRIES = 1024;  // of a block
 
@@ -22,8 +23,8 @@ struct FewParams {
 	float* hiddenPart;      // backward: [few_blocks()][rows][width]; null: hidden_diff is not wanted
 };
 
-int few_entries(int vocabulary);
-int few_blocks(int vocabulary);
+int few_entries(int rows, int vocabulary);
+int few_blocks(int rows, int vocabulary);
 int few_forward(const FewParams& p, cudaStream_t stream);
 int few_backward(const FewParams& p, float* hiddenDiff, long long hiddenDiffRow, cudaStream_t stream);
 

@@ -12,7 +12,7 @@
 //   of two that puts the largest loss_diff at 2^14, because softmax values of 1e-7 are below what a half holds; dz between 1
 //   and 2^-38 of the largest then keeps some or all of its bits.  hidden_diff is summed in fp32 over the pieces.
 // fp32: the same with three bf16 planes of each operand (product16.cuh), a piece of the weights split at a time: six times the
-// multiply-adds, and results as exact as fp32 sums in order give them.  Up to eight rows of fp32: vocabulary_few.cu.
+// multiply-adds, and results as exact as fp32 sums in order give them.  Few rows of fp32: vocabulary_few.cu.
 #include "product16.cuh"
 #include "vocabulary_few.cuh"
 
@@ -354,16 +354,22 @@ struct Aligned {
 	long long row, plane;
 };
 
-// Few rows of fp32 go to kernels of their own, whose blocks have stretches of the vocabulary: not where it is shorter than the rows (6 x
-// 4007 rows over 119 entries, two blocks: 240 us).
-bool few_rows(const Problem& q) { return q.type == NB200_TYPE_FP32 && q.rows <= FEW_ROWS && q.vocabulary >= q.width; }
+// Few rows of fp32 go to kernels of their own, whose blocks have stretches of the vocabulary: up to eight where it is not shorter than the
+// rows (6 x 4007 rows over 119 entries, two blocks: 240 us), more, forward only, where half of the SMs have a stretch (16 x 2048 rows over
+// 12000 entries 58 us, by planes 116; 24 x 3596 over 6319 118 and 113, 9 x 1031 over 8000 49 and 43).
+bool few_rows(const Problem& q, bool backward)
+{
+	if(q.type != NB200_TYPE_FP32) return false;
+	if(q.rows <= FEW_ROWS) return q.vocabulary >= q.width;
+	return !backward && q.rows <= FEW_FORWARD_ROWS && q.vocabulary >= 64 * sm_count();
+}
 
 struct FewRoom {
 	float2* partial;
 	float *labelled, *hiddenPart;
 	FewRoom(const Problem& q, bool backward, Room& room)
 	{
-		const size_t blocks = few_blocks(q.vocabulary);
+		const size_t blocks = few_blocks(q.rows, q.vocabulary);
 		partial = backward ? nullptr : room.take<float2>(blocks * q.rows);
 		labelled = backward ? nullptr : room.take<float>(q.rows);
 		hiddenPart = backward ? room.take<float>(blocks * q.rows * q.width) : nullptr;
@@ -482,7 +488,7 @@ FewParams few_params(const Problem& q, const int* labels)
 {
 	FewParams p = {};
 	p.hidden = static_cast<const float*>(q.hidden); p.weights = static_cast<const float*>(q.weights); p.hiddenRow = q.hiddenRow; p.weightsRow = q.weightsRow;
-	p.rows = q.rows; p.width = q.width; p.vocabulary = q.vocabulary; p.perBlock = few_entries(q.vocabulary);
+	p.rows = q.rows; p.width = q.width; p.vocabulary = q.vocabulary; p.perBlock = few_entries(q.rows, q.vocabulary);
 	p.labels = labels;
 	return p;
 }
@@ -498,13 +504,13 @@ void join_partials(const Problem& q, const float2* partial, int parts, const flo
 int forward(const Problem& q, const int* labels, float* loss, float* logSum, void* scratch, cudaStream_t stream)
 {
 	Room room = { static_cast<uint8_t*>(scratch) };
-	if(few_rows(q)) {
+	if(few_rows(q, false)) {
 		const FewRoom w(q, false, room);
 		FewParams p = few_params(q, labels);
 		p.partial = w.partial; p.labelled = w.labelled;
 		const int rc = few_forward(p, stream);
 		if(rc != NB200_OK) return rc;
-		join_partials(q, w.partial, few_blocks(q.vocabulary), w.labelled, labels, loss, logSum, stream);
+		join_partials(q, w.partial, few_blocks(q.rows, q.vocabulary), w.labelled, labels, loss, logSum, stream);
 		return check_launch();
 	}
 	const Forward f(q, room);
@@ -551,7 +557,7 @@ int backward(const Problem& q, const float* lossDiff, const int* labels, const f
 	void* weightsDiff, long long weightsDiffRow, void* scratch, cudaStream_t stream)
 {
 	Room room = { static_cast<uint8_t*>(scratch) };
-	if(few_rows(q)) {
+	if(few_rows(q, true)) {
 		const FewRoom few(q, true, room);
 		FewParams p = few_params(q, labels);
 		p.logSum = logSum; p.lossDiff = lossDiff;
@@ -632,7 +638,7 @@ size_t nb200_vocabulary_cross_entropy_scratch_bytes(int type, const void* hidden
 	const Problem q = { type, rows, width, vocabulary, hidden, weights, hidden_row_size, weights_row_size };
 	if(!valid(q) || rows == 0 || too_big(q)) return 0;
 	Room room = { nullptr };
-	if(few_rows(q)) FewRoom(q, backward != 0, room);
+	if(few_rows(q, backward != 0)) FewRoom(q, backward != 0, room);
 	else if(backward) Backward(q, room);
 	else Forward(q, room);
 	return room.used;

@@ -318,3 +318,32 @@ def test_negated_views_are_refused():
         ops.GatedRecurrence(x[None], torch._neg_view(x[None]))
     with pytest.raises(AssertionError, match="negated"):
         ops.DistillationLoss(torch._neg_view(x), torch.zeros(4, 2), torch.zeros(4, 2, dtype=torch.int32))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,width,v", [(9, 33, 9600), (12, 1, 40000), (16, 130, 20011), (17, 64, 30003), (24, 36, 12001), (25, 1031, 9500), (32, 206, 10007), (32, 512, 9999),
+                                          (33, 206, 10007)])
+def test_some_rows_of_fp32(rows, width, v):
+    x, w, labels = _case(torch.float32, rows, width, v)
+    labels[0], labels[-1] = 0, v - 1
+    _check(x, w, labels)
+    first = ops.VocabularyCrossEntropy(x, w, labels)
+    assert all(torch.equal(a, b) for a, b in zip(first, ops.VocabularyCrossEntropy(x, w, labels)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("first,row", [(0, 72), (2, 70), (1, 72), (2, 69)])
+def test_some_rows_of_fp32_in_views(first, row):
+    x, w, labels = _case(torch.float32, 20, row, 9700)
+    x, w = x[:, first:first + 64], w[:, first:first + 64]
+    got, want = (ops.VocabularyCrossEntropy(*pair, labels) for pair in ((x, w), (x.contiguous(), w.contiguous())))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    # a row without a target, whatever it holds, and its neighbours
+    x = x.clone()
+    labels[3] = -1
+    before = ops.VocabularyCrossEntropy(x, w, labels)
+    x[3] = float("nan")
+    after = ops.VocabularyCrossEntropy(x, w, labels)
+    others = torch.arange(20, device="cuda") != 3
+    assert torch.equal(before[0], after[0]) and torch.equal(before[1][others], after[1][others])
+
