@@ -152,23 +152,26 @@ __global__ void __launch_bounds__(THREADS, 1) product16_kernel(const Product16Pa
 		if(elect_one()) {
 			int it = 0;
 			bool ok = true;
+			// rows of A that do not exist are left out of the box: what their place in the stage holds reaches no other row of the
+			// accumulator.  (Leaving out boxes across that lie behind m or n as well, by a test each, made gradients of 1023 x 768 rows over
+			// 30011 entries 2.5 % slower.)
+			const uint32_t bytes = (A_ACROSS ? A_BYTES : p.boxA * BK * 2) + BN * BK * 2;
 			auto load = [&](const Tile& t, int kb, int planeA, int planeB) {
 				const int s = it % STAGES;
 				if(it >= STAGES && !mbar_wait_bounded(bars + B_EMPTY + s, (it / STAGES - 1) & 1, abortFlag, p.status, (KERNEL_ID << 8) | SITE_LOAD)) return false;
 				uint64_t* const full = bars + B_FULL + s;
 				const uint32_t a = smemBase + s * STAGE_BYTES, b = a + A_BYTES;
-				// boxes and rows that nothing of the result needs are left out: what their place in the stage holds reaches no other row
-				// or column of the accumulator
-				const int boxesA = A_ACROSS ? min(BM / 64, (p.m - t.m0 + 63) / 64) : 1, boxesB = B_ACROSS ? min(BN / 64, (p.n - t.n0 + 63) / 64) : 1;
-				mbar_arrive_expect_tx(full, (A_ACROSS ? boxesA * 8192 : p.boxA * BK * 2) + (B_ACROSS ? boxesB * 8192 : BN * BK * 2));
+				mbar_arrive_expect_tx(full, bytes);
 				const int k = kb * BK;
 				if constexpr(A_ACROSS) {
-					for(int i = 0; i < boxesA; ++i) tma_load_3d(a + i * 8192, &mapA, full, t.m0 + i * 64, k, planeA);
+#pragma unroll
+					for(int i = 0; i < BM / 64; ++i) tma_load_3d(a + i * 8192, &mapA, full, t.m0 + i * 64, k, planeA);
 				} else {
 					tma_load_3d(a, &mapA, full, k, t.m0, planeA);
 				}
 				if constexpr(B_ACROSS) {
-					for(int i = 0; i < boxesB; ++i) tma_load_3d(b + i * 8192, &mapB, full, t.n0 + i * 64, k, planeB);
+#pragma unroll
+					for(int i = 0; i < BN / 64; ++i) tma_load_3d(b + i * 8192, &mapB, full, t.n0 + i * 64, k, planeB);
 				} else {
 					tma_load_3d(b, &mapB, full, k, t.n0, planeB);
 				}
