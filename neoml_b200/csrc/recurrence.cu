@@ -16,6 +16,8 @@
 //            mbarrier: a cluster-wide barrier would wait for the results' stores to global memory too, every round
 // The next round's loads are issued before this one is folded.
 // The gates' pre-activations are the inputs: a gate of 0.999 rounded to bf16 is 1 and would never forget.
+// The backward pass takes h_{t-1} from the result as it was stored.  In 16-bit types that is half a step of it in d(forget) (36 x 8 x 46
+// bf16: the gradients together 2.2e-3 off, 1.7e-3 by fp32 states), where fp32 states would be twice the bytes of the result, to write and to read.
 #include "product16.cuh"
 #include <cooperative_groups.h>
 #include <cuda.h>
