@@ -348,7 +348,9 @@ NB200_API int nb200_gated_recurrence(void* stream, int type, const nb200_recurre
 	const void* forget, const void* input, const float* initial_state, const int* lengths, void* result, float* final_state);
 /* Its gradients (QrnnFPoolingBackward, QrnnIfPoolingBackward; the slope of VectorSigmoid, NME.h:311, inside): of update,
  * forget and input (dense, zero behind a sequence's end; input_diff is NULL exactly where input is) and of the initial
- * state, from those of the result and of the final state (NULL: zeros).  `result` is what the forward pass wrote. */
+ * state, from those of the result and of the final state (NULL: zeros).  `result` is what the forward pass wrote; of 16-bit
+ * types it is rounded, and the states are formed again in fp32 from the inputs.  update_diff of 16-bit types shares no memory with
+ * result_diff, update, forget or input (NB200_EINVAL). */
 NB200_API int nb200_gated_recurrence_backward(void* stream, int type, const nb200_recurrence_desc* desc,
 	const void* result_diff, long long result_diff_batch, long long result_diff_row, const void* result, const void* update,
 	const void* forget, const void* input, const float* initial_state, const float* final_state_diff, const int* lengths,

@@ -16,8 +16,9 @@
 //            mbarrier: a cluster-wide barrier would wait for the results' stores to global memory too, every round
 // The next round's loads are issued before this one is folded.
 // The gates' pre-activations are the inputs: a gate of 0.999 rounded to bf16 is 1 and would never forget.
-// The backward pass takes h_{t-1} from the result as it was stored.  In 16-bit types that is half a step of it in d(forget) (36 x 8 x 46
-// bf16: the gradients together 2.2e-3 off, 1.7e-3 by fp32 states), where fp32 states would be twice the bytes of the result, to write and to read.
+// The backward pass of fp32 takes h_{t-1} from the result.  In 16-bit types the result is rounded (half a step of it in d(forget), and an infinite
+// one where a half ends), so the states are formed again in fp32: a pass over the inputs stores one in front of every eight steps, which costs
+// a quarter of an array's bytes, and a thread of the backward kernel goes through its own steps from there.
 #include "product16.cuh"
 #include <cooperative_groups.h>
 #include <cuda.h>
@@ -109,6 +110,36 @@ __device__ __forceinline__ void store_raw(T* p, Num<W> v, int second)
 		p[0] = from_float<T>(v.v.x);
 		if(second != 0) p[1] = from_float<T>(v.v.y);
 	}
+}
+
+// A pair of states in front of a stretch of steps, kept in 16-bit memory that the stretch's gradients take later: the upper halves of both in
+// the stretch's first row, the lower halves in its second one.  Who reads them is the thread that writes the gradients there.
+template<typename T, bool SPLIT>
+__device__ __forceinline__ void store_parts(T* at, int row, Num<2> v, int second)
+{
+	const uint32_t x = __float_as_uint(v.v.x), y = __float_as_uint(v.v.y);
+	const uint32_t parts[2] = { __byte_perm(x, y, 0x7632), __byte_perm(x, y, 0x5410) };
+#pragma unroll
+	for(int k = 0; k < 2; ++k) {
+		unsigned short* const to = reinterpret_cast<unsigned short*>(at + static_cast<long long>(k) * row);
+		if constexpr(SPLIT) {
+			to[0] = static_cast<unsigned short>(parts[k]);
+			if(second != 0) to[1] = static_cast<unsigned short>(parts[k] >> 16);
+		} else {
+			*reinterpret_cast<uint32_t*>(to) = parts[k];
+		}
+	}
+}
+template<typename T, bool SPLIT>
+__device__ __forceinline__ uint2 load_parts(const T* at, int row, int second)
+{
+	return make_uint2(load_raw<T, SPLIT>(at, second), load_raw<T, SPLIT>(at + row, second));
+}
+template<int W>
+__device__ __forceinline__ Num<W> from_parts(uint2 parts)
+{
+	if constexpr(W == 2) return { make_float2(__uint_as_float(__byte_perm(parts.y, parts.x, 0x5410)), __uint_as_float(__byte_perm(parts.y, parts.x, 0x7632))) };
+	else return all<W>(0.f); // fp32 states are not kept in parts
 }
 
 template<int W>
@@ -282,7 +313,17 @@ struct Operand {
 struct Yes { static constexpr bool value = true; };
 struct No { static constexpr bool value = false; };
 
-template<typename T, int W, bool INPUT, bool DENSE, bool SPLIT>
+// The same pass over the inputs, but of the states only those in front of every STEPS-th step are stored, for the backward pass of 16-bit
+// types (store_parts): stretches end at a sequence's end then, as they do there, and the first of them may begin in front of step 0.
+template<bool STATES>
+struct Stretches {
+	int n;
+	__device__ __forceinline__ int begin(int stride) const { return STATES ? n - (n + stride - 1) / stride * stride : 0; }
+	__device__ __forceinline__ bool in(int t) const { return STATES ? t >= 0 && t < n : t < n; }
+	__device__ __forceinline__ bool whole(int t, int steps) const { return (!STATES || t >= 0) && t + steps <= n; }
+};
+
+template<typename T, int W, bool INPUT, bool DENSE, bool SPLIT, bool STATES>
 __global__ void __launch_bounds__(MAX_WARPS * 32, W == 1 ? 3 : 2) recurrence_forward_kernel(const RecurrenceParams p)
 {
 	extern __shared__ __align__(128) uint8_t sharedRoom[];
@@ -298,12 +339,14 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, W == 1 ? 3 : 2) recurrence_for
 	const int second = c + 1 < p.channels ? 1 : 0;
 	const int n = sequence_length(p, b);
 	const int span = warps * STEPS, stride = span * blocks;
-	const int first = rank * span + warp * STEPS;
-	Operand<T, DENSE> z = { static_cast<const uint8_t*>(p.z) + b * p.zBatch * sizeof(T), p.zRow * static_cast<long long>(sizeof(T)) };
-	Operand<T, DENSE> f = { static_cast<const uint8_t*>(p.f) + b * p.fBatch * sizeof(T), p.fRow * static_cast<long long>(sizeof(T)) };
-	Operand<T, DENSE> i = { static_cast<const uint8_t*>(p.i) + b * p.iBatch * sizeof(T), p.iRow * static_cast<long long>(sizeof(T)) };
+	const Stretches<STATES> all_steps = { n };
+	const int begin = all_steps.begin(stride), first = rank * span + warp * STEPS;
+	const long long back = DENSE ? static_cast<long long>(begin) * p.channels * static_cast<long long>(sizeof(T)) : 0; // nothing in front of step 0 is read
+	Operand<T, DENSE> z = { static_cast<const uint8_t*>(p.z) + b * p.zBatch * sizeof(T) + back, p.zRow * static_cast<long long>(sizeof(T)) };
+	Operand<T, DENSE> f = { static_cast<const uint8_t*>(p.f) + b * p.fBatch * sizeof(T) + back, p.fRow * static_cast<long long>(sizeof(T)) };
+	Operand<T, DENSE> i = { static_cast<const uint8_t*>(p.i) + b * p.iBatch * sizeof(T) + back, p.iRow * static_cast<long long>(sizeof(T)) };
 	T* const out = static_cast<T*>(p.out) + static_cast<long long>(b) * p.length * p.channels;
-	uint8_t* outRound = reinterpret_cast<uint8_t*>(out);
+	uint8_t* outRound = reinterpret_cast<uint8_t*>(out) + back;
 	const long long roundBytes = static_cast<long long>(stride) * p.channels * sizeof(T);
 	uint32_t offset[STEPS];
 #pragma unroll
@@ -315,14 +358,14 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, W == 1 ? 3 : 2) recurrence_for
 	auto load = [&](int t, auto full) {
 #pragma unroll
 		for(int k = 0; k < STEPS; ++k) {
-			const bool in = decltype(full)::value || t + k < n;
+			const bool in = decltype(full)::value || all_steps.in(t + k);
 			rz[k] = in ? load_raw<T, SPLIT>(z.at(offset[k], t + k, c), second) : 0u;
 			rf[k] = in ? load_raw<T, SPLIT>(f.at(offset[k], t + k, c), second) : 0u;
 			if constexpr(INPUT) ri[k] = in ? load_raw<T, SPLIT>(i.at(offset[k], t + k, c), second) : 0u;
 		}
 	};
-	int round = 0, t = first;
-	if(t + STEPS <= n) load(t, Yes());
+	int round = 0, t = begin + first;
+	if(all_steps.whole(t, STEPS)) load(t, Yes());
 	else load(t, No());
 	// the whole cluster agrees on n, and on the number of rounds
 	for(; round * stride < n; ++round) {
@@ -331,7 +374,7 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, W == 1 ? 3 : 2) recurrence_for
 		auto fold = [&](auto full) {
 #pragma unroll
 			for(int k = 0; k < STEPS; ++k) {
-				const bool in = decltype(full)::value || t + k < n;
+				const bool in = decltype(full)::value || all_steps.in(t + k);
 				const Gate<W> forget = gate<T, W>(rf[k]);
 				Num<W> take = forget.take;
 				if constexpr(INPUT) take = sigmoid<T, W>(ri[k]);
@@ -341,7 +384,7 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, W == 1 ? 3 : 2) recurrence_for
 				mine.a = mul(mine.a, a[k]);
 			}
 		};
-		const bool whole = t + STEPS <= n;
+		const bool whole = all_steps.whole(t, STEPS);
 		if(whole) fold(Yes());
 		else fold(No());
 		if constexpr(DENSE) {
@@ -349,7 +392,7 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, W == 1 ? 3 : 2) recurrence_for
 			f.base += roundBytes;
 			if constexpr(INPUT) i.base += roundBytes;
 		}
-		if(t + stride + STEPS <= n) load(t + stride, Yes());
+		if(all_steps.whole(t + stride, STEPS)) load(t + stride, Yes());
 		else load(t + stride, No());
 		Num<W> state;
 		join<W>(s, mine, round, rank, blocks, warps, p.status, carry, state);
@@ -361,13 +404,17 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, W == 1 ? 3 : 2) recurrence_for
 				if(on && (decltype(full)::value || t + k < n)) store_raw<T, W, SPLIT>(to, state, second);
 			}
 		};
-		if(whole) apply(Yes());
-		else apply(No());
+		if constexpr(STATES) {
+			if(on && t > 0) store_parts<T, SPLIT>(DENSE ? reinterpret_cast<T*>(outRound + offset[0]) : out + static_cast<long long>(t) * p.channels + c, p.channels, state, second);
+		} else {
+			if(whole) apply(Yes());
+			else apply(No());
+		}
 		outRound += roundBytes;
 		t += stride;
 	}
 	// behind the sequence the results are zeros
-	for(int k = n + rank * warps + warp; k < p.length; k += blocks * warps) {
+	for(int k = n + rank * warps + warp; !STATES && k < p.length; k += blocks * warps) {
 		if(on) store_raw<T, W, SPLIT>(out + static_cast<long long>(k) * p.channels + c, all<W>(0.f), second);
 	}
 	if(blocks > 1) cg::this_cluster().sync(); // nobody leaves while its shared memory may be written
@@ -379,6 +426,7 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, W == 1 ? 3 : 2) recurrence_for
 template<typename T, int W, bool INPUT, bool DENSE, bool SPLIT>
 __global__ void __launch_bounds__(MAX_WARPS * 32, 2) recurrence_backward_kernel(const RecurrenceParams p)
 {
+	constexpr bool STORED = sizeof(T) == 4; // the result holds the states as they were
 	extern __shared__ __align__(128) uint8_t sharedRoom[];
 	__shared__ uint64_t arrived[2];
 	__shared__ int abortFlag;
@@ -423,7 +471,8 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 2) recurrence_backward_kernel(
 	}
 	// The gates and the gradients are wanted when a round begins, the rest only when its state has arrived: the former are
 	// loaded a whole round ahead, the latter while the round before them ends.
-	uint32_t rz[STEPS], rf[STEPS], ri[STEPS], rd[STEPS], nd[STEPS], rh[STEPS];
+	uint32_t rz[STEPS], rf[STEPS], ri[STEPS], rd[STEPS], nd[STEPS], rh[STORED ? STEPS : 1];
+	uint2 parts = make_uint2(0u, 0u); // the state in front of the stretch
 	auto load_gates = [&](int t, auto full) {
 #pragma unroll
 		for(int k = 0; k < STEPS; ++k) {
@@ -432,22 +481,26 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 2) recurrence_backward_kernel(
 			nd[k] = in ? load_raw<T, SPLIT>(dh.at(offset[k], t - k, c), second) : 0u;
 		}
 	};
-	auto load_rest = [&](int t, auto full) {
+	auto load_rest = [&](int t, long long round, auto full) {
+		if constexpr(!STORED && decltype(full)::value) {
+			parts = load_parts<T, SPLIT>(DENSE ? reinterpret_cast<const T*>(reinterpret_cast<const uint8_t*>(dz) + round + offset[STEPS - 1])
+				: dz + static_cast<long long>(t - STEPS + 1) * p.channels + c, p.channels, second);
+		}
 #pragma unroll
 		for(int k = 0; k < STEPS; ++k) {
 			const bool in = decltype(full)::value || t - k >= 0;
 			rz[k] = in ? load_raw<T, SPLIT>(z.at(offset[k], t - k, c), second) : 0u;
-			rh[k] = decltype(full)::value || t - k > 0 ? load_raw<T, SPLIT>(h.at(offset[k], t - k, c), second) : 0u;
+			if constexpr(STORED) rh[k] = decltype(full)::value || t - k > 0 ? load_raw<T, SPLIT>(h.at(offset[k], t - k, c), second) : 0u;
 			if constexpr(INPUT) ri[k] = in ? load_raw<T, SPLIT>(i.at(offset[k], t - k, c), second) : 0u;
 		}
 	};
 	int round = 0, t = n - 1 - back;
 	if(t - STEPS >= 0) {
 		load_gates(t, Yes());
-		load_rest(t, Yes());
+		load_rest(t, outRound, Yes());
 	} else {
 		load_gates(t, No());
-		load_rest(t, No());
+		load_rest(t, outRound, No());
 	}
 	for(; round * stride < n; ++round) {
 		Num<W> a[STEPS], u[STEPS];
@@ -477,22 +530,36 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 2) recurrence_backward_kernel(
 		Num<W> state;
 		join<W>(s, mine, round, rank, blocks, warps, p.status, carry, state);
 		auto apply = [&](auto full) {
+			// d(forget) of a step: S times this, which takes the state in front of it
+			Num<W> slope[STEPS];
+			Num<W> running = first;
+			if constexpr(!STORED && decltype(full)::value) running = from_parts<W>(parts);
+#pragma unroll
+			for(int k = STEPS - 1; k >= 0; --k) {
+				const Num<W> value = number<T, W>(rz[k]);
+				Num<W> before = running;
+				if constexpr(STORED) {
+					before = number<T, W>(rh[k]);
+					if(!decltype(full)::value && t - k == 0) before = first;
+				} else { // steps in front of the first one: a is one, the value zero
+					Num<W> take = u[k];
+					if constexpr(INPUT) take = sigmoid<T, W>(ri[k]);
+					running = fma(a[k], before, mul(take, value));
+				}
+				slope[k] = mul(mul(a[k], u[k]), INPUT ? before : fma(value, all<W>(-1.f), before));
+			}
 #pragma unroll
 			for(int k = 0; k < STEPS; ++k) {
-				const Num<W> S = add(state, number<T, W>(rd[k])), value = number<T, W>(rz[k]);
-				Num<W> before = number<T, W>(rh[k]);
-				if(!decltype(full)::value && t - k == 0) before = first;
-				const Num<W> slope = mul(a[k], u[k]);
-				Num<W> oz, of, oi = S;
+				const Num<W> S = add(state, number<T, W>(rd[k]));
+				Num<W> oz, oi = S;
 				if constexpr(INPUT) {
 					const Gate<W> take = gate<T, W>(ri[k]);
 					oz = mul(S, take.keep);
-					of = mul(mul(S, before), slope);
-					oi = mul(mul(oz, value), take.take);
+					oi = mul(mul(oz, number<T, W>(rz[k])), take.take);
 				} else {
 					oz = mul(S, u[k]);
-					of = mul(mul(S, fma(value, all<W>(-1.f), before)), slope);
 				}
+				const Num<W> of = mul(S, slope[k]);
 				state = mul(a[k], S);
 				if(on && (decltype(full)::value || t - k >= 0)) {
 					const long long step = DENSE ? 0 : static_cast<long long>(t - k) * p.channels + c;
@@ -511,8 +578,8 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 2) recurrence_backward_kernel(
 			h.base -= roundBytes;
 			if constexpr(INPUT) i.base -= roundBytes;
 		}
-		if(nextWhole) load_rest(t - stride, Yes());
-		else load_rest(t - stride, No());
+		if(nextWhole) load_rest(t - stride, outRound - roundBytes, Yes());
+		else load_rest(t - stride, outRound - roundBytes, No());
 		outRound -= roundBytes;
 		t -= stride;
 	}
@@ -529,6 +596,7 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 2) recurrence_backward_kernel(
 struct Maps {
 	CUtensorMap z, f, i, dh, h;
 };
+__host__ __device__ constexpr int backward_arrays(bool input, bool stored) { return 3 + (stored ? 1 : 0) + (input ? 1 : 0); }
 
 // One warp's ring: `arrays` boxes a stage.
 template<int S>
@@ -571,7 +639,7 @@ __device__ __forceinline__ void stage_read()
 	fence_proxy_async_smem();
 }
 
-template<typename T, int W, bool INPUT, int S, int DEPTH>
+template<typename T, int W, bool INPUT, int S, int DEPTH, bool STATES>
 __global__ void __launch_bounds__(MAX_WARPS * 32, S == 8 ? 3 : 2) recurrence_forward_stream_kernel(const RecurrenceParams p, const __grid_constant__ Maps maps)
 {
 	extern __shared__ __align__(128) uint8_t sharedRoom[];
@@ -590,19 +658,20 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, S == 8 ? 3 : 2) recurrence_for
 	const bool on = c < p.channels;
 	const int n = sequence_length(p, b);
 	const int span = warps * S, stride = span * blocks;
-	const int first = rank * span + warp * S;
+	const Stretches<STATES> all_steps = { n };
+	const int first = all_steps.begin(stride) + rank * span + warp * S;
 	T* const out = static_cast<T*>(p.out) + static_cast<long long>(b) * p.length * p.channels;
-	uint8_t* outRound = reinterpret_cast<uint8_t*>(out);
+	uint8_t* outRound = reinterpret_cast<uint8_t*>(out) + static_cast<long long>(all_steps.begin(stride)) * p.channels * static_cast<long long>(sizeof(T));
 	const long long roundBytes = static_cast<long long>(stride) * p.channels * sizeof(T);
 	uint32_t offset[S];
 #pragma unroll
-	for(int k = 0; k < S; ++k) offset[k] = (static_cast<uint32_t>(first + k) * p.channels + c) * static_cast<uint32_t>(sizeof(T));
+	for(int k = 0; k < S; ++k) offset[k] = (static_cast<uint32_t>(rank * span + warp * S + k) * p.channels + c) * static_cast<uint32_t>(sizeof(T));
 	const long long state0 = static_cast<long long>(b) * p.channels + c;
 	Num<W> carry = all<W>(0.f);
 	if(on) carry = load_state<W>(p.first, state0, 1);
 	auto ask = [&](int round) {
 		const int t = first + round * stride;
-		if(t >= n || lane != 0) return;
+		if(t >= n || lane != 0) return; // (a box may lie in front of step 0: rounds that a warp leaves out are the last ones)
 		const uint32_t at = ring.begin(round);
 		uint64_t* const bar = ring.full + round % DEPTH;
 		tma_load_3d(at, &maps.z, bar, tile, t, b);
@@ -618,7 +687,7 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, S == 8 ? 3 : 2) recurrence_for
 			const uint32_t *z = ring.box(round, 0) + lane, *f = ring.box(round, 1) + lane, *i = ring.box(round, INPUT ? 2 : 0) + lane;
 #pragma unroll
 			for(int k = 0; k < S; ++k) {
-				const bool in = decltype(full)::value || t + k < n;
+				const bool in = decltype(full)::value || all_steps.in(t + k);
 				const Gate<W> forget = gate<T, W>(f[k * 32]);
 				Num<W> take = forget.take;
 				if constexpr(INPUT) take = sigmoid<T, W>(i[k * 32]);
@@ -628,7 +697,7 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, S == 8 ? 3 : 2) recurrence_for
 				mine.a = mul(mine.a, a[k]);
 			}
 		};
-		const bool whole = t + S <= n;
+		const bool whole = all_steps.whole(t, S);
 		if(t < n) ring.wait(round, s.abortFlag, p.status);
 		if(whole) fold(Yes());
 		else if(t < n) fold(No());
@@ -643,12 +712,20 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, S == 8 ? 3 : 2) recurrence_for
 				if(on && (decltype(full)::value || t + k < n)) store_raw<T, W, false>(reinterpret_cast<T*>(outRound + offset[k]), state, 1);
 			}
 		};
-		if(whole) apply(Yes());
-		else if(t < n) apply(No());
+		if constexpr(STATES) {
+#pragma unroll
+			for(int k = 0; k < S; ++k) {
+				if(k % STEPS == 0 && on && t + k > 0) store_parts<T, false>(reinterpret_cast<T*>(outRound + offset[k]), p.channels, state, 1);
+				state = fma(a[k], state, h[k]);
+			}
+		} else {
+			if(whole) apply(Yes());
+			else if(t < n) apply(No());
+		}
 		outRound += roundBytes;
 	}
 	// behind the sequence the results are zeros
-	for(int k = n + rank * warps + warp; k < p.length; k += blocks * warps) {
+	for(int k = n + rank * warps + warp; !STATES && k < p.length; k += blocks * warps) {
 		if(on) store_raw<T, W, false>(out + static_cast<long long>(k) * p.channels + c, all<W>(0.f), 1);
 	}
 	if(blocks > 1) cg::this_cluster().sync(); // nobody leaves while its shared memory may be written
@@ -663,7 +740,9 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 2) recurrence_backward_stream_
 	__shared__ uint64_t arrived[2];
 	__shared__ int abortFlag;
 	__shared__ uint64_t bars[MAX_WARPS][DEPTH];
-	constexpr int ARRAYS = INPUT ? 5 : 4;
+	constexpr bool STORED = sizeof(T) == 4; // the result holds the states as they were
+	constexpr int ARRAYS = backward_arrays(INPUT, STORED), INPUT_AT = ARRAYS - 1;
+	static_assert(STORED || S % STEPS == 0, "a state in front of every stretch");
 	const int blocks = gridDim.y, rank = blockIdx.y;
 	const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 	constexpr int BOX_BYTES = Ring<S>::BOX_BYTES;
@@ -699,8 +778,8 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 2) recurrence_backward_stream_
 		tma_load_3d(at, &maps.f, bar, tile, from, b);
 		tma_load_3d(at + BOX_BYTES, &maps.dh, bar, tile, from, b);
 		tma_load_3d(at + 2 * BOX_BYTES, &maps.z, bar, tile, from, b);
-		tma_load_3d(at + 3 * BOX_BYTES, &maps.h, bar, tile, from - 1, b); // the step before
-		if constexpr(INPUT) tma_load_3d(at + 4 * BOX_BYTES, &maps.i, bar, tile, from, b);
+		if constexpr(STORED) tma_load_3d(at + 3 * BOX_BYTES, &maps.h, bar, tile, from - 1, b); // the step before
+		if constexpr(INPUT) tma_load_3d(at + INPUT_AT * BOX_BYTES, &maps.i, bar, tile, from, b);
 	};
 	for(int k = 0; k < DEPTH; ++k) ask(k);
 	// behind the sequence the gradients are zeros
@@ -716,7 +795,7 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 2) recurrence_backward_stream_
 		Num<W> a[S], u[S];
 		Fold<W> mine = { all<W>(1.f), all<W>(0.f) };
 		const uint32_t *f = ring.box(round, 0) + lane, *d = ring.box(round, 1) + lane, *z = ring.box(round, 2) + lane,
-			*h = ring.box(round, 3) + lane, *i = ring.box(round, INPUT ? 4 : 0) + lane;
+			*h = ring.box(round, STORED ? 3 : 0) + lane, *i = ring.box(round, INPUT ? INPUT_AT : 0) + lane;
 		auto fold = [&](auto full) {
 #pragma unroll
 			for(int k = 0; k < S; ++k) {
@@ -730,29 +809,48 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 2) recurrence_backward_stream_
 			}
 		};
 		const bool whole = t - S >= 0;
+		uint2 parts = make_uint2(0u, 0u); // the state in front of the stretch
+		if constexpr(!STORED) {
+			if(on && whole) parts = load_parts<T, false>(reinterpret_cast<const T*>(dz + outRound + offset[S - 1]), p.channels, 1);
+		}
 		if(t >= 0) ring.wait(round, s.abortFlag, p.status);
 		if(whole) fold(Yes());
 		else if(t >= 0) fold(No());
 		Num<W> state;
 		join<W>(s, mine, round, rank, blocks, warps, p.status, carry, state);
 		auto apply = [&](auto full) {
+			// d(forget) of a step: S times this, which takes the state in front of it
+			Num<W> slope[S];
+			Num<W> running = first;
+			if constexpr(!STORED && decltype(full)::value) running = from_parts<W>(parts);
+#pragma unroll
+			for(int k = S - 1; k >= 0; --k) {
+				const int row = (S - 1 - k) * 32;
+				const Num<W> value = number<T, W>(z[row]);
+				Num<W> before = running;
+				if constexpr(STORED) {
+					before = number<T, W>(h[row]);
+					if(!decltype(full)::value && t - k == 0) before = first;
+				} else { // steps in front of the first one: a is one, the value zero
+					Num<W> take = u[k];
+					if constexpr(INPUT) take = sigmoid<T, W>(i[row]);
+					running = fma(a[k], before, mul(take, value));
+				}
+				slope[k] = mul(mul(a[k], u[k]), INPUT ? before : fma(value, all<W>(-1.f), before));
+			}
 #pragma unroll
 			for(int k = 0; k < S; ++k) {
 				const int row = (S - 1 - k) * 32;
-				const Num<W> S = add(state, number<T, W>(d[row])), value = number<T, W>(z[row]);
-				Num<W> before = number<T, W>(h[row]);
-				if(!decltype(full)::value && t - k == 0) before = first;
-				const Num<W> slope = mul(a[k], u[k]);
-				Num<W> oz, of, oi = S;
+				const Num<W> S = add(state, number<T, W>(d[row]));
+				Num<W> oz, oi = S;
 				if constexpr(INPUT) {
 					const Gate<W> take = gate<T, W>(i[row]);
 					oz = mul(S, take.keep);
-					of = mul(mul(S, before), slope);
-					oi = mul(mul(oz, value), take.take);
+					oi = mul(mul(oz, number<T, W>(z[row])), take.take);
 				} else {
 					oz = mul(S, u[k]);
-					of = mul(mul(S, fma(value, all<W>(-1.f), before)), slope);
 				}
+				const Num<W> of = mul(S, slope[k]);
 				state = mul(a[k], S);
 				if(on && (decltype(full)::value || t - k >= 0)) {
 					store_raw<T, W, false>(reinterpret_cast<T*>(dz + outRound + offset[k]), oz, 1);
@@ -773,46 +871,55 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 2) recurrence_backward_stream_
 
 using Kernel = void (*)(const RecurrenceParams);
 
-template<typename T, int W, bool SPLIT, bool BACKWARD>
+enum Pass {
+	FORWARD,
+	STATES,  // of 16-bit types, in front of BACKWARD: the states in front of every STEPS-th step
+	BACKWARD
+};
+
+template<typename T, int W, bool SPLIT, Pass PASS>
 Kernel kernel_of(bool input, bool dense)
 {
-	if(BACKWARD) {
+	if(PASS == BACKWARD) {
 		if(dense) return input ? recurrence_backward_kernel<T, W, true, true, SPLIT> : recurrence_backward_kernel<T, W, false, true, SPLIT>;
 		return input ? recurrence_backward_kernel<T, W, true, false, SPLIT> : recurrence_backward_kernel<T, W, false, false, SPLIT>;
 	}
-	if(dense) return input ? recurrence_forward_kernel<T, W, true, true, SPLIT> : recurrence_forward_kernel<T, W, false, true, SPLIT>;
-	return input ? recurrence_forward_kernel<T, W, true, false, SPLIT> : recurrence_forward_kernel<T, W, false, false, SPLIT>;
+	constexpr bool S = PASS == STATES;
+	if(dense) return input ? recurrence_forward_kernel<T, W, true, true, SPLIT, S> : recurrence_forward_kernel<T, W, false, true, SPLIT, S>;
+	return input ? recurrence_forward_kernel<T, W, true, false, SPLIT, S> : recurrence_forward_kernel<T, W, false, false, SPLIT, S>;
 }
 
-template<bool BACKWARD>
+template<Pass PASS>
 Kernel kernel_for(int type, bool pair, bool input, bool dense)
 {
-	if(type == NB200_TYPE_FP32) return kernel_of<float, 1, false, BACKWARD>(input, dense);
-	if(type == NB200_TYPE_FP16) return pair ? kernel_of<__half, 2, false, BACKWARD>(input, dense) : kernel_of<__half, 2, true, BACKWARD>(input, dense);
-	return pair ? kernel_of<__nv_bfloat16, 2, false, BACKWARD>(input, dense) : kernel_of<__nv_bfloat16, 2, true, BACKWARD>(input, dense);
+	if(type == NB200_TYPE_FP16) return pair ? kernel_of<__half, 2, false, PASS>(input, dense) : kernel_of<__half, 2, true, PASS>(input, dense);
+	if(type == NB200_TYPE_BF16) return pair ? kernel_of<__nv_bfloat16, 2, false, PASS>(input, dense) : kernel_of<__nv_bfloat16, 2, true, PASS>(input, dense);
+	if constexpr(PASS == STATES) return nullptr;
+	else return kernel_of<float, 1, false, PASS>(input, dense);
 }
 
 // Rounds that a warp's loads are ahead of its work, by what fits beside one another in 16 or more warps' shared memory.
 constexpr int FORWARD_STEPS = 16, FORWARD_DEPTH = 2, FORWARD_INPUT_DEPTH = 2, BACKWARD_STEPS = 8, BACKWARD_DEPTH = 2,
-	BACKWARD_INPUT_STEPS = 16, BACKWARD_INPUT_DEPTH = 2;
+	BACKWARD_INPUT_STEPS = 8, BACKWARD_INPUT_STEPS_FP32 = 16, BACKWARD_INPUT_DEPTH = 2; // (16 steps of 16-bit gates and states spill: 570 us for 275)
 
 using StreamKernel = void (*)(const RecurrenceParams, const Maps);
 
-template<bool BACKWARD, typename T, int W>
+template<Pass PASS, typename T, int W>
 StreamKernel stream_of(bool input)
 {
-	if(BACKWARD) return input ? recurrence_backward_stream_kernel<T, W, true, BACKWARD_INPUT_STEPS, BACKWARD_INPUT_DEPTH>
+	if(PASS == BACKWARD) return input ? recurrence_backward_stream_kernel<T, W, true, W == 1 ? BACKWARD_INPUT_STEPS_FP32 : BACKWARD_INPUT_STEPS, BACKWARD_INPUT_DEPTH>
 		: recurrence_backward_stream_kernel<T, W, false, BACKWARD_STEPS, BACKWARD_DEPTH>;
-	return input ? recurrence_forward_stream_kernel<T, W, true, FORWARD_STEPS, FORWARD_INPUT_DEPTH>
-		: recurrence_forward_stream_kernel<T, W, false, FORWARD_STEPS, FORWARD_DEPTH>;
+	return input ? recurrence_forward_stream_kernel<T, W, true, FORWARD_STEPS, FORWARD_INPUT_DEPTH, PASS == STATES>
+		: recurrence_forward_stream_kernel<T, W, false, FORWARD_STEPS, FORWARD_DEPTH, PASS == STATES>;
 }
-template<bool BACKWARD>
+template<Pass PASS>
 StreamKernel stream_for(int type, bool input)
 {
-	return type == NB200_TYPE_FP32 ? stream_of<BACKWARD, float, 1>(input)
-		: type == NB200_TYPE_FP16 ? stream_of<BACKWARD, __half, 2>(input) : stream_of<BACKWARD, __nv_bfloat16, 2>(input);
+	if(type == NB200_TYPE_FP16) return stream_of<PASS, __half, 2>(input);
+	if(type == NB200_TYPE_BF16) return stream_of<PASS, __nv_bfloat16, 2>(input);
+	if constexpr(PASS == STATES) return nullptr;
+	else return stream_of<PASS, float, 1>(input);
 }
-
 // Maps of the operands; false where one of them does not lie as TMA takes it (or a step's distance does not fit 32 bits of a round's offsets).
 bool make_maps(Maps& maps, int type, bool backward, const RecurrenceParams& p, int batch, int steps)
 {
@@ -823,7 +930,7 @@ bool make_maps(Maps& maps, int type, bool backward, const RecurrenceParams& p, i
 		return sequence_map(&map, base, type, p.channels, p.length, batch, row, batch > 1 ? batchStride : row * p.length, steps);
 	};
 	return one(maps.z, p.z, p.zBatch, p.zRow) && one(maps.f, p.f, p.fBatch, p.fRow) && (p.i == nullptr || one(maps.i, p.i, p.iBatch, p.iRow))
-		&& (!backward || (one(maps.dh, p.dh, p.dhBatch, p.dhRow) && one(maps.h, p.h, dense * p.length, dense)));
+		&& (!backward || one(maps.dh, p.dh, p.dhBatch, p.dhRow)) && (!backward || size != 4 || one(maps.h, p.h, dense * p.length, dense));
 }
 
 // How many warps and blocks share a sequence's time axis: the fewest that fill three quarters of the warps that the SMs hold
@@ -832,13 +939,15 @@ bool make_maps(Maps& maps, int type, bool backward, const RecurrenceParams& p, i
 // two; 64 x 100 x 4096 fp16 39 + 57 in blocks of two, 60 + 94 of eight.  Where there are few channels (2 x 16384 x 2048 bf16) clusters of eight
 // blocks of four: 84 + 141, in clusters of four 116 + 199, without 352 + 617.  By loads into registers the three take 93 + 181, 43 + 77 and
 // 104 + 213 in the same shapes.
-int launch(int type, bool pair, bool backward, RecurrenceParams p, int batch, cudaStream_t stream)
+int launch(int type, bool pair, Pass pass, RecurrenceParams p, int batch, cudaStream_t stream)
 {
+	const bool backward = pass == BACKWARD;
 	const bool input = p.i != nullptr;
 	const long long row = p.channels;
 	const bool dense = row * type_size(type) * (MAX_CLUSTER + 1) * MAX_WARPS * STEPS < (1ll << 32)
 		&& (p.length <= 1 || (p.zRow == row && p.fRow == row && (!input || p.iRow == row) && (!backward || p.dhRow == row)));
-	const Kernel kernel = backward ? kernel_for<true>(type, pair, input, dense) : kernel_for<false>(type, pair, input, dense);
+	const Kernel kernel = backward ? kernel_for<BACKWARD>(type, pair, input, dense) : pass == STATES ? kernel_for<STATES>(type, pair, input, dense)
+		: kernel_for<FORWARD>(type, pair, input, dense);
 	p.status = device_status_word();
 	const int channelsPerLane = type == NB200_TYPE_FP32 ? 1 : 2;
 	const int tiles = (p.channels + 32 * channelsPerLane - 1) / (32 * channelsPerLane);
@@ -853,10 +962,10 @@ int launch(int type, bool pair, bool backward, RecurrenceParams p, int batch, cu
 	Maps maps = {};
 	StreamKernel stream_kernel = nullptr;
 	int depth = 0;
-	const int steps = !backward ? FORWARD_STEPS : input ? BACKWARD_INPUT_STEPS : BACKWARD_STEPS;
+	const int steps = !backward ? FORWARD_STEPS : !input ? BACKWARD_STEPS : type == NB200_TYPE_FP32 ? BACKWARD_INPUT_STEPS_FP32 : BACKWARD_INPUT_STEPS;
 	// (their stores go by whole words; maps ask more of what is read)
 	if((pair || channelsPerLane == 1) && p.length >= 2 * warps * blocks * steps && make_maps(maps, type, backward, p, batch, steps)) {
-		stream_kernel = backward ? stream_for<true>(type, input) : stream_for<false>(type, input);
+		stream_kernel = backward ? stream_for<BACKWARD>(type, input) : pass == STATES ? stream_for<STATES>(type, input) : stream_for<FORWARD>(type, input);
 		depth = backward ? (input ? BACKWARD_INPUT_DEPTH : BACKWARD_DEPTH) : (input ? FORWARD_INPUT_DEPTH : FORWARD_DEPTH);
 	}
 	cudaLaunchConfig_t config = {};
@@ -872,7 +981,7 @@ int launch(int type, bool pair, bool backward, RecurrenceParams p, int batch, cu
 	config.attrs = attribute;
 	config.numAttrs = blocks > 1 ? 1 : 0;
 	if(stream_kernel != nullptr) {
-		const int arrays = (backward ? 4 : 2) + (input ? 1 : 0);
+		const int arrays = backward ? backward_arrays(input, type == NB200_TYPE_FP32) : 2 + (input ? 1 : 0);
 		const int perWarp = depth * arrays * steps * 128;
 		config.dynamicSmemBytes += static_cast<size_t>(warps) * perWarp;
 		// the most that the kernel is ever launched with: another thread may be between this and its own launch
@@ -900,6 +1009,17 @@ bool pairs_aligned(int type, int batch, int length, int channels, const Strided*
 		if((batch > 1 && s[k].batch % 2 != 0) || (length > 1 && s[k].row % 2 != 0)) return false;
 	}
 	return true;
+}
+
+// Elements from an operand's first to behind its last.
+long long extent(const nb200_recurrence_desc* d, long long batch, long long row)
+{
+	return (d->batch - 1) * batch + (d->length - 1) * row + d->channels;
+}
+bool apart(const void* a, long long aBytes, const void* b, long long bBytes)
+{
+	const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+	return a == nullptr || b == nullptr || (x < y ? y - x >= static_cast<uintptr_t>(aBytes) : x - y >= static_cast<uintptr_t>(bBytes));
 }
 
 bool desc_valid(int type, const nb200_recurrence_desc* d)
@@ -938,7 +1058,7 @@ int nb200_gated_recurrence(void* stream, int type, const nb200_recurrence_desc* 
 	p.length = d->length; p.channels = d->channels;
 	const Strided all[] = { { update, d->update_batch, d->update_row }, { forget, d->forget_batch, d->forget_row },
 		{ input, d->input_batch, d->input_row }, { result, 0, 0 } };
-	return launch(type, pairs_aligned(type, d->batch, d->length, d->channels, all, 4), false, p, d->batch, as_stream(stream));
+	return launch(type, pairs_aligned(type, d->batch, d->length, d->channels, all, 4), FORWARD, p, d->batch, as_stream(stream));
 }
 
 int nb200_gated_recurrence_backward(void* stream, int type, const nb200_recurrence_desc* d, const void* result_diff,
@@ -956,6 +1076,13 @@ int nb200_gated_recurrence_backward(void* stream, int type, const nb200_recurren
 		if(!type_aligned(t, type)) return NB200_EINVAL;
 	}
 	if(!words_aligned(initial_state, final_state_diff, lengths, initial_state_diff)) return NB200_EINVAL;
+	if(type != NB200_TYPE_FP32 && d->length > 0) { // update_diff holds states before it holds gradients
+		const long long size = 2, own = extent(d, static_cast<long long>(d->length) * d->channels, d->channels) * size;
+		if(!apart(update_diff, own, result_diff, extent(d, result_diff_batch, result_diff_row) * size)
+			|| !apart(update_diff, own, update, extent(d, d->update_batch, d->update_row) * size)
+			|| !apart(update_diff, own, forget, extent(d, d->forget_batch, d->forget_row) * size)
+			|| !apart(update_diff, own, input, extent(d, d->input_batch, d->input_row) * size)) return NB200_EINVAL;
+	}
 	if(d->batch > 65535 || d->length > (1 << 30)) return NB200_ETOOBIG;
 	if(device_status_word() == nullptr) return NB200_ENODEVICE;
 	RecurrenceParams p = {};
@@ -968,7 +1095,14 @@ int nb200_gated_recurrence_backward(void* stream, int type, const nb200_recurren
 	const Strided all[] = { { update, d->update_batch, d->update_row }, { forget, d->forget_batch, d->forget_row },
 		{ input, d->input_batch, d->input_row }, { result_diff, result_diff_batch, result_diff_row }, { result, 0, 0 },
 		{ update_diff, 0, 0 }, { forget_diff, 0, 0 }, { input_diff, 0, 0 } };
-	return launch(type, pairs_aligned(type, d->batch, d->length, d->channels, all, 8), true, p, d->batch, as_stream(stream));
+	const bool pair = pairs_aligned(type, d->batch, d->length, d->channels, all, 8);
+	if(type != NB200_TYPE_FP32 && d->length > STEPS) { // the states in front of stretches, in update_diff's memory
+		RecurrenceParams q = p;
+		q.last = nullptr;
+		const int rc = launch(type, pair, STATES, q, d->batch, as_stream(stream));
+		if(rc != NB200_OK) return rc;
+	}
+	return launch(type, pair, BACKWARD, p, d->batch, as_stream(stream));
 }
 
 } // extern "C"

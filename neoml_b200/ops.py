@@ -564,8 +564,8 @@ def GatedRecurrence(update, forget, input=None, *, initial_state=None, lengths=N
 def GatedRecurrenceBackward(result_diff, result, update, forget, input=None, *, initial_state=None, final_state_diff=None,
                             lengths=None):
     """The gradients of GatedRecurrence: (update_diff, forget_diff, input_diff, initial_state_diff); input_diff is None
-    without input gates.  `result` is what the forward pass returned; final_state_diff (fp32, None: zeros) is the gradient
-    of the last state.  Gradients are dense, one for every element that an expanded input stands for, and zero behind a
+    without input gates.  `result` is what the forward pass returned (the states themselves are fp32 here too: those of 16-bit
+    types are formed again from the inputs); final_state_diff (fp32, None: zeros) is the gradient of the last state.  Gradients are dense, one for every element that an expanded input stands for, and zero behind a
     sequence's end."""
     done = _native().gated_recurrence_backward(result_diff, result, update, forget, input, initial_state, final_state_diff, lengths)
     if done is not None:
