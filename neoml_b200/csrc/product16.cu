@@ -9,12 +9,16 @@
 // indices x 64 k lands as 64 rows of 128 bytes; eight rows are a swizzle atom of 1024 bytes (stride byte offset), the next 64
 // indices lie 8192 bytes further (leading byte offset).  Every wait is bounded (common.cuh).
 //
-// The tensor core's own additions cut off rather than round: a running sum loses about 3e-9 of itself with each MMA, always towards zero
-// (measured: 1.3e-6 after 384 of them, 3.5e-5 after 11250).  16-bit results do not show it, and
-// losses of 16-bit rows, fp32, are 3e-7 off (48 x 1024 bf16 over 32000; fp32 sums 5e-8).  For fp32 operands the K loop
-// is cut into chunks of 256 whose sums the epilogue warps add up in registers, and within a chunk the small products go first, so that
-// only the 16 MMAs of hi hi work on a sum of full size.  Gradients of 1023 x 768 rows over 30011 entries are 3.7e-7 off then
-// (1.3e-6 with chunks of 1024, 6.7e-7 of 512, fp32 arithmetic 5.7e-7), and take as long: the additions hide behind the MMAs.
+// The tensor core's own additions cut off rather than round, each MMA a unit or two in the last place of the running sum: all of it in one
+// direction where the sum has one sign (7.8e-6 of logits of 4096 positive products, 1.9e-4 of a gradient summed over 30000 entries), less where signs
+// alternate (1.3e-6 after 384 MMAs, 3.5e-5 after 11250).  So the K loop is cut into chunks whose sums the epilogue warps add up in registers:
+//   fp32        256 elements, the small products first, so that only the 16 MMAs of hi hi work on a sum of full size.  Gradients
+//               of 1023 x 768 rows over 30011 entries are 3.7e-7 off then (1.3e-6 with chunks of 1024, 6.7e-7 of 512, fp32 arithmetic 5.7e-7), and
+//               take as long: the additions hide behind six times the MMAs.
+//   16 bits     512 for the statistics, whose results are fp32: log_sum 1.6e-7 off at any width (whole K 3.2e-7 at 1024, 1.3e-6 at 4096; chunks of
+//               256 9e-8).  8192 x 2048 rows over 50257 entries take 1.06 ms (whole 1.02, chunks of 256 1.17).  1024 for gradients, which end as 16 bits: 1.6e-5
+//               of the sum above, 1 to 2 % of the time (2048: 3e-5, within the noise; 512: 9e-6, 3 %).  None for dz, which is rounded to 16 bits
+//               as it is formed, and none where K is no longer than a chunk.
 #include "product16.cuh"
 
 #include <cuda.h>
@@ -43,7 +47,8 @@ __device__ __forceinline__ float exp2_fast(float x)
 
 // The products of planes in the order of their MMAs, small ones first: 0 hi, 1 mid, 2 lo.
 __device__ constexpr int PLANE_A[6] = { 2, 0, 1, 1, 0, 0 }, PLANE_B[6] = { 0, 2, 1, 0, 1, 0 };
-constexpr int CHUNK = 256 / BK; // K blocks of fp32 operands that are summed in tensor memory
+// K blocks that are summed in tensor memory before the epilogue warps add them up in registers.
+template<int EPILOGUE, bool FP32> constexpr int CHUNK = FP32 ? 256 / BK : EPILOGUE == PRODUCT16_STATS ? 512 / BK : 1024 / BK;
 
 // MN-major operand of 16-bit elements: see the head of this file.
 __device__ __forceinline__ uint64_t desc_across(uint32_t smemAddr)
@@ -107,11 +112,12 @@ __device__ __forceinline__ uint32_t pack16(float a, float b, int bf16)
 	return bf16 ? pack2<__nv_bfloat16>(a, b) : pack2<__half>(a, b);
 }
 
-template<int EPILOGUE, bool A_ACROSS, bool B_ACROSS, bool FP32, bool NARROW>
+template<int EPILOGUE, bool A_ACROSS, bool B_ACROSS, bool FP32, bool NARROW, bool CHUNKED>
 __global__ void __launch_bounds__(THREADS, 1) product16_kernel(const Product16Params p, const __grid_constant__ CUtensorMap mapA,
 	const __grid_constant__ CUtensorMap mapB)
 {
-	constexpr int TERMS = FP32 ? 6 : 1;
+	constexpr int TERMS = FP32 ? 6 : 1, CHUNKS = CHUNK<EPILOGUE, FP32>;
+	static_assert(CHUNKED || !FP32, "the terms of fp32 operands come chunk by chunk");
 	constexpr int BN = NARROW ? PRODUCT16_NARROW : PRODUCT16_N, COLUMNS = BN / 2; // of a tile, and of an epilogue warp
 	constexpr int STAGE_BYTES = A_BYTES + BN * BK * 2, STAGES = RING_BYTES / STAGE_BYTES;
 	static_assert(STAGES * STAGE_BYTES == RING_BYTES && STAGE_BYTES % 1024 == 0, "stages fill the ring");
@@ -181,7 +187,7 @@ __global__ void __launch_bounds__(THREADS, 1) product16_kernel(const Product16Pa
 			};
 			for(int tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x) {
 				const Tile t = tile_of<BN>(p, tile);
-				const int chunk = FP32 ? CHUNK : p.kBlocks;
+				const int chunk = CHUNKED ? CHUNKS : p.kBlocks;
 				for(int k0 = t.kBegin; ok && k0 < t.kEnd; k0 += chunk) {
 					const int k1 = min(t.kEnd, k0 + chunk);
 					for(int term = 0; ok && term < TERMS; ++term) {
@@ -205,7 +211,7 @@ __global__ void __launch_bounds__(THREADS, 1) product16_kernel(const Product16Pa
 			bool ok = true;
 			for(int tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x) {
 				const Tile t = tile_of<BN>(p, tile);
-				const int chunk = FP32 ? CHUNK : p.kBlocks;
+				const int chunk = CHUNKED ? CHUNKS : p.kBlocks;
 				int k0 = t.kBegin;
 				do { // a part of K without steps takes its turn too
 					const int acc = n & 1;
@@ -410,7 +416,7 @@ __global__ void __launch_bounds__(THREADS, 1) product16_kernel(const Product16Pa
 				}
 			};
 			const bool empty = t.kBegin >= t.kEnd; // a part of K without steps: nothing was multiplied
-			if constexpr(FP32) {
+			if constexpr(CHUNKED) {
 				float total[COLUMNS / 32][32];
 				int k0 = t.kBegin;
 				do {
@@ -429,7 +435,7 @@ __global__ void __launch_bounds__(THREADS, 1) product16_kernel(const Product16Pa
 					tc_fence_before_sync();
 					if(lane == 0) mbar_arrive(bars + B_ACCEMPTY + acc);
 					++n;
-					k0 += CHUNK;
+					k0 += CHUNKS;
 				} while(k0 < t.kEnd);
 				if(!ok) break;
 #pragma unroll
@@ -485,11 +491,19 @@ EncodeTiledFn encoder()
 
 using Kernel = void (*)(const Product16Params, const CUtensorMap, const CUtensorMap);
 
+template<int EPILOGUE, bool A_ACROSS, bool B_ACROSS, bool NARROW>
+Kernel kernel_for(const Product16Params& p)
+{
+	if(p.fp32) return product16_kernel<EPILOGUE, A_ACROSS, B_ACROSS, true, NARROW, true>;
+	if constexpr(EPILOGUE != PRODUCT16_DIFF) { // (whose exponentials are rounded to the operands' type)
+		if(p.kBlocksPerSplit > CHUNK<EPILOGUE, false>) return product16_kernel<EPILOGUE, A_ACROSS, B_ACROSS, false, NARROW, true>;
+	}
+	return product16_kernel<EPILOGUE, A_ACROSS, B_ACROSS, false, NARROW, false>;
+}
 template<int EPILOGUE>
 Kernel rows_kernel(const Product16Params& p)
 {
-	if(p.narrow) return p.fp32 ? product16_kernel<EPILOGUE, false, false, true, true> : product16_kernel<EPILOGUE, false, false, false, true>;
-	return p.fp32 ? product16_kernel<EPILOGUE, false, false, true, false> : product16_kernel<EPILOGUE, false, false, false, false>;
+	return p.narrow ? kernel_for<EPILOGUE, false, false, true>(p) : kernel_for<EPILOGUE, false, false, false>(p);
 }
 
 } // namespace
@@ -529,9 +543,9 @@ int product16(Product16Epilogue epilogue, bool aAcross, bool bAcross, const Prod
 	Kernel kernel = nullptr;
 	if(epilogue == PRODUCT16_STATS && !aAcross && !bAcross) kernel = rows_kernel<PRODUCT16_STATS>(p);
 	else if(epilogue == PRODUCT16_DIFF && !aAcross && !bAcross) kernel = rows_kernel<PRODUCT16_DIFF>(p);
-	else if(epilogue == PRODUCT16_SUM && !aAcross && bAcross && !p.narrow) kernel = p.fp32 ? product16_kernel<PRODUCT16_SUM, false, true, true, false> : product16_kernel<PRODUCT16_SUM, false, true, false, false>;
-	else if(epilogue == PRODUCT16_SUM && aAcross && bAcross && !p.narrow) kernel = p.fp32 ? product16_kernel<PRODUCT16_SUM, true, true, true, false> : product16_kernel<PRODUCT16_SUM, true, true, false, false>;
-	else if(epilogue == PRODUCT16_STORE && aAcross && bAcross && !p.narrow) kernel = p.fp32 ? product16_kernel<PRODUCT16_STORE, true, true, true, false> : product16_kernel<PRODUCT16_STORE, true, true, false, false>;
+	else if(epilogue == PRODUCT16_SUM && !aAcross && bAcross && !p.narrow) kernel = kernel_for<PRODUCT16_SUM, false, true, false>(p);
+	else if(epilogue == PRODUCT16_SUM && aAcross && bAcross && !p.narrow) kernel = kernel_for<PRODUCT16_SUM, true, true, false>(p);
+	else if(epilogue == PRODUCT16_STORE && aAcross && bAcross && !p.narrow) kernel = kernel_for<PRODUCT16_STORE, true, true, false>(p);
 	else return NB200_EINVAL;
 	const long long tiles = static_cast<long long>(p.mTiles) * p.nTiles * p.splits;
 	if(tiles > 0x7fffffffLL - 1024) return NB200_ETOOBIG;

@@ -1,0 +1,51 @@
+"""What VocabularyCrossEntropy's 16-bit products lose in one direction: errors of a common sign, which norms of random data do not show."""
+import pytest
+import torch
+
+from neoml_b200 import ops
+
+HALVES = [torch.float16, torch.bfloat16]
+
+
+def _made(t, *shape, seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return torch.randn(*shape, generator=g, device="cuda").to(t)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", HALVES)
+@pytest.mark.parametrize("rows,width,v", [(64, 4096, 2000), (300, 8200, 700), (3, 4104, 9000)])
+def test_long_sums_of_one_sign(t, rows, width, v):
+    """The tensor core's additions cut off: a sum of 512 elements is 32 of them, each of which loses about a unit in the last place (2^-23) of
+    what has been summed, which on the way up comes to 16.5 of the whole.  Those sums are added up to nearest; the row's maximum, its
+    logarithm and their sum round a few times more."""
+    x, w = _made(t, rows, width, seed=1).abs(), (_made(torch.float32, v, width, seed=2).abs() * (20 / width)).to(t)
+    labels = torch.arange(rows, device="cuda", dtype=torch.int32) % v
+    loss, log_sum = ops.VocabularyCrossEntropy(x, w, labels)
+    z = x.double() @ w.double().T
+    want = torch.logsumexp(z, 1)
+    bound = (16.5 * 2.0 ** -23 + (width / 512 + 16) * 2.0 ** -24) * want
+    assert ((log_sum.double() - want).abs() <= bound).all()
+    assert ((loss.double() - (want - z.gather(1, labels.long()[:, None])[:, 0])).abs() <= 2 * bound).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,width,v", [(4096, 768, 30000), (5001, 520, 24001)])
+def test_gradient_of_many_entries_of_one_sign(rows, width, v):
+    """hidden_diff of positive weights whose labelled entry has a softmax of zero, so that its part of dz is exact, by
+    enough rows for the sum not to be cut into parts.  The vocabulary is summed 1024 entries at a time in 64 additions of 17 addends each (16
+    products and the sum so far), which are cut off at the last place of the largest: less than 17 units of 2^-23 of the sum so far, and as that
+    grows evenly 32.5 times that of the whole.  A half's own rounding, which has no direction, is 2^-11 over the root of how many there are."""
+    t = torch.float16
+    x, w = _made(t, rows, width, seed=1), _made(t, v, width, seed=2).abs() * 0.05
+    x[:, 0], w[:, 0], w[7, 0] = 4.0, 1.0, -8.0
+    labels = torch.full((rows,), 7, dtype=torch.int32, device="cuda")
+    dloss = torch.full((rows,), 1024.0, device="cuda")
+    _, log_sum = ops.VocabularyCrossEntropy(x, w, labels)
+    dx, _ = ops.VocabularyCrossEntropyBackward(dloss, x, w, labels, log_sum, weights_diff=False)
+    part = 1024 * torch.cat([torch.softmax(cut.double() @ w.double().T, 1) @ w.double() for cut in x.split(1024)])[:, 1:]
+    want = part - 1024 * w[7, 1:].double()
+    lost = (dx[:, 1:].double() - want).sum() / part.sum()
+    noise = 2.0 ** -11 * want.abs().max() / part.mean() / (rows * (width - 1)) ** 0.5
+    assert lost.abs() <= 32.5 * 17 * 2.0 ** -23 + 64 * 2.0 ** -24 + 3 * noise
