@@ -268,7 +268,7 @@ __global__ void __launch_bounds__(THREADS, 1) product16_kernel(const Product16Pa
 			}
 			if(on && EPILOGUE == PRODUCT16_DIFF) {
 				logSum2 = __ldg(p.logSum + row) * LOG2E;
-				by = __ldg(p.rowScale + row) * __ldg(p.scale);
+				by = __fdiv_rn(__ldg(p.rowScale + row), __ldg(p.scale)) * __ldg(p.scale + 1);
 				if(label < 0) by = 0.f;
 			}
 			if(EPILOGUE == PRODUCT16_STORE) by = __ldg(p.resultScale);

@@ -36,7 +36,7 @@ struct Product16Params {
 	int columns;         // of all: columns behind are left out
 	// DIFF
 	const float* logSum; // [m]
-	const float* rowScale; // [m], times *scale
+	const float* rowScale; // [m], over scale[0] and times scale[1]
 	const float* scale;
 	// DIFF, STORE
 	void* out;           // STORE: 16-bit or fp32

@@ -7,10 +7,13 @@
 // 8 bytes per row leave the SM for 128 logits (product16.cu).  The backward pass forms the logits anew, piece by piece of the vocabulary: a product
 // whose epilogue turns them into dz, and the two products that consume it.  Bound by the tensor core: 8 rows vocabulary
 // width multiply-adds in all for forward and backward, where keeping the logits would take 6 and rows x vocabulary memory.
-//   dz is kept in the operands' type for those products: the tensor core multiplies like types, and its rounding, half a
-//   step per element with no common direction, is of the size of the results' own.  In fp16 it is scaled by a power
-//   of two that puts the largest loss_diff at 2^14, because softmax values of 1e-7 are below what a half holds; dz between 1
-//   and 2^-38 of the largest then keeps some or all of its bits.  hidden_diff is summed in fp32 over the pieces.
+//   dz is kept in the operands' type for those products: the tensor core multiplies like types, and two planes of dz would make six
+//   products of four.  It is rounded over the largest |loss_diff|, so that one loss_diff for all rows (a mean's 1 / rows) costs nothing: rounded
+//   with it, the labels' elements, which are almost -loss_diff, would all be off alike (1 / 921 in bf16: both gradients 2.2e-3 too small).
+//   What is left is half a step per element of the softmax, in no common direction, and a label's p where p - 1 rounds to -1; rows whose
+//   loss_diff is another are off by up to half a step each.  Gradients of 4096 x 1024 rows over 50257 entries differ in 5e-4 from those of
+//   fp32 dz rounded the same way, 1.66e-3 being that rounding.  In fp16 dz is times 2^14, because softmax values of 1e-7 are below what a
+//   half holds; dz between 1 and 2^-38 of the largest then keeps some or all of its bits.  hidden_diff is summed in fp32 over the pieces.
 // fp32: the same with three bf16 planes of each operand (product16.cuh), a piece of the weights split at a time: six times the
 // multiply-adds, and results as exact as fp32 sums in order give them.  Few rows of fp32: vocabulary_few.cu.
 #include "product16.cuh"
@@ -52,14 +55,14 @@ __device__ __forceinline__ void row_unit(long long i, int perRow, int* row, int*
 	*unit = static_cast<int>(i - static_cast<long long>(r) * perRow);
 }
 
-// The scale of dz (the head of this file) and its inverse: one block.
+// What dz is over and times (the head of this file), and what undoes both: one block.
 __global__ void __launch_bounds__(256) diff_scale_kernel(int rows, const int* __restrict__ labels, const float* __restrict__ lossDiff,
-	int vocabulary, float* scale, int fp16)
+	int vocabulary, float* scale, int type)
 {
 	__shared__ float slots[8];
 	dependent_wait();
 	float most = 0.f;
-	if(fp16) {
+	if(type != NB200_TYPE_FP32) {
 		for(int r = threadIdx.x; r < rows; r += blockDim.x) {
 			if(has_target(labels, r, vocabulary)) most = fmaxf(most, fabsf(lossDiff[r]));
 		}
@@ -69,13 +72,11 @@ __global__ void __launch_bounds__(256) diff_scale_kernel(int rows, const int* __
 	__syncthreads();
 	if(threadIdx.x == 0) {
 		for(int i = 1; i < 8; ++i) most = fmaxf(most, slots[i]);
-		int e = 0;
-		if(most > 0.f && most < INFINITY) {
-			e = 14 - ilogbf(most);
-			e = e > 100 ? 100 : e < -100 ? -100 : e;
-		}
-		scale[0] = ldexpf(1.f, e);
-		scale[1] = ldexpf(1.f, -e);
+		if(!(most > 0.f && most < INFINITY)) most = 1.f;
+		const float by = type == NB200_TYPE_FP16 ? 16384.f : 1.f;
+		scale[0] = most;
+		scale[1] = by;
+		scale[2] = most / by;
 	}
 }
 
@@ -411,7 +412,7 @@ struct Backward {
 		hiddenSplits = splits_of(mTiles * dTiles, piece / PRODUCT16_K);
 		// its result goes straight to the caller where K is not split
 		weightsSplits = splits_of(piece / PRODUCT16_M * dTiles, (q.rows + PRODUCT16_K - 1) / PRODUCT16_K);
-		scale = room.take<float>(2);
+		scale = room.take<float>(3);
 		hidden = room.take<uint16_t>(planes * q.rows * ld);
 		weights = fp32 ? room.take<uint16_t>(3 * piece * ld) : rows_for_tma(q.weights, q.weightsRow) ? nullptr : room.take<uint16_t>(q.vocabulary * ld);
 		diff = room.take<uint16_t>(planes * q.rows * piece);
@@ -570,7 +571,7 @@ int backward(const Problem& q, const float* lossDiff, const int* labels, const f
 	const long long ld = round_up(q.width, 8), hiddenPlane = fp32 ? q.rows * ld : 0, diffPlane = fp32 ? static_cast<long long>(q.rows) * w.piece : 0;
 	if(fp32) split_rows(q.hidden, q.hiddenRow, q.rows, q.width, w.hidden, hiddenPlane, labels, lossDiff, q.vocabulary, stream);
 	else copy_rows(q.hidden, q.hiddenRow, q.rows, q.width, w.hidden, labels, lossDiff, q.vocabulary, stream);
-	launch_dependent(true, diff_scale_kernel, dim3(1), dim3(256), 0, stream, q.rows, labels, lossDiff, q.vocabulary, w.scale, q.type == NB200_TYPE_FP16 ? 1 : 0);
+	launch_dependent(true, diff_scale_kernel, dim3(1), dim3(256), 0, stream, q.rows, labels, lossDiff, q.vocabulary, w.scale, q.type);
 	count_launch();
 	if(!fp32 && w.weights != nullptr) copy_rows(q.weights, q.weightsRow, q.vocabulary, q.width, w.weights, nullptr, nullptr, 0, stream);
 	CUtensorMap hidden, hiddenAcross, rows, across, diff, diffAcross;
@@ -603,11 +604,11 @@ int backward(const Problem& q, const float* lossDiff, const int* labels, const f
 				p.plane = w.weightsPlanes; p.ldPlane = ld;
 				rc = product16(PRODUCT16_SUM, true, true, p, &diffAcross, &hiddenAcross, stream);
 				if(rc != NB200_OK) return rc;
-				sum_planes(q, w.weightsPlanes, p.splits, columns, w.scale + 1, out, weightsDiffRow, stream);
+				sum_planes(q, w.weightsPlanes, p.splits, columns, w.scale + 2, out, weightsDiffRow, stream);
 			} else {
 				p.out = w.weightsRows != nullptr ? w.weightsRows : out;
 				p.ldOut = w.weightsRows != nullptr ? ld : weightsDiffRow;
-				p.resultScale = w.scale + 1;
+				p.resultScale = w.scale + 2;
 				rc = product16(PRODUCT16_STORE, true, true, p, &diffAcross, &hiddenAcross, stream);
 				if(rc != NB200_OK) return rc;
 				if(w.weightsRows != nullptr) {
@@ -618,7 +619,7 @@ int backward(const Problem& q, const float* lossDiff, const int* labels, const f
 			}
 		}
 	}
-	if(hiddenDiff != nullptr) sum_planes(q, w.hiddenPlanes, w.hiddenSplits, q.rows, w.scale + 1, hiddenDiff, hiddenDiffRow, stream);
+	if(hiddenDiff != nullptr) sum_planes(q, w.hiddenPlanes, w.hiddenSplits, q.rows, w.scale + 2, hiddenDiff, hiddenDiffRow, stream);
 	return check_launch();
 }
 

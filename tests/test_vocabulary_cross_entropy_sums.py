@@ -49,3 +49,32 @@ def test_gradient_of_many_entries_of_one_sign(rows, width, v):
     lost = (dx[:, 1:].double() - want).sum() / part.sum()
     noise = 2.0 ** -11 * want.abs().max() / part.mean() / (rows * (width - 1)) ** 0.5
     assert lost.abs() <= 32.5 * 17 * 2.0 ** -23 + 64 * 2.0 ** -24 + 3 * noise
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", HALVES)
+@pytest.mark.parametrize("rows,width,v", [(921, 512, 30000), (48, 1024, 32000), (1843, 200, 9001)])
+@pytest.mark.parametrize("every", [1, 3])
+def test_mean_losses(t, rows, width, v, every):
+    """One loss_diff for all rows that count, 1 / their number as a mean has it, which 16 bits do not hold: neither gradient may be off in a
+    common direction.  A rounding has a deviation of at most a half step over the root of three; dz rounds the softmax's part, a tenth
+    of it here.  The label's element, p - 1, may round to -1, which is off by p; sums lose a few 2^-17 (above)."""
+    x, w = _made(t, rows, width, seed=1), (_made(torch.float32, v, width, seed=2) * (2 / width ** 0.5)).to(t)
+    labels = (torch.arange(rows, device="cuda", dtype=torch.int32) * 7919 % v // 16 * 16).int()   # many of them repeated
+    labels[every::every + 1] = -1
+    scale = 4096.0 if t == torch.float16 else 1.0
+    dloss = torch.full((rows,), scale / (labels >= 0).sum().item(), device="cuda")
+    _, log_sum = ops.VocabularyCrossEntropy(x, w, labels)
+    dx, dw = ops.VocabularyCrossEntropyBackward(dloss, x, w, labels, log_sum)
+    used = labels >= 0
+    p = torch.softmax(x.double() @ w.double().T, 1)
+    at = labels.clamp(min=0).long()[:, None]
+    own = p.gather(1, at)[used].mean()
+    dz = (p.scatter_add(1, at, torch.full_like(at, -1.0, dtype=torch.float64)) * dloss.double()[:, None])[used]
+    half = torch.finfo(t).eps / 2
+    for got, want in ((dx[used], dz @ w.double()), (dw[at[used][:, 0].unique()], (dz.T @ x[used].double())[at[used][:, 0].unique()])):
+        off = got.double() - want
+        tiny = 2.0 ** -25 * want.numel() ** 0.5 if t == torch.float16 else 0.0   # of halves below their normal numbers
+        assert off.norm() <= 1.03 * half / 3 ** 0.5 * want.norm() + tiny
+        lost = (off * want.sign()).sum() / want.abs().sum()
+        assert lost.abs() <= 5 * half / (3 * want.numel()) ** 0.5 * want.norm() / want.abs().mean() / want.numel() ** 0.5 + own + 2.0 ** -15
