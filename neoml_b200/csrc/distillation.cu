@@ -63,8 +63,8 @@ struct Taught {
 	float top, sum, cross;
 	__device__ __forceinline__ void join(const Taught& o)
 	{
+		if(sum == 0.f && o.sum == 0.f) return; // neither has an entry (one that is not a number makes the sum none, and leaves no maximum)
 		const float t = fmaxf(top, o.top);
-		if(t == -INFINITY) return; // neither has an entry
 		const float d1 = top - t, d2 = o.top - t, f1 = exp2_fast(d1), f2 = exp2_fast(d2);
 		// what has vanished adds nothing, not even an infinite loss times zero
 		cross = (f1 == 0.f ? 0.f : f1 * fmaf(d1 * LN2, sum, cross)) + (f2 == 0.f ? 0.f : f2 * fmaf(d2 * LN2, o.sum, o.cross));
@@ -186,7 +186,7 @@ __global__ void __launch_bounds__(THREADS) distillation_forward_kernel(const Dis
 	if(rank == 0) {
 #pragma unroll
 		for(int e = 0; e < ENTRIES; ++e) {
-			// (not a number counts as an entry)
+			// (not a number is an entry too)
 			if(entries[e].at >= 0 && entries[e].x != -INFINITY) taught.join({ entries[e].x, 1.f, -entries[e].z / p.temperature });
 		}
 	}
