@@ -44,32 +44,39 @@ __device__ __forceinline__ float exp2_fast(float x)
 	return y;
 }
 
-// Maximum and the sum of 2^(x - maximum).
+// Maximum of x and the sum of 2^(c (x - maximum)).
 struct Running {
 	float top, sum;
-	__device__ __forceinline__ void join(const Running& o)
+	__device__ __forceinline__ void join(const Running& o, float c)
 	{
 		const float t = fmaxf(top, o.top);
 		const float at = t == -INFINITY ? 0.f : t;
-		sum = sum * exp2_fast(top - at) + o.sum * exp2_fast(o.top - at);
+		sum = sum * exp2_fast((top - at) * c) + o.sum * exp2_fast((o.top - at) * c);
 		top = t;
 	}
+	// log sum exp((x - base) / temperature); the maximum's distance from the base is exact where both are of one size
+	__device__ __forceinline__ float log_sum_over(float base, float temperature) const { return (top - base) / temperature + logf(sum); }
 };
 
 // The teacher's side of a row, or of some of its entries: maximum of x = log2(e) teacher / tau, sum of 2^(x - maximum), and the sum of
-// 2^(x - maximum) (ln 2 (x - maximum) - z / tau), z being the student's logit.  The loss is then
-// tau^2 (cross / sum - ln sum + log_sum): no term is larger than the distributions' logarithms, whatever the logits' common offset.
+// 2^(x - maximum) (ln 2 (x - maximum) - (z - base) / tau), z being the student's logit and base that of the likeliest entry.  The loss is then
+// tau^2 (cross / sum - ln sum + log_sum - base / tau), where the last two are formed as one (log_sum_over): no term is larger than the
+// distributions' logarithms, whatever the logits' common offset.
 struct Taught {
-	float top, sum, cross;
-	__device__ __forceinline__ void join(const Taught& o)
+	float top, sum, cross, base;
+	__device__ __forceinline__ void join(const Taught& o, float overTemperature)
 	{
 		if(sum == 0.f && o.sum == 0.f) return; // neither has an entry (one that is not a number makes the sum none, and leaves no maximum)
 		const float t = fmaxf(top, o.top);
 		const float d1 = top - t, d2 = o.top - t, f1 = exp2_fast(d1), f2 = exp2_fast(d2);
+		// the base is that of the likeliest entry: one that hardly counts may lie at its type's lowest value
+		const float from = top >= o.top ? base : o.base;
+		const float mine = fmaf((from - base) * overTemperature, sum, cross), its = fmaf((from - o.base) * overTemperature, o.sum, o.cross);
 		// what has vanished adds nothing, not even an infinite loss times zero
-		cross = (f1 == 0.f ? 0.f : f1 * fmaf(d1 * LN2, sum, cross)) + (f2 == 0.f ? 0.f : f2 * fmaf(d2 * LN2, o.sum, o.cross));
+		cross = (f1 == 0.f ? 0.f : f1 * fmaf(d1 * LN2, sum, mine)) + (f2 == 0.f ? 0.f : f2 * fmaf(d2 * LN2, o.sum, its));
 		sum = f1 * sum + f2 * o.sum;
 		top = t;
+		base = from;
 	}
 };
 
@@ -135,6 +142,7 @@ __global__ void __launch_bounds__(THREADS) distillation_forward_kernel(const Dis
 	row.end = x + p.vocabulary;
 	Entry entries[ENTRIES];
 	if(rank == 0) load_entries<T, P, THREADS>(p, r, x, entries);
+	// exponents are formed of differences: a type's lowest value times c would be infinite
 	Running mine = { -INFINITY, 0.f };
 	for(int u0 = rank * perBlock; u0 < end; u0 += THREADS * UNROLL) {
 		uint4 raw[UNROLL];
@@ -145,16 +153,16 @@ __global__ void __launch_bounds__(THREADS) distillation_forward_kernel(const Dis
 			float top = unit_top<T>(raw[0]);
 #pragma unroll
 			for(int k = 1; k < UNROLL; ++k) top = fmaxf(top, unit_top<T>(raw[k]));
-			top = fmaxf(mine.top, top * c);
+			top = fmaxf(mine.top, top);
 			const float at = top == -INFINITY ? 0.f : top;
-			float2 sums = make_float2(mine.sum * exp2_fast(mine.top - at), 0.f);
+			float2 sums = make_float2(mine.sum * exp2_fast((mine.top - at) * c), 0.f);
 #pragma unroll
 			for(int k = 0; k < UNROLL; ++k) {
 				float v[V];
 				unit_floats<T, V>(raw[k], v);
 #pragma unroll
 				for(int j = 0; j < V; j += 2) {
-					const float2 e = fma2(make_float2(v[j], v[j + 1]), both(c), both(-at));
+					const float2 e = mul2(add2(make_float2(v[j], v[j + 1]), both(-at)), both(c));
 					sums = add2(sums, make_float2(exp2_fast(e.x), exp2_fast(e.y)));
 				}
 			}
@@ -171,30 +179,35 @@ __global__ void __launch_bounds__(THREADS) distillation_forward_kernel(const Dis
 				float top = mine.top;
 #pragma unroll
 				for(int j = 0; j < V; ++j) {
-					v[j] = inside<V>(first, j, p.vocabulary) ? v[j] * c : -INFINITY;
+					if(!inside<V>(first, j, p.vocabulary)) v[j] = -INFINITY;
 					top = fmaxf(top, v[j]);
 				}
 				const float at = top == -INFINITY ? 0.f : top;
-				mine.sum *= exp2_fast(mine.top - at);
+				mine.sum *= exp2_fast((mine.top - at) * c);
 #pragma unroll
-				for(int j = 0; j < V; ++j) mine.sum += exp2_fast(v[j] - at);
+				for(int j = 0; j < V; ++j) mine.sum += exp2_fast((v[j] - at) * c);
 				mine.top = top;
 			}
 		}
 	}
-	Taught taught = { -INFINITY, 0.f, 0.f };
+	Taught taught = { -INFINITY, 0.f, 0.f, 0.f };
+	const float overTemperature = 1.f / p.temperature;
 	if(rank == 0) {
 #pragma unroll
 		for(int e = 0; e < ENTRIES; ++e) {
 			// (not a number is an entry too)
-			if(entries[e].at >= 0 && entries[e].x != -INFINITY) taught.join({ entries[e].x, 1.f, -entries[e].z / p.temperature });
+			if(entries[e].at >= 0 && entries[e].x != -INFINITY) {
+				// no base are infinite or undefined logits, and those whose multiples would be
+				const bool base = fabsf(entries[e].z) < 1e30f;
+				taught.join({ entries[e].x, 1.f, base ? 0.f : -entries[e].z * overTemperature, base ? entries[e].z : 0.f }, overTemperature);
+			}
 		}
 	}
 #pragma unroll
 	for(int o = 16; o > 0; o >>= 1) {
-		mine.join({ __shfl_xor_sync(0xffffffffu, mine.top, o), __shfl_xor_sync(0xffffffffu, mine.sum, o) });
+		mine.join({ __shfl_xor_sync(0xffffffffu, mine.top, o), __shfl_xor_sync(0xffffffffu, mine.sum, o) }, c);
 		taught.join({ __shfl_xor_sync(0xffffffffu, taught.top, o), __shfl_xor_sync(0xffffffffu, taught.sum, o),
-			__shfl_xor_sync(0xffffffffu, taught.cross, o) });
+			__shfl_xor_sync(0xffffffffu, taught.cross, o), __shfl_xor_sync(0xffffffffu, taught.base, o) }, overTemperature);
 	}
 	if((threadIdx.x & 31) == 0) {
 		warpsOf[threadIdx.x >> 5] = mine;
@@ -204,7 +217,7 @@ __global__ void __launch_bounds__(THREADS) distillation_forward_kernel(const Dis
 	if(blocks > 1) {
 		cg::cluster_group cluster = cg::this_cluster();
 		if(threadIdx.x == 0) {
-			for(int w = 1; w < WARPS; ++w) mine.join(warpsOf[w]);
+			for(int w = 1; w < WARPS; ++w) mine.join(warpsOf[w], c);
 			*cluster.map_shared_rank(&parts[rank], 0) = mine;
 		}
 		cluster.sync();
@@ -212,13 +225,12 @@ __global__ void __launch_bounds__(THREADS) distillation_forward_kernel(const Dis
 	if(rank != 0 || threadIdx.x != 0) return;
 	const Running* const all = blocks > 1 ? parts : warpsOf;
 	mine = all[0];
-	for(int k = 1; k < (blocks > 1 ? blocks : WARPS); ++k) mine.join(all[k]);
-	for(int w = 1; w < WARPS; ++w) taught.join(taughtOf[w]);
-	const float logSum = mine.top * LN2 + logf(mine.sum); // mine.top is in units of log 2
-	p.logSum[r] = logSum;
+	for(int k = 1; k < (blocks > 1 ? blocks : WARPS); ++k) mine.join(all[k], c);
+	for(int w = 1; w < WARPS; ++w) taught.join(taughtOf[w], overTemperature);
+	p.logSum[r] = mine.log_sum_over(0.f, p.temperature);
 	// no entry, or nothing but minus infinity: no loss
 	p.loss[r] = taught.top == -INFINITY && taught.sum == 0.f ? 0.f
-		: p.temperature * p.temperature * (taught.cross / taught.sum - logf(taught.sum) + logSum);
+		: p.temperature * p.temperature * (taught.cross / taught.sum - logf(taught.sum) + mine.log_sum_over(taught.base, p.temperature));
 }
 
 template<typename T, typename P, int V, int THREADS>
@@ -247,16 +259,16 @@ __global__ void __launch_bounds__(THREADS) distillation_backward_kernel(const Di
 			keptAt[k] = entries[e].at;
 			keptX[k] = entries[e].x;
 		}
-		if(entries[e].at >= 0 && entries[e].x != -INFINITY) teacher.join({ entries[e].x, 1.f });
+		if(entries[e].at >= 0 && entries[e].x != -INFINITY) teacher.join({ entries[e].x, 1.f }, 1.f);
 	}
 #pragma unroll
-	for(int o = 16; o > 0; o >>= 1) teacher.join({ __shfl_xor_sync(0xffffffffu, teacher.top, o), __shfl_xor_sync(0xffffffffu, teacher.sum, o) });
+	for(int o = 16; o > 0; o >>= 1) teacher.join({ __shfl_xor_sync(0xffffffffu, teacher.top, o), __shfl_xor_sync(0xffffffffu, teacher.sum, o) }, 1.f);
 	if((threadIdx.x & 31) == 0) warpsOf[threadIdx.x >> 5] = teacher;
 	const float diff = p.temperature * __ldg(p.lossDiff + r), log2Sum = __ldg(p.logSum + r) * LOG2E;
 	__syncthreads();
 	teacher = warpsOf[0];
 #pragma unroll
-	for(int w = 1; w < WARPS; ++w) teacher.join(warpsOf[w]);
+	for(int w = 1; w < WARPS; ++w) teacher.join(warpsOf[w], 1.f);
 	const bool used = !(teacher.top == -INFINITY && teacher.sum == 0.f);
 	Row<T, V> row;
 	row.p = x;
