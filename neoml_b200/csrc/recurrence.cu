@@ -228,6 +228,15 @@ __device__ __forceinline__ Shared<W> begin_sharing(uint8_t* room, uint64_t* arri
 	return { reinterpret_cast<Fold<W>*>(room), warps, blocks, arrived, abortFlag };
 }
 
+// A wait of the whole warp; once one of the block's has given up, the others do as soon as they would have to wait.  A block then sends and
+// asks for nothing more, since its barriers' phases are no longer those of its rounds, but goes through them with what is there: every
+// block has to reach the end.
+__device__ __forceinline__ void wait_warp(uint64_t* bar, uint32_t parity, volatile int* abortFlag, int* status, int site)
+{
+	if(__all_sync(0xffffffffu, mbar_try_wait(bar, parity)) || *abortFlag != 0) return;
+	mbar_wait_bounded_warp(bar, parity, abortFlag, status, site);
+}
+
 // Joins the folds of a round: `mine` is this thread's stretch; the state before it is returned in `state`, and `carry` moves on by
 // the whole round.  Stretches follow one another warp by warp, block by block.
 //   A set of folds is written again two rounds later.  Within the block, the barrier of the round between keeps the writers
@@ -251,7 +260,8 @@ __device__ __forceinline__ void join(const Shared<W>& s, const Fold<W>& mine, in
 	if(warp == warps - 1) { // the block's fold, to every block of the cluster, this one too
 		Fold<W> whole = before;
 		after(whole, mine);
-		if(blocks == 1) { // launched without a cluster: st.async is not an instruction of such a kernel
+		if(*static_cast<volatile int*>(s.abortFlag) != 0) {
+		} else if(blocks == 1) { // launched without a cluster: st.async is not an instruction of such a kernel
 			s.block(set, 0, lane) = whole;
 			__syncwarp();
 			if(lane == 0) mbar_arrive(s.arrived + set);
@@ -260,8 +270,7 @@ __device__ __forceinline__ void join(const Shared<W>& s, const Fold<W>& mine, in
 			for(int k = 0; k < blocks; ++k) send(whole, &s.block(set, rank, lane), s.arrived + set, k);
 		}
 	}
-	// should the wait give up, the rounds go on with what is there: every block has to reach the end
-	mbar_wait_bounded_warp(s.arrived + set, (round >> 1) & 1, s.abortFlag, status, (KERNEL_ID << 8) | 1);
+	wait_warp(s.arrived + set, (round >> 1) & 1, s.abortFlag, status, (KERNEL_ID << 8) | 1);
 	Num<W> start = carry;
 	for(int k = 0; k < blocks; ++k) {
 		if(k == rank) start = carry;
@@ -604,6 +613,7 @@ struct Ring {
 	static constexpr int BOX_BYTES = S * 128;
 	uint8_t* stages;
 	uint64_t* full;
+	int* asked; // rounds asked for
 	int arrays, depth;
 	__device__ __forceinline__ const uint32_t* box(int round, int array) const
 	{
@@ -611,21 +621,32 @@ struct Ring {
 	}
 	__device__ __forceinline__ uint32_t begin(int round) const // by one lane
 	{
+		*asked = round + 1;
 		mbar_arrive_expect_tx(full + round % depth, arrays * BOX_BYTES);
 		return smem_u32(stages + (round % depth) * arrays * BOX_BYTES);
 	}
 	__device__ __forceinline__ void wait(int round, volatile int* abortFlag, int* status) const
 	{
-		mbar_wait_bounded_warp(full + round % depth, (round / depth) & 1, abortFlag, status, (KERNEL_ID << 8) | 2);
+		wait_warp(full + round % depth, (round / depth) & 1, abortFlag, status, (KERNEL_ID << 8) | 2);
+	}
+	// Once a wait has given up: what was asked for lands before the shared memory goes (rounds that have landed come back at once).
+	__device__ __forceinline__ void drain() const
+	{
+		__syncwarp();
+		for(int round = max(*asked - depth, 0); round < *asked; ++round) {
+			int ignored = 0;
+			mbar_wait_bounded_warp(full + round % depth, (round / depth) & 1, &ignored, nullptr, 0);
+		}
 	}
 };
 
 template<int S, int DEPTH>
-__device__ __forceinline__ Ring<S> make_ring(uint8_t* room, uint64_t (&bars)[MAX_WARPS][DEPTH], int arrays)
+__device__ __forceinline__ Ring<S> make_ring(uint8_t* room, uint64_t (&bars)[MAX_WARPS][DEPTH], int (&asked)[MAX_WARPS], int arrays)
 {
 	const int warp = threadIdx.x >> 5;
-	Ring<S> ring = { room + warp * DEPTH * arrays * Ring<S>::BOX_BYTES, bars[warp], arrays, DEPTH };
+	Ring<S> ring = { room + warp * DEPTH * arrays * Ring<S>::BOX_BYTES, bars[warp], asked + warp, arrays, DEPTH };
 	if((threadIdx.x & 31) == 0) {
+		asked[warp] = 0;
 		for(int k = 0; k < DEPTH; ++k) mbar_init(ring.full + k, 1);
 		mbar_init_fence();
 	}
@@ -640,17 +661,18 @@ __device__ __forceinline__ void stage_read()
 }
 
 template<typename T, int W, bool INPUT, int S, int DEPTH, bool STATES>
-__global__ void __launch_bounds__(MAX_WARPS * 32, S == 8 ? 3 : 2) recurrence_forward_stream_kernel(const RecurrenceParams p, const __grid_constant__ Maps maps)
+__global__ void __launch_bounds__(MAX_WARPS * 32, 2) recurrence_forward_stream_kernel(const RecurrenceParams p, const __grid_constant__ Maps maps)
 {
 	extern __shared__ __align__(128) uint8_t sharedRoom[];
 	__shared__ uint64_t arrived[2];
 	__shared__ int abortFlag;
 	__shared__ uint64_t bars[MAX_WARPS][DEPTH];
+	__shared__ int asked[MAX_WARPS];
 	constexpr int ARRAYS = INPUT ? 3 : 2;
 	const int blocks = gridDim.y, rank = blockIdx.y;
 	const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 	constexpr int BOX_BYTES = Ring<S>::BOX_BYTES;
-	const Ring<S> ring = make_ring<S, DEPTH>(sharedRoom + shared_bytes(warps, blocks, W), bars, ARRAYS);
+	const Ring<S> ring = make_ring<S, DEPTH>(sharedRoom + shared_bytes(warps, blocks, W), bars, asked, ARRAYS);
 	const Shared<W> s = begin_sharing<W>(sharedRoom, arrived, &abortFlag, warps, blocks);
 	const int b = blockIdx.z;
 	const int tile = blockIdx.x * 32 * W;
@@ -671,7 +693,7 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, S == 8 ? 3 : 2) recurrence_for
 	if(on) carry = load_state<W>(p.first, state0, 1);
 	auto ask = [&](int round) {
 		const int t = first + round * stride;
-		if(t >= n || lane != 0) return; // (a box may lie in front of step 0: rounds that a warp leaves out are the last ones)
+		if(t >= n || lane != 0 || *static_cast<volatile int*>(s.abortFlag) != 0) return; // (a box may lie in front of step 0: rounds that a warp leaves out are the last ones)
 		const uint32_t at = ring.begin(round);
 		uint64_t* const bar = ring.full + round % DEPTH;
 		tma_load_3d(at, &maps.z, bar, tile, t, b);
@@ -724,6 +746,7 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, S == 8 ? 3 : 2) recurrence_for
 		}
 		outRound += roundBytes;
 	}
+	if(*static_cast<volatile int*>(s.abortFlag) != 0) ring.drain();
 	// behind the sequence the results are zeros
 	for(int k = n + rank * warps + warp; !STATES && k < p.length; k += blocks * warps) {
 		if(on) store_raw<T, W, false>(out + static_cast<long long>(k) * p.channels + c, all<W>(0.f), 1);
@@ -740,13 +763,14 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 2) recurrence_backward_stream_
 	__shared__ uint64_t arrived[2];
 	__shared__ int abortFlag;
 	__shared__ uint64_t bars[MAX_WARPS][DEPTH];
+	__shared__ int asked[MAX_WARPS];
 	constexpr bool STORED = sizeof(T) == 4; // the result holds the states as they were
 	constexpr int ARRAYS = backward_arrays(INPUT, STORED), INPUT_AT = ARRAYS - 1;
 	static_assert(STORED || S % STEPS == 0, "a state in front of every stretch");
 	const int blocks = gridDim.y, rank = blockIdx.y;
 	const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 	constexpr int BOX_BYTES = Ring<S>::BOX_BYTES;
-	const Ring<S> ring = make_ring<S, DEPTH>(sharedRoom + shared_bytes(warps, blocks, W), bars, ARRAYS);
+	const Ring<S> ring = make_ring<S, DEPTH>(sharedRoom + shared_bytes(warps, blocks, W), bars, asked, ARRAYS);
 	const Shared<W> s = begin_sharing<W>(sharedRoom, arrived, &abortFlag, warps, blocks);
 	const int b = blockIdx.z;
 	const int tile = blockIdx.x * 32 * W;
@@ -772,7 +796,7 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 2) recurrence_backward_stream_
 	}
 	auto ask = [&](int round) {
 		const int t = n - 1 - back - round * stride, from = t - S + 1; // a box may begin in front of step 0
-		if(t < 0 || lane != 0) return;
+		if(t < 0 || lane != 0 || *static_cast<volatile int*>(s.abortFlag) != 0) return;
 		const uint32_t at = ring.begin(round);
 		uint64_t* const bar = ring.full + round % DEPTH;
 		tma_load_3d(at, &maps.f, bar, tile, from, b);
@@ -865,6 +889,7 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 2) recurrence_backward_stream_
 		ask(round + DEPTH);
 		outRound -= roundBytes;
 	}
+	if(*static_cast<volatile int*>(s.abortFlag) != 0) ring.drain();
 	if(blocks > 1) cg::this_cluster().sync();
 	if(on && p.last != nullptr && rank == 0 && warp == 0) store_state<W>(p.last, state0, carry, 1);
 }

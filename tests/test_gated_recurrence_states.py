@@ -130,3 +130,8 @@ def test_gradients_in_place_of_an_operand_are_refused():
         near[13] = good[7] + off
         if not torch.cuda.is_available():   # nothing to refuse but the device
             assert lib.nb200_gated_recurrence_backward(*near) == capi.ENODEVICE
+
+
+@pytest.mark.gpu
+def test_no_wait_gave_up():
+    assert capi.load().nb200_device_status(None, 0) == 0
