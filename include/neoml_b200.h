@@ -339,7 +339,7 @@ NB200_API int nb200_layer_normalization_backward(void* stream, int type, int par
  * h[t]; initial_state (NULL: zeros) and final_state (NULL: not wanted) are fp32 [batch][channels], and may be the same
  * memory.  lengths (NULL: all of `length`) ends sequences early: behind a sequence's end nothing is read, the result is
  * zero and the state stays (values outside 0..length count as the nearer of the two).  Strides of the three inputs are in elements, channels are adjacent; a stride of
- * zero repeats a sequence or a step. */
+ * zero repeats a sequence or a step.  At most 65535 sequences, 2^30 steps and 2^30 channels (NB200_ETOOBIG). */
 typedef struct nb200_recurrence_desc {
 	int batch, length, channels;
 	long long update_batch, update_row, forget_batch, forget_row, input_batch, input_row; /* from sequence to sequence, step to step */

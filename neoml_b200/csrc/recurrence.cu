@@ -32,6 +32,7 @@ namespace cg = cooperative_groups;
 constexpr int STEPS = 8;       // of a thread
 constexpr int MAX_WARPS = 8;   // of a block
 constexpr int MAX_CLUSTER = 8;
+constexpr int MAX_BATCH = 65535; // sequences are the grid's third dimension
 constexpr int KERNEL_ID = 0x71; // in the status word: (KERNEL_ID << 8) | site
 
 struct RecurrenceParams {
@@ -1074,7 +1075,7 @@ int nb200_gated_recurrence(void* stream, int type, const nb200_recurrence_desc* 
 	if(d->length > 0 && (update == nullptr || forget == nullptr || result == nullptr)) return NB200_EINVAL;
 	if(!type_aligned(update, type) || !type_aligned(forget, type) || !type_aligned(input, type) || !type_aligned(result, type)
 		|| !words_aligned(initial_state, final_state, lengths)) return NB200_EINVAL;
-	if(d->batch > 65535 || d->length > (1 << 30)) return NB200_ETOOBIG;
+	if(d->batch > MAX_BATCH || d->length > (1 << 30) || d->channels > (1 << 30)) return NB200_ETOOBIG;
 	if(device_status_word() == nullptr) return NB200_ENODEVICE;
 	RecurrenceParams p = {};
 	p.z = update; p.f = forget; p.i = input; p.out = result; p.first = initial_state; p.last = final_state; p.lengths = lengths;
@@ -1108,7 +1109,7 @@ int nb200_gated_recurrence_backward(void* stream, int type, const nb200_recurren
 			|| !apart(update_diff, own, forget, extent(d, d->forget_batch, d->forget_row) * size)
 			|| !apart(update_diff, own, input, extent(d, d->input_batch, d->input_row) * size)) return NB200_EINVAL;
 	}
-	if(d->batch > 65535 || d->length > (1 << 30)) return NB200_ETOOBIG;
+	if(d->batch > MAX_BATCH || d->length > (1 << 30) || d->channels > (1 << 30)) return NB200_ETOOBIG;
 	if(device_status_word() == nullptr) return NB200_ENODEVICE;
 	RecurrenceParams p = {};
 	p.z = update; p.f = forget; p.i = input; p.dh = result_diff; p.h = result;

@@ -540,7 +540,7 @@ def GatedRecurrence(update, forget, input=None, *, initial_state=None, lengths=N
     final_state): every h[t] in the update's type, and the last state, fp32 [batch, channels].  initial_state is fp32 too
     (None: zeros); `final_state` may be the same tensor, as when tokens are served one at a time.  lengths (int32 [batch])
     ends sequences early: behind their end the result is zero and the state stays.  The three inputs may be strided views or
-    expanded; channels are adjacent."""
+    expanded; channels are adjacent.  At most 65535 sequences."""
     done = _native().gated_recurrence(update, forget, input, initial_state, lengths, result, final_state)
     if done is not None:
         return _checked("GatedRecurrence", done)

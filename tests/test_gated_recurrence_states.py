@@ -132,6 +132,15 @@ def test_gradients_in_place_of_an_operand_are_refused():
             assert lib.nb200_gated_recurrence_backward(*near) == capi.ENODEVICE
 
 
+def test_sizes_beyond_the_limits_are_refused():
+    lib = capi.load()
+    for head in ((65536, 3, 4), (1, 2 ** 30 + 1, 1), (1, 1, 2 ** 30 + 1), (1, 1, 2 ** 31 - 1)):
+        desc = ctypes.byref(capi.RecurrenceDesc(*head, 0, 0, 0, 0, 0, 0))
+        assert lib.nb200_gated_recurrence(None, 1, desc, 64, 64, None, None, None, 64, None) == capi.ETOOBIG, head
+        backward = [None, 0, desc, 64, 0, 0, 64, 64, 64, None, None, None, None, 64, 64, None, None]
+        assert lib.nb200_gated_recurrence_backward(*backward) == capi.ETOOBIG, head
+
+
 @pytest.mark.gpu
 def test_no_wait_gave_up():
     assert capi.load().nb200_device_status(None, 0) == 0
