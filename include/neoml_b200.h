@@ -379,15 +379,16 @@ NB200_API int nb200_distillation_loss_backward(void* stream, int type, int teach
  * gradient, whatever the row holds.  Both matrices are of `type`; sums are fp32.  `scratch` holds nb200_vocabulary_cross_entropy_scratch_bytes(...) bytes, 256-byte
  * aligned: for the logits' partial sums (8 bytes per row and 128 entries), for copies of operands whose rows do not begin on 16-byte boundaries
  * (of 16-bit types), for the hidden rows and up to 1 GB of the weights in the tensor core's parts (fp32), and for one piece of the
- * gradient by the logits (backward), 256 MB or 256 columns if that is more. */
+ * gradient by the logits (backward), 256 MB or 256 columns if that is more.  At most 2^24 rows and elements of a row, 2^28 vocabulary
+ * entries (NB200_ETOOBIG). */
 NB200_API size_t nb200_vocabulary_cross_entropy_scratch_bytes(int type, const void* hidden, int rows, int width,
 	long long hidden_row_size, const void* weights, int vocabulary, long long weights_row_size, int backward);
 NB200_API int nb200_vocabulary_cross_entropy(void* stream, int type, const void* hidden, int rows, int width,
 	long long hidden_row_size, const void* weights, int vocabulary, long long weights_row_size, const int* labels, float* loss,
 	float* log_sum, void* scratch);
 /* Its gradients by hidden and weights, each NULL where not wanted: with dz = loss_diff[r] * (softmax(z) - [j = label[r]]) the
- * products dz * weights and dz^T * hidden (NME.h:529-532, NME.h:580-582).  log_sum is the forward pass's.  No atomics: the
- * same bits from run to run. */
+ * products dz * weights and dz^T * hidden (NME.h:529-532, NME.h:580-582).  log_sum is the forward pass's.  dz of 16-bit types is rounded
+ * to the type, over the largest |loss_diff|.  No atomics: the same bits from run to run. */
 NB200_API int nb200_vocabulary_cross_entropy_backward(void* stream, int type, const float* loss_diff, const void* hidden,
 	int rows, int width, long long hidden_row_size, const void* weights, int vocabulary, long long weights_row_size,
 	const int* labels, const float* log_sum, void* hidden_diff, long long hidden_diff_row_size, void* weights_diff,

@@ -651,9 +651,9 @@ int nb200_vocabulary_cross_entropy(void* stream, int type, const void* hidden, i
 	const Problem q = { type, rows, width, vocabulary, hidden, weights, hidden_row_size, weights_row_size };
 	if(!valid(q)) return NB200_EINVAL;
 	if(rows == 0) return NB200_OK;
+	if(too_big(q)) return NB200_ETOOBIG; // before the scratch memory, which has no size then
 	if(hidden == nullptr || weights == nullptr || labels == nullptr || loss == nullptr || log_sum == nullptr || !scratch_valid(scratch)
 		|| !words_aligned(labels, loss, log_sum)) return NB200_EINVAL;
-	if(too_big(q)) return NB200_ETOOBIG;
 	if(device_status_word() == nullptr) return NB200_ENODEVICE;
 	return forward(q, labels, loss, log_sum, scratch, as_stream(stream));
 }
@@ -667,9 +667,9 @@ int nb200_vocabulary_cross_entropy_backward(void* stream, int type, const float*
 	if((hidden_diff != nullptr && hidden_diff_row_size < width) || (weights_diff != nullptr && weights_diff_row_size < width)
 		|| !type_aligned(hidden_diff, type) || !type_aligned(weights_diff, type)) return NB200_EINVAL;
 	if(hidden_diff == nullptr && weights_diff == nullptr) return NB200_OK;
+	if(too_big(q)) return NB200_ETOOBIG;
 	if(rows > 0 && (hidden == nullptr || weights == nullptr || labels == nullptr || loss_diff == nullptr || log_sum == nullptr
 		|| !scratch_valid(scratch) || !words_aligned(loss_diff, labels, log_sum))) return NB200_EINVAL;
-	if(too_big(q)) return NB200_ETOOBIG;
 	if(rows == 0 && weights_diff == nullptr) return NB200_OK;
 	if(device_status_word() == nullptr) return NB200_ENODEVICE;
 	if(rows == 0) { // sums over no rows

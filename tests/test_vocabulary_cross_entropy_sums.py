@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+from neoml_b200 import _capi as capi
 from neoml_b200 import ops
 
 HALVES = [torch.float16, torch.bfloat16]
@@ -78,3 +79,14 @@ def test_mean_losses(t, rows, width, v, every):
         assert off.norm() <= 1.03 * half / 3 ** 0.5 * want.norm() + tiny
         lost = (off * want.sign()).sum() / want.abs().sum()
         assert lost.abs() <= 5 * half / (3 * want.numel()) ** 0.5 * want.norm() / want.abs().mean() / want.numel() ** 0.5 + own + 2.0 ** -15
+
+
+def test_sizes_beyond_the_limits_are_named():
+    """Their scratch memory has no size, so none can be given."""
+    lib = capi.load()
+    for rows, width, v in ((2 ** 24 + 1, 8, 10), (4, 2 ** 24 + 8, 10), (4, 8, 2 ** 28 + 1)):
+        for t in (0, 2):
+            assert lib.nb200_vocabulary_cross_entropy_scratch_bytes(t, 64, rows, width, width, 64, v, width, 1) == 0
+            assert lib.nb200_vocabulary_cross_entropy(None, t, 64, rows, width, width, 64, v, width, 64, 64, 64, None) == capi.ETOOBIG
+            assert lib.nb200_vocabulary_cross_entropy_backward(None, t, 64, 64, rows, width, width, 64, v, width, 64, 64, 64, width, 64, width,
+                                                               None) == capi.ETOOBIG
