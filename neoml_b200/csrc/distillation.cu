@@ -37,13 +37,6 @@ struct DistillParams {
 	float temperature;
 };
 
-__device__ __forceinline__ float exp2_fast(float x)
-{
-	float y;
-	asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-	return y;
-}
-
 // Maximum of x and the sum of 2^(c (x - maximum)).
 struct Running {
 	float top, sum;

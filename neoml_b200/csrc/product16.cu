@@ -38,13 +38,6 @@ constexpr int KERNEL_ID = 0x70;       // in the status word: (KERNEL_ID << 8) | 
 constexpr float LOG2E = 1.4426950408889634f;
 enum { SITE_LOAD = 1, SITE_MMA = 2, SITE_MMA_ACC = 3, SITE_EPILOGUE = 4 };
 
-__device__ __forceinline__ float exp2_fast(float x)
-{
-	float y;
-	asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-	return y;
-}
-
 // The products of planes in the order of their MMAs, small ones first: 0 hi, 1 mid, 2 lo.
 __device__ constexpr int PLANE_A[6] = { 2, 0, 1, 1, 0, 0 }, PLANE_B[6] = { 0, 2, 1, 0, 1, 0 };
 // K blocks that are summed in tensor memory before the epilogue warps add them up in registers.

@@ -69,12 +69,6 @@ template<int W> __device__ __forceinline__ Num<W> pick(bool yes, Num<W> a, Num<W
 	else return { make_float2(yes ? a.v.x : b.v.x, yes ? a.v.y : b.v.y) };
 }
 
-__device__ __forceinline__ float exp2_fast(float x)
-{
-	float y;
-	asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-	return y;
-}
 __device__ __forceinline__ float inverse_fast(float x)
 {
 	float y;

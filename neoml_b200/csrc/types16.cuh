@@ -204,6 +204,13 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
 }
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
+__device__ __forceinline__ float exp2_fast(float x)
+{
+	float y;
+	asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+	return y;
+}
+
 __device__ __forceinline__ float warp_sum_all(float v)
 {
 #pragma unroll

@@ -24,13 +24,6 @@ constexpr int TILE = FEW_TILE;       // vocabulary entries
 constexpr int CHUNK = 64;            // elements of them at a time
 constexpr int PITCH = CHUNK + 4;     // 8 entries x 4 elements of a warp's read lie in 32 different banks
 
-__device__ __forceinline__ float exp2_fast(float x)
-{
-	float y;
-	asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-	return y;
-}
-
 // What a warp has in hand of a chunk: its eight entries' elements lane and lane + 32.
 struct Staged {
 	static constexpr int ROWS = TILE / WARPS;
