@@ -17,8 +17,9 @@
 // The next round's loads are issued before this one is folded.
 // The gates' pre-activations are the inputs: a gate of 0.999 rounded to bf16 is 1 and would never forget.
 // The backward pass of fp32 takes h_{t-1} from the result.  In 16-bit types the result is rounded (half a step of it in d(forget), and an infinite
-// one where a half ends), so the states are formed again in fp32: a pass over the inputs stores one in front of every eight steps, which costs
-// a quarter of an array's bytes, and a thread of the backward kernel goes through its own steps from there.
+// one where a half ends), so the states are formed again in fp32: a pass over the inputs stores one in front of every eight steps, a quarter of an
+// array's bytes, and a thread of the backward kernel goes through its own steps from there while the folds are under way (16 x 2048 x 2048
+// bf16: 60 us and 132; by rounded states 141 without that pass, and gradients 1.77e-3 off instead of 1.66e-3).
 #include "product16.cuh"
 #include <cooperative_groups.h>
 #include <cuda.h>
@@ -237,9 +238,10 @@ __device__ __forceinline__ void wait_warp(uint64_t* bar, uint32_t parity, volati
 //   A set of folds is written again two rounds later.  Within the block, the barrier of the round between keeps the writers
 // behind the readers.  Between blocks: a block sends its fold of a round after its own barrier, when all its warps have read
 // the set of the round before, and nobody sends the round after next without having received that fold.
-template<int W>
+// `meanwhile` is what can be done without the state, while the folds are under way.
+template<int W, typename F>
 __device__ __forceinline__ void join(const Shared<W>& s, const Fold<W>& mine, int round, int rank, int blocks, int warps, int* status,
-	Num<W>& carry, Num<W>& state)
+	Num<W>& carry, Num<W>& state, F&& meanwhile)
 {
 	const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, set = round & 1;
 	Fold<W> before = { all<W>(1.f), all<W>(0.f) };
@@ -265,6 +267,7 @@ __device__ __forceinline__ void join(const Shared<W>& s, const Fold<W>& mine, in
 			for(int k = 0; k < blocks; ++k) send(whole, &s.block(set, rank, lane), s.arrived + set, k);
 		}
 	}
+	meanwhile();
 	wait_warp(s.arrived + set, (round >> 1) & 1, s.abortFlag, status, (KERNEL_ID << 8) | 1);
 	Num<W> start = carry;
 	for(int k = 0; k < blocks; ++k) {
@@ -399,7 +402,7 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, W == 1 ? 3 : 2) recurrence_for
 		if(all_steps.whole(t + stride, STEPS)) load(t + stride, Yes());
 		else load(t + stride, No());
 		Num<W> state;
-		join<W>(s, mine, round, rank, blocks, warps, p.status, carry, state);
+		join<W>(s, mine, round, rank, blocks, warps, p.status, carry, state, [] {});
 		auto apply = [&](auto full) {
 #pragma unroll
 			for(int k = 0; k < STEPS; ++k) {
@@ -531,11 +534,9 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 2) recurrence_backward_kernel(
 		}
 		if(nextWhole) load_gates(t - stride, Yes());
 		else load_gates(t - stride, No());
-		Num<W> state;
-		join<W>(s, mine, round, rank, blocks, warps, p.status, carry, state);
-		auto apply = [&](auto full) {
-			// d(forget) of a step: S times this, which takes the state in front of it
-			Num<W> slope[STEPS];
+		// d(forget) of a step: S times this, which takes the state in front of it
+		Num<W> slope[STEPS];
+		auto slopes = [&](auto full) {
 			Num<W> running = first;
 			if constexpr(!STORED && decltype(full)::value) running = from_parts<W>(parts);
 #pragma unroll
@@ -552,6 +553,13 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 2) recurrence_backward_kernel(
 				}
 				slope[k] = mul(mul(a[k], u[k]), INPUT ? before : fma(value, all<W>(-1.f), before));
 			}
+		};
+		Num<W> state;
+		join<W>(s, mine, round, rank, blocks, warps, p.status, carry, state, [&] {
+			if(whole) slopes(Yes());
+			else slopes(No());
+		});
+		auto apply = [&](auto full) {
 #pragma unroll
 			for(int k = 0; k < STEPS; ++k) {
 				const Num<W> S = add(state, number<T, W>(rd[k]));
@@ -594,7 +602,7 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 2) recurrence_backward_kernel(
 // ---- the same fed by TMA ----------------------------------------------------------------------------------------------
 // Long sequences whose rows begin on 16-byte boundaries: a warp's stretches come as boxes of S steps x 128 bytes into a ring of its
 // own in shared memory, several rounds ahead, by one lane's instructions; steps and channels that do not exist come as zeros.  Loads into
-// registers are one round ahead at most: the kernels above take 1.1 to 1.5 times as long (launch()'s comment).  A ring needs no
+// registers are one round ahead at most: the kernels above take 1.1 to 1.3 times as long (launch()'s comment).  A ring needs no
 // barrier for free stages: its warp has read a stage when it asks for the next round in its place.
 
 struct Maps {
@@ -721,7 +729,7 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 2) recurrence_forward_stream_k
 		stage_read();
 		ask(round + DEPTH);
 		Num<W> state;
-		join<W>(s, mine, round, rank, blocks, warps, p.status, carry, state);
+		join<W>(s, mine, round, rank, blocks, warps, p.status, carry, state, [] {});
 		auto apply = [&](auto full) {
 #pragma unroll
 			for(int k = 0; k < S; ++k) {
@@ -810,6 +818,13 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 2) recurrence_backward_stream_
 		if constexpr(INPUT) store_raw<T, W, false>(reinterpret_cast<T*>(di + at), all<W>(0.f), 1);
 	}
 	int t = n - 1 - back;
+	uint2 parts = make_uint2(0u, 0u); // the state in front of the stretch, a round ahead
+	auto load_next = [&](int t, long long round) {
+		if constexpr(!STORED) {
+			if(on && t - S >= 0) parts = load_parts<T, false>(reinterpret_cast<const T*>(dz + round + offset[S - 1]), p.channels, 1);
+		}
+	};
+	load_next(t, outRound);
 	for(int round = 0; round * stride < n; ++round, t -= stride) {
 		Num<W> a[S], u[S];
 		Fold<W> mine = { all<W>(1.f), all<W>(0.f) };
@@ -828,18 +843,12 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 2) recurrence_backward_stream_
 			}
 		};
 		const bool whole = t - S >= 0;
-		uint2 parts = make_uint2(0u, 0u); // the state in front of the stretch
-		if constexpr(!STORED) {
-			if(on && whole) parts = load_parts<T, false>(reinterpret_cast<const T*>(dz + outRound + offset[S - 1]), p.channels, 1);
-		}
 		if(t >= 0) ring.wait(round, s.abortFlag, p.status);
 		if(whole) fold(Yes());
 		else if(t >= 0) fold(No());
-		Num<W> state;
-		join<W>(s, mine, round, rank, blocks, warps, p.status, carry, state);
-		auto apply = [&](auto full) {
-			// d(forget) of a step: S times this, which takes the state in front of it
-			Num<W> slope[S];
+		// d(forget) of a step: S times this, which takes the state in front of it
+		Num<W> slope[S];
+		auto slopes = [&](auto full) {
 			Num<W> running = first;
 			if constexpr(!STORED && decltype(full)::value) running = from_parts<W>(parts);
 #pragma unroll
@@ -857,6 +866,14 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 2) recurrence_backward_stream_
 				}
 				slope[k] = mul(mul(a[k], u[k]), INPUT ? before : fma(value, all<W>(-1.f), before));
 			}
+		};
+		Num<W> state;
+		join<W>(s, mine, round, rank, blocks, warps, p.status, carry, state, [&] {
+			if(whole) slopes(Yes());
+			else if(t >= 0) slopes(No());
+			load_next(t - stride, outRound - roundBytes);
+		});
+		auto apply = [&](auto full) {
 #pragma unroll
 			for(int k = 0; k < S; ++k) {
 				const int row = (S - 1 - k) * 32;
@@ -955,10 +972,11 @@ bool make_maps(Maps& maps, int type, bool backward, const RecurrenceParams& p, i
 
 // How many warps and blocks share a sequence's time axis: the fewest that fill three quarters of the warps that the SMs hold
 // (16, or 24 in the kernels of fewer registers); up to four warps before more blocks, which exchange folds through the cluster.  Measured,
-// forward + backward by TMA: 16 x 2048 x 2048 bf16 73 + 141 us in blocks of four, 100 + 170 of two, 78 + 140 of eight, 80 + 144 in clusters of
-// two; 64 x 100 x 4096 fp16 39 + 57 in blocks of two, 60 + 94 of eight.  Where there are few channels (2 x 16384 x 2048 bf16) clusters of eight
-// blocks of four: 84 + 141, in clusters of four 116 + 199, without 352 + 617.  By loads into registers the three take 93 + 181, 43 + 77 and
-// 104 + 213 in the same shapes.
+// forward + both backward passes by TMA: 16 x 2048 x 2048 bf16 75 + 192 us in blocks of four, 105 + 269 of two, 81 + 206 of eight, 81 + 210 in
+// clusters of two; 64 x 100 x 4096 fp16 40 + 91 in blocks of two, 50 + 110 of four, 60 + 144 of eight.  Where there are few channels (2 x 16384 x 2048 bf16)
+// clusters of eight blocks of four: 86 + 216, in clusters of four 120 + 300, without 373 + 958.  By loads into registers the three take 94 + 248,
+// 43 + 112 and 105 + 289 in the same shapes.  fp32: 16 x 2048 x 2048 142 + 290 (0.87 and 0.85 of the copy rate), 24 x 1021 x 1024 with input
+// gates 78 + 142.
 int launch(int type, bool pair, Pass pass, RecurrenceParams p, int batch, cudaStream_t stream)
 {
 	const bool backward = pass == BACKWARD;
