@@ -90,3 +90,28 @@ def test_sizes_beyond_the_limits_are_named():
             assert lib.nb200_vocabulary_cross_entropy(None, t, 64, rows, width, width, 64, v, width, 64, 64, 64, None) == capi.ETOOBIG
             assert lib.nb200_vocabulary_cross_entropy_backward(None, t, 64, 64, rows, width, width, 64, v, width, 64, 64, 64, width, 64, width,
                                                                None) == capi.ETOOBIG
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", [torch.float32, *HALVES])
+@pytest.mark.parametrize("rows,width,v", [(5, 64, 3000), (20, 64, 9600), (200, 96, 1001), (40, 130, 40000)])   # few rows, some, wide and narrow tiles
+@pytest.mark.parametrize("offset", [0.0, 200.0, -500.0])
+def test_losses_of_confident_rows(t, rows, width, v, offset):
+    """The label has nearly all of the probability, all logits a common part: the loss is small and does not know that part.  What a
+    product's rounding moves of the logits, a few units of their terms' size, counts as far as the other entries do.  The sum of
+    exponentials is about one and rounded at that size: 8 + 2 additions of a thread's 32 columns, 4 of its groups of them (by the kernels for few
+    rows, 16 entries one after another, twice each), 3 + 5 joins of the parts, the exponential and the logarithm two each: 48 at most."""
+    x, w = _made(t, rows, width, seed=1), (_made(torch.float32, v, width, seed=2) / width ** 0.5).to(t)
+    labels = torch.full((rows,), 5, dtype=torch.int32, device="cuda")
+    x[:, 0], w[:, 0] = 8.0, offset / 8
+    at = labels.long()[:, None]
+    x[:, 1], w[:, 1], w[5, 1] = 4.0, 0.0, 4.0       # 16 above the others
+    z = x.double() @ w.double().T
+    loss, log_sum = ops.VocabularyCrossEntropy(x, w, labels)
+    p = torch.softmax(z, 1)
+    rest = p.scatter(1, at, 0.0).sum(1)
+    want = -torch.log1p(-rest)
+    moved = (x.double().abs() @ w.double().abs().T).amax(1) * 2.0 ** -20
+    assert rest.max() < 0.2
+    assert ((loss.double() - want).abs() <= 2 * rest * (moved + (32 + v / 128) * 2.0 ** -24) + 48 * 2.0 ** -24 * (1 + want)).all()
+    assert ((log_sum.double() - torch.logsumexp(z, 1)).abs() <= moved + 2.0 ** -22 * (1 + log_sum.double().abs())).all()
