@@ -56,22 +56,25 @@ __device__ __forceinline__ void row_unit(long long i, int perRow, int* row, int*
 }
 
 // What dz is over and times (the head of this file), and what undoes both: one block.
-__global__ void __launch_bounds__(256) diff_scale_kernel(int rows, const int* __restrict__ labels, const float* __restrict__ lossDiff,
+constexpr int SCALE_THREADS = 1024;
+__global__ void __launch_bounds__(SCALE_THREADS) diff_scale_kernel(int rows, const int* __restrict__ labels, const float* __restrict__ lossDiff,
 	int vocabulary, float* scale, int type)
 {
-	__shared__ float slots[8];
+	__shared__ float slots[SCALE_THREADS / 32];
 	dependent_wait();
 	float most = 0.f;
 	if(type != NB200_TYPE_FP32) {
-		for(int r = threadIdx.x; r < rows; r += blockDim.x) {
-			if(has_target(labels, r, vocabulary)) most = fmaxf(most, fabsf(lossDiff[r]));
+#pragma unroll 8
+		for(int r = threadIdx.x; r < rows; r += SCALE_THREADS) {
+			const float diff = fabsf(__ldg(lossDiff + r));
+			most = fmaxf(most, has_target(labels, r, vocabulary) ? diff : 0.f);
 		}
 	}
 	most = warp_max_all(most);
 	if((threadIdx.x & 31) == 0) slots[threadIdx.x >> 5] = most;
 	__syncthreads();
 	if(threadIdx.x == 0) {
-		for(int i = 1; i < 8; ++i) most = fmaxf(most, slots[i]);
+		for(int i = 1; i < SCALE_THREADS / 32; ++i) most = fmaxf(most, slots[i]);
 		if(!(most > 0.f && most < INFINITY)) most = 1.f;
 		const float by = type == NB200_TYPE_FP16 ? 16384.f : 1.f;
 		scale[0] = most;
@@ -580,7 +583,7 @@ int backward(const Problem& q, const float* lossDiff, const int* labels, const f
 	const long long ld = round_up(q.width, 8), hiddenPlane = fp32 ? q.rows * ld : 0, diffPlane = fp32 ? static_cast<long long>(q.rows) * w.piece : 0;
 	if(fp32) split_rows(q.hidden, q.hiddenRow, q.rows, q.width, w.hidden, hiddenPlane, labels, lossDiff, q.vocabulary, stream);
 	else copy_rows(q.hidden, q.hiddenRow, q.rows, q.width, w.hidden, labels, lossDiff, q.vocabulary, stream);
-	launch_dependent(true, diff_scale_kernel, dim3(1), dim3(256), 0, stream, q.rows, labels, lossDiff, q.vocabulary, w.scale, q.type);
+	launch_dependent(true, diff_scale_kernel, dim3(1), dim3(SCALE_THREADS), 0, stream, q.rows, labels, lossDiff, q.vocabulary, w.scale, q.type);
 	count_launch();
 	if(!fp32 && w.weights != nullptr) copy_rows(q.weights, q.weightsRow, q.vocabulary, q.width, w.weights, nullptr, nullptr, 0, stream);
 	CUtensorMap hidden, hiddenAcross, rows, across, diff, diffAcross;
